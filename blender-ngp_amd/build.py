@@ -23,7 +23,9 @@ KERNEL_SOURCES = ["density_grid.hip", "train_samples.hip", "network.hip", "loss.
 HOST_SOURCES = ["testbed.cpp", "python_api.cpp", "mini_json.cpp", "snapshot.cpp", "nerf_renderer.cpp", "nerf_loader.cpp", "png_reader.cpp", "exr_reader.cpp", "jpeg_reader.cpp", "hdr_reader.cpp", "image_io.cpp", "plumbing.cpp", "dp.cpp"]
 
 # -ffp-contract=off: the index / count paths must round exactly like the CPU oracle; network.hip re-enables contraction locally.
-HIP_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off", "-Wall", "-Wno-unused-function", "-Wno-unused-variable"] + os.environ.get("NGP_EXTRA_HIP_FLAGS", "").split()
+# -packed-fp32-ops: some forms of the packed fp32 instructions hipcc makes by itself have given wrong results on this hardware now and then; none are generated.
+HIP_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off", "-Wall", "-Wno-unused-function", "-Wno-unused-variable",
+             "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"] + os.environ.get("NGP_EXTRA_HIP_FLAGS", "").split()
 
 
 def _newer(src_list, out):
