@@ -162,5 +162,10 @@ RENDER_EXTRAS = np.dtype([("render_masks", "<u8"), ("n_render_masks", "<u4"), ("
                           ("distortion", "<u8"), ("distortion_res", "<i4", 2), ("quilting_dims", "<i4", 2), ("render_mode", "<i4"), ("frame_buffer", "<u8"),
                           ("row_begin", "<i4"), ("row_end", "<i4"), ("tile_order", "<i4")], align=True)   # NgpRenderExtras
 
+GATED_FFN = np.dtype([("n_in", "<u4"), ("n_hidden", "<u4"), ("n_out", "<u4"), ("dtype", "<i4"), ("activation", "<i4")])   # NgpGatedFfn
+DTYPE_F16, DTYPE_BF16, DTYPE_F32 = 0, 1, 2
+ACT_NONE, ACT_RELU, ACT_LOGISTIC, ACT_EXPONENTIAL, ACT_SILU, ACT_GELU = range(6)
+FFN_BACKWARD, FFN_ANY_LAYOUT = 1, 2
+
 assert AABB.itemsize == 24 and RAY.itemsize == 24 and XFORM.itemsize == 96 and COORD.itemsize == 28 and PAYLOAD.itemsize == 40
 assert NET_DESC.itemsize == 8 + 16 * 16

@@ -1,0 +1,228 @@
+// matmul_mfma.cuh — tiled matrix products C[m][n] = sum_k M[m][k] N[n][k] on v_mfma_f32_32x32x16_{f16,bf16}, the core of the gated feed-forward block (gated_ffn.hip)
+// and of the Muon step (muon.hip).
+//
+// Scheme.  A workgroup owns a BN x BM tile and walks k in steps of 64.  Both operands of a step go from memory into LDS by DMA (buffer_load ... lds, 16 bytes a lane: no
+// registers, no ds_write), one step ahead of the matrix instructions (two LDS buffers).  The buffer descriptor of a step ends where the operand ends, and the hardware returns
+// zero behind it, so the last rows and the last k of any size need no branch; a chunk behind k in the middle of a row asks for an offset behind the descriptor.
+// Operands come in two layouts:
+//   KC   [rows][k], k contiguous:     LDS [row][64 k], a fragment (lane: one row, 8 k) is one ds_read_b128;
+//   RC   [k][rows], rows contiguous:  LDS [64 k][row], a fragment is two ds_read_b64_tr_b16 (the LDS unit transposes 4 x 16 blocks on the way out).
+// Bank conflicts: the DMA writes LDS linearly, so the 16-byte chunks of a row are permuted by which chunk each lane ASKS for: chunk ^ (row & 7) for KC (eight rows of one chunk
+// column cover all banks), chunk ^ 4 (k & 3) for RC (the four k rows of a transposed block and its neighbour fall on different 32-byte units).
+// The N side is the A operand of the MFMA: a lane then holds four consecutive n of one m per register quad, which is the contiguous direction of the output.
+#pragma once
+
+#include "ngp_device.cuh"
+
+#pragma clang fp contract(fast)
+
+namespace ngp {
+namespace mm {
+
+typedef _Float16 f16;
+typedef __bf16 b16;
+typedef f16 f16x8 __attribute__((ext_vector_type(8)));
+typedef b16 b16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x2 __attribute__((ext_vector_type(2)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) char lds_char;
+
+enum { KC = 0, RC = 1 };
+constexpr int BK = 64;   // k per step: 128-byte rows for KC, four MFMA k-blocks
+
+struct Mat {             // rows x k, see above; ld in elements, a multiple of 8; p 16-byte aligned; KC: k a multiple of 8
+	const void* p;
+	uint64_t ld;
+	uint32_t rows, k;
+};
+
+template <class T> __device__ __forceinline__ f32x16 mfma(i32x4 a, i32x4 b, f32x16 c);
+template <> __device__ __forceinline__ f32x16 mfma<f16>(i32x4 a, i32x4 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0); }
+template <> __device__ __forceinline__ f32x16 mfma<b16>(i32x4 a, i32x4 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b16x8, a), __builtin_bit_cast(b16x8, b), c, 0, 0, 0); }
+
+__device__ __forceinline__ lds_char* lds_of(void* p) { return (lds_char*)(__attribute__((address_space(3))) void*)p; }
+
+// 16 bytes of every lane straight into LDS at `lds` + 16 lane.  The instruction returns nothing to a register, and the compiler, told of it as a builtin, would wait for ALL
+// DMA in flight before each LDS read; written here, the waits are the two below and stand where the buffers change hands.
+__device__ __forceinline__ void dma16(i32x4 rsrc, lds_char* lds, int voff) {
+	asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"((uint32_t)(uintptr_t)lds), "v"(voff), "s"(rsrc) : "memory");
+}
+// every DMA of this wave has landed, every LDS read of it has returned; then all waves
+__device__ __forceinline__ void wait_and_sync() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// One operand's tile of BR rows x 64 k: who loads what, and how a fragment is read back.
+template <int LAY, int BR, int THREADS>
+struct Tile {
+	static constexpr int BYTES = BR * BK * 2;
+	static constexpr int CHUNKS = LAY == KC ? 8 : BR / 8;            // 16-byte chunks per LDS row
+	static constexpr int LOADS = BYTES / 16 / THREADS;
+	static_assert(BYTES % (16 * THREADS) == 0, "every thread issues the same number of loads");
+	static __device__ __forceinline__ int swizzle(int r) { return LAY == KC ? (r & 7) : CHUNKS >= 16 ? (r & 3) << 2 : (r & 2) << 1; }
+
+	const char* base;        // of this step (uniform)
+	int64_t left;            // bytes from base to the operand's end
+	int64_t step_bytes;
+	int k_here;              // KC: k of this thread's chunk in the step; beyond `k_left` it reads zero
+	int k_left;
+	int voff[LOADS];
+
+	__device__ __forceinline__ void init(const Mat& m, uint32_t row0, int tid) {
+		if (LAY == KC) {
+			base = (const char*)m.p + (uint64_t)row0 * m.ld * 2;
+			left = row0 < m.rows ? (int64_t)(((uint64_t)(m.rows - row0 - 1) * m.ld + m.k) * 2) : 0;
+			step_bytes = BK * 2;
+		} else {
+			base = (const char*)m.p + (uint64_t)row0 * 2;
+			left = row0 < m.rows ? (int64_t)(((uint64_t)(m.k - 1) * m.ld + m.rows - row0) * 2) : 0;
+			step_bytes = (int64_t)m.ld * BK * 2;
+		}
+		k_left = (int)m.k;
+#pragma unroll
+		for (int i = 0; i < LOADS; ++i) {
+			const int slot = i * THREADS + tid, r = slot / CHUNKS, c = (slot % CHUNKS) ^ swizzle(r);
+			voff[i] = (int)((uint32_t)r * (uint32_t)m.ld * 2u) + c * 16;
+			if (LAY == KC && i == 0) k_here = c * 8;   // the same for every i: a thread's rows differ by a multiple of 8
+		}
+	}
+	// DMA of the current step into `lds` (wave-uniform), then on to the next step
+	__device__ __forceinline__ void issue(lds_char* lds, int wave) {
+		const uint32_t records = left > 0x7fffffff ? 0x7fffffffu : left < 0 ? 0u : (uint32_t)left;
+		const uint64_t b = (uint64_t)base;
+		i32x4 r = {(int)(uint32_t)b, (int)((uint32_t)(b >> 32) & 0xffffu), (int)records, 0x00020000};
+		asm volatile("s_nop 4" : "+s"(r));   // a descriptor word that came from the VALU must be five wait states old when a memory instruction reads it
+#pragma unroll
+		for (int i = 0; i < LOADS; ++i) {
+			const int v = LAY == KC && k_here >= k_left ? (int)0x80000000 : voff[i];
+			dma16(r, lds + (i * THREADS + wave * 64) * 16, v);
+		}
+		base += step_bytes;
+		left -= step_bytes;
+		k_left -= BK;
+	}
+	// fragment of rows row0 .. row0 + 31, k-block ks (16 k): lane l has row l & 31 and k = 8 (l >> 5) .. + 7
+	static __device__ __forceinline__ i32x4 frag(const lds_char* lds, int row0, int ks, int lane) {
+		if (LAY == KC) {
+			const int r = row0 + (lane & 31), c = (ks * 2 + (lane >> 5)) ^ (lane & 7);
+			return *(const __attribute__((address_space(3))) i32x4*)(lds + r * 128 + c * 16);
+		}
+		const int k = ks * 16 + 8 * (lane >> 5) + ((lane & 15) >> 2), c = row0 / 8 + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+		const lds_char* p = lds + k * (CHUNKS * 16) + (c ^ swizzle((lane & 15) >> 2)) * 16 + (lane & 1) * 8;   // k & 3 = (lane & 15) >> 2 (CHUNKS < 16: only bit 1 counts)
+		const i32x2 lo = __builtin_bit_cast(i32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p));
+		const i32x2 hi = __builtin_bit_cast(i32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(p + 4 * CHUNKS * 16)));
+		return i32x4{lo.x, lo.y, hi.x, hi.y};
+	}
+};
+
+// LDS of `STAGES` steps and the product's main loop.  NM N-side matrices of BN rows each share one M-side tile of BM rows (gate and up projection: NM = 2).
+// WN x WM waves; a wave owns BN / WN rows of every N-side matrix and BM / WM rows of the M side.
+template <class T, int NLAY, int MLAY, int NM, int BN, int BM, int WN, int WM>
+struct Product {
+	static constexpr int THREADS = 64 * WN * WM, NB = BN / WN / 32, MB = BM / WM / 32;
+	using NT = Tile<NLAY, BN, THREADS>;
+	using MT = Tile<MLAY, BM, THREADS>;
+	static constexpr int STAGE_BYTES = NM * NT::BYTES + MT::BYTES, LDS_BYTES = 2 * STAGE_BYTES;
+
+	// acc[j][nb][mb] += the product over `k` (in steps of 64) of rows n0.. of n[j] and m0.. of m.  Every thread of the workgroup calls it; LDS is free again on return
+	// of the last wave (a barrier stands at the start of each call and step).
+	static __device__ __forceinline__ void run(f32x16 (&acc)[NM][NB][MB], const Mat* n, const Mat& m, uint32_t n0, uint32_t m0, uint32_t k0, uint32_t k1, lds_char* lds) {
+		const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wn = wave % WN, wm = wave / WN;
+		NT nt[NM];
+		MT mt;
+#pragma unroll
+		for (int j = 0; j < NM; ++j) nt[j].init(n[j], n0, tid);
+		mt.init(m, m0, tid);
+		if (k0) {
+			const int64_t skip = k0 / BK;
+#pragma unroll
+			for (int j = 0; j < NM; ++j) { nt[j].base += skip * nt[j].step_bytes; nt[j].left -= skip * nt[j].step_bytes; nt[j].k_left -= (int)k0; }
+			mt.base += skip * mt.step_bytes; mt.left -= skip * mt.step_bytes; mt.k_left -= (int)k0;
+		}
+		const int steps = (int)((k1 - k0 + BK - 1) / BK);
+		auto issue = [&](int stage) {
+			lds_char* p = lds + stage * STAGE_BYTES;
+#pragma unroll
+			for (int j = 0; j < NM; ++j) nt[j].issue(p + j * NT::BYTES, wave);
+			mt.issue(p + NM * NT::BYTES, wave);
+		};
+		wait_and_sync();   // the LDS may still be read by what ran before
+		issue(0);
+		for (int s = 0; s < steps; ++s) {
+			wait_and_sync();   // this step's tiles have landed; the other buffer has been read
+			if (s + 1 < steps) issue((s + 1) & 1);
+			const lds_char* p = lds + (s & 1) * STAGE_BYTES;
+#pragma unroll
+			for (int ks = 0; ks < BK / 16; ++ks) {
+				i32x4 fm[MB];
+#pragma unroll
+				for (int b = 0; b < MB; ++b) fm[b] = MT::frag(p + NM * NT::BYTES, wm * (BM / WM) + b * 32, ks, lane);
+#pragma unroll
+				for (int j = 0; j < NM; ++j) {
+					i32x4 fn[NB];
+#pragma unroll
+					for (int b = 0; b < NB; ++b) fn[b] = NT::frag(p + j * NT::BYTES, wn * (BN / WN) + b * 32, ks, lane);
+#pragma unroll
+					for (int b = 0; b < NB; ++b)
+#pragma unroll
+						for (int c = 0; c < MB; ++c) acc[j][b][c] = mfma<T>(fn[b], fm[c], acc[j][b][c]);
+				}
+			}
+		}
+	}
+};
+
+// ---- which tile a workgroup takes --------------------------------------------------------------------------------------------------------
+// Workgroups go to the 8 XCDs in turn, each with its own L2: give an XCD one contiguous run of the tile order, and walk that order eight tile rows at a time, so that the
+// tiles in flight on one XCD share both operands' panels.
+__device__ __forceinline__ void tile_of(uint32_t pid, uint32_t total, uint32_t tiles_n, uint32_t tiles_m, uint32_t& tn, uint32_t& tm, uint32_t& split) {
+	const uint32_t xcd = pid & 7, per = total >> 3, rem = total & 7;
+	uint32_t t = xcd * per + (xcd < rem ? xcd : rem) + (pid >> 3);
+	const uint32_t tiles = tiles_n * tiles_m;
+	split = t / tiles;
+	t -= split * tiles;
+	constexpr uint32_t G = 8;
+	const uint32_t group = t / (G * tiles_n), first = group * G, size = tiles_m - first < G ? tiles_m - first : G;
+	t -= group * G * tiles_n;
+	tm = first + t % size;
+	tn = t / size;
+}
+
+// ---- epilogue ----------------------------------------------------------------------------------------------------------------------------
+template <class T> struct Out { T* p; uint64_t ld; uint32_t rows, cols; };   // row-major; columns are the N side
+
+// One wave writes v = 32 rows (m0 ..) x NBLK * 32 columns (n0 ..) through LDS (`lds`: 32 * (NBLK * 64 + 16) bytes of its own), so that a row's columns leave in 16-byte pieces.
+// Rounds once, to nearest even.  Register layout of a 32 x 32 block: lane l holds column m = l & 31 and rows n = 8 (i >> 2) + 4 (l >> 5) + (i & 3).
+template <class T, int NBLK>
+__device__ __forceinline__ void store_rows(const f32x16* v, const Out<T>& o, uint32_t n0, uint32_t m0, lds_char* lds, int lane) {
+	typedef T t4 __attribute__((ext_vector_type(4)));
+	typedef T t8 __attribute__((ext_vector_type(8)));
+	constexpr int PITCH = NBLK * 64 + 16, PIECES = NBLK * 4, ROWS = 64 / PIECES;
+#pragma unroll
+	for (int b = 0; b < NBLK; ++b)
+#pragma unroll
+		for (int q = 0; q < 4; ++q) {
+			const t4 h = {(T)v[b][4 * q], (T)v[b][4 * q + 1], (T)v[b][4 * q + 2], (T)v[b][4 * q + 3]};
+			*(__attribute__((address_space(3))) t4*)(lds + (lane & 31) * PITCH + (b * 32 + q * 8 + 4 * (lane >> 5)) * 2) = h;
+		}
+	const bool wide = (((uint64_t)o.p | (o.ld * 2)) & 15) == 0;
+	const int piece = lane % PIECES;
+	const uint32_t n = n0 + piece * 8;
+#pragma unroll
+	for (int r = 0; r < 32; r += ROWS) {
+		const int row = r + lane / PIECES;
+		const t8 h = *(const __attribute__((address_space(3))) t8*)(lds + row * PITCH + piece * 16);   // same wave, LDS is in order: no barrier
+		const uint32_t m = m0 + row;
+		if (m >= o.rows) continue;
+		T* p = o.p + (uint64_t)m * o.ld + n;
+		if (wide && n + 8 <= o.cols) *(t8*)p = h;
+		else
+#pragma unroll
+			for (int e = 0; e < 8; ++e)
+				if (n + e < o.cols) p[e] = h[e];
+	}
+}
+
+} // namespace mm
+} // namespace ngp

@@ -79,7 +79,8 @@ typedef struct {                                                     /* tcnn Gri
 
 /* enums mirror include/neural-graphics-primitives/common.h:103-141 */
 enum { NGP_LOSS_L2 = 0, NGP_LOSS_L1 = 1, NGP_LOSS_MAPE = 2, NGP_LOSS_SMAPE = 3, NGP_LOSS_HUBER = 4, NGP_LOSS_LOG_L1 = 5, NGP_LOSS_RELATIVE_L2 = 6 };
-enum { NGP_ACT_NONE = 0, NGP_ACT_RELU = 1, NGP_ACT_LOGISTIC = 2, NGP_ACT_EXPONENTIAL = 3 };
+enum { NGP_ACT_NONE = 0, NGP_ACT_RELU = 1, NGP_ACT_LOGISTIC = 2, NGP_ACT_EXPONENTIAL = 3, NGP_ACT_SILU = 4, NGP_ACT_GELU = 5 };   /* the last two: gated blocks only */
+enum { NGP_DTYPE_F16 = 0, NGP_DTYPE_BF16 = 1, NGP_DTYPE_F32 = 2 };   /* element type of the tensors of an entry point that takes void* */
 enum { NGP_COLOR_LINEAR = 0, NGP_COLOR_SRGB = 1 };
 enum { NGP_TONEMAP_IDENTITY = 0, NGP_TONEMAP_ACES = 1, NGP_TONEMAP_HABLE = 2, NGP_TONEMAP_REINHARD = 3 };
 
@@ -470,6 +471,27 @@ int ngp_hip_grid_backward(void* stream, uint32_t n_dims, const NgpNetDesc* desc_
  * run-merging walk, which finds nothing to merge there (what ngp_hip_gridmlp_backward runs).  Bit-identical results: the sums are exact either way. */
 int ngp_hip_grid_backward_unordered(void* stream, uint32_t n_dims, const NgpNetDesc* desc_dev, const float* pos, uint32_t pos_stride_floats, uint32_t n,
                           const uint16_t* dL_dx_planes, uint16_t* grid_grad, void* scratch, uint64_t scratch_bytes);
+
+/* ============================ gated feed-forward block ============================
+ * y = (act(x Wg^T) * (x Wu^T)) Wd^T: the gated form of the fully connected block, of any width, next to the FullyFusedMLP of the configs above (no reference counterpart).
+ *   x [n_rows][n_in], y [n_rows][n_out] with a row stride in elements; w_gate, w_up [n_hidden][n_in] and w_down [n_out][n_hidden] row-major and contiguous, as every matrix
+ *   of a parameter vector here.  All tensors are of `dtype` (F16 or BF16); products accumulate in fp32, the hidden row is rounded once, every output is rounded once.
+ *   activation: NGP_ACT_NONE (bilinear), RELU, LOGISTIC, SILU or GELU (the exact one, with erf); applied to x Wg^T.
+ * Widths 1 .. 2^20 and rows 0 .. 2^31 of any remainder.  Rows whose width, stride and base are multiples of 8 elements / 16 bytes are read in place; others cost one padded copy.
+ * Nothing outside y, dx, the gradients and the workspace is written; bytes between rows of a strided output stay as they are.  No atomics: the same inputs give the same bits.
+ * A call only enqueues (capturable); two calls that may overlap need workspaces of their own. */
+typedef struct { uint32_t n_in, n_hidden, n_out; int32_t dtype, activation; } NgpGatedFfn;   /* host struct */
+enum { NGP_FFN_BACKWARD = 1,     /* the workspace of the backward call */
+       NGP_FFN_ANY_LAYOUT = 2 }; /* ... where a base address or a row stride is no multiple of 16 bytes although its width is */
+/* bytes of workspace a call of n_rows rows needs (it may be used for fewer rows of the same block); 0 for a block that is refused.  Host only. */
+uint64_t ngp_hip_gated_ffn_workspace_bytes(const NgpGatedFfn* block_host, uint64_t n_rows, uint32_t flags);
+int ngp_hip_gated_ffn_forward(void* stream, const NgpGatedFfn* block_host, uint64_t n_rows, const void* x, uint64_t x_stride, const void* w_gate, const void* w_up,
+                              const void* w_down, void* y, uint64_t y_stride, void* workspace, uint64_t workspace_bytes);
+/* The gradients of dy [n_rows][n_out], overwritten (not added to): dx [n_rows][n_in], or NULL; dw_gate, dw_up, dw_down in the weights' layout, or all three NULL.  The block's
+ * inner values are computed again from x: the forward call leaves nothing behind that has to be kept. */
+int ngp_hip_gated_ffn_backward(void* stream, const NgpGatedFfn* block_host, uint64_t n_rows, const void* x, uint64_t x_stride, const void* w_gate, const void* w_up,
+                               const void* w_down, const void* dy, uint64_t dy_stride, void* dx, uint64_t dx_stride, void* dw_gate, void* dw_up, void* dw_down,
+                               void* workspace, uint64_t workspace_bytes);
 
 /* ============================ plumbing configs P1 (2-D image) / P2 (SDF): grid encoding -> one FullyFusedMLP ============================
  * tcnn NetworkWithInputEncoding as Testbed::reset_network builds it for Image / Sdf mode (src/testbed.cu:2397-2445): HashGrid (16 levels x 2
