@@ -163,6 +163,7 @@ RENDER_EXTRAS = np.dtype([("render_masks", "<u8"), ("n_render_masks", "<u4"), ("
                           ("row_begin", "<i4"), ("row_end", "<i4"), ("tile_order", "<i4")], align=True)   # NgpRenderExtras
 
 GATED_FFN = np.dtype([("n_in", "<u4"), ("n_hidden", "<u4"), ("n_out", "<u4"), ("dtype", "<i4"), ("activation", "<i4")])   # NgpGatedFfn
+MUON_MATRIX = np.dtype([("offset", "<u8"), ("rows", "<u4"), ("cols", "<u4")])   # NgpMuonMatrix
 DTYPE_F16, DTYPE_BF16, DTYPE_F32 = 0, 1, 2
 ACT_NONE, ACT_RELU, ACT_LOGISTIC, ACT_EXPONENTIAL, ACT_SILU, ACT_GELU = range(6)
 FFN_BACKWARD, FFN_ANY_LAYOUT = 1, 2

@@ -472,6 +472,20 @@ int ngp_hip_grid_backward(void* stream, uint32_t n_dims, const NgpNetDesc* desc_
 int ngp_hip_grid_backward_unordered(void* stream, uint32_t n_dims, const NgpNetDesc* desc_dev, const float* pos, uint32_t pos_stride_floats, uint32_t n,
                           const uint16_t* dL_dx_planes, uint16_t* grid_grad, void* scratch, uint64_t scratch_bytes);
 
+/* ============================ Muon ============================
+ * The optimizer step of matrix parameters next to Adam (ngp_hip_optimizer_step; no reference counterpart): momentum, the update orthogonalised by Newton-Schulz products, the weights.
+ *   g = grads / loss_scale;  m <- momentum m + g;  u = nesterov ? g + momentum m : m;  X = u / (|u|_F + epsilon)
+ *   n_iterations times  X <- 3.4445 X + (-4.7750 A + 2.0315 A^2) X with A = X X^T (on the shorter side)
+ *   master <- (1 - learning_rate weight_decay) master - learning_rate sqrt(max(1, rows / cols)) X;  params <- master, rounded to dtype
+ * grads, master, params and momentum_buffer are whole parameter vectors; matrices_host names the row-major matrices in them, in ascending order and without overlap (nothing else is
+ * read or written: the encoding behind the matrices belongs to Adam).  dtype: of grads and params (F16, BF16; F32: grads alone, params NULL); params may be NULL.
+ * Products run on pairs of fp16 halves (22 bits) with fp32 sums, norms in 64 bits: X agrees with 64-bit arithmetic to about 1e-6 of its norm.  No atomics: the same inputs give the
+ * same bits.  A gradient that is not finite makes its matrix not finite, no other.  A zero update leaves X = 0.  Enqueues only (capturable: matrices_host is read during the call). */
+typedef struct { uint64_t offset; uint32_t rows, cols; } NgpMuonMatrix;   /* offset in elements from the start of the vectors; rows, cols 1 .. 65536 */
+uint64_t ngp_hip_muon_workspace_bytes(uint32_t n_matrices, const NgpMuonMatrix* matrices_host);   /* Host only; 0 for a list that is refused */
+int ngp_hip_muon_step(void* stream, uint32_t n_matrices, const NgpMuonMatrix* matrices_host, float learning_rate, float momentum, float weight_decay, float epsilon, int nesterov,
+                      uint32_t n_iterations, float loss_scale, int dtype, const void* grads, float* master, void* params, float* momentum_buffer, void* workspace, uint64_t workspace_bytes);
+
 /* ============================ gated feed-forward block ============================
  * y = (act(x Wg^T) * (x Wu^T)) Wd^T: the gated form of the fully connected block, of any width, next to the FullyFusedMLP of the configs above (no reference counterpart).
  *   x [n_rows][n_in], y [n_rows][n_out] with a row stride in elements; w_gate, w_up [n_hidden][n_in] and w_down [n_out][n_hidden] row-major and contiguous, as every matrix
