@@ -33,6 +33,14 @@ __device__ __forceinline__ float2 activate(int act, float g) {
 	return make_float2(g * s, s * (1.0f + g * (1.0f - s)));   // NGP_ACT_SILU
 }
 
+} // namespace ffn
+} // namespace ngp
+
+#include "gated_ffn_narrow.cuh"
+
+namespace ngp {
+namespace ffn {
+
 template <bool BIG> struct Shape;   // BIG: 256 x 256 x 64 in 8 waves, one workgroup a CU; else 128 x 128 x 64 in 4 waves, two a CU
 template <> struct Shape<true> { static constexpr int N = 256, M = 256, WN = 2, WM = 4, THREADS = 512; };
 template <> struct Shape<false> { static constexpr int N = 128, M = 128, WN = 2, WM = 2, THREADS = 256; };
@@ -127,15 +135,26 @@ __global__ void __launch_bounds__(Shape<BIG>::THREADS, 2) product_kernel(Pair p0
 	store_tile<T, P::NB, P::MB>(acc, out, n0 + wn * (P::NB * 32), m0 + wm * (P::MB * 32), lds_of(lds) + wave * (32 * (P::NB * 64 + 16)), lane);
 }
 
-// the splits of a tile, added in order, rounded once
+// `splits` partials -> ceil(splits / SUM_FAN) in the first of them, sixteen neighbours in their order: a long list of splits would otherwise be one workgroup's serial work
+constexpr uint32_t SUM_FAN = 16;
+__global__ void __launch_bounds__(256) split_fold_kernel(float* partial, uint32_t splits, uint64_t floats) {   // floats: of one split, a multiple of 1024
+	const uint64_t blocks = floats / 1024, at = (blockIdx.x % blocks) * 1024 + threadIdx.x * 4;
+	const uint32_t first = (uint32_t)(blockIdx.x / blocks) * SUM_FAN, end = min(first + SUM_FAN, splits);
+	f32x4 v = *(const f32x4*)(partial + first * floats + at);
+#pragma unroll 4
+	for (uint32_t s = first + 1; s < end; ++s) v += *(const f32x4*)(partial + s * floats + at);
+	*(f32x4*)(partial + first * floats + at) = v;
+}
+
+// the splits of a tile (every `every`-th of them), added in order, rounded once
 template <class T, bool BIG>
-__global__ void __launch_bounds__(Shape<BIG>::THREADS) split_sum_kernel(const float* partial, uint32_t splits, Rows2<T> out, uint32_t tiles_n, uint32_t tiles_m) {
+__global__ void __launch_bounds__(Shape<BIG>::THREADS) split_sum_kernel(const float* partial, uint32_t splits, uint32_t every, Rows2<T> out, uint32_t tiles_n, uint32_t tiles_m) {
 	using S = Shape<BIG>;
 	constexpr int NB = S::N / S::WN / 32, MB = S::M / S::WM / 32;
 	__shared__ __attribute__((aligned(16))) char lds[S::WN * S::WM * 32 * (NB * 64 + 16)];
 	const uint32_t tn = blockIdx.x % tiles_n, tm = blockIdx.x / tiles_n;
 	const float* q = partial + (uint64_t)blockIdx.x * (S::N * S::M) + threadIdx.x * 4;
-	const uint64_t stride = (uint64_t)tiles_n * tiles_m * (S::N * S::M);
+	const uint64_t stride = (uint64_t)every * tiles_n * tiles_m * (S::N * S::M);
 	const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wn = wave % S::WN, wm = wave / S::WN;
 	f32x16 acc[1][NB][MB];
 	clear(acc);
@@ -276,6 +295,66 @@ static bool dma_ready(const Tensor& t) { return ((uintptr_t)t.p & 15) == 0 && t.
 
 static uint32_t copy_grid(uint64_t n) { return (uint32_t)std::min<uint64_t>(ceil_div(n, 256), 4096); }
 
+// ---- narrow blocks: which, and their launches
+
+constexpr uint32_t NARROW_GROUPS = 512;   // of the backward pass: two to three workgroups a CU, and the fewer, the less there is to add at the end
+
+static uint32_t narrow_forward_lds(const NgpGatedFfn& b) {   // 0: not narrow
+	if (b.n_in > 128 || b.n_out > 128) return 0;
+	const uint32_t kb = b.n_in <= 16 ? 1 : b.n_in <= 32 ? 2 : b.n_in <= 64 ? 4 : 8, ob = b.n_out <= 32 ? 1 : b.n_out <= 64 ? 2 : 4;
+	const uint64_t bytes = ceil_div(b.n_hidden, 32) * (2 * kb + 2 * ob) * 1024;
+	return bytes <= 128 * 1024 ? (uint32_t)bytes : 0;
+}
+static bool narrow_backward(const NgpGatedFfn& b) { return b.n_in <= 64 && b.n_out <= 64 && b.n_hidden <= 128; }
+static uint64_t narrow_partial_bytes(const NgpGatedFfn& b, uint64_t rows) {
+	const uint64_t db = ceil_div(b.n_in, 32), fb = b.n_hidden <= 32 ? 1 : b.n_hidden <= 64 ? 2 : 4, ob = ceil_div(b.n_out, 32);
+	return std::min<uint64_t>(NARROW_GROUPS, ceil_div(rows, 64)) * (2 * fb * db + fb * ob) * 4096;
+}
+
+template <class T, int DB, int OB, bool VEC>
+static void launch_narrow_forward(hipStream_t st, const NarrowArgs& a, uint32_t lds) {
+	if (lds > 64 * 1024) (void)hipFuncSetAttribute((const void*)narrow_forward_kernel<T, DB, OB, VEC>, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+	const uint32_t per_cu = std::max(1u, std::min(6u, 160 * 1024 / lds));
+	hipLaunchKernelGGL((narrow_forward_kernel<T, DB, OB, VEC>), dim3(std::min((a.rows + 127) / 128, 256 * per_cu)), dim3(256), lds, st, a);
+}
+template <class T, int DB, int OB> static void pick_narrow_forward(hipStream_t st, const NarrowArgs& a, uint32_t lds, bool vec) {
+	if (vec) launch_narrow_forward<T, DB, OB, true>(st, a, lds);
+	else launch_narrow_forward<T, DB, OB, false>(st, a, lds);
+}
+template <class T, int DB> static void pick_narrow_forward(hipStream_t st, const NarrowArgs& a, uint32_t lds, bool vec) {
+	if (a.o <= 32) pick_narrow_forward<T, DB, 1>(st, a, lds, vec);
+	else if (a.o <= 64) pick_narrow_forward<T, DB, 2>(st, a, lds, vec);
+	else pick_narrow_forward<T, DB, 4>(st, a, lds, vec);
+}
+template <class T> static int run_narrow_forward(hipStream_t st, const NarrowArgs& a, uint32_t lds, bool vec) {
+	if (a.d <= 16) pick_narrow_forward<T, 1>(st, a, lds, vec);
+	else if (a.d <= 32) pick_narrow_forward<T, 2>(st, a, lds, vec);
+	else if (a.d <= 64) pick_narrow_forward<T, 4>(st, a, lds, vec);
+	else pick_narrow_forward<T, 8>(st, a, lds, vec);
+	NGP_LAUNCH_CHECK("narrow_forward_kernel");
+	return 0;
+}
+
+template <class T, int DB, int FB, int OB> static void launch_narrow_backward(hipStream_t st, const NarrowArgs& a, bool vec, void* dwg, void* dwu, void* dwd) {
+	const uint32_t groups = std::min<uint32_t>(NARROW_GROUPS, (a.rows + 63) / 64);
+	if (vec) hipLaunchKernelGGL((narrow_backward_kernel<T, DB, FB, OB, true>), dim3(groups), dim3(256), 0, st, a);
+	else hipLaunchKernelGGL((narrow_backward_kernel<T, DB, FB, OB, false>), dim3(groups), dim3(256), 0, st, a);
+	constexpr uint32_t blocks = NarrowBackward<DB, FB, OB>::BLOCKS;
+	if (a.partial) hipLaunchKernelGGL((narrow_sum_kernel<T>), dim3(blocks * 16), dim3(1024), 0, st, (const float*)a.partial, groups, blocks, (uint32_t)DB, (uint32_t)FB, (uint32_t)OB, a.d, a.f, a.o, (T*)dwg, (T*)dwu, (T*)dwd);
+}
+template <class T, int DB, int OB> static void pick_narrow_backward(hipStream_t st, const NarrowArgs& a, bool vec, void* dwg, void* dwu, void* dwd) {
+	if (a.f <= 32) launch_narrow_backward<T, DB, 1, OB>(st, a, vec, dwg, dwu, dwd);
+	else if (a.f <= 64) launch_narrow_backward<T, DB, 2, OB>(st, a, vec, dwg, dwu, dwd);
+	else launch_narrow_backward<T, DB, 4, OB>(st, a, vec, dwg, dwu, dwd);
+}
+template <class T> static int run_narrow_backward(hipStream_t st, const NarrowArgs& a, bool vec, void* dwg, void* dwu, void* dwd) {
+	if (a.d <= 32) { if (a.o <= 32) pick_narrow_backward<T, 1, 1>(st, a, vec, dwg, dwu, dwd); else pick_narrow_backward<T, 1, 2>(st, a, vec, dwg, dwu, dwd); }
+	else { if (a.o <= 32) pick_narrow_backward<T, 2, 1>(st, a, vec, dwg, dwu, dwd); else pick_narrow_backward<T, 2, 2>(st, a, vec, dwg, dwu, dwd); }
+	NGP_LAUNCH_CHECK("narrow_backward_kernel");
+	return 0;
+}
+static bool vector_rows(const void* p, uint64_t ld, uint32_t cols) { return ((uintptr_t)p & 15) == 0 && ld % 8 == 0 && cols % 8 == 0; }
+
 // What a call keeps in its workspace.  `any`: room for padded copies of every input, else of those whose width is no multiple of 8.
 struct Space {
 	uint32_t d8, f8, o8, fp;                                   // widths as the copies have them; fp: row pitch of h, dg and du
@@ -286,6 +365,12 @@ struct Space {
 	bool has_copies(uint32_t width, bool any) const { return any || width % 8; }
 	Space(char* base, const NgpGatedFfn& b, uint64_t rows, bool backward, bool any) {
 		Arena a{base};
+		bytes = 0;
+		if (backward ? narrow_backward(b) : narrow_forward_lds(b) != 0) {
+			if (backward) partial = (float*)a.take(narrow_partial_bytes(b, rows));
+			bytes = a.used;
+			return;
+		}
 		d8 = (uint32_t)up8(b.n_in); f8 = (uint32_t)up8(b.n_hidden); o8 = (uint32_t)up8(b.n_out); fp = (f8 + 31) & ~31u;
 		if (has_copies(b.n_in, any)) { x = a.take(rows * d8 * 2); wg = a.take((uint64_t)b.n_hidden * d8 * 2); wu = a.take((uint64_t)b.n_hidden * d8 * 2); }
 		if (has_copies(b.n_hidden, any)) wd = a.take((uint64_t)b.n_out * f8 * 2);
@@ -332,8 +417,14 @@ struct Launch {
 		if (p.big) hipLaunchKernelGGL((product_kernel<T, NLAY, MLAY, true>), grid, dim3(512), 0, st, p0, p1 ? *p1 : p0, p1 ? 2 : 1, out, p.tiles_n, p.tiles_m, p.splits, p.k_split, part);
 		else hipLaunchKernelGGL((product_kernel<T, NLAY, MLAY, false>), grid, dim3(256), 0, st, p0, p1 ? *p1 : p0, p1 ? 2 : 1, out, p.tiles_n, p.tiles_m, p.splits, p.k_split, part);
 		if (!ok("product_kernel") || !part) return;
-		if (p.big) hipLaunchKernelGGL((split_sum_kernel<T, true>), dim3(tiles), dim3(512), 0, st, (const float*)part, p.partials, out, p.tiles_n, p.tiles_m);
-		else hipLaunchKernelGGL((split_sum_kernel<T, false>), dim3(tiles), dim3(256), 0, st, (const float*)part, p.partials, out, p.tiles_n, p.tiles_m);
+		uint32_t splits = p.partials, every = 1;
+		if (splits > SUM_FAN) {
+			const uint64_t floats = (uint64_t)tiles * 128 * 128;
+			hipLaunchKernelGGL(split_fold_kernel, dim3((uint32_t)(floats / 1024 * ceil_div(splits, SUM_FAN))), dim3(256), 0, st, part, splits, floats);
+			splits = (uint32_t)ceil_div(splits, SUM_FAN);
+			every = SUM_FAN;
+		}
+		hipLaunchKernelGGL((split_sum_kernel<T, false>), dim3(tiles), dim3(256), 0, st, (const float*)part, splits, every, out, p.tiles_n, p.tiles_m);
 		ok("split_sum_kernel");
 	}
 };
@@ -406,6 +497,11 @@ int ngp_hip_gated_ffn_forward(void* stream, const NgpGatedFfn* b, uint64_t n_row
 	if (x_stride < b->n_in || y_stride < b->n_out) return refuse("ngp_hip_gated_ffn_forward: a row stride is smaller than its row");
 	if (((uintptr_t)x | (uintptr_t)w_gate | (uintptr_t)w_up | (uintptr_t)w_down | (uintptr_t)y) & 1) return refuse("ngp_hip_gated_ffn_forward: a tensor is not aligned to its elements");
 	const Tensor tx{x, x_stride, n_rows, b->n_in}, tg{w_gate, b->n_in, b->n_hidden, b->n_in}, tu{w_up, b->n_in, b->n_hidden, b->n_in}, td{w_down, b->n_hidden, b->n_out, b->n_hidden};
+	if (const uint32_t lds = narrow_forward_lds(*b)) {
+		const NarrowArgs a{x, w_gate, w_up, w_down, nullptr, y, nullptr, x_stride, y_stride, 0, 0, (uint32_t)n_rows, b->n_in, b->n_hidden, b->n_out, b->activation, nullptr};
+		const bool vec = vector_rows(x, x_stride, b->n_in);
+		return b->dtype == NGP_DTYPE_F16 ? run_narrow_forward<f16>((hipStream_t)stream, a, lds, vec) : run_narrow_forward<b16>((hipStream_t)stream, a, lds, vec);
+	}
 	const bool plain = (b->n_in % 8 || (dma_ready(tx) && dma_ready(tg) && dma_ready(tu))) && (b->n_hidden % 8 || dma_ready(td));
 	const Space s((char*)workspace, *b, n_rows, false, !plain);
 	if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < s.bytes) return refuse("ngp_hip_gated_ffn_forward: workspace null, not 16-byte aligned or too small (ngp_hip_gated_ffn_workspace_bytes; rows that are not 16-byte aligned: NGP_FFN_ANY_LAYOUT)");
@@ -435,6 +531,13 @@ int ngp_hip_gated_ffn_backward(void* stream, const NgpGatedFfn* b, uint64_t n_ro
 	if (x_stride < b->n_in || dy_stride < b->n_out || (dx && dx_stride < b->n_in)) return refuse("ngp_hip_gated_ffn_backward: a row stride is smaller than its row");
 	if (((uintptr_t)x | (uintptr_t)w_gate | (uintptr_t)w_up | (uintptr_t)w_down | (uintptr_t)dy) & 1) return refuse("ngp_hip_gated_ffn_backward: a tensor is not aligned to its elements");
 	const Tensor tx{x, x_stride, n_rows, b->n_in}, tg{w_gate, b->n_in, b->n_hidden, b->n_in}, tu{w_up, b->n_in, b->n_hidden, b->n_in}, td{w_down, b->n_hidden, b->n_out, b->n_hidden}, ty{dy, dy_stride, n_rows, b->n_out};
+	if (narrow_backward(*b)) {
+		const uint64_t need = dw_gate ? narrow_partial_bytes(*b, n_rows) : 0;
+		if (need && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < need)) return refuse("ngp_hip_gated_ffn_backward: workspace null, not 16-byte aligned or too small (ngp_hip_gated_ffn_workspace_bytes)");
+		const NarrowArgs a{x, w_gate, w_up, w_down, dy, nullptr, dx, x_stride, 0, dy_stride, dx_stride, (uint32_t)n_rows, b->n_in, b->n_hidden, b->n_out, b->activation, need ? (float*)workspace : nullptr};
+		const bool vec = vector_rows(x, x_stride, b->n_in) && vector_rows(dy, dy_stride, b->n_out);
+		return b->dtype == NGP_DTYPE_F16 ? run_narrow_backward<f16>(st, a, vec, dw_gate, dw_up, dw_down) : run_narrow_backward<b16>(st, a, vec, dw_gate, dw_up, dw_down);
+	}
 	const bool plain = (b->n_in % 8 || (dma_ready(tx) && dma_ready(tg) && dma_ready(tu))) && (b->n_hidden % 8 || dma_ready(td)) && (b->n_out % 8 || dma_ready(ty));
 	const Space s((char*)workspace, *b, n_rows, true, !plain);
 	if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < s.bytes) return refuse("ngp_hip_gated_ffn_backward: workspace null, not 16-byte aligned or too small (ngp_hip_gated_ffn_workspace_bytes; rows that are not 16-byte aligned: NGP_FFN_ANY_LAYOUT)");
