@@ -19,24 +19,36 @@ namespace ffn {
 using namespace mm;
 
 // act(g) and act'(g)
-__device__ __forceinline__ float2 activate(int act, float g) {
-	switch (act) {
-		case NGP_ACT_NONE: return make_float2(g, 1.0f);
-		case NGP_ACT_RELU: return g <= 0.0f ? make_float2(0.0f, 0.0f) : make_float2(g, 1.0f);   // a NaN stays one
-		case NGP_ACT_GELU: {   // g Phi(g); erfc keeps the small tail's digits
-			const float phi = 0.5f * erfcf(g * -0.70710678f);
-			return make_float2(g * phi, phi + g * 0.39894228f * __expf(-0.5f * g * g));
-		}
+template <int ACT>
+__device__ __forceinline__ float2 activate(float g) {
+	if (ACT == NGP_ACT_NONE) return make_float2(g, 1.0f);
+	if (ACT == NGP_ACT_RELU) return g <= 0.0f ? make_float2(0.0f, 0.0f) : make_float2(g, 1.0f);   // a NaN stays one
+	if (ACT == NGP_ACT_GELU) {   // g Phi(g); erfc keeps the small tail's digits
+		const float phi = 0.5f * erfcf(g * -0.70710678f);
+		return make_float2(g * phi, phi + g * 0.39894228f * __expf(-0.5f * g * g));
 	}
-	const float s = 1.0f / (1.0f + __expf(-g));
-	if (act == NGP_ACT_LOGISTIC) return make_float2(s, s * (1.0f - s));
-	return make_float2(g * s, s * (1.0f + g * (1.0f - s)));   // NGP_ACT_SILU
+	const float s = __builtin_amdgcn_rcpf(1.0f + __expf(-g));   // both within 2 ulp
+	if (ACT == NGP_ACT_LOGISTIC) return make_float2(s, s * (1.0f - s));
+	return make_float2(g * s, s * (1.0f + g * (1.0f - s)));     // NGP_ACT_SILU
+}
+template <int V> struct Constant { static constexpr int value = V; };
+// f(Constant<act>): the choice is made once, outside the loops over a tile
+template <class F>
+__device__ __forceinline__ void with_activation(int act, F f) {
+	switch (act) {
+		case NGP_ACT_NONE: f(Constant<NGP_ACT_NONE>()); break;
+		case NGP_ACT_RELU: f(Constant<NGP_ACT_RELU>()); break;
+		case NGP_ACT_LOGISTIC: f(Constant<NGP_ACT_LOGISTIC>()); break;
+		case NGP_ACT_SILU: f(Constant<NGP_ACT_SILU>()); break;
+		default: f(Constant<NGP_ACT_GELU>());
+	}
 }
 
 } // namespace ffn
 } // namespace ngp
 
 #include "gated_ffn_narrow.cuh"
+#include "gated_ffn_few.cuh"
 
 namespace ngp {
 namespace ffn {
@@ -71,14 +83,19 @@ __global__ void __launch_bounds__(Shape<BIG>::THREADS, 2) gate_up_kernel(Mat x, 
 	P::run(acc, w, x, n0, m0, 0, x.k, lds_of(lds));
 	const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wn = wave % S::WN, wm = wave / S::WN;
 	wait_and_sync();
+	lds_char* mine = lds_of(lds) + wave * Rows<P::NB>::BYTES;
 #pragma unroll
 	for (int c = 0; c < P::MB; ++c) {
-		f32x16 v[P::NB];
 #pragma unroll
-		for (int b = 0; b < P::NB; ++b)
+		for (int b = 0; b < P::NB; ++b) {
+			f32x16 v;
+			with_activation(act, [&](auto a) {
 #pragma unroll
-			for (int i = 0; i < 16; ++i) v[b][i] = activate(act, acc[0][b][c][i]).x * acc[1][b][c][i];
-		store_rows<T, P::NB>(v, h, n0 + wn * (P::NB * 32), m0 + wm * (P::MB * 32) + c * 32, lds_of(lds) + wave * (32 * (P::NB * 64 + 16)), lane);
+				for (int i = 0; i < 16; ++i) v[i] = activate<decltype(a)::value>(acc[0][b][c][i]).x * acc[1][b][c][i];
+			});
+			put_block<T, P::NB>(v, b, mine, lane);
+		}
+		store_rows<T, P::NB>(h, n0 + wn * (P::NB * 32), m0 + wm * (P::MB * 32) + c * 32, mine, lane);
 	}
 }
 
@@ -89,12 +106,11 @@ template <class T, int NB, int MB>
 __device__ __forceinline__ void store_tile(f32x16 (&acc)[1][NB][MB], const Rows2<T>& o, uint32_t n0, uint32_t m0, lds_char* lds, int lane) {
 #pragma unroll
 	for (int c = 0; c < MB; ++c) {
-		f32x16 v[NB];
 #pragma unroll
-		for (int b = 0; b < NB; ++b) v[b] = acc[0][b][c];
+		for (int b = 0; b < NB; ++b) put_block<T, NB>(acc[0][b][c], b, lds, lane);
 		const uint32_t m = m0 + c * 32;   // a_rows is a multiple of 32 wherever b is used: 32 rows never lie on both sides
-		if (m < o.a_rows) store_rows<T, NB>(v, o.a, n0, m, lds, lane);
-		else store_rows<T, NB>(v, o.b, n0, m - o.a_rows, lds, lane);
+		if (m < o.a_rows) store_rows<T, NB>(o.a, n0, m, lds, lane);
+		else store_rows<T, NB>(o.b, n0, m - o.a_rows, lds, lane);
 	}
 }
 
@@ -132,7 +148,7 @@ __global__ void __launch_bounds__(Shape<BIG>::THREADS, 2) product_kernel(Pair p0
 		return;
 	}
 	wait_and_sync();
-	store_tile<T, P::NB, P::MB>(acc, out, n0 + wn * (P::NB * 32), m0 + wm * (P::MB * 32), lds_of(lds) + wave * (32 * (P::NB * 64 + 16)), lane);
+	store_tile<T, P::NB, P::MB>(acc, out, n0 + wn * (P::NB * 32), m0 + wm * (P::MB * 32), lds_of(lds) + wave * Rows<P::NB>::BYTES, lane);
 }
 
 // `splits` partials -> ceil(splits / SUM_FAN) in the first of them, sixteen neighbours in their order: a long list of splits would otherwise be one workgroup's serial work
@@ -151,7 +167,7 @@ template <class T, bool BIG>
 __global__ void __launch_bounds__(Shape<BIG>::THREADS) split_sum_kernel(const float* partial, uint32_t splits, uint32_t every, Rows2<T> out, uint32_t tiles_n, uint32_t tiles_m) {
 	using S = Shape<BIG>;
 	constexpr int NB = S::N / S::WN / 32, MB = S::M / S::WM / 32;
-	__shared__ __attribute__((aligned(16))) char lds[S::WN * S::WM * 32 * (NB * 64 + 16)];
+	__shared__ __attribute__((aligned(16))) char lds[S::WN * S::WM * Rows<NB>::BYTES];
 	const uint32_t tn = blockIdx.x % tiles_n, tm = blockIdx.x / tiles_n;
 	const float* q = partial + (uint64_t)blockIdx.x * (S::N * S::M) + threadIdx.x * 4;
 	const uint64_t stride = (uint64_t)every * tiles_n * tiles_m * (S::N * S::M);
@@ -169,7 +185,7 @@ __global__ void __launch_bounds__(Shape<BIG>::THREADS) split_sum_kernel(const fl
 #pragma unroll
 					for (int e = 0; e < 4; ++e) acc[0][b][c][4 * i + e] += v[e];
 				}
-	store_tile<T, NB, MB>(acc, out, tn * S::N + wn * (NB * 32), tm * S::M + wm * (MB * 32), lds_of(lds) + wave * (32 * (NB * 64 + 16)), lane);
+	store_tile<T, NB, MB>(acc, out, tn * S::N + wn * (NB * 32), tm * S::M + wm * (MB * 32), lds_of(lds) + wave * Rows<NB>::BYTES, lane);
 }
 
 // g, u and dh of a tile in one set of registers; from them dg, du (next to each other: d[m][0 .. f8) and d[m][f8 .. 2 f8)) and h
@@ -191,29 +207,32 @@ __global__ void __launch_bounds__(Shape<BIG>::THREADS, 2) hidden_backward_kernel
 	Q::run(dh, &wd, dy, n0, m0, 0, dy.k, lds_of(lds));
 	const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wn = wave % S::WN, wm = wave / S::WN;
 	wait_and_sync();
-	lds_char* mine = lds_of(lds) + wave * (32 * (P::NB * 64 + 16));
+	lds_char* mine = lds_of(lds) + wave * (3 * Rows<P::NB>::BYTES);
+	static_assert(S::WN * S::WM * 3 * Rows<P::NB>::BYTES <= P::LDS_BYTES, "three results of every wave at once");
 	const uint32_t n = n0 + wn * (P::NB * 32);
 #pragma unroll
 	for (int c = 0; c < P::MB; ++c) {
 		const uint32_t m = m0 + wm * (P::MB * 32) + c * 32;
-		f32x16 v[P::NB];
 #pragma unroll
-		for (int b = 0; b < P::NB; ++b)
+		for (int b = 0; b < P::NB; ++b) {
+			f32x16 g = gu[0][b][c], u = gu[1][b][c], v = dh[0][b][c];
+			with_activation(act, [&](auto kind) {
 #pragma unroll
-			for (int i = 0; i < 16; ++i) {
-				const float2 a = activate(act, gu[0][b][c][i]);
-				const float u = gu[1][b][c][i], d = dh[0][b][c][i];
-				v[b][i] = a.x * u;
-				gu[0][b][c][i] = d * u * a.y;
-				gu[1][b][c][i] = d * a.x;
-			}
-		store_rows<T, P::NB>(v, h, n, m, mine, lane);
-#pragma unroll
-		for (int b = 0; b < P::NB; ++b) v[b] = gu[0][b][c];
-		store_rows<T, P::NB>(v, dg, n, m, mine, lane);
-#pragma unroll
-		for (int b = 0; b < P::NB; ++b) v[b] = gu[1][b][c];
-		store_rows<T, P::NB>(v, du, n, m, mine, lane);
+				for (int i = 0; i < 16; ++i) {
+					const float2 a = activate<decltype(kind)::value>(g[i]);
+					const float d = v[i];
+					v[i] = a.x * u[i];
+					g[i] = d * u[i] * a.y;
+					u[i] = d * a.x;
+				}
+			});
+			put_block<T, P::NB>(v, b, mine, lane);
+			put_block<T, P::NB>(g, b, mine + Rows<P::NB>::BYTES, lane);
+			put_block<T, P::NB>(u, b, mine + 2 * Rows<P::NB>::BYTES, lane);
+		}
+		store_rows<T, P::NB>(h, n, m, mine, lane);
+		store_rows<T, P::NB>(dg, n, m, mine + Rows<P::NB>::BYTES, lane);
+		store_rows<T, P::NB>(du, n, m, mine + 2 * Rows<P::NB>::BYTES, lane);
 	}
 }
 
@@ -314,7 +333,7 @@ static uint64_t narrow_partial_bytes(const NgpGatedFfn& b, uint64_t rows) {
 template <class T, int DB, int OB, bool VEC>
 static void launch_narrow_forward(hipStream_t st, const NarrowArgs& a, uint32_t lds) {
 	if (lds > 64 * 1024) (void)hipFuncSetAttribute((const void*)narrow_forward_kernel<T, DB, OB, VEC>, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
-	const uint32_t per_cu = std::max(1u, std::min(6u, 160 * 1024 / lds));
+	const uint32_t per_cu = std::max(1u, std::min((uint32_t)narrow_waves(DB, OB, VEC), 160 * 1024 / lds));
 	hipLaunchKernelGGL((narrow_forward_kernel<T, DB, OB, VEC>), dim3(std::min((a.rows + 127) / 128, 256 * per_cu)), dim3(256), lds, st, a);
 }
 template <class T, int DB, int OB> static void pick_narrow_forward(hipStream_t st, const NarrowArgs& a, uint32_t lds, bool vec) {
@@ -353,6 +372,26 @@ template <class T> static int run_narrow_backward(hipStream_t st, const NarrowAr
 	NGP_LAUNCH_CHECK("narrow_backward_kernel");
 	return 0;
 }
+// ---- few rows: a launch for h and one for y.  Workgroups of 4 to 16 waves (8 for the pair of matrices, whose sums take twice the LDS): about 2048 waves, 8 a CU.
+template <class T, int NM, int MB> static void launch_few(hipStream_t st, const T* x, uint64_t x_ld, uint32_t rows, const T* w0, const T* w1, uint32_t n, uint32_t k, T* out, uint64_t out_ld, int act) {
+	const uint32_t groups = (n + 15) / 16;
+	uint32_t waves = 4;
+	while (waves < (NM == 2 ? 8 : 16) && groups * waves < 2048 && waves * (FEW_CHUNK * 32) < k) waves *= 2;
+	hipLaunchKernelGGL((few_rows_kernel<T, NM, MB>), dim3(groups), dim3(64 * waves), 0, st, x, x_ld, rows, w0, w1, n, k, out, out_ld, act);
+}
+template <class T, int NM> static void pick_few(hipStream_t st, const T* x, uint64_t x_ld, uint32_t rows, const T* w0, const T* w1, uint32_t n, uint32_t k, T* out, uint64_t out_ld, int act) {
+	if (rows <= 16) launch_few<T, NM, 1>(st, x, x_ld, rows, w0, w1, n, k, out, out_ld, act);
+	else if (rows <= 32) launch_few<T, NM, 2>(st, x, x_ld, rows, w0, w1, n, k, out, out_ld, act);
+	else launch_few<T, NM, 4>(st, x, x_ld, rows, w0, w1, n, k, out, out_ld, act);
+}
+template <class T> static int run_few(hipStream_t st, const NgpGatedFfn& b, uint32_t rows, const void* x, uint64_t x_ld, const void* wg, const void* wu, const void* wd, void* y, uint64_t y_ld, void* h) {
+	const uint32_t pitch = (b.n_hidden + 31) & ~31u;
+	pick_few<T, 2>(st, (const T*)x, x_ld, rows, (const T*)wg, (const T*)wu, b.n_hidden, b.n_in, (T*)h, pitch, b.activation);
+	pick_few<T, 1>(st, (const T*)h, pitch, rows, (const T*)wd, nullptr, b.n_out, b.n_hidden, (T*)y, y_ld, 0);
+	NGP_LAUNCH_CHECK("few_rows_kernel");
+	return 0;
+}
+
 static bool vector_rows(const void* p, uint64_t ld, uint32_t cols) { return ((uintptr_t)p & 15) == 0 && ld % 8 == 0 && cols % 8 == 0; }
 
 // What a call keeps in its workspace.  `any`: room for padded copies of every input, else of those whose width is no multiple of 8.
@@ -366,12 +405,17 @@ struct Space {
 	Space(char* base, const NgpGatedFfn& b, uint64_t rows, bool backward, bool any) {
 		Arena a{base};
 		bytes = 0;
+		d8 = (uint32_t)up8(b.n_in); f8 = (uint32_t)up8(b.n_hidden); o8 = (uint32_t)up8(b.n_out); fp = (f8 + 31) & ~31u;
 		if (backward ? narrow_backward(b) : narrow_forward_lds(b) != 0) {
 			if (backward) partial = (float*)a.take(narrow_partial_bytes(b, rows));
 			bytes = a.used;
 			return;
 		}
-		d8 = (uint32_t)up8(b.n_in); f8 = (uint32_t)up8(b.n_hidden); o8 = (uint32_t)up8(b.n_out); fp = (f8 + 31) & ~31u;
+		if (!backward && rows <= FEW_ROWS) {
+			h = a.take(rows * fp * 2);
+			bytes = a.used;
+			return;
+		}
 		if (has_copies(b.n_in, any)) { x = a.take(rows * d8 * 2); wg = a.take((uint64_t)b.n_hidden * d8 * 2); wu = a.take((uint64_t)b.n_hidden * d8 * 2); }
 		if (has_copies(b.n_hidden, any)) wd = a.take((uint64_t)b.n_out * f8 * 2);
 		if (backward && has_copies(b.n_out, any)) dy = a.take(rows * o8 * 2);
@@ -505,6 +549,8 @@ int ngp_hip_gated_ffn_forward(void* stream, const NgpGatedFfn* b, uint64_t n_row
 	const bool plain = (b->n_in % 8 || (dma_ready(tx) && dma_ready(tg) && dma_ready(tu))) && (b->n_hidden % 8 || dma_ready(td));
 	const Space s((char*)workspace, *b, n_rows, false, !plain);
 	if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < s.bytes) return refuse("ngp_hip_gated_ffn_forward: workspace null, not 16-byte aligned or too small (ngp_hip_gated_ffn_workspace_bytes; rows that are not 16-byte aligned: NGP_FFN_ANY_LAYOUT)");
+	if (n_rows <= FEW_ROWS) return b->dtype == NGP_DTYPE_F16 ? run_few<f16>((hipStream_t)stream, *b, (uint32_t)n_rows, x, x_stride, w_gate, w_up, w_down, y, y_stride, s.h)
+	                                                         : run_few<b16>((hipStream_t)stream, *b, (uint32_t)n_rows, x, x_stride, w_gate, w_up, w_down, y, y_stride, s.h);
 	if (b->dtype == NGP_DTYPE_F16) return forward<f16>((hipStream_t)stream, *b, s, tx, tg, tu, td, y, y_stride);
 	return forward<b16>((hipStream_t)stream, *b, s, tx, tg, tu, td, y, y_stride);
 }

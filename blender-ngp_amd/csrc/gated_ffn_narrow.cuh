@@ -15,7 +15,10 @@ __device__ __forceinline__ i32x4 load8(const T* row, uint32_t k, uint32_t width)
 	typedef T t8 __attribute__((ext_vector_type(8)));
 	t8 v;
 #pragma unroll
-	for (int e = 0; e < 8; ++e) v[e] = k + e < width ? row[k + e] : (T)0.0f;
+	for (int e = 0; e < 8; ++e) {   // a load that is always allowed and a choice: no branch between the loads
+		const T r = row[min(k + e, width ? width - 1 : 0)];
+		v[e] = k + e < width ? r : (T)0.0f;
+	}
 	return __builtin_bit_cast(i32x4, v);
 }
 template <class T> __device__ __forceinline__ int pack2(float a, float b) {
@@ -60,7 +63,8 @@ __device__ __forceinline__ void stage_fragment(lds_char* dst, const T* w, uint32
 	for (int j = 0; j < 8; ++j) {
 		const uint32_t k = k0 + (perm ? 8 * (j >> 2) + 4 * (lane >> 5) + (j & 3) : 8 * (lane >> 5) + j);
 		const uint32_t a = turned ? k : r, b = turned ? r : k;   // turned: the operand is w^T
-		v[j] = a < rows && b < cols ? w[(uint64_t)a * cols + b] : (T)0.0f;
+		const T e = w[(uint64_t)min(a, rows - 1) * cols + min(b, cols - 1)];
+		v[j] = a < rows && b < cols ? e : (T)0.0f;
 	}
 	*(__attribute__((address_space(3))) t8*)(dst + lane * 16) = v;
 }
@@ -75,19 +79,15 @@ struct NarrowArgs {
 };
 
 // ---- forward: DB k-blocks of 16 input columns, OB blocks of 32 output columns, any number of blocks of 32 hidden columns ----
+// workgroups a CU that the registers leave room for without spilling
+constexpr int narrow_waves(int db, int ob, bool vec) { return ob == 4 ? (db <= 2 ? 3 : 2) : db <= 2 || (vec && db == 4) ? 4 : 2; }
+
 template <class T, int DB, int OB, bool VEC>
-__global__ void __launch_bounds__(256) narrow_forward_kernel(NarrowArgs a) {
+__global__ void __launch_bounds__(256, narrow_waves(DB, OB, VEC)) narrow_forward_kernel(NarrowArgs a) {
 	extern __shared__ __attribute__((aligned(1024))) char smem[];
 	lds_char* const lds = lds_of(smem);
 	constexpr int PER = 2 * DB + 2 * OB;   // fragments of 1 KiB per hidden block: gate, up (DB each), down (2 k-blocks x OB)
 	const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-	const uint32_t fb_n = (a.f + 31) / 32;
-	for (uint32_t i = wave; i < fb_n * PER; i += 4) {
-		const uint32_t fb = i / PER, c = i % PER;
-		if (c < 2 * DB) stage_fragment<T>(lds + i * 1024, (const T*)(c < DB ? a.wg : a.wu), a.f, a.d, fb * 32, (c % DB) * 16, false, false, lane);
-		else stage_fragment<T>(lds + i * 1024, (const T*)a.wd, a.o, a.f, (c - 2 * DB) / 2 * 32, fb * 32 + (c & 1) * 16, false, true, lane);
-	}
-	__syncthreads();
 	const uint32_t tiles = (a.rows + 31) / 32, step = gridDim.x * 4;
 	const bool wide = ((a.y_ld & 7) | ((uintptr_t)a.y & 15)) == 0;
 	i32x4 x[DB], next[DB];
@@ -99,6 +99,13 @@ __global__ void __launch_bounds__(256) narrow_forward_kernel(NarrowArgs a) {
 	};
 	uint32_t tile = blockIdx.x * 4 + wave;
 	if (tile < tiles) load(tile, next);
+	const uint32_t fb_n = (a.f + 31) / 32;
+	for (uint32_t i = wave; i < fb_n * PER; i += 4) {
+		const uint32_t fb = i / PER, c = i % PER;
+		if (c < 2 * DB) stage_fragment<T>(lds + i * 1024, (const T*)(c < DB ? a.wg : a.wu), a.f, a.d, fb * 32, (c % DB) * 16, false, false, lane);
+		else stage_fragment<T>(lds + i * 1024, (const T*)a.wd, a.o, a.f, (c - 2 * DB) / 2 * 32, fb * 32 + (c & 1) * 16, false, true, lane);
+	}
+	__syncthreads();
 	for (; tile < tiles; tile += step) {
 #pragma unroll
 		for (int k = 0; k < DB; ++k) x[k] = next[k];
@@ -114,8 +121,10 @@ __global__ void __launch_bounds__(256) narrow_forward_kernel(NarrowArgs a) {
 				g = mfma<T>(*(const __attribute__((address_space(3))) i32x4*)(w + k * 1024), x[k], g);
 				u = mfma<T>(*(const __attribute__((address_space(3))) i32x4*)(w + (DB + k) * 1024), x[k], u);
 			}
+			with_activation(a.act, [&](auto kind) {
 #pragma unroll
-			for (int i = 0; i < 16; ++i) g[i] = activate(a.act, g[i]).x * u[i];
+				for (int i = 0; i < 16; ++i) g[i] = activate<decltype(kind)::value>(g[i]).x * u[i];
+			});
 #pragma unroll
 			for (int t = 0; t < 2; ++t) {
 				const i32x4 h = as_operand<T>(g, t);
@@ -152,24 +161,12 @@ __device__ __forceinline__ i32x4 turned_fragment(const lds_char* tile, int pitch
 }
 
 template <class T, int DB, int FB, int OB, bool VEC>
-__global__ void __launch_bounds__(256) narrow_backward_kernel(NarrowArgs a) {
+__global__ void __launch_bounds__(256, NarrowBackward<DB, FB, OB>::LDS_BYTES <= 80 * 1024 ? 2 : 1) narrow_backward_kernel(NarrowArgs a) {
 	using S = NarrowBackward<DB, FB, OB>;
 	__shared__ __attribute__((aligned(1024))) char smem[S::LDS_BYTES];
 	lds_char* const lds = lds_of(smem);
 	lds_char* const w = lds + S::OFF_W;
 	const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-	for (int i = wave; i < 2 * S::W_GU + S::W_D + 2 * S::W_T; i += 4) {
-		if (i < 2 * S::W_GU) {
-			const int c = i % S::W_GU;
-			stage_fragment<T>(w + i * 1024, (const T*)(i < S::W_GU ? a.wg : a.wu), a.f, a.d, c / (2 * DB) * 32, c % (2 * DB) * 16, false, false, lane);
-		} else if (i < 2 * S::W_GU + S::W_D) {
-			const int c = i - 2 * S::W_GU;
-			stage_fragment<T>(w + i * 1024, (const T*)a.wd, a.o, a.f, c / (2 * OB) * 32, c % (2 * OB) * 16, true, false, lane);
-		} else {
-			const int c = i - 2 * S::W_GU - S::W_D;
-			stage_fragment<T>(w + i * 1024, (const T*)(c < S::W_T ? a.wg : a.wu), a.f, a.d, (c % S::W_T) / (2 * FB) * 32, c % (2 * FB) * 16, true, false, lane);
-		}
-	}
 	auto weight = [&](int i) { return *(const __attribute__((address_space(3))) i32x4*)(w + i * 1024 + lane * 16); };
 	f32x16 acc[S::OWN];
 #pragma unroll
@@ -190,6 +187,18 @@ __global__ void __launch_bounds__(256) narrow_backward_kernel(NarrowArgs a) {
 	};
 	uint32_t tile = blockIdx.x;
 	if (tile < tiles) load(tile);
+	for (int i = wave; i < 2 * S::W_GU + S::W_D + 2 * S::W_T; i += 4) {
+		if (i < 2 * S::W_GU) {
+			const int c = i % S::W_GU;
+			stage_fragment<T>(w + i * 1024, (const T*)(i < S::W_GU ? a.wg : a.wu), a.f, a.d, c / (2 * DB) * 32, c % (2 * DB) * 16, false, false, lane);
+		} else if (i < 2 * S::W_GU + S::W_D) {
+			const int c = i - 2 * S::W_GU;
+			stage_fragment<T>(w + i * 1024, (const T*)a.wd, a.o, a.f, c / (2 * OB) * 32, c % (2 * OB) * 16, true, false, lane);
+		} else {
+			const int c = i - 2 * S::W_GU - S::W_D;
+			stage_fragment<T>(w + i * 1024, (const T*)(c < S::W_T ? a.wg : a.wu), a.f, a.d, (c % S::W_T) / (2 * FB) * 32, c % (2 * FB) * 16, true, false, lane);
+		}
+	}
 	for (; tile < tiles; tile += gridDim.x) {
 		__syncthreads();   // phase 2 of the rows before has been read (first time: the weights are there)
 		i32x4 x[2 * DB], y[2 * OB];
@@ -218,20 +227,22 @@ __global__ void __launch_bounds__(256) narrow_backward_kernel(NarrowArgs a) {
 				}
 #pragma unroll
 				for (int k = 0; k < 2 * OB; ++k) dh = mfma<T>(weight(2 * S::W_GU + fb * 2 * OB + k), y[k], dh);
+				with_activation(a.act, [&](auto kind) {
+#pragma unroll
+					for (int i = 0; i < 16; ++i) {
+						const float2 r = activate<decltype(kind)::value>(g[i]);
+						const float up = u[i];
+						u[i] = dh[i] * r.x;
+						g[i] = dh[i] * up * r.y;
+						dh[i] = r.x * up;   // now du, dg, h
+					}
+				});
 #pragma unroll
 				for (int q = 0; q < 4; ++q) {
-					float vg[4], vu[4], vh[4];
-#pragma unroll
-					for (int e = 0; e < 4; ++e) {
-						const float2 r = activate(a.act, g[4 * q + e]);
-						vh[e] = r.x * u[4 * q + e];
-						vg[e] = dh[4 * q + e] * u[4 * q + e] * r.y;
-						vu[e] = dh[4 * q + e] * r.x;
-					}
 					const int at = mine * S::PF + (fb * 32 + 8 * q + 4 * (lane >> 5)) * 2;
-					*(__attribute__((address_space(3))) i32x2*)(lds + S::OFF_G + at) = i32x2{pack2<T>(vg[0], vg[1]), pack2<T>(vg[2], vg[3])};
-					*(__attribute__((address_space(3))) i32x2*)(lds + S::OFF_U + at) = i32x2{pack2<T>(vu[0], vu[1]), pack2<T>(vu[2], vu[3])};
-					*(__attribute__((address_space(3))) i32x2*)(lds + S::OFF_H + at) = i32x2{pack2<T>(vh[0], vh[1]), pack2<T>(vh[2], vh[3])};
+					*(__attribute__((address_space(3))) i32x2*)(lds + S::OFF_G + at) = i32x2{pack2<T>(g[4 * q], g[4 * q + 1]), pack2<T>(g[4 * q + 2], g[4 * q + 3])};
+					*(__attribute__((address_space(3))) i32x2*)(lds + S::OFF_U + at) = i32x2{pack2<T>(u[4 * q], u[4 * q + 1]), pack2<T>(u[4 * q + 2], u[4 * q + 3])};
+					*(__attribute__((address_space(3))) i32x2*)(lds + S::OFF_H + at) = i32x2{pack2<T>(dh[4 * q], dh[4 * q + 1]), pack2<T>(dh[4 * q + 2], dh[4 * q + 3])};
 				}
 			}
 		}
@@ -284,6 +295,7 @@ __global__ void __launch_bounds__(1024) narrow_sum_kernel(const float* partial, 
 	const uint32_t b = blockIdx.x >> 4, e = blockIdx.x & 15;   // block of 32 x 32, register of it
 	float s = 0.0f;
 	const float* p = partial + (uint64_t)b * 1024 + e * 64 + lane;
+#pragma unroll 8
 	for (uint32_t g = wave; g < groups; g += 16) s += p[(uint64_t)g * blocks * 1024];
 	sums[wave][lane] = s;
 	__syncthreads();

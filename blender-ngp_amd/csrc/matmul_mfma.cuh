@@ -192,27 +192,32 @@ __device__ __forceinline__ void tile_of(uint32_t pid, uint32_t total, uint32_t t
 // ---- epilogue ----------------------------------------------------------------------------------------------------------------------------
 template <class T> struct Out { T* p; uint64_t ld; uint32_t rows, cols; };   // row-major; columns are the N side
 
-// One wave writes v = 32 rows (m0 ..) x NBLK * 32 columns (n0 ..) through LDS (`lds`: 32 * (NBLK * 64 + 16) bytes of its own), so that a row's columns leave in 16-byte pieces.
-// Rounds once, to nearest even.  Register layout of a 32 x 32 block: lane l holds column m = l & 31 and rows n = 8 (i >> 2) + 4 (l >> 5) + (i & 3).
+// A wave brings 32 rows x NBLK * 32 columns of results into row order through LDS of its own (Rows<NBLK>::BYTES), so that a row's columns leave in 16-byte pieces: put_block rounds one
+// 32 x 32 block (once, to nearest even) into it, store_rows writes the rows.  Register layout of a block: lane l holds column m = l & 31 and rows n = 8 (i >> 2) + 4 (l >> 5) + (i & 3).
+// The wave's own LDS operations are in order: no barrier between the two.
+template <int NBLK> struct Rows { static constexpr int PITCH = NBLK * 64 + 16, BYTES = 32 * PITCH; };
+
 template <class T, int NBLK>
-__device__ __forceinline__ void store_rows(const f32x16* v, const Out<T>& o, uint32_t n0, uint32_t m0, lds_char* lds, int lane) {
+__device__ __forceinline__ void put_block(const f32x16& v, int b, lds_char* lds, int lane) {
 	typedef T t4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+	for (int q = 0; q < 4; ++q) {
+		const t4 h = {(T)v[4 * q], (T)v[4 * q + 1], (T)v[4 * q + 2], (T)v[4 * q + 3]};
+		*(__attribute__((address_space(3))) t4*)(lds + (lane & 31) * Rows<NBLK>::PITCH + (b * 32 + q * 8 + 4 * (lane >> 5)) * 2) = h;
+	}
+}
+
+template <class T, int NBLK>
+__device__ __forceinline__ void store_rows(const Out<T>& o, uint32_t n0, uint32_t m0, const lds_char* lds, int lane) {
 	typedef T t8 __attribute__((ext_vector_type(8)));
-	constexpr int PITCH = NBLK * 64 + 16, PIECES = NBLK * 4, ROWS = 64 / PIECES;
-#pragma unroll
-	for (int b = 0; b < NBLK; ++b)
-#pragma unroll
-		for (int q = 0; q < 4; ++q) {
-			const t4 h = {(T)v[b][4 * q], (T)v[b][4 * q + 1], (T)v[b][4 * q + 2], (T)v[b][4 * q + 3]};
-			*(__attribute__((address_space(3))) t4*)(lds + (lane & 31) * PITCH + (b * 32 + q * 8 + 4 * (lane >> 5)) * 2) = h;
-		}
+	constexpr int PIECES = NBLK * 4, ROWS = 64 / PIECES;
 	const bool wide = (((uint64_t)o.p | (o.ld * 2)) & 15) == 0;
 	const int piece = lane % PIECES;
 	const uint32_t n = n0 + piece * 8;
 #pragma unroll
 	for (int r = 0; r < 32; r += ROWS) {
 		const int row = r + lane / PIECES;
-		const t8 h = *(const __attribute__((address_space(3))) t8*)(lds + row * PITCH + piece * 16);   // same wave, LDS is in order: no barrier
+		const t8 h = *(const __attribute__((address_space(3))) t8*)(lds + row * Rows<NBLK>::PITCH + piece * 16);
 		const uint32_t m = m0 + row;
 		if (m >= o.rows) continue;
 		T* p = o.p + (uint64_t)m * o.ld + n;
