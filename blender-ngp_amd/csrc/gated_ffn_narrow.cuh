@@ -161,7 +161,7 @@ __device__ __forceinline__ i32x4 turned_fragment(const lds_char* tile, int pitch
 }
 
 template <class T, int DB, int FB, int OB, bool VEC>
-__global__ void __launch_bounds__(256, NarrowBackward<DB, FB, OB>::LDS_BYTES <= 80 * 1024 ? 2 : 1) narrow_backward_kernel(NarrowArgs a) {
+__global__ void __launch_bounds__(256, (NarrowBackward<DB, FB, OB>::LDS_BYTES <= 80 * 1024 ? 2 : 1)) narrow_backward_kernel(NarrowArgs a) {
 	using S = NarrowBackward<DB, FB, OB>;
 	__shared__ __attribute__((aligned(1024))) char smem[S::LDS_BYTES];
 	lds_char* const lds = lds_of(smem);

@@ -7,8 +7,8 @@
 // Operands come in two layouts:
 //   KC   [rows][k], k contiguous:     LDS [row][64 k], a fragment (lane: one row, 8 k) is one ds_read_b128;
 //   RC   [k][rows], rows contiguous:  LDS [64 k][row], a fragment is two ds_read_b64_tr_b16 (the LDS unit transposes 4 x 16 blocks on the way out).
-// Bank conflicts: the DMA writes LDS linearly, so the 16-byte chunks of a row are permuted by which chunk each lane ASKS for: chunk ^ (row & 7) for KC (eight rows of one chunk
-// column cover all banks), chunk ^ 4 (k & 3) for RC (the four k rows of a transposed block and its neighbour fall on different 32-byte units).
+// Bank conflicts: the DMA writes LDS linearly, so the 16-byte chunks of a row are permuted by which chunk each lane ASKS for: chunk ^ ((row / 2) & 7) for KC (16 rows of one
+// chunk column, two to a line of 64 banks, cover every bank once), chunk ^ 4 (k & 3) for RC (the four k rows of a transposed block and its neighbour fall on different 32-byte units).
 // The N side is the A operand of the MFMA: a lane then holds four consecutive n of one m per register quad, which is the contiguous direction of the output.
 #pragma once
 
@@ -60,7 +60,7 @@ struct Tile {
 	static constexpr int CHUNKS = LAY == KC ? 8 : BR / 8;            // 16-byte chunks per LDS row
 	static constexpr int LOADS = BYTES / 16 / THREADS;
 	static_assert(BYTES % (16 * THREADS) == 0, "every thread issues the same number of loads");
-	static __device__ __forceinline__ int swizzle(int r) { return LAY == KC ? (r & 7) : CHUNKS >= 16 ? (r & 3) << 2 : (r & 2) << 1; }
+	static __device__ __forceinline__ int swizzle(int r) { return LAY == KC ? (r >> 1) & 7 : CHUNKS >= 16 ? (r & 3) << 2 : (r & 2) << 1; }
 
 	const char* base;        // of this step (uniform)
 	int64_t left;            // bytes from base to the operand's end
@@ -84,7 +84,7 @@ struct Tile {
 		for (int i = 0; i < LOADS; ++i) {
 			const int slot = i * THREADS + tid, r = slot / CHUNKS, c = (slot % CHUNKS) ^ swizzle(r);
 			voff[i] = (int)((uint32_t)r * (uint32_t)m.ld * 2u) + c * 16;
-			if (LAY == KC && i == 0) k_here = c * 8;   // the same for every i: a thread's rows differ by a multiple of 8
+			if (LAY == KC && i == 0) k_here = c * 8;   // the same for every i: a thread's rows differ by a multiple of 16
 		}
 	}
 	// DMA of the current step into `lds` (wave-uniform), then on to the next step
@@ -105,7 +105,7 @@ struct Tile {
 	// fragment of rows row0 .. row0 + 31, k-block ks (16 k): lane l has row l & 31 and k = 8 (l >> 5) .. + 7
 	static __device__ __forceinline__ i32x4 frag(const lds_char* lds, int row0, int ks, int lane) {
 		if (LAY == KC) {
-			const int r = row0 + (lane & 31), c = (ks * 2 + (lane >> 5)) ^ (lane & 7);
+			const int r = row0 + (lane & 31), c = (ks * 2 + (lane >> 5)) ^ ((lane >> 1) & 7);
 			return *(const __attribute__((address_space(3))) i32x4*)(lds + r * 128 + c * 16);
 		}
 		const int k = ks * 16 + 8 * (lane >> 5) + ((lane & 15) >> 2), c = row0 / 8 + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
