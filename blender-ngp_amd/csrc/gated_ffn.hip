@@ -53,49 +53,46 @@ __device__ __forceinline__ void with_activation(int act, F f) {
 namespace ngp {
 namespace ffn {
 
-template <bool BIG> struct Shape;   // BIG: 256 x 256 x 64 in 8 waves, one workgroup a CU; else 128 x 128 x 64 in 4 waves, two a CU
-template <> struct Shape<true> { static constexpr int N = 256, M = 256, WN = 2, WM = 4, THREADS = 512; };
-template <> struct Shape<false> { static constexpr int N = 128, M = 128, WN = 2, WM = 2, THREADS = 256; };
+template <bool BIG> struct Shape;   // BIG: 256 x 256 in 8 waves, one workgroup a CU; else 128 x 128 in 4 waves, two a CU
+template <> struct Shape<true> { static constexpr int N = 256, M = 256, WN = 2, WM = 4, THREADS = 512, RESIDENT = 2; };
+template <> struct Shape<false> { static constexpr int N = 128, M = 128, WN = 2, WM = 2, THREADS = 256, RESIDENT = 2; };
 
-template <int NM, int NB, int MB> __device__ __forceinline__ void clear(f32x16 (&acc)[NM][NB][MB]) {
+template <int NM, int NB, int MB> __device__ __forceinline__ void clear(f32x4 (&acc)[NM][NB][MB]) {
 #pragma unroll
 	for (int j = 0; j < NM; ++j)
 #pragma unroll
 		for (int a = 0; a < NB; ++a)
 #pragma unroll
-			for (int b = 0; b < MB; ++b)
-#pragma unroll
-				for (int i = 0; i < 16; ++i) acc[j][a][b][i] = 0.0f;
+			for (int b = 0; b < MB; ++b) acc[j][a][b] = f32x4{0, 0, 0, 0};
 }
 
 // h = act(x Wg^T) * (x Wu^T): one tile of rows of x against N / 2 gate rows and the same N / 2 up rows, so that both factors of an h meet in one lane
 template <class T, bool BIG>
-__global__ void __launch_bounds__(Shape<BIG>::THREADS, 2) gate_up_kernel(Mat x, Mat wg, Mat wu, Out<T> h, int act, uint32_t tiles_n, uint32_t tiles_m) {
+__global__ void __launch_bounds__(Shape<BIG>::THREADS, Shape<BIG>::RESIDENT) gate_up_kernel(Mat x, Mat wg, Mat wu, Out<T> h, int act, uint32_t tiles_n, uint32_t tiles_m) {
 	using S = Shape<BIG>;
 	using P = Product<T, KC, KC, 2, S::N / 2, S::M, S::WN, S::WM>;
 	__shared__ __attribute__((aligned(1024))) char lds[P::LDS_BYTES];
 	uint32_t tn, tm, split;
 	tile_of(blockIdx.x, gridDim.x, tiles_n, tiles_m, tn, tm, split);
-	f32x16 acc[2][P::NB][P::MB];
+	f32x4 acc[2][P::NB][P::MB];
 	clear(acc);
 	const Mat w[2] = {wg, wu};
 	const uint32_t n0 = tn * (S::N / 2), m0 = tm * S::M;
 	P::run(acc, w, x, n0, m0, 0, x.k, lds_of(lds));
 	const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wn = wave % S::WN, wm = wave / S::WN;
-	wait_and_sync();
 	lds_char* mine = lds_of(lds) + wave * Rows<P::NB>::BYTES;
 #pragma unroll
 	for (int c = 0; c < P::MB; ++c) {
+		with_activation(act, [&](auto a) {
 #pragma unroll
-		for (int b = 0; b < P::NB; ++b) {
-			f32x16 v;
-			with_activation(act, [&](auto a) {
+			for (int b = 0; b < P::NB; ++b) {
+				f32x4 v;
 #pragma unroll
-				for (int i = 0; i < 16; ++i) v[i] = activate<decltype(a)::value>(acc[0][b][c][i]).x * acc[1][b][c][i];
-			});
-			put_block<T, P::NB>(v, b, mine, lane);
-		}
-		store_rows<T, P::NB>(h, n0 + wn * (P::NB * 32), m0 + wm * (P::MB * 32) + c * 32, mine, lane);
+				for (int i = 0; i < 4; ++i) v[i] = activate<decltype(a)::value>(acc[0][b][c][i]).x * acc[1][b][c][i];
+				put_block<T, P::NB>(v, b, c & 1, mine, lane);
+			}
+		});
+		if (c & 1) store_rows<T, P::NB>(h, n0 + wn * (P::NB * 16), m0 + wm * (P::MB * 16) + (c - 1) * 16, mine, lane);
 	}
 }
 
@@ -103,12 +100,13 @@ struct Pair { Mat n, m; };                        // one product's operands
 template <class T> struct Rows2 { Out<T> a, b; uint32_t a_rows; };   // rows 0 .. a_rows - 1 of the result go to a, the rest to b (b starts at row a_rows)
 
 template <class T, int NB, int MB>
-__device__ __forceinline__ void store_tile(f32x16 (&acc)[1][NB][MB], const Rows2<T>& o, uint32_t n0, uint32_t m0, lds_char* lds, int lane) {
+__device__ __forceinline__ void store_tile(f32x4 (&acc)[1][NB][MB], const Rows2<T>& o, uint32_t n0, uint32_t m0, lds_char* lds, int lane) {
 #pragma unroll
 	for (int c = 0; c < MB; ++c) {
 #pragma unroll
-		for (int b = 0; b < NB; ++b) put_block<T, NB>(acc[0][b][c], b, lds, lane);
-		const uint32_t m = m0 + c * 32;   // a_rows is a multiple of 32 wherever b is used: 32 rows never lie on both sides
+		for (int b = 0; b < NB; ++b) put_block<T, NB>(acc[0][b][c], b, c & 1, lds, lane);
+		if (!(c & 1)) continue;
+		const uint32_t m = m0 + (c - 1) * 16;   // a_rows is a multiple of 32 wherever b is used: 32 rows never lie on both sides
 		if (m < o.a_rows) store_rows<T, NB>(o.a, n0, m, lds, lane);
 		else store_rows<T, NB>(o.b, n0, m - o.a_rows, lds, lane);
 	}
@@ -117,13 +115,13 @@ __device__ __forceinline__ void store_tile(f32x16 (&acc)[1][NB][MB], const Rows2
 // C = sum of up to two products of the same k (dx = dg Wg + du Wu), all of it or one split.  With splits, a workgroup leaves its accumulators in `partial` as they lie in the registers,
 // and split_sum_kernel adds the splits in their order: the result does not depend on which workgroup ends first.
 template <class T, int NLAY, int MLAY, bool BIG>
-__global__ void __launch_bounds__(Shape<BIG>::THREADS, 2) product_kernel(Pair p0, Pair p1, int n_products, Rows2<T> out, uint32_t tiles_n, uint32_t tiles_m, uint32_t splits, uint32_t k_split, float* partial) {
+__global__ void __launch_bounds__(Shape<BIG>::THREADS, Shape<BIG>::RESIDENT) product_kernel(Pair p0, Pair p1, int n_products, Rows2<T> out, uint32_t tiles_n, uint32_t tiles_m, uint32_t splits, uint32_t k_split, float* partial) {
 	using S = Shape<BIG>;
 	using P = Product<T, NLAY, MLAY, 1, S::N, S::M, S::WN, S::WM>;
 	__shared__ __attribute__((aligned(1024))) char lds[P::LDS_BYTES];
 	uint32_t tn, tm, split;
 	tile_of(blockIdx.x, gridDim.x, tiles_n, tiles_m, tn, tm, split);
-	f32x16 acc[1][P::NB][P::MB];
+	f32x4 acc[1][P::NB][P::MB];
 	clear(acc);
 	const uint32_t n0 = tn * S::N, m0 = tm * S::M;
 	if (partial) {   // split s of product s / splits
@@ -141,14 +139,10 @@ __global__ void __launch_bounds__(Shape<BIG>::THREADS, 2) product_kernel(Pair p0
 #pragma unroll
 		for (int b = 0; b < P::NB; ++b)
 #pragma unroll
-			for (int c = 0; c < P::MB; ++c)
-#pragma unroll
-				for (int i = 0; i < 4; ++i)
-					*(f32x4*)(q + ((b * P::MB + c) * 4 + i) * (S::THREADS * 4)) = f32x4{acc[0][b][c][4 * i], acc[0][b][c][4 * i + 1], acc[0][b][c][4 * i + 2], acc[0][b][c][4 * i + 3]};
+			for (int c = 0; c < P::MB; ++c) *(f32x4*)(q + (b * P::MB + c) * (S::THREADS * 4)) = acc[0][b][c];
 		return;
 	}
-	wait_and_sync();
-	store_tile<T, P::NB, P::MB>(acc, out, n0 + wn * (P::NB * 32), m0 + wm * (P::MB * 32), lds_of(lds) + wave * Rows<P::NB>::BYTES, lane);
+	store_tile<T, P::NB, P::MB>(acc, out, n0 + wn * (P::NB * 16), m0 + wm * (P::MB * 16), lds_of(lds) + wave * Rows<P::NB>::BYTES, lane);
 }
 
 // `splits` partials -> ceil(splits / SUM_FAN) in the first of them, sixteen neighbours in their order: a long list of splits would otherwise be one workgroup's serial work
@@ -166,31 +160,25 @@ __global__ void __launch_bounds__(256) split_fold_kernel(float* partial, uint32_
 template <class T, bool BIG>
 __global__ void __launch_bounds__(Shape<BIG>::THREADS) split_sum_kernel(const float* partial, uint32_t splits, uint32_t every, Rows2<T> out, uint32_t tiles_n, uint32_t tiles_m) {
 	using S = Shape<BIG>;
-	constexpr int NB = S::N / S::WN / 32, MB = S::M / S::WM / 32;
+	constexpr int NB = S::N / S::WN / 16, MB = S::M / S::WM / 16;
 	__shared__ __attribute__((aligned(16))) char lds[S::WN * S::WM * Rows<NB>::BYTES];
 	const uint32_t tn = blockIdx.x % tiles_n, tm = blockIdx.x / tiles_n;
 	const float* q = partial + (uint64_t)blockIdx.x * (S::N * S::M) + threadIdx.x * 4;
 	const uint64_t stride = (uint64_t)every * tiles_n * tiles_m * (S::N * S::M);
 	const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wn = wave % S::WN, wm = wave / S::WN;
-	f32x16 acc[1][NB][MB];
+	f32x4 acc[1][NB][MB];
 	clear(acc);
 	for (uint32_t s = 0; s < splits; ++s, q += stride)
 #pragma unroll
 		for (int b = 0; b < NB; ++b)
 #pragma unroll
-			for (int c = 0; c < MB; ++c)
-#pragma unroll
-				for (int i = 0; i < 4; ++i) {
-					const f32x4 v = *(const f32x4*)(q + ((b * MB + c) * 4 + i) * (S::THREADS * 4));
-#pragma unroll
-					for (int e = 0; e < 4; ++e) acc[0][b][c][4 * i + e] += v[e];
-				}
-	store_tile<T, NB, MB>(acc, out, tn * S::N + wn * (NB * 32), tm * S::M + wm * (MB * 32), lds_of(lds) + wave * Rows<NB>::BYTES, lane);
+			for (int c = 0; c < MB; ++c) acc[0][b][c] += *(const f32x4*)(q + (b * MB + c) * (S::THREADS * 4));
+	store_tile<T, NB, MB>(acc, out, tn * S::N + wn * (NB * 16), tm * S::M + wm * (MB * 16), lds_of(lds) + wave * Rows<NB>::BYTES, lane);
 }
 
 // g, u and dh of a tile in one set of registers; from them dg, du (next to each other: d[m][0 .. f8) and d[m][f8 .. 2 f8)) and h
 template <class T, bool BIG>
-__global__ void __launch_bounds__(Shape<BIG>::THREADS, 2) hidden_backward_kernel(Mat x, Mat wg, Mat wu, Mat dy, Mat wd, Out<T> dg, Out<T> du, Out<T> h, int act, uint32_t tiles_n, uint32_t tiles_m) {
+__global__ void __launch_bounds__(Shape<BIG>::THREADS, Shape<BIG>::RESIDENT) hidden_backward_kernel(Mat x, Mat wg, Mat wu, Mat dy, Mat wd, Out<T> dg, Out<T> du, Out<T> h, int act, uint32_t tiles_n, uint32_t tiles_m) {
 	using S = Shape<BIG>;
 	using P = Product<T, KC, KC, 2, S::N / 2, S::M, S::WN, S::WM>;
 	using Q = Product<T, RC, KC, 1, S::N / 2, S::M, S::WN, S::WM>;
@@ -198,38 +186,38 @@ __global__ void __launch_bounds__(Shape<BIG>::THREADS, 2) hidden_backward_kernel
 	static_assert(Q::LDS_BYTES <= P::LDS_BYTES, "one buffer for both");
 	uint32_t tn, tm, split;
 	tile_of(blockIdx.x, gridDim.x, tiles_n, tiles_m, tn, tm, split);
-	f32x16 gu[2][P::NB][P::MB], dh[1][P::NB][P::MB];
+	f32x4 gu[2][P::NB][P::MB], dh[1][P::NB][P::MB];
 	clear(gu);
-	clear(dh);
 	const Mat w[2] = {wg, wu};
 	const uint32_t n0 = tn * (S::N / 2), m0 = tm * S::M;
 	P::run(gu, w, x, n0, m0, 0, x.k, lds_of(lds));
+	clear(dh);
 	Q::run(dh, &wd, dy, n0, m0, 0, dy.k, lds_of(lds));
 	const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wn = wave % S::WN, wm = wave / S::WN;
-	wait_and_sync();
 	lds_char* mine = lds_of(lds) + wave * (3 * Rows<P::NB>::BYTES);
 	static_assert(S::WN * S::WM * 3 * Rows<P::NB>::BYTES <= P::LDS_BYTES, "three results of every wave at once");
-	const uint32_t n = n0 + wn * (P::NB * 32);
+	const uint32_t n = n0 + wn * (P::NB * 16);
 #pragma unroll
 	for (int c = 0; c < P::MB; ++c) {
-		const uint32_t m = m0 + wm * (P::MB * 32) + c * 32;
+		with_activation(act, [&](auto kind) {
 #pragma unroll
-		for (int b = 0; b < P::NB; ++b) {
-			f32x16 g = gu[0][b][c], u = gu[1][b][c], v = dh[0][b][c];
-			with_activation(act, [&](auto kind) {
+			for (int b = 0; b < P::NB; ++b) {
+				f32x4 g, u, v;
 #pragma unroll
-				for (int i = 0; i < 16; ++i) {
-					const float2 a = activate<decltype(kind)::value>(g[i]);
-					const float d = v[i];
-					v[i] = a.x * u[i];
-					g[i] = d * u[i] * a.y;
+				for (int i = 0; i < 4; ++i) {
+					const float2 a = activate<decltype(kind)::value>(gu[0][b][c][i]);
+					const float up = gu[1][b][c][i], d = dh[0][b][c][i];
+					v[i] = a.x * up;
+					g[i] = d * up * a.y;
 					u[i] = d * a.x;
 				}
-			});
-			put_block<T, P::NB>(v, b, mine, lane);
-			put_block<T, P::NB>(g, b, mine + Rows<P::NB>::BYTES, lane);
-			put_block<T, P::NB>(u, b, mine + 2 * Rows<P::NB>::BYTES, lane);
-		}
+				put_block<T, P::NB>(v, b, c & 1, mine, lane);
+				put_block<T, P::NB>(g, b, c & 1, mine + Rows<P::NB>::BYTES, lane);
+				put_block<T, P::NB>(u, b, c & 1, mine + 2 * Rows<P::NB>::BYTES, lane);
+			}
+		});
+		if (!(c & 1)) continue;
+		const uint32_t m = m0 + wm * (P::MB * 16) + (c - 1) * 16;
 		store_rows<T, P::NB>(h, n, m, mine, lane);
 		store_rows<T, P::NB>(dg, n, m, mine + Rows<P::NB>::BYTES, lane);
 		store_rows<T, P::NB>(du, n, m, mine + 2 * Rows<P::NB>::BYTES, lane);
@@ -458,7 +446,7 @@ struct Launch {
 		const uint32_t tiles = p.tiles_n * p.tiles_m;
 		float* part = p.partials ? partial : nullptr;
 		const dim3 grid(tiles * std::max(1u, p.partials));
-		if (p.big) hipLaunchKernelGGL((product_kernel<T, NLAY, MLAY, true>), grid, dim3(512), 0, st, p0, p1 ? *p1 : p0, p1 ? 2 : 1, out, p.tiles_n, p.tiles_m, p.splits, p.k_split, part);
+		if (p.big) hipLaunchKernelGGL((product_kernel<T, NLAY, MLAY, true>), grid, dim3(Shape<true>::THREADS), 0, st, p0, p1 ? *p1 : p0, p1 ? 2 : 1, out, p.tiles_n, p.tiles_m, p.splits, p.k_split, part);
 		else hipLaunchKernelGGL((product_kernel<T, NLAY, MLAY, false>), grid, dim3(256), 0, st, p0, p1 ? *p1 : p0, p1 ? 2 : 1, out, p.tiles_n, p.tiles_m, p.splits, p.k_split, part);
 		if (!ok("product_kernel") || !part) return;
 		uint32_t splits = p.partials, every = 1;
@@ -485,7 +473,7 @@ static int forward(hipStream_t st, const NgpGatedFfn& b, const Space& s, Tensor 
 	const Out<T> h{(T*)s.h, s.fp, (uint32_t)x.rows, s.fp};
 	const bool big = ceil_div(s.fp, 128) * ceil_div(x.rows, 256) >= 192;
 	const uint32_t tn = (uint32_t)ceil_div(s.fp, big ? 128 : 64), tm = (uint32_t)ceil_div(x.rows, big ? 256 : 128);
-	if (big) hipLaunchKernelGGL((gate_up_kernel<T, true>), dim3(tn * tm), dim3(512), 0, st, kc(x), kc(wg), kc(wu), h, b.activation, tn, tm);
+	if (big) hipLaunchKernelGGL((gate_up_kernel<T, true>), dim3(tn * tm), dim3(Shape<true>::THREADS), 0, st, kc(x), kc(wg), kc(wu), h, b.activation, tn, tm);
 	else hipLaunchKernelGGL((gate_up_kernel<T, false>), dim3(tn * tm), dim3(256), 0, st, kc(x), kc(wg), kc(wu), h, b.activation, tn, tm);
 	l.ok("gate_up_kernel");
 	const Tensor th{s.h, s.fp, x.rows, s.f8};
@@ -503,7 +491,7 @@ static int backward(hipStream_t st, const NgpGatedFfn& b, const Space& s, Tensor
 	const Out<T> h{(T*)s.h, s.fp, rows, s.fp}, dg{d, 2ull * s.fp, rows, s.fp}, du{d + s.fp, 2ull * s.fp, rows, s.fp};
 	const bool big = ceil_div(s.fp, 128) * ceil_div(rows, 256) >= 192;
 	const uint32_t tn = (uint32_t)ceil_div(s.fp, big ? 128 : 64), tm = (uint32_t)ceil_div(rows, big ? 256 : 128);
-	if (big) hipLaunchKernelGGL((hidden_backward_kernel<T, true>), dim3(tn * tm), dim3(512), 0, st, kc(x), kc(wg), kc(wu), kc(dy), rc(wd), dg, du, h, b.activation, tn, tm);
+	if (big) hipLaunchKernelGGL((hidden_backward_kernel<T, true>), dim3(tn * tm), dim3(Shape<true>::THREADS), 0, st, kc(x), kc(wg), kc(wu), kc(dy), rc(wd), dg, du, h, b.activation, tn, tm);
 	else hipLaunchKernelGGL((hidden_backward_kernel<T, false>), dim3(tn * tm), dim3(256), 0, st, kc(x), kc(wg), kc(wu), kc(dy), rc(wd), dg, du, h, b.activation, tn, tm);
 	l.ok("hidden_backward_kernel");
 	const Tensor tdg{dg.p, dg.ld, rows, s.f8}, tdu{du.p, du.ld, rows, s.f8}, tboth{d, 2ull * s.fp, rows, 2 * s.fp}, th{s.h, s.fp, rows, s.fp};

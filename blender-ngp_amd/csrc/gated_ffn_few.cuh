@@ -9,10 +9,6 @@
 namespace ngp {
 namespace ffn {
 
-template <class T> __device__ __forceinline__ f32x4 mfma16(i32x4 a, i32x4 b, f32x4 c);
-template <> __device__ __forceinline__ f32x4 mfma16<f16>(i32x4 a, i32x4 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0); }
-template <> __device__ __forceinline__ f32x4 mfma16<b16>(i32x4 a, i32x4 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b16x8, a), __builtin_bit_cast(b16x8, b), c, 0, 0, 0); }
-
 typedef i32x4 i32x4_any __attribute__((aligned(2)));
 
 constexpr int FEW_ROWS = 64, FEW_CHUNK = 8;   // k-blocks of 32 per wave and turn

@@ -1,14 +1,18 @@
-// matmul_mfma.cuh — tiled matrix products C[m][n] = sum_k M[m][k] N[n][k] on v_mfma_f32_32x32x16_{f16,bf16}, the core of the gated feed-forward block (gated_ffn.hip)
+// matmul_mfma.cuh — tiled matrix products C[m][n] = sum_k M[m][k] N[n][k] on v_mfma_f32_16x16x32_{f16,bf16}, the core of the gated feed-forward block (gated_ffn.hip)
 // and of the Muon step (muon.hip).
 //
-// Scheme.  A workgroup owns a BN x BM tile and walks k in steps of 64.  Both operands of a step go from memory into LDS by DMA (buffer_load ... lds, 16 bytes a lane: no
-// registers, no ds_write), one step ahead of the matrix instructions (two LDS buffers).  The buffer descriptor of a step ends where the operand ends, and the hardware returns
+// Scheme.  A workgroup owns a BN x BM tile and walks k in steps of 32.  Both operands of a step go from memory into LDS by DMA (buffer_load ... lds, 16 bytes a lane: no
+// registers, no ds_write), three steps ahead of the matrix instructions (a ring of four LDS buffers).  The buffer descriptor of a step ends where the operand ends, and the hardware returns
 // zero behind it, so the last rows and the last k of any size need no branch; a chunk behind k in the middle of a row asks for an offset behind the descriptor.
 // Operands come in two layouts:
-//   KC   [rows][k], k contiguous:     LDS [row][64 k], a fragment (lane: one row, 8 k) is one ds_read_b128;
-//   RC   [k][rows], rows contiguous:  LDS [64 k][row], a fragment is two ds_read_b64_tr_b16 (the LDS unit transposes 4 x 16 blocks on the way out).
-// Bank conflicts: the DMA writes LDS linearly, so the 16-byte chunks of a row are permuted by which chunk each lane ASKS for: chunk ^ ((row / 2) & 7) for KC (16 rows of one
-// chunk column, two to a line of 64 banks, cover every bank once), chunk ^ 4 (k & 3) for RC (the four k rows of a transposed block and its neighbour fall on different 32-byte units).
+//   KC   [rows][k], k contiguous:     LDS [row][k], a fragment (lane: one row, 8 k) is one ds_read_b128;
+//   RC   [k][rows], rows contiguous:  LDS [k][row], a fragment is two ds_read_b64_tr_b16 (the LDS unit transposes 4 x 16 blocks on the way out).
+// Bank conflicts: the DMA writes LDS linearly, so the 16-byte chunks of a row are permuted by which chunk each lane ASKS for, chunk ^ swizzle(row): for KC such that 16 rows of
+// one chunk column cover every bank once, for RC such that the four k rows of a transposed block and its neighbour fall on different 32-byte units.  (The KC order that repeats
+// every 8 rows instead cost half of the LDS cycles in conflicts.)
+// What bounds it.  The matrix pipes and, below them, power: at 8192 x 4096 x 8192 the clock falls to about 1.7 GHz.  Three things keep the pipes fed: fragments are read half a step
+// ahead of the MFMAs that take them; the DMA instructions stand between MFMAs, two to a half step (eight in a row block the wave's issue, and with it its MFMAs, until the memory
+// pipe has taken them); and the only waits are for data that was asked for two steps ago.
 // The N side is the A operand of the MFMA: a lane then holds four consecutive n of one m per register quad, which is the contiguous direction of the output.
 #pragma once
 
@@ -31,7 +35,6 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) char lds_char;
 
 enum { KC = 0, RC = 1 };
-constexpr int BK = 64;   // k per step: 128-byte rows for KC, four MFMA k-blocks
 
 struct Mat {             // rows x k, see above; ld in elements, a multiple of 8; p 16-byte aligned; KC: k a multiple of 8
 	const void* p;
@@ -39,6 +42,9 @@ struct Mat {             // rows x k, see above; ld in elements, a multiple of 8
 	uint32_t rows, k;
 };
 
+template <class T> __device__ __forceinline__ f32x4 mfma16(i32x4 a, i32x4 b, f32x4 c);
+template <> __device__ __forceinline__ f32x4 mfma16<f16>(i32x4 a, i32x4 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0); }
+template <> __device__ __forceinline__ f32x4 mfma16<b16>(i32x4 a, i32x4 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b16x8, a), __builtin_bit_cast(b16x8, b), c, 0, 0, 0); }
 template <class T> __device__ __forceinline__ f32x16 mfma(i32x4 a, i32x4 b, f32x16 c);
 template <> __device__ __forceinline__ f32x16 mfma<f16>(i32x4 a, i32x4 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0); }
 template <> __device__ __forceinline__ f32x16 mfma<b16>(i32x4 a, i32x4 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b16x8, a), __builtin_bit_cast(b16x8, b), c, 0, 0, 0); }
@@ -50,23 +56,27 @@ __device__ __forceinline__ lds_char* lds_of(void* p) { return (lds_char*)(__attr
 __device__ __forceinline__ void dma16(i32x4 rsrc, lds_char* lds, int voff) {
 	asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"((uint32_t)(uintptr_t)lds), "v"(voff), "s"(rsrc) : "memory");
 }
-// every DMA of this wave has landed, every LDS read of it has returned; then all waves
-__device__ __forceinline__ void wait_and_sync() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+// every DMA of this wave but the last PENDING has landed, every LDS read of it has returned; then all waves
+template <int PENDING = 0> __device__ __forceinline__ void wait_and_sync() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(PENDING) : "memory"); }
 
-// One operand's tile of BR rows x 64 k: who loads what, and how a fragment is read back.
-template <int LAY, int BR, int THREADS>
+// One operand's tile of BR rows x BK k: who loads what, and how a fragment is read back.
+template <int LAY, int BR, int THREADS, int BK>
 struct Tile {
 	static constexpr int BYTES = BR * BK * 2;
-	static constexpr int CHUNKS = LAY == KC ? 8 : BR / 8;            // 16-byte chunks per LDS row
+	static constexpr int CHUNKS = LAY == KC ? BK / 8 : BR / 8;       // 16-byte chunks per LDS row
 	static constexpr int LOADS = BYTES / 16 / THREADS;
 	static_assert(BYTES % (16 * THREADS) == 0, "every thread issues the same number of loads");
-	static __device__ __forceinline__ int swizzle(int r) { return LAY == KC ? (r >> 1) & 7 : CHUNKS >= 16 ? (r & 3) << 2 : (r & 2) << 1; }
+	static __device__ __forceinline__ int swizzle(int r) {
+		if (LAY == KC) return BK == 64 ? (r >> 1) & 7 : (r >> 2) & 3;
+		return CHUNKS >= 16 ? (r & 3) << 1 | (r & 8) : (r & 2) | (r & 8) >> 1;
+	}
 
 	const char* base;        // of this step (uniform)
 	int64_t left;            // bytes from base to the operand's end
 	int64_t step_bytes;
 	int k_here;              // KC: k of this thread's chunk in the step; beyond `k_left` it reads zero
 	int k_left;
+	bool k_past;
 	int voff[LOADS];
 
 	__device__ __forceinline__ void init(const Mat& m, uint32_t row0, int tid) {
@@ -87,47 +97,57 @@ struct Tile {
 			if (LAY == KC && i == 0) k_here = c * 8;   // the same for every i: a thread's rows differ by a multiple of 16
 		}
 	}
-	// DMA of the current step into `lds` (wave-uniform), then on to the next step
-	__device__ __forceinline__ void issue(lds_char* lds, int wave) {
-		const uint32_t records = left > 0x7fffffff ? 0x7fffffffu : left < 0 ? 0u : (uint32_t)left;
+	// descriptor of the current step (what lies behind the operand's end reads as zero), then on to the next
+	__device__ __forceinline__ i32x4 next() {
 		const uint64_t b = (uint64_t)base;
-		i32x4 r = {(int)(uint32_t)b, (int)((uint32_t)(b >> 32) & 0xffffu), (int)records, 0x00020000};
+		const int records = left > 0x7fffffff ? 0x7fffffff : left < 0 ? 0 : (int)left;
+		i32x4 r = {(int)(uint32_t)b, (int)((uint32_t)(b >> 32) & 0xffffu), records, 0x00020000};
 		asm volatile("s_nop 4" : "+s"(r));   // a descriptor word that came from the VALU must be five wait states old when a memory instruction reads it
-#pragma unroll
-		for (int i = 0; i < LOADS; ++i) {
-			const int v = LAY == KC && k_here >= k_left ? (int)0x80000000 : voff[i];
-			dma16(r, lds + (i * THREADS + wave * 64) * 16, v);
-		}
+		k_past = LAY == KC && k_here >= k_left;
 		base += step_bytes;
 		left -= step_bytes;
 		k_left -= BK;
+		return r;
 	}
-	// fragment of rows row0 .. row0 + 31, k-block ks (16 k): lane l has row l & 31 and k = 8 (l >> 5) .. + 7
-	static __device__ __forceinline__ i32x4 frag(const lds_char* lds, int row0, int ks, int lane) {
+	// the i-th DMA of the step that next() gave into `lds` (wave-uniform)
+	__device__ __forceinline__ void issue(const i32x4& r, int i, lds_char* lds, int wave) const {
+		dma16(r, lds + (i * THREADS + wave * 64) * 16, k_past ? (int)0x80000000 : voff[i]);
+	}
+	// fragment of rows row0 .. row0 + 31, k-block ks of 16 (KC): lane l has row l & 31 and k = 8 (l >> 5) .. + 7
+	static __device__ __forceinline__ i32x4 frag32(const lds_char* lds, int row0, int ks, int lane) {
+		static_assert(LAY == KC, "the 32-row fragments are read along k");
+		const int r = row0 + (lane & 31), c = (ks * 2 + (lane >> 5)) ^ swizzle(lane & 31);
+		return *(const __attribute__((address_space(3))) i32x4*)(lds + r * (BK * 2) + c * 16);
+	}
+	// fragment of rows row0 .. row0 + 15, all 32 k: lane l has row l & 15 and k = 8 (l >> 4) .. + 7
+	static __device__ __forceinline__ i32x4 frag(const lds_char* lds, int row0, int lane) {
+		static_assert(BK == 32, "one k-block a step");
 		if (LAY == KC) {
-			const int r = row0 + (lane & 31), c = (ks * 2 + (lane >> 5)) ^ ((lane >> 1) & 7);
-			return *(const __attribute__((address_space(3))) i32x4*)(lds + r * 128 + c * 16);
+			const int r = row0 + (lane & 15), c = (lane >> 4) ^ swizzle(lane & 15);
+			return *(const __attribute__((address_space(3))) i32x4*)(lds + r * 64 + c * 16);
 		}
-		const int k = ks * 16 + 8 * (lane >> 5) + ((lane & 15) >> 2), c = row0 / 8 + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-		const lds_char* p = lds + k * (CHUNKS * 16) + (c ^ swizzle((lane & 15) >> 2)) * 16 + (lane & 1) * 8;   // k & 3 = (lane & 15) >> 2 (CHUNKS < 16: only bit 1 counts)
+		const int k = 8 * (lane >> 4) + ((lane & 15) >> 2), c = row0 / 8 + ((lane & 3) >> 1);   // the four lanes of a k bring 16 rows; k + 4 has the same swizzle
+		const lds_char* p = lds + k * (CHUNKS * 16) + (c ^ swizzle(k)) * 16 + (lane & 1) * 8;
 		const i32x2 lo = __builtin_bit_cast(i32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p));
 		const i32x2 hi = __builtin_bit_cast(i32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(p + 4 * CHUNKS * 16)));
 		return i32x4{lo.x, lo.y, hi.x, hi.y};
 	}
 };
 
-// LDS of `STAGES` steps and the product's main loop.  NM N-side matrices of BN rows each share one M-side tile of BM rows (gate and up projection: NM = 2).
-// WN x WM waves; a wave owns BN / WN rows of every N-side matrix and BM / WM rows of the M side.
+// The product's main loop.  NM N-side matrices of BN rows each share one M-side tile of BM rows (gate and up projection: NM = 2).  WN x WM waves; a wave owns BN / WN rows of every
+// N-side matrix and BM / WM rows of the M side.
 template <class T, int NLAY, int MLAY, int NM, int BN, int BM, int WN, int WM>
 struct Product {
-	static constexpr int THREADS = 64 * WN * WM, NB = BN / WN / 32, MB = BM / WM / 32;
-	using NT = Tile<NLAY, BN, THREADS>;
-	using MT = Tile<MLAY, BM, THREADS>;
-	static constexpr int STAGE_BYTES = NM * NT::BYTES + MT::BYTES, LDS_BYTES = 2 * STAGE_BYTES;
+	static constexpr int BK = 32, STAGES = 4;
+	static constexpr int THREADS = 64 * WN * WM, NB = BN / WN / 16, MB = BM / WM / 16, HALF = NM * NB / 2;
+	using NT = Tile<NLAY, BN, THREADS, BK>;
+	using MT = Tile<MLAY, BM, THREADS, BK>;
+	static constexpr int STAGE_BYTES = NM * NT::BYTES + MT::BYTES, LDS_BYTES = STAGES * STAGE_BYTES;
+	static constexpr int LOADS = NM * NT::LOADS + MT::LOADS, EARLY = LOADS / 2;   // a step's DMA: the first EARLY beside its first half of MFMAs, the others beside its second
 
-	// acc[j][nb][mb] += the product over `k` (in steps of 64) of rows n0.. of n[j] and m0.. of m.  Every thread of the workgroup calls it; LDS is free again on return
-	// of the last wave (a barrier stands at the start of each call and step).
-	static __device__ __forceinline__ void run(f32x16 (&acc)[NM][NB][MB], const Mat* n, const Mat& m, uint32_t n0, uint32_t m0, uint32_t k0, uint32_t k1, lds_char* lds) {
+	// acc[j][nb][mb] += the product over k0 .. k1 of rows n0.. of n[j] and m0.. of m.  Every thread of the workgroup calls it; LDS is
+	// free again on return.
+	static __device__ __forceinline__ void run(f32x4 (&acc)[NM][NB][MB], const Mat* n, const Mat& m, uint32_t n0, uint32_t m0, uint32_t k0, uint32_t k1, lds_char* lds) {
 		const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wn = wave % WN, wm = wave / WN;
 		NT nt[NM];
 		MT mt;
@@ -141,35 +161,77 @@ struct Product {
 			mt.base += skip * mt.step_bytes; mt.left -= skip * mt.step_bytes; mt.k_left -= (int)k0;
 		}
 		const int steps = (int)((k1 - k0 + BK - 1) / BK);
-		auto issue = [&](int stage) {
-			lds_char* p = lds + stage * STAGE_BYTES;
+		// Steps are issued without end (those behind the last one would bring the next split's or, behind the operand, zeros: nothing reads them), so that the count of DMA in flight is
+		// the same in every step and the waits can be counted.
+		i32x4 rn[NM], rm;
+		int ahead = 0;
+		lds_char* to = lds;
+		auto next_step = [&]() {
 #pragma unroll
-			for (int j = 0; j < NM; ++j) nt[j].issue(p + j * NT::BYTES, wave);
-			mt.issue(p + NM * NT::BYTES, wave);
+			for (int j = 0; j < NM; ++j) rn[j] = nt[j].next();
+			rm = mt.next();
+			to = lds + (ahead & (STAGES - 1)) * STAGE_BYTES;
+			++ahead;
 		};
-		wait_and_sync();   // the LDS may still be read by what ran before
-		issue(0);
-		for (int s = 0; s < steps; ++s) {
-			wait_and_sync();   // this step's tiles have landed; the other buffer has been read
-			if (s + 1 < steps) issue((s + 1) & 1);
-			const lds_char* p = lds + (s & 1) * STAGE_BYTES;
+		auto issue = [&](int i) {   // i is a constant where it is called
+			if (i < NM * NT::LOADS) nt[i / NT::LOADS].issue(rn[i / NT::LOADS], i % NT::LOADS, to + (i / NT::LOADS) * NT::BYTES, wave);
+			else mt.issue(rm, i - NM * NT::LOADS, to + NM * NT::BYTES, wave);
+		};
+		i32x4 fm[2][MB], fn[2][HALF];   // M side of this step and the next; N side of this half and the next
+		auto read_m = [&](int set, const lds_char* p) {
 #pragma unroll
-			for (int ks = 0; ks < BK / 16; ++ks) {
-				i32x4 fm[MB];
+			for (int b = 0; b < MB; ++b) fm[set][b] = MT::frag(p + NM * NT::BYTES, wm * (BM / WM) + b * 16, lane);
+		};
+		auto read_n = [&](int half, const lds_char* p) {
 #pragma unroll
-				for (int b = 0; b < MB; ++b) fm[b] = MT::frag(p + NM * NT::BYTES, wm * (BM / WM) + b * 32, ks, lane);
-#pragma unroll
-				for (int j = 0; j < NM; ++j) {
-					i32x4 fn[NB];
-#pragma unroll
-					for (int b = 0; b < NB; ++b) fn[b] = NT::frag(p + j * NT::BYTES, wn * (BN / WN) + b * 32, ks, lane);
-#pragma unroll
-					for (int b = 0; b < NB; ++b)
-#pragma unroll
-						for (int c = 0; c < MB; ++c) acc[j][b][c] = mfma<T>(fn[b], fm[c], acc[j][b][c]);
-				}
+			for (int i = 0; i < HALF; ++i) {
+				const int u = half * HALF + i;
+				fn[half][i] = NT::frag(p + u / NB * NT::BYTES, wn * (BN / WN) + u % NB * 16, lane);
 			}
+		};
+		// half a step's MFMAs, with DMA first .. last - 1 spread between them
+		auto multiply = [&](int half, int set, int first, int last) {
+			constexpr int COUNT = HALF * MB;
+			__builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+			for (int i = 0; i < COUNT; ++i) {
+				const int u = half * HALF + i / MB, c = i % MB;
+				acc[u / NB][u % NB][c] = mfma16<T>(fn[half][i / MB], fm[set][c], acc[u / NB][u % NB][c]);
+#pragma unroll
+				for (int d = first; d < last; ++d)
+					if ((d - first) * COUNT / (last - first) + 1 == i) {
+						__builtin_amdgcn_sched_barrier(0);
+						issue(d);
+						__builtin_amdgcn_sched_barrier(0);
+					}
+			}
+			__builtin_amdgcn_sched_barrier(0);
+		};
+#pragma unroll
+		for (int s = 0; s < STAGES - 1; ++s) {
+			next_step();
+#pragma unroll
+			for (int i = 0; i < LOADS; ++i) issue(i);
 		}
+		wait_and_sync<(STAGES - 2) * LOADS>();
+		read_m(0, lds);
+		read_n(0, lds);
+		auto step = [&](int s, int set) {   // set: s & 1, a constant
+			next_step();
+			read_n(1, lds + (s & (STAGES - 1)) * STAGE_BYTES);
+			multiply(0, set, 0, EARLY);
+			wait_and_sync<(STAGES - 3) * LOADS + EARLY>();   // the next step has landed, this one has been read: its buffer is the next to be filled
+			read_m(set ^ 1, lds + ((s + 1) & (STAGES - 1)) * STAGE_BYTES);   // behind the last step: not used
+			read_n(0, lds + ((s + 1) & (STAGES - 1)) * STAGE_BYTES);
+			multiply(1, set, EARLY, LOADS);
+		};
+		int s = 0;
+		for (; s + 1 < steps; s += 2) {
+			step(s, 0);
+			step(s + 1, 1);
+		}
+		if (s < steps) step(s, 0);
+		wait_and_sync();   // the DMA behind the last step too: LDS may belong to another workgroup next
 	}
 };
 
@@ -192,25 +254,21 @@ __device__ __forceinline__ void tile_of(uint32_t pid, uint32_t total, uint32_t t
 // ---- epilogue ----------------------------------------------------------------------------------------------------------------------------
 template <class T> struct Out { T* p; uint64_t ld; uint32_t rows, cols; };   // row-major; columns are the N side
 
-// A wave brings 32 rows x NBLK * 32 columns of results into row order through LDS of its own (Rows<NBLK>::BYTES), so that a row's columns leave in 16-byte pieces: put_block rounds one
-// 32 x 32 block (once, to nearest even) into it, store_rows writes the rows.  Register layout of a block: lane l holds column m = l & 31 and rows n = 8 (i >> 2) + 4 (l >> 5) + (i & 3).
+// A wave brings 32 rows x NBLK * 16 columns of results into row order through LDS of its own (Rows<NBLK>::BYTES), so that a row's columns leave in 16-byte pieces: put_block rounds a
+// 16 x 16 block (once, to nearest even) into it, store_rows writes the rows.  Register layout of a block: lane l holds row m = l & 15 and columns n = 4 (l >> 4) .. + 3.
 // The wave's own LDS operations are in order: no barrier between the two.
-template <int NBLK> struct Rows { static constexpr int PITCH = NBLK * 64 + 16, BYTES = 32 * PITCH; };
+template <int NBLK> struct Rows { static constexpr int PITCH = NBLK * 32 + 16, BYTES = 32 * PITCH; };
 
 template <class T, int NBLK>
-__device__ __forceinline__ void put_block(const f32x16& v, int b, lds_char* lds, int lane) {
+__device__ __forceinline__ void put_block(const f32x4& v, int b, int upper, lds_char* lds, int lane) {   // block b of the row; upper: rows 16 .. 31
 	typedef T t4 __attribute__((ext_vector_type(4)));
-#pragma unroll
-	for (int q = 0; q < 4; ++q) {
-		const t4 h = {(T)v[4 * q], (T)v[4 * q + 1], (T)v[4 * q + 2], (T)v[4 * q + 3]};
-		*(__attribute__((address_space(3))) t4*)(lds + (lane & 31) * Rows<NBLK>::PITCH + (b * 32 + q * 8 + 4 * (lane >> 5)) * 2) = h;
-	}
+	*(__attribute__((address_space(3))) t4*)(lds + (upper * 16 + (lane & 15)) * Rows<NBLK>::PITCH + (b * 16 + 4 * (lane >> 4)) * 2) = t4{(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
 }
 
 template <class T, int NBLK>
 __device__ __forceinline__ void store_rows(const Out<T>& o, uint32_t n0, uint32_t m0, const lds_char* lds, int lane) {
 	typedef T t8 __attribute__((ext_vector_type(8)));
-	constexpr int PIECES = NBLK * 4, ROWS = 64 / PIECES;
+	constexpr int PIECES = NBLK * 2, ROWS = 64 / PIECES;
 	const bool wide = (((uint64_t)o.p | (o.ld * 2)) & 15) == 0;
 	const int piece = lane % PIECES;
 	const uint32_t n = n0 + piece * 8;

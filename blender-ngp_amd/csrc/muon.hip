@@ -134,7 +134,8 @@ __global__ void __launch_bounds__(256) split_kernel(Jobs jobs, Step s) {
 // ---- products of split matrices ------------------------------------------------------------------------------------------------------------
 
 struct Shape { static constexpr int N = 128, M = 128, WN = 2, WM = 2, THREADS = 256; };
-using T = Tile<KC, 128, 256>;
+constexpr int BK = 64;   // 32 k, both halves
+using T = Tile<KC, 128, 256, BK>;
 constexpr int NB = 2, MB = 2;
 
 // acc[nb][mb] = rows n0 .. of n times rows m0 .. of m; steps of 32 k
@@ -151,8 +152,12 @@ __device__ __forceinline__ void split_product(f32x16 (&acc)[NB][MB], const Mat& 
 	mt.init(m, m0, tid);
 	const int steps = (int)(n.k / BK);
 	auto issue = [&](int stage) {
-		nt.issue(lds + stage * 2 * T::BYTES, wave);
-		mt.issue(lds + stage * 2 * T::BYTES + T::BYTES, wave);
+		const i32x4 rn = nt.next(), rm = mt.next();
+#pragma unroll
+		for (int i = 0; i < T::LOADS; ++i) {
+			nt.issue(rn, i, lds + stage * 2 * T::BYTES, wave);
+			mt.issue(rm, i, lds + stage * 2 * T::BYTES + T::BYTES, wave);
+		}
 	};
 	issue(0);
 	for (int s = 0; s < steps; ++s) {
@@ -163,9 +168,9 @@ __device__ __forceinline__ void split_product(f32x16 (&acc)[NB][MB], const Mat& 
 		for (int ks = 0; ks < 2; ++ks) {
 			i32x4 nh[NB], nl[NB], mh[MB], ml[MB];
 #pragma unroll
-			for (int b = 0; b < NB; ++b) { nh[b] = T::frag(p, wn * 64 + b * 32, ks, lane); nl[b] = T::frag(p, wn * 64 + b * 32, ks + 2, lane); }
+			for (int b = 0; b < NB; ++b) { nh[b] = T::frag32(p, wn * 64 + b * 32, ks, lane); nl[b] = T::frag32(p, wn * 64 + b * 32, ks + 2, lane); }
 #pragma unroll
-			for (int b = 0; b < MB; ++b) { mh[b] = T::frag(p + T::BYTES, wm * 64 + b * 32, ks, lane); ml[b] = T::frag(p + T::BYTES, wm * 64 + b * 32, ks + 2, lane); }
+			for (int b = 0; b < MB; ++b) { mh[b] = T::frag32(p + T::BYTES, wm * 64 + b * 32, ks, lane); ml[b] = T::frag32(p + T::BYTES, wm * 64 + b * 32, ks + 2, lane); }
 #pragma unroll
 			for (int a = 0; a < NB; ++a)
 #pragma unroll
