@@ -25,7 +25,7 @@ using namespace mm;
 
 constexpr float SX = 32768.0f, SA = 8192.0f;                      // scales of X and of A, B
 constexpr float NS_A = 3.4445f, NS_B = -4.7750f, NS_C = 2.0315f;
-constexpr uint32_t MAX_JOBS = 24, MAX_SIDE = 65536, SUM_BLOCKS = 256;
+constexpr uint32_t MAX_JOBS = 24, MAX_SIDE = 65536, SUM_BLOCKS = 1024;
 
 struct Job {
 	uint64_t offset;                    // of the matrix in the parameter vector, in elements
@@ -37,7 +37,7 @@ struct Job {
 enum { START_SUM, START_SPLIT, START_SYM, START_APPLY, N_STARTS };
 struct Jobs {
 	Job job[MAX_JOBS];
-	uint32_t start[N_STARTS][MAX_JOBS + 1];   // first workgroup of each job, per kind of kernel
+	uint32_t start[N_STARTS][MAX_JOBS + 1];   // first workgroup of each job, per kind of kernel (the products': of the tile chosen by use_tile)
 	uint32_t count;
 };
 
@@ -60,6 +60,14 @@ __device__ __forceinline__ float load_grad(const Step& s, uint64_t i) {
 	return g * s.inv_loss_scale;
 }
 
+__device__ __forceinline__ void update_weight(const Step& s, uint64_t at, float keep, float change) {
+	const float w = keep * s.master[at] - change;
+	s.master[at] = w;
+	if (!s.params) return;
+	if (s.dtype == NGP_DTYPE_F16) ((f16*)s.params)[at] = (f16)w;
+	else ((b16*)s.params)[at] = (b16)w;
+}
+
 __device__ __forceinline__ double block_sum(double v, double* lds) {   // 256 threads, a fixed order
 	for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
 	if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
@@ -69,16 +77,41 @@ __device__ __forceinline__ double block_sum(double v, double* lds) {   // 256 th
 	return v;
 }
 
-// m <- beta m + g, and the squares of u.  In 64 bits: gradients of single precision may square to what fp32 cannot hold.
+// four gradients from i on (i and the vector's base aligned to four elements)
+__device__ __forceinline__ f32x4 load_grad4(const Step& s, uint64_t i) {
+	typedef f16 h4 __attribute__((ext_vector_type(4)));
+	typedef b16 b4 __attribute__((ext_vector_type(4)));
+	f32x4 g;
+	if (s.dtype == NGP_DTYPE_F32) g = *(const f32x4*)((const float*)s.grads + i);
+	else if (s.dtype == NGP_DTYPE_F16) g = __builtin_convertvector(*(const h4*)((const f16*)s.grads + i), f32x4);
+	else g = __builtin_convertvector(*(const b4*)((const b16*)s.grads + i), f32x4);
+	return g * s.inv_loss_scale;
+}
+
+// m <- beta m + g, and the squares of u.  In 64 bits: gradients of single precision may square to what fp32 cannot hold.  Bound by memory: 10 bytes an element of 16-bit gradients.
 __global__ void __launch_bounds__(256) momentum_kernel(Jobs jobs, Step s) {
 	__shared__ double lds[4];
 	uint32_t pid = blockIdx.x;
 	const uint32_t ji = job_of(jobs, START_SUM, pid);
 	const Job& j = jobs.job[ji];
 	const uint32_t blocks = jobs.start[START_SUM][ji + 1] - jobs.start[START_SUM][ji];
-	const uint64_t total = (uint64_t)j.rows * j.cols;
+	const uint64_t total = (uint64_t)j.rows * j.cols, step = (uint64_t)blocks * 256;
+	const bool wide = ((j.offset & 3) | ((uintptr_t)s.buffer & 15) | ((uintptr_t)s.grads & (s.dtype == NGP_DTYPE_F32 ? 15 : 7))) == 0;
+	const uint64_t quads = wide ? total / 4 : 0;
 	double sum = 0.0;
-	for (uint64_t i = (uint64_t)pid * 256 + threadIdx.x; i < total; i += (uint64_t)blocks * 256) {
+	for (uint64_t q = (uint64_t)pid * 256 + threadIdx.x; q < quads; q += step) {
+		const uint64_t i = j.offset + 4 * q;
+		const f32x4 g = load_grad4(s, i), old = *(const f32x4*)(s.buffer + i);
+		f32x4 m;
+#pragma unroll
+		for (int e = 0; e < 4; ++e) {
+			m[e] = s.momentum * old[e] + g[e];
+			const double u = s.nesterov ? g[e] + s.momentum * m[e] : m[e];
+			sum += u * u;
+		}
+		*(f32x4*)(s.buffer + i) = m;
+	}
+	for (uint64_t i = 4 * quads + (uint64_t)pid * 256 + threadIdx.x; i < total; i += step) {
 		const float g = load_grad(s, j.offset + i), m = s.momentum * s.buffer[j.offset + i] + g;
 		s.buffer[j.offset + i] = m;
 		const double u = s.nesterov ? g + s.momentum * m : m;
@@ -99,7 +132,9 @@ __global__ void __launch_bounds__(256) split_kernel(Jobs jobs, Step s) {
 	const uint32_t ji = job_of(jobs, START_SPLIT, pid);
 	const Job& j = jobs.job[ji];
 	const uint32_t blocks = jobs.start[START_SUM][ji + 1] - jobs.start[START_SUM][ji];
-	const double sum = block_sum(threadIdx.x < blocks ? j.sums[threadIdx.x] : 0.0, lds);
+	double mine = 0.0;
+	for (uint32_t i = threadIdx.x; i < blocks; i += 256) mine += j.sums[i];
+	const double sum = block_sum(mine, lds);
 	const double norm = sqrt(sum) + (double)s.eps, scale = norm == 0.0 ? 0.0 : (double)SX / norm;   // a zero update stays zero also without eps
 	const uint32_t tiles_k = (j.kp + 63) / 64, m0 = pid / tiles_k * 64, n0 = pid % tiles_k * 64;
 	const bool turn = j.rows > j.cols;   // X = u^T
@@ -133,158 +168,220 @@ __global__ void __launch_bounds__(256) split_kernel(Jobs jobs, Step s) {
 
 // ---- products of split matrices ------------------------------------------------------------------------------------------------------------
 
-struct Shape { static constexpr int N = 128, M = 128, WN = 2, WM = 2, THREADS = 256; };
-constexpr int BK = 64;   // 32 k, both halves
-using T = Tile<KC, 128, 256, BK>;
-constexpr int NB = 2, MB = 2;
-
-// acc[nb][mb] = rows n0 .. of n times rows m0 .. of m; steps of 32 k
-__device__ __forceinline__ void split_product(f32x16 (&acc)[NB][MB], const Mat& n, const Mat& m, uint32_t n0, uint32_t m0, lds_char* lds) {
-	const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wn = wave % Shape::WN, wm = wave / Shape::WN;
-#pragma unroll
-	for (int a = 0; a < NB; ++a)
-#pragma unroll
-		for (int b = 0; b < MB; ++b)
-#pragma unroll
-			for (int i = 0; i < 16; ++i) acc[a][b][i] = 0.0f;
-	T nt, mt;
-	nt.init(n, n0, tid);
-	mt.init(m, m0, tid);
-	const int steps = (int)(n.k / BK);
-	auto issue = [&](int stage) {
-		const i32x4 rn = nt.next(), rm = mt.next();
-#pragma unroll
-		for (int i = 0; i < T::LOADS; ++i) {
-			nt.issue(rn, i, lds + stage * 2 * T::BYTES, wave);
-			mt.issue(rm, i, lds + stage * 2 * T::BYTES + T::BYTES, wave);
-		}
-	};
-	issue(0);
-	for (int s = 0; s < steps; ++s) {
-		wait_and_sync();
-		if (s + 1 < steps) issue((s + 1) & 1);
-		const lds_char* p = lds + (s & 1) * 2 * T::BYTES;
-#pragma unroll
-		for (int ks = 0; ks < 2; ++ks) {
-			i32x4 nh[NB], nl[NB], mh[MB], ml[MB];
-#pragma unroll
-			for (int b = 0; b < NB; ++b) { nh[b] = T::frag32(p, wn * 64 + b * 32, ks, lane); nl[b] = T::frag32(p, wn * 64 + b * 32, ks + 2, lane); }
-#pragma unroll
-			for (int b = 0; b < MB; ++b) { mh[b] = T::frag32(p + T::BYTES, wm * 64 + b * 32, ks, lane); ml[b] = T::frag32(p + T::BYTES, wm * 64 + b * 32, ks + 2, lane); }
-#pragma unroll
-			for (int a = 0; a < NB; ++a)
-#pragma unroll
-				for (int b = 0; b < MB; ++b) {
-					acc[a][b] = mfma<f16>(nl[a], mh[b], acc[a][b]);
-					acc[a][b] = mfma<f16>(nh[a], ml[b], acc[a][b]);
-					acc[a][b] = mfma<f16>(nh[a], mh[b], acc[a][b]);
-				}
-		}
-	}
-}
-
 typedef f16 f16x4 __attribute__((ext_vector_type(4)));
 
-// a 32 x 32 block into a split matrix, as it lies (row m) and / or transposed (row n); lane layout: matmul_mfma.cuh store_rows
-__device__ __forceinline__ void store_split(const f32x16& v, f16* p, uint32_t cols2, uint32_t rows, uint32_t cols, f16* pt, uint32_t colst2, uint32_t rowst, uint32_t colst, uint32_t n0, uint32_t m0, int lane) {
-	const uint32_t m = m0 + (lane & 31);
+// acc[nb][mb] = rows n0 .. of n times rows m0 .. of m (16 x 16 blocks), in steps of 32 k: 64 columns, both halves.  A ring of STAGES buffers, DMA spread between the MFMAs, counted
+// waits: the scheme of mm::Product, with three MFMAs to a pair of fragments' halves.
+template <int BN, int BM, int WN, int WM, int STAGES>
+struct SplitProduct {
+	static constexpr int THREADS = 64 * WN * WM, NB = BN / WN / 16, MB = BM / WM / 16, N = BN, M = BM, WAVES_N = WN, WAVES_M = WM;
+	using NT = Tile<KC, BN, THREADS, 64>;
+	using MT = Tile<KC, BM, THREADS, 64>;
+	static constexpr int STAGE_BYTES = NT::BYTES + MT::BYTES, LOADS = NT::LOADS + MT::LOADS, LDS_BYTES = STAGES * STAGE_BYTES;
+	static_assert(LDS_BYTES >= WN * WM * 32 * 144, "the epilogue's rows");
+
+	// rows row0 .. + 15, half 0 (hi) or 1 (lo): lane l has row l & 15 and k = 8 (l >> 4) .. + 7
+	template <class TT> static __device__ __forceinline__ i32x4 frag(const lds_char* p, int row0, int half, int lane) {
+		return *(const __attribute__((address_space(3))) i32x4*)(p + (row0 + (lane & 15)) * 128 + ((half * 4 + (lane >> 4)) ^ TT::swizzle(lane & 15)) * 16);
+	}
+	static __device__ __forceinline__ void run(f32x4 (&acc)[NB][MB], const Mat& n, const Mat& m, uint32_t n0, uint32_t m0, lds_char* lds) {
+		const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wn = wave % WN, wm = wave / WN;
 #pragma unroll
-	for (int q = 0; q < 4; ++q) {
-		const uint32_t n = n0 + 8 * q + 4 * (lane >> 5);
-		f16x4 hi, lo;
+		for (int a = 0; a < NB; ++a)
 #pragma unroll
-		for (int e = 0; e < 4; ++e) { f16 h, l; split2(v[4 * q + e], h, l); hi[e] = h; lo[e] = l; }
-		if (p && m < rows && n < cols) {   // cols is a multiple of 32: a quad never straddles it
-			f16* d = p + (uint64_t)m * cols2 + split_col(n);
-			*(f16x4*)d = hi; *(f16x4*)(d + 32) = lo;
+			for (int b = 0; b < MB; ++b) acc[a][b] = f32x4{0, 0, 0, 0};
+		NT nt;
+		MT mt;
+		nt.init(n, n0, tid);
+		mt.init(m, m0, tid);
+		const int steps = (int)(n.k / 64);
+		i32x4 rn, rm;
+		int slot = 0;
+		lds_char* to = lds;
+		auto next_step = [&]() {
+			rn = nt.next();
+			rm = mt.next();
+			to = lds + slot * STAGE_BYTES;
+			slot = slot + 1 == STAGES ? 0 : slot + 1;
+		};
+		auto issue = [&](int i) {
+			if (i < NT::LOADS) nt.issue(rn, i, to, wave);
+			else mt.issue(rm, i - NT::LOADS, to + NT::BYTES, wave);
+		};
+#pragma unroll
+		for (int s = 0; s < STAGES - 1; ++s) {   // the steps behind the last one read zeros
+			next_step();
+#pragma unroll
+			for (int i = 0; i < LOADS; ++i) issue(i);
 		}
-		if (pt && m < colst)
+		int at = 0;
+		for (int s = 0; s < steps; ++s) {
+			wait_and_sync<(STAGES - 2) * LOADS>();   // this step has landed; the one before has been read
+			const lds_char* p = lds + at * STAGE_BYTES;
+			at = at + 1 == STAGES ? 0 : at + 1;
+			next_step();
+			i32x4 mh[MB], ml[MB], nh[NB], nl[NB];
 #pragma unroll
-			for (int e = 0; e < 4; ++e)
-				if (n + e < rowst) {
-					f16* d = pt + (uint64_t)(n + e) * colst2 + split_col(m);
-					d[0] = hi[e]; d[32] = lo[e];
+			for (int b = 0; b < MB; ++b) mh[b] = frag<MT>(p + NT::BYTES, wm * (BM / WM) + b * 16, 0, lane);
+#pragma unroll
+			for (int b = 0; b < NB; ++b) nh[b] = frag<NT>(p, wn * (BN / WN) + b * 16, 0, lane);
+#pragma unroll
+			for (int b = 0; b < MB; ++b) ml[b] = frag<MT>(p + NT::BYTES, wm * (BM / WM) + b * 16, 1, lane);
+#pragma unroll
+			for (int b = 0; b < NB; ++b) nl[b] = frag<NT>(p, wn * (BN / WN) + b * 16, 1, lane);
+			constexpr int COUNT = NB * MB;
+#pragma unroll
+			for (int part = 0; part < 3; ++part)
+#pragma unroll
+				for (int i = 0; i < COUNT; ++i) {
+					const int a = i / MB, b = i % MB;
+					acc[a][b] = part == 0 ? mfma16<f16>(nh[a], mh[b], acc[a][b]) : part == 1 ? mfma16<f16>(nh[a], ml[b], acc[a][b]) : mfma16<f16>(nl[a], mh[b], acc[a][b]);
+#pragma unroll
+					for (int d = 0; d < LOADS; ++d)
+						if (d * (2 * COUNT) / LOADS == part * COUNT + i) {   // within the first two thirds
+							__builtin_amdgcn_sched_barrier(0);
+							issue(d);
+							__builtin_amdgcn_sched_barrier(0);
+						}
 				}
+		}
+		wait_and_sync();   // the DMA behind the last step too
+	}
+};
+using Large = SplitProduct<128, 256, 2, 4, 3>;   // 144 KB of LDS
+using Middle = SplitProduct<128, 128, 4, 2, 4>;  // 128 KB
+using Little = SplitProduct<64, 64, 2, 2, 4>;    // 64 KB: two workgroups a CU
+
+// A wave's 32 x 32 block (2 x 2 of 16) of a split matrix, through LDS of its own (32 rows of 144 bytes) into rows of 64 hi and 64 lo bytes: as it lies (rows m), or transposed (rows n)
+__device__ __forceinline__ void put_split(const f32x4& v, bool turned, int nb, int mb, lds_char* lds, int lane) {   // block nb, mb of the four
+	typedef __attribute__((address_space(3))) f16x4 lds_f16x4;
+	typedef __attribute__((address_space(3))) f16 lds_f16;
+	f16x4 hi, lo;
+#pragma unroll
+	for (int e = 0; e < 4; ++e) { f16 h, l; split2(v[e], h, l); hi[e] = h; lo[e] = l; }
+	const int m = mb * 16 + (lane & 15), n = nb * 16 + 4 * (lane >> 4);
+	if (!turned) {
+		*(lds_f16x4*)(lds + m * 144 + n * 2) = hi;
+		*(lds_f16x4*)(lds + m * 144 + 64 + n * 2) = lo;
+	} else
+#pragma unroll
+		for (int e = 0; e < 4; ++e) {
+			*(lds_f16*)(lds + (n + e) * 144 + m * 2) = hi[e];
+			*(lds_f16*)(lds + (n + e) * 144 + 64 + m * 2) = lo[e];
+		}
+}
+// rows row0 .. + 31 below `rows`, columns col0 .. + 31 (all below `cols` or none) of the split matrix p with rows of `pitch` elements
+__device__ __forceinline__ void write_split(f16* p, uint32_t pitch, uint32_t rows, uint32_t cols, uint32_t row0, uint32_t col0, const lds_char* lds, int lane) {
+	if (col0 >= cols) return;
+#pragma unroll
+	for (int r = 0; r < 32; r += 8) {
+		const uint32_t row = row0 + r + (lane >> 3);
+		const i32x4 q = *(const __attribute__((address_space(3))) i32x4*)(lds + (r + (lane >> 3)) * 144 + (lane & 7) * 16);
+		if (row < rows) *(i32x4*)(p + (uint64_t)row * pitch + (uint64_t)col0 * 2 + (lane & 7) * 8) = q;
 	}
 }
 
-// A = X X^T (POLY 0), or B = a I + b A + c A^2 (POLY 1): tiles on and below the diagonal
-template <int POLY>
-__global__ void __launch_bounds__(256, 2) symmetric_kernel(Jobs jobs) {
-	__shared__ __attribute__((aligned(1024))) char lds[4 * T::BYTES];
+// Tiles that hold an element on or below the diagonal, by rows of tiles; a tile row's last tiles (M / N of them) are its square on the diagonal, whole, the others are written twice.
+template <class P> __host__ __device__ inline uint32_t symmetric_tiles(uint32_t n) {
+	const uint32_t tm = (n + P::M - 1) / P::M, tn = (n + P::N - 1) / P::N, r = P::M / P::N;
+	uint32_t t = 0;
+	for (uint32_t i = 0; i < tm; ++i) t += r * (i + 1) < tn ? r * (i + 1) : tn;
+	return t;
+}
+
+// A = X X^T (POLY 0), or B = a I + b A + c A^2 (POLY 1)
+template <class P, int POLY>
+__global__ void __launch_bounds__(P::THREADS, P::LDS_BYTES <= 80 * 1024 ? 2 : 1) symmetric_kernel(Jobs jobs) {
+	__shared__ __attribute__((aligned(1024))) char lds[P::LDS_BYTES];
 	uint32_t pid = xcd_order(blockIdx.x, gridDim.x);
 	const Job& j = jobs.job[job_of(jobs, START_SYM, pid)];
-	uint32_t tm = (uint32_t)((sqrtf(8.0f * pid + 1.0f) - 1.0f) * 0.5f);
-	while (tm * (tm + 1) / 2 > pid) --tm;
-	while ((tm + 1) * (tm + 2) / 2 <= pid) ++tm;
-	const uint32_t tn = pid - tm * (tm + 1) / 2;
+	constexpr uint32_t R = P::M / P::N;
+	uint32_t tm = 0;
+	for (uint32_t t = pid;; ++tm) {   // tile rows of R, 2 R, 3 R ... tiles
+		if (t < R * (tm + 1)) { pid = t; break; }
+		t -= R * (tm + 1);
+	}
+	const uint32_t tn = pid;
 	const uint32_t width = 2 * (POLY ? j.np : j.kp);
 	const Mat mat{POLY ? j.a : j.x, width, j.n, width};
-	f32x16 acc[NB][MB];
-	split_product(acc, mat, mat, tn * 128, tm * 128, lds_of(lds));
-	const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wn = wave % Shape::WN, wm = wave / Shape::WN;
+	f32x4 acc[P::NB][P::MB];
+	P::run(acc, mat, mat, tn * P::N, tm * P::M, lds_of(lds));
+	const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wn = wave % P::WAVES_N, wm = wave / P::WAVES_N;
+	lds_char* mine = lds_of(lds) + wave * (32 * 144);
+	f16* const out = POLY ? j.b : j.a;
+	const bool twice = tn < tm * R;
 #pragma unroll
-	for (int a = 0; a < NB; ++a)
+	for (int a = 0; a < P::NB; a += 2)
 #pragma unroll
-		for (int b = 0; b < MB; ++b) {
-			const uint32_t n0 = tn * 128 + wn * 64 + a * 32, m0 = tm * 128 + wm * 64 + b * 32, m = m0 + (lane & 31);
-			f32x16 v;
+		for (int b = 0; b < P::MB; b += 2) {
+			const uint32_t n0 = tn * P::N + wn * (P::NB * 16) + a * 16, m0 = tm * P::M + wm * (P::MB * 16) + b * 16;
+			f32x4 v[2][2];
 #pragma unroll
-			for (int q = 0; q < 4; ++q) {
-				const uint32_t n = n0 + 8 * q + 4 * (lane >> 5);
-				f16x4 hi = {0, 0, 0, 0}, lo = {0, 0, 0, 0};
-				if (POLY && m < j.n && n < j.np) {
-					const f16* d = j.a + (uint64_t)m * 2 * j.np + split_col(n);
-					hi = *(const f16x4*)d; lo = *(const f16x4*)(d + 32);
+			for (int x = 0; x < 2; ++x)
+#pragma unroll
+				for (int y = 0; y < 2; ++y) {
+					v[x][y] = acc[a + x][b + y];
+					if (POLY) {
+						const uint32_t m = m0 + y * 16 + (lane & 15), n = n0 + x * 16 + 4 * (lane >> 4);
+						f16x4 hi = {0, 0, 0, 0}, lo = {0, 0, 0, 0};
+						if (m < j.n && n < j.np) {
+							const f16* d = j.a + (uint64_t)m * 2 * j.np + split_col(n);
+							hi = *(const f16x4*)d; lo = *(const f16x4*)(d + 32);
+						}
+#pragma unroll
+						for (int e = 0; e < 4; ++e) v[x][y][e] = NS_C / SA * v[x][y][e] + NS_B * ((float)hi[e] + (float)lo[e]) + (m == n + e && m < j.n ? NS_A * SA : 0.0f);
+					} else v[x][y] *= SA / (SX * SX);
+					put_split(v[x][y], false, x, y, mine, lane);
 				}
+			write_split(out, 2 * j.np, j.n, j.np, m0, n0, mine, lane);
+			if (!twice) continue;
 #pragma unroll
-				for (int e = 0; e < 4; ++e) {
-					if (POLY) v[4 * q + e] = NS_C / SA * acc[a][b][4 * q + e] + NS_B * ((float)hi[e] + (float)lo[e]) + (m == n + e && m < j.n ? NS_A * SA : 0.0f);
-					else v[4 * q + e] = acc[a][b][4 * q + e] * (SA / (SX * SX));
-				}
-			}
-			f16* const out = POLY ? j.b : j.a;
-			store_split(v, out, 2 * j.np, j.n, j.np, tm != tn ? out : nullptr, 2 * j.np, j.n, j.np, n0, m0, lane);
+			for (int x = 0; x < 2; ++x)
+#pragma unroll
+				for (int y = 0; y < 2; ++y) put_split(v[x][y], true, x, y, mine, lane);
+			write_split(out, 2 * j.np, j.n, j.np, n0, m0, mine, lane);
 		}
 }
 
 // X <- B X: into both orientations, or (LAST) straight into the weights
-template <int LAST>
-__global__ void __launch_bounds__(256, 2) apply_kernel(Jobs jobs, Step s, int from) {
-	__shared__ __attribute__((aligned(1024))) char lds[4 * T::BYTES];
+template <class P, int LAST>
+__global__ void __launch_bounds__(P::THREADS, P::LDS_BYTES <= 80 * 1024 ? 2 : 1) apply_kernel(Jobs jobs, Step s, int from) {
+	__shared__ __attribute__((aligned(1024))) char lds[P::LDS_BYTES];
 	uint32_t pid = xcd_order(blockIdx.x, gridDim.x);
 	const Job& j = jobs.job[job_of(jobs, START_APPLY, pid)];
-	const uint32_t tiles_m = (j.n + 127) / 128, tm = pid % tiles_m, tn = pid / tiles_m;
-	f32x16 acc[NB][MB];
-	split_product(acc, Mat{j.xt[from], 2ull * j.np, j.k, 2 * j.np}, Mat{j.b, 2ull * j.np, j.n, 2 * j.np}, tn * 128, tm * 128, lds_of(lds));
-	const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wn = wave % Shape::WN, wm = wave / Shape::WN;
+	const uint32_t tiles_m = (j.n + P::M - 1) / P::M, tm = pid % tiles_m, tn = pid / tiles_m;
+	f32x4 acc[P::NB][P::MB];
+	P::run(acc, Mat{j.xt[from], 2ull * j.np, j.k, 2 * j.np}, Mat{j.b, 2ull * j.np, j.n, 2 * j.np}, tn * P::N, tm * P::M, lds_of(lds));
+	const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wn = wave % P::WAVES_N, wm = wave / P::WAVES_N;
+	lds_char* mine = lds_of(lds) + wave * (32 * 144);
 	const bool turn = j.rows > j.cols;
 	const float keep = 1.0f - s.lr * s.decay, rate = s.lr * sqrtf(fmaxf(1.0f, (float)j.rows / (float)j.cols)) / (SA * SX);
 #pragma unroll
-	for (int a = 0; a < NB; ++a)
+	for (int a = 0; a < P::NB; a += 2)
 #pragma unroll
-		for (int b = 0; b < MB; ++b) {
-			const uint32_t n0 = tn * 128 + wn * 64 + a * 32, m0 = tm * 128 + wm * 64 + b * 32, m = m0 + (lane & 31);
+		for (int b = 0; b < P::MB; b += 2) {
+			const uint32_t n0 = tn * P::N + wn * (P::NB * 16) + a * 16, m0 = tm * P::M + wm * (P::MB * 16) + b * 16;
 			if (!LAST) {
-				f32x16 v;
 #pragma unroll
-				for (int i = 0; i < 16; ++i) v[i] = acc[a][b][i] * (1.0f / SA);
-				store_split(v, j.x, 2 * j.kp, j.n, j.kp, j.xt[1 - from], 2 * j.np, j.k, j.np, n0, m0, lane);
+				for (int turned = 0; turned < 2; ++turned) {
+#pragma unroll
+					for (int x = 0; x < 2; ++x)
+#pragma unroll
+						for (int y = 0; y < 2; ++y) put_split(acc[a + x][b + y] * (1.0f / SA), turned, x, y, mine, lane);
+					if (!turned) write_split(j.x, 2 * j.kp, j.n, j.kp, m0, n0, mine, lane);
+					else write_split(j.xt[1 - from], 2 * j.np, j.k, j.np, n0, m0, mine, lane);
+				}
 				continue;
 			}
-			if (m >= j.n) continue;
 #pragma unroll
-			for (int i = 0; i < 16; ++i) {
-				const uint32_t n = n0 + 8 * (i >> 2) + 4 * (lane >> 5) + (i & 3);
-				if (n >= j.k) continue;
-				const uint64_t at = j.offset + (turn ? (uint64_t)n * j.cols + m : (uint64_t)m * j.cols + n);
-				const float w = keep * s.master[at] - rate * acc[a][b][i];
-				s.master[at] = w;
-				if (s.params) {
-					if (s.dtype == NGP_DTYPE_F16) ((f16*)s.params)[at] = (f16)w;
-					else ((b16*)s.params)[at] = (b16)w;
-				}
-			}
+			for (int x = 0; x < 2; ++x)
+#pragma unroll
+				for (int y = 0; y < 2; ++y)
+#pragma unroll
+					for (int e = 0; e < 4; ++e) {
+						const uint32_t m = m0 + y * 16 + (lane & 15), n = n0 + x * 16 + 4 * (lane >> 4) + e;
+						if (m < j.n && n < j.k) update_weight(s, j.offset + (turn ? (uint64_t)n * j.cols + m : (uint64_t)m * j.cols + n), keep, rate * acc[a + x][b + y][e]);
+					}
 		}
 }
 
@@ -323,11 +420,30 @@ static uint64_t lay_out(Jobs& jobs, const NgpMuonMatrix* m, char* base) {
 		j.a = (f16*)take((uint64_t)j.n * j.np * 4);
 		j.b = (f16*)take((uint64_t)j.n * j.np * 4);
 		j.sums = (double*)take(blocks * 8);
-		const uint32_t tn = (j.n + 127) / 128, tk = (j.k + 127) / 128;
-		const uint32_t n[N_STARTS] = {blocks, ((j.np + 63) / 64) * ((j.kp + 63) / 64), tn * (tn + 1) / 2, tn * tk};
-		for (int kind = 0; kind < N_STARTS; ++kind) jobs.start[kind][i + 1] = jobs.start[kind][i] + n[kind];
+		jobs.start[START_SUM][i + 1] = jobs.start[START_SUM][i] + blocks;
+		jobs.start[START_SPLIT][i + 1] = jobs.start[START_SPLIT][i] + ((j.np + 63) / 64) * ((j.kp + 63) / 64);
 	}
 	return used;
+}
+
+template <class P> static void use_tile(Jobs& jobs) {
+	for (uint32_t i = 0; i < jobs.count; ++i) {
+		const Job& j = jobs.job[i];
+		jobs.start[START_SYM][i + 1] = jobs.start[START_SYM][i] + symmetric_tiles<P>(j.n);
+		jobs.start[START_APPLY][i + 1] = jobs.start[START_APPLY][i] + ((j.n + P::M - 1) / P::M) * ((j.k + P::N - 1) / P::N);
+	}
+}
+
+template <class P> static void iterate(hipStream_t st, Jobs& jobs, const Step& s, uint32_t n_iterations) {
+	use_tile<P>(jobs);
+	const uint32_t c = jobs.count;
+	const dim3 block(P::THREADS), sym(jobs.start[START_SYM][c]), apply(jobs.start[START_APPLY][c]);
+	for (uint32_t i = 0; i < n_iterations; ++i) {
+		hipLaunchKernelGGL((symmetric_kernel<P, 0>), sym, block, 0, st, jobs);
+		hipLaunchKernelGGL((symmetric_kernel<P, 1>), sym, block, 0, st, jobs);
+		if (i + 1 < n_iterations) hipLaunchKernelGGL((apply_kernel<P, 0>), apply, block, 0, st, jobs, s, (int)(i & 1));
+		else hipLaunchKernelGGL((apply_kernel<P, 1>), apply, block, 0, st, jobs, s, (int)(i & 1));
+	}
 }
 
 } // namespace muon
@@ -372,12 +488,12 @@ int ngp_hip_muon_step(void* stream, uint32_t n_matrices, const NgpMuonMatrix* ma
 		const uint32_t c = jobs.count;
 		hipLaunchKernelGGL(momentum_kernel, dim3(jobs.start[START_SUM][c]), dim3(256), 0, st, jobs, s);
 		hipLaunchKernelGGL(split_kernel, dim3(jobs.start[START_SPLIT][c]), dim3(256), 0, st, jobs, s);
-		for (uint32_t i = 0; i < n_iterations; ++i) {
-			hipLaunchKernelGGL(symmetric_kernel<0>, dim3(jobs.start[START_SYM][c]), dim3(256), 0, st, jobs);
-			hipLaunchKernelGGL(symmetric_kernel<1>, dim3(jobs.start[START_SYM][c]), dim3(256), 0, st, jobs);
-			if (i + 1 < n_iterations) hipLaunchKernelGGL(apply_kernel<0>, dim3(jobs.start[START_APPLY][c]), dim3(256), 0, st, jobs, s, (int)(i & 1));
-			else hipLaunchKernelGGL(apply_kernel<1>, dim3(jobs.start[START_APPLY][c]), dim3(256), 0, st, jobs, s, (int)(i & 1));
-		}
+		use_tile<Middle>(jobs);
+		const uint32_t middle = jobs.start[START_SYM][c];
+		use_tile<Large>(jobs);
+		if (jobs.start[START_SYM][c] >= 512) iterate<Large>(st, jobs, s, n_iterations);
+		else if (middle >= 200) iterate<Middle>(st, jobs, s, n_iterations);
+		else iterate<Little>(st, jobs, s, n_iterations);
 		NGP_LAUNCH_CHECK("ngp_hip_muon_step");
 	}
 	return 0;
