@@ -9,7 +9,10 @@
 // operands of 11 (fp16) or 8 bits.  fp32 matrix instructions would do at 1/16 of the fp16 rate; instead every matrix is kept as two fp16 halves, v = hi + lo with
 // hi = fp16(v) and lo = fp16(v - hi): 22 bits, and a product is three fp16 ones (hi hi + hi lo + lo hi, fp32 accumulation; lo lo is below the last bit kept).  Powers of two keep both
 // halves inside fp16's normal range: X is held as 2^15 X (|X_ij| <= 1.21, typically 1 / sqrt(n k)), A and B as 2^13 of themselves (spectral norms at most 1.5 and 3.5).
-// Layout of such a matrix: row-major, per 32 columns 32 hi values and 32 lo values: one 64-wide step of the product core brings both halves of 32 k.
+// Layout of such a matrix: row-major, per 32 columns 32 hi values and 32 lo values: 128 bytes of a row are both halves of 32 k.
+//
+// X is kept transposed, [k][n], and only so: A = X X^T reads it with k as the rows (transposed LDS reads on both sides), X^T <- X^T B with B, which is symmetric, along rows.  One
+// orientation to write instead of two: for matrices that do not stay in the cache between launches the iterations are as much bound by memory as by the products.
 #include <algorithm>
 #include <math.h>
 #include <stdio.h>
@@ -30,8 +33,8 @@ constexpr uint32_t MAX_JOBS = 24, MAX_SIDE = 65536, SUM_BLOCKS = 1024;
 struct Job {
 	uint64_t offset;                    // of the matrix in the parameter vector, in elements
 	uint32_t rows, cols, n, k;          // n = min, k = max of rows and cols
-	uint32_t np, kp;                    // n and k up to a multiple of 32
-	f16 *x, *xt[2], *a, *b;             // X [n][2 kp], its transpose [k][2 np] (two: an iteration reads one and writes the other), A and B [n][2 np]
+	uint32_t np;                        // n up to a multiple of 32
+	f16 *xt[2], *a, *b;                 // X^T [k][2 np] (two: an iteration reads one and writes the other), A and B [n][2 np]
 	double* sums;
 };
 enum { START_SUM, START_SPLIT, START_SYM, START_APPLY, N_STARTS };
@@ -43,9 +46,9 @@ struct Jobs {
 
 struct Step { float lr, momentum, decay, eps, inv_loss_scale; int nesterov, dtype; const void* grads; float* master; void* params; float* buffer; };
 
+// the job of a workgroup, which becomes its number within the job: every lane compares one job's end
 __device__ __forceinline__ uint32_t job_of(const Jobs& j, int kind, uint32_t& pid) {
-	uint32_t i = 0;
-	while (i + 1 < j.count && pid >= j.start[kind][i + 1]) ++i;
+	const uint32_t lane = threadIdx.x & 63, i = (uint32_t)__popcll(__ballot(lane < j.count && j.start[kind][lane < j.count ? lane + 1 : 0] <= pid));
 	pid -= j.start[kind][i];
 	return i;
 }
@@ -60,8 +63,7 @@ __device__ __forceinline__ float load_grad(const Step& s, uint64_t i) {
 	return g * s.inv_loss_scale;
 }
 
-__device__ __forceinline__ void update_weight(const Step& s, uint64_t at, float keep, float change) {
-	const float w = keep * s.master[at] - change;
+__device__ __forceinline__ void set_weight(const Step& s, uint64_t at, float w) {
 	s.master[at] = w;
 	if (!s.params) return;
 	if (s.dtype == NGP_DTYPE_F16) ((f16*)s.params)[at] = (f16)w;
@@ -124,10 +126,12 @@ __global__ void __launch_bounds__(256) momentum_kernel(Jobs jobs, Step s) {
 __device__ __forceinline__ void split2(float v, f16& hi, f16& lo) { hi = (f16)v; lo = (f16)(v - (float)hi); }
 __device__ __forceinline__ uint64_t split_col(uint32_t c) { return (uint64_t)(c >> 5) * 64 + (c & 31); }   // of the hi half; lo is 32 behind it
 
-// X_0 in halves, in both orientations, zeros up to the padded widths.  A workgroup takes 64 x 64 elements of X.
+typedef f16 f16x4 __attribute__((ext_vector_type(4)));
+
+// X_0^T in halves, zeros up to the padded width.  A workgroup takes 64 x 64 elements, through LDS where the matrix lies the other way round.
 __global__ void __launch_bounds__(256) split_kernel(Jobs jobs, Step s) {
 	__shared__ double lds[4];
-	__shared__ float tile[64][65];
+	__shared__ float tile[64][65];   // [long][short]
 	uint32_t pid = blockIdx.x;
 	const uint32_t ji = job_of(jobs, START_SPLIT, pid);
 	const Job& j = jobs.job[ji];
@@ -136,55 +140,51 @@ __global__ void __launch_bounds__(256) split_kernel(Jobs jobs, Step s) {
 	for (uint32_t i = threadIdx.x; i < blocks; i += 256) mine += j.sums[i];
 	const double sum = block_sum(mine, lds);
 	const double norm = sqrt(sum) + (double)s.eps, scale = norm == 0.0 ? 0.0 : (double)SX / norm;   // a zero update stays zero also without eps
-	const uint32_t tiles_k = (j.kp + 63) / 64, m0 = pid / tiles_k * 64, n0 = pid % tiles_k * 64;
-	const bool turn = j.rows > j.cols;   // X = u^T
-	for (uint32_t e = threadIdx.x; e < 4096; e += 256) {   // e runs along the rows of u
-		const uint32_t a = e >> 6, b = e & 63, m = m0 + (turn ? b : a), n = n0 + (turn ? a : b);
-		float v = 0.0f;
-		if (m < j.n && n < j.k) {
-			const uint64_t i = j.offset + (turn ? (uint64_t)n * j.cols + m : (uint64_t)m * j.cols + n);
-			const float buf = s.buffer[i];
-			v = (float)((double)(s.nesterov ? load_grad(s, i) + s.momentum * buf : buf) * scale);
-		}
-		tile[m - m0][n - n0] = v;
+	const uint32_t tiles_n = (j.np + 63) / 64, k0 = pid / tiles_n * 64, n0 = pid % tiles_n * 64;
+	const bool turn = j.rows > j.cols;   // the matrix is X^T as it lies
+#pragma unroll 4
+	for (uint32_t e = threadIdx.x; e < 4096; e += 256) {   // e runs along the matrix's rows
+		const uint32_t a = e >> 6, b = e & 63, k = k0 + (turn ? a : b), n = n0 + (turn ? b : a);
+		const bool in = k < j.k && n < j.n;
+		const uint64_t i = j.offset + (in ? (turn ? (uint64_t)k * j.cols + n : (uint64_t)n * j.cols + k) : 0);
+		const float m = s.buffer[i], g = s.nesterov ? load_grad(s, i) : 0.0f;
+		tile[k - k0][n - n0] = in ? (float)((double)(s.nesterov ? g + s.momentum * m : m) * scale) : 0.0f;
 	}
 	__syncthreads();
-	for (uint32_t e = threadIdx.x; e < 4096; e += 256) {
-		const uint32_t m = m0 + (e >> 6), n = n0 + (e & 63);
-		f16 hi, lo;
-		if (m < j.n && n < j.kp) {
-			split2(tile[e >> 6][e & 63], hi, lo);
-			f16* p = j.x + (uint64_t)m * 2 * j.kp + split_col(n);
-			p[0] = hi; p[32] = lo;
-		}
-		const uint32_t mt = m0 + (e & 63), nt = n0 + (e >> 6);
-		if (mt < j.np && nt < j.k) {
-			split2(tile[e & 63][e >> 6], hi, lo);
-			f16* p = j.xt[0] + (uint64_t)nt * 2 * j.np + split_col(mt);
-			p[0] = hi; p[32] = lo;
-		}
+#pragma unroll
+	for (uint32_t e = threadIdx.x; e < 1024; e += 256) {
+		const uint32_t k = e >> 4, n = (e & 15) * 4;
+		f16x4 hi, lo;
+#pragma unroll
+		for (int q = 0; q < 4; ++q) { f16 h, l; split2(tile[k][n + q], h, l); hi[q] = h; lo[q] = l; }
+		if (k0 + k >= j.k || n0 + n >= j.np) continue;
+		f16* p = j.xt[0] + (uint64_t)(k0 + k) * 2 * j.np + split_col(n0 + n);
+		*(f16x4*)p = hi;
+		*(f16x4*)(p + 32) = lo;
 	}
 }
 
 // ---- products of split matrices ------------------------------------------------------------------------------------------------------------
 
-typedef f16 f16x4 __attribute__((ext_vector_type(4)));
-
 // acc[nb][mb] = rows n0 .. of n times rows m0 .. of m (16 x 16 blocks), in steps of 32 k: 64 columns, both halves.  A ring of STAGES buffers, DMA spread between the MFMAs, counted
 // waits: the scheme of mm::Product, with three MFMAs to a pair of fragments' halves.
-template <int BN, int BM, int WN, int WM, int STAGES>
+// KC: the operands' rows have k along them (a step: 64 columns, both halves of 32 k).  RC: k is their rows (a step: 32 of them, both halves of the tile's columns).
+template <int BN_, int BM_, int WN_, int WM_, int STAGES_> struct Geometry { static constexpr int BN = BN_, BM = BM_, WN = WN_, WM = WM_, STAGES = STAGES_, THREADS = 64 * WN_ * WM_; };
+template <class G, int LAY>
 struct SplitProduct {
-	static constexpr int THREADS = 64 * WN * WM, NB = BN / WN / 16, MB = BM / WM / 16, N = BN, M = BM, WAVES_N = WN, WAVES_M = WM;
-	using NT = Tile<KC, BN, THREADS, 64>;
-	using MT = Tile<KC, BM, THREADS, 64>;
+	static constexpr int BN = G::BN, BM = G::BM, WN = G::WN, WM = G::WM, STAGES = G::STAGES;
+	static constexpr int THREADS = G::THREADS, NB = BN / WN / 16, MB = BM / WM / 16, N = BN, M = BM, WAVES_N = WN, WAVES_M = WM;
+	using NT = Tile<LAY, LAY == KC ? BN : 2 * BN, THREADS, LAY == KC ? 64 : 32>;
+	using MT = Tile<LAY, LAY == KC ? BM : 2 * BM, THREADS, LAY == KC ? 64 : 32>;
 	static constexpr int STAGE_BYTES = NT::BYTES + MT::BYTES, LOADS = NT::LOADS + MT::LOADS, LDS_BYTES = STAGES * STAGE_BYTES;
 	static_assert(LDS_BYTES >= WN * WM * 32 * 144, "the epilogue's rows");
 
 	// rows row0 .. + 15, half 0 (hi) or 1 (lo): lane l has row l & 15 and k = 8 (l >> 4) .. + 7
 	template <class TT> static __device__ __forceinline__ i32x4 frag(const lds_char* p, int row0, int half, int lane) {
+		if constexpr (LAY == RC) return TT::frag(p, (row0 >> 5) * 64 + half * 32 + (row0 & 31), lane);
 		return *(const __attribute__((address_space(3))) i32x4*)(p + (row0 + (lane & 15)) * 128 + ((half * 4 + (lane >> 4)) ^ TT::swizzle(lane & 15)) * 16);
 	}
-	static __device__ __forceinline__ void run(f32x4 (&acc)[NB][MB], const Mat& n, const Mat& m, uint32_t n0, uint32_t m0, lds_char* lds) {
+	static __device__ __forceinline__ void run(f32x4 (&acc)[NB][MB], const Mat& n, const Mat& m, uint32_t n0, uint32_t m0, lds_char* lds) {   // RC: n.rows, m.rows in columns of both halves
 		const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wn = wave % WN, wm = wave / WN;
 #pragma unroll
 		for (int a = 0; a < NB; ++a)
@@ -192,9 +192,9 @@ struct SplitProduct {
 			for (int b = 0; b < MB; ++b) acc[a][b] = f32x4{0, 0, 0, 0};
 		NT nt;
 		MT mt;
-		nt.init(n, n0, tid);
-		mt.init(m, m0, tid);
-		const int steps = (int)(n.k / 64);
+		nt.init(n, LAY == KC ? n0 : 2 * n0, tid);
+		mt.init(m, LAY == KC ? m0 : 2 * m0, tid);
+		const int steps = (int)(LAY == KC ? n.k / 64 : (n.k + 31) / 32);
 		i32x4 rn, rm;
 		int slot = 0;
 		lds_char* to = lds;
@@ -248,9 +248,9 @@ struct SplitProduct {
 		wait_and_sync();   // the DMA behind the last step too
 	}
 };
-using Large = SplitProduct<128, 256, 2, 4, 3>;   // 144 KB of LDS
-using Middle = SplitProduct<128, 128, 4, 2, 4>;  // 128 KB
-using Little = SplitProduct<64, 64, 2, 2, 4>;    // 64 KB: two workgroups a CU
+using Large = Geometry<128, 256, 2, 4, 3>;   // 144 KB of LDS
+using Middle = Geometry<128, 128, 4, 2, 4>;  // 128 KB
+using Little = Geometry<64, 64, 2, 2, 4>;    // 64 KB: two workgroups a CU
 
 // A wave's 32 x 32 block (2 x 2 of 16) of a split matrix, through LDS of its own (32 rows of 144 bytes) into rows of 64 hi and 64 lo bytes: as it lies (rows m), or transposed (rows n)
 __device__ __forceinline__ void put_split(const f32x4& v, bool turned, int nb, int mb, lds_char* lds, int lane) {   // block nb, mb of the four
@@ -282,16 +282,17 @@ __device__ __forceinline__ void write_split(f16* p, uint32_t pitch, uint32_t row
 }
 
 // Tiles that hold an element on or below the diagonal, by rows of tiles; a tile row's last tiles (M / N of them) are its square on the diagonal, whole, the others are written twice.
-template <class P> __host__ __device__ inline uint32_t symmetric_tiles(uint32_t n) {
-	const uint32_t tm = (n + P::M - 1) / P::M, tn = (n + P::N - 1) / P::N, r = P::M / P::N;
+template <class G> inline uint32_t symmetric_tiles(uint32_t n) {
+	const uint32_t tm = (n + G::BM - 1) / G::BM, tn = (n + G::BN - 1) / G::BN, r = G::BM / G::BN;
 	uint32_t t = 0;
 	for (uint32_t i = 0; i < tm; ++i) t += r * (i + 1) < tn ? r * (i + 1) : tn;
 	return t;
 }
 
 // A = X X^T (POLY 0), or B = a I + b A + c A^2 (POLY 1)
-template <class P, int POLY>
-__global__ void __launch_bounds__(P::THREADS, P::LDS_BYTES <= 80 * 1024 ? 2 : 1) symmetric_kernel(Jobs jobs) {
+template <class G, int POLY>
+__global__ void __launch_bounds__(G::THREADS, (SplitProduct<G, KC>::LDS_BYTES <= 80 * 1024 ? 2 : 1)) symmetric_kernel(Jobs jobs, int from) {
+	using P = SplitProduct<G, POLY ? KC : RC>;
 	__shared__ __attribute__((aligned(1024))) char lds[P::LDS_BYTES];
 	uint32_t pid = xcd_order(blockIdx.x, gridDim.x);
 	const Job& j = jobs.job[job_of(jobs, START_SYM, pid)];
@@ -302,8 +303,7 @@ __global__ void __launch_bounds__(P::THREADS, P::LDS_BYTES <= 80 * 1024 ? 2 : 1)
 		t -= R * (tm + 1);
 	}
 	const uint32_t tn = pid;
-	const uint32_t width = 2 * (POLY ? j.np : j.kp);
-	const Mat mat{POLY ? j.a : j.x, width, j.n, width};
+	const Mat mat = POLY ? Mat{j.a, 2ull * j.np, j.n, 2 * j.np} : Mat{j.xt[from], 2ull * j.np, 2 * j.np, j.k};
 	f32x4 acc[P::NB][P::MB];
 	P::run(acc, mat, mat, tn * P::N, tm * P::M, lds_of(lds));
 	const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wn = wave % P::WAVES_N, wm = wave / P::WAVES_N;
@@ -343,15 +343,16 @@ __global__ void __launch_bounds__(P::THREADS, P::LDS_BYTES <= 80 * 1024 ? 2 : 1)
 		}
 }
 
-// X <- B X: into both orientations, or (LAST) straight into the weights
-template <class P, int LAST>
-__global__ void __launch_bounds__(P::THREADS, P::LDS_BYTES <= 80 * 1024 ? 2 : 1) apply_kernel(Jobs jobs, Step s, int from) {
+// X^T <- X^T B, or (LAST) straight into the weights
+template <class G, int LAST>
+__global__ void __launch_bounds__(G::THREADS, (SplitProduct<G, KC>::LDS_BYTES <= 80 * 1024 ? 2 : 1)) apply_kernel(Jobs jobs, Step s, int from) {
+	using P = SplitProduct<G, KC>;
 	__shared__ __attribute__((aligned(1024))) char lds[P::LDS_BYTES];
 	uint32_t pid = xcd_order(blockIdx.x, gridDim.x);
 	const Job& j = jobs.job[job_of(jobs, START_APPLY, pid)];
-	const uint32_t tiles_m = (j.n + P::M - 1) / P::M, tm = pid % tiles_m, tn = pid / tiles_m;
+	const uint32_t tiles_n = (j.n + P::N - 1) / P::N, tn = pid % tiles_n, tm = pid / tiles_n;
 	f32x4 acc[P::NB][P::MB];
-	P::run(acc, Mat{j.xt[from], 2ull * j.np, j.k, 2 * j.np}, Mat{j.b, 2ull * j.np, j.n, 2 * j.np}, tn * P::N, tm * P::M, lds_of(lds));
+	P::run(acc, Mat{j.b, 2ull * j.np, j.n, 2 * j.np}, Mat{j.xt[from], 2ull * j.np, j.k, 2 * j.np}, tn * P::N, tm * P::M, lds_of(lds));
 	const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wn = wave % P::WAVES_N, wm = wave / P::WAVES_N;
 	lds_char* mine = lds_of(lds) + wave * (32 * 144);
 	const bool turn = j.rows > j.cols;
@@ -363,25 +364,30 @@ __global__ void __launch_bounds__(P::THREADS, P::LDS_BYTES <= 80 * 1024 ? 2 : 1)
 			const uint32_t n0 = tn * P::N + wn * (P::NB * 16) + a * 16, m0 = tm * P::M + wm * (P::MB * 16) + b * 16;
 			if (!LAST) {
 #pragma unroll
-				for (int turned = 0; turned < 2; ++turned) {
+				for (int x = 0; x < 2; ++x)
 #pragma unroll
-					for (int x = 0; x < 2; ++x)
-#pragma unroll
-						for (int y = 0; y < 2; ++y) put_split(acc[a + x][b + y] * (1.0f / SA), turned, x, y, mine, lane);
-					if (!turned) write_split(j.x, 2 * j.kp, j.n, j.kp, m0, n0, mine, lane);
-					else write_split(j.xt[1 - from], 2 * j.np, j.k, j.np, n0, m0, mine, lane);
-				}
+					for (int y = 0; y < 2; ++y) put_split(acc[a + x][b + y] * (1.0f / SA), false, x, y, mine, lane);
+				write_split(j.xt[1 - from], 2 * j.np, j.k, j.np, m0, n0, mine, lane);
 				continue;
 			}
+			float w[2][2][4];   // all loads, then all stores
+			auto each = [&](auto f) {
 #pragma unroll
-			for (int x = 0; x < 2; ++x)
+				for (int x = 0; x < 2; ++x)
 #pragma unroll
-				for (int y = 0; y < 2; ++y)
+					for (int y = 0; y < 2; ++y)
 #pragma unroll
-					for (int e = 0; e < 4; ++e) {
-						const uint32_t m = m0 + y * 16 + (lane & 15), n = n0 + x * 16 + 4 * (lane >> 4) + e;
-						if (m < j.n && n < j.k) update_weight(s, j.offset + (turn ? (uint64_t)n * j.cols + m : (uint64_t)m * j.cols + n), keep, rate * acc[a + x][b + y][e]);
-					}
+						for (int e = 0; e < 4; ++e) {
+							const uint32_t m = m0 + y * 16 + (lane & 15), n = n0 + x * 16 + 4 * (lane >> 4) + e;   // long, short
+							const bool in = m < j.k && n < j.n;
+							f(x, y, e, in, j.offset + (in ? (turn ? (uint64_t)m * j.cols + n : (uint64_t)n * j.cols + m) : 0));
+						}
+			};
+			each([&](int x, int y, int e, bool, uint64_t at) { w[x][y][e] = s.master[at]; });
+			each([&](int x, int y, int e, bool in, uint64_t at) {
+				const float v = keep * w[x][y][e] - rate * acc[a + x][b + y][e];
+				if (in) set_weight(s, at, v);
+			});
 		}
 }
 
@@ -412,16 +418,15 @@ static uint64_t lay_out(Jobs& jobs, const NgpMuonMatrix* m, char* base) {
 		Job& j = jobs.job[i];
 		j.offset = m[i].offset; j.rows = m[i].rows; j.cols = m[i].cols;
 		j.n = std::min(j.rows, j.cols); j.k = std::max(j.rows, j.cols);
-		j.np = (j.n + 31) & ~31u; j.kp = (j.k + 31) & ~31u;
+		j.np = (j.n + 31) & ~31u;
 		const uint32_t blocks = (uint32_t)std::min<uint64_t>(SUM_BLOCKS, ((uint64_t)j.rows * j.cols + 4095) / 4096);
-		j.x = (f16*)take((uint64_t)j.n * j.kp * 4);
 		j.xt[0] = (f16*)take((uint64_t)j.k * j.np * 4);
 		j.xt[1] = (f16*)take((uint64_t)j.k * j.np * 4);
 		j.a = (f16*)take((uint64_t)j.n * j.np * 4);
 		j.b = (f16*)take((uint64_t)j.n * j.np * 4);
 		j.sums = (double*)take(blocks * 8);
 		jobs.start[START_SUM][i + 1] = jobs.start[START_SUM][i] + blocks;
-		jobs.start[START_SPLIT][i + 1] = jobs.start[START_SPLIT][i] + ((j.np + 63) / 64) * ((j.kp + 63) / 64);
+		jobs.start[START_SPLIT][i + 1] = jobs.start[START_SPLIT][i] + ((j.np + 63) / 64) * ((j.k + 63) / 64);
 	}
 	return used;
 }
@@ -430,7 +435,7 @@ template <class P> static void use_tile(Jobs& jobs) {
 	for (uint32_t i = 0; i < jobs.count; ++i) {
 		const Job& j = jobs.job[i];
 		jobs.start[START_SYM][i + 1] = jobs.start[START_SYM][i] + symmetric_tiles<P>(j.n);
-		jobs.start[START_APPLY][i + 1] = jobs.start[START_APPLY][i] + ((j.n + P::M - 1) / P::M) * ((j.k + P::N - 1) / P::N);
+		jobs.start[START_APPLY][i + 1] = jobs.start[START_APPLY][i] + ((j.n + P::BN - 1) / P::BN) * ((j.k + P::BM - 1) / P::BM);
 	}
 }
 
@@ -439,8 +444,8 @@ template <class P> static void iterate(hipStream_t st, Jobs& jobs, const Step& s
 	const uint32_t c = jobs.count;
 	const dim3 block(P::THREADS), sym(jobs.start[START_SYM][c]), apply(jobs.start[START_APPLY][c]);
 	for (uint32_t i = 0; i < n_iterations; ++i) {
-		hipLaunchKernelGGL((symmetric_kernel<P, 0>), sym, block, 0, st, jobs);
-		hipLaunchKernelGGL((symmetric_kernel<P, 1>), sym, block, 0, st, jobs);
+		hipLaunchKernelGGL((symmetric_kernel<P, 0>), sym, block, 0, st, jobs, (int)(i & 1));
+		hipLaunchKernelGGL((symmetric_kernel<P, 1>), sym, block, 0, st, jobs, 0);
 		if (i + 1 < n_iterations) hipLaunchKernelGGL((apply_kernel<P, 0>), apply, block, 0, st, jobs, s, (int)(i & 1));
 		else hipLaunchKernelGGL((apply_kernel<P, 1>), apply, block, 0, st, jobs, s, (int)(i & 1));
 	}
