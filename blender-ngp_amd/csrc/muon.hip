@@ -63,11 +63,35 @@ __device__ __forceinline__ float load_grad(const Step& s, uint64_t i) {
 	return g * s.inv_loss_scale;
 }
 
-__device__ __forceinline__ void set_weight(const Step& s, uint64_t at, float w) {
-	s.master[at] = w;
+// N gradients at once, and N weights: the choice of type is made once, and the loads (the stores) follow each other
+template <int N> __device__ __forceinline__ void load_grads(const Step& s, const uint64_t (&at)[N], float (&g)[N]) {
+	if (s.dtype == NGP_DTYPE_F32) {
+#pragma unroll
+		for (int i = 0; i < N; ++i) g[i] = ((const float*)s.grads)[at[i]];
+	} else if (s.dtype == NGP_DTYPE_F16) {
+#pragma unroll
+		for (int i = 0; i < N; ++i) g[i] = (float)((const f16*)s.grads)[at[i]];
+	} else {
+#pragma unroll
+		for (int i = 0; i < N; ++i) g[i] = (float)((const b16*)s.grads)[at[i]];
+	}
+#pragma unroll
+	for (int i = 0; i < N; ++i) g[i] *= s.inv_loss_scale;
+}
+template <int N> __device__ __forceinline__ void set_weights(const Step& s, const uint64_t (&at)[N], const float (&w)[N], const bool (&in)[N]) {
+#pragma unroll
+	for (int i = 0; i < N; ++i)
+		if (in[i]) s.master[at[i]] = w[i];
 	if (!s.params) return;
-	if (s.dtype == NGP_DTYPE_F16) ((f16*)s.params)[at] = (f16)w;
-	else ((b16*)s.params)[at] = (b16)w;
+	if (s.dtype == NGP_DTYPE_F16) {
+#pragma unroll
+		for (int i = 0; i < N; ++i)
+			if (in[i]) ((f16*)s.params)[at[i]] = (f16)w[i];
+	} else {
+#pragma unroll
+		for (int i = 0; i < N; ++i)
+			if (in[i]) ((b16*)s.params)[at[i]] = (b16)w[i];
+	}
 }
 
 __device__ __forceinline__ double block_sum(double v, double* lds) {   // 256 threads, a fixed order
@@ -370,26 +394,185 @@ __global__ void __launch_bounds__(G::THREADS, (SplitProduct<G, KC>::LDS_BYTES <=
 				write_split(j.xt[1 - from], 2 * j.np, j.k, j.np, m0, n0, mine, lane);
 				continue;
 			}
-			float w[2][2][4];   // all loads, then all stores
-			auto each = [&](auto f) {
+			float w[16];
+			uint64_t at[16];
+			bool in[16];
 #pragma unroll
-				for (int x = 0; x < 2; ++x)
+			for (int i = 0; i < 16; ++i) {
+				const uint32_t m = m0 + (i >> 2 & 1) * 16 + (lane & 15), n = n0 + (i >> 3) * 16 + 4 * (lane >> 4) + (i & 3);   // long, short
+				in[i] = m < j.k && n < j.n;
+				at[i] = j.offset + (in[i] ? (turn ? (uint64_t)m * j.cols + n : (uint64_t)n * j.cols + m) : 0);
+				w[i] = s.master[at[i]];
+			}
 #pragma unroll
-					for (int y = 0; y < 2; ++y)
-#pragma unroll
-						for (int e = 0; e < 4; ++e) {
-							const uint32_t m = m0 + y * 16 + (lane & 15), n = n0 + x * 16 + 4 * (lane >> 4) + e;   // long, short
-							const bool in = m < j.k && n < j.n;
-							f(x, y, e, in, j.offset + (in ? (turn ? (uint64_t)m * j.cols + n : (uint64_t)n * j.cols + m) : 0));
-						}
-			};
-			each([&](int x, int y, int e, bool, uint64_t at) { w[x][y][e] = s.master[at]; });
-			each([&](int x, int y, int e, bool in, uint64_t at) {
-				const float v = keep * w[x][y][e] - rate * acc[a + x][b + y][e];
-				if (in) set_weight(s, at, v);
-			});
+			for (int i = 0; i < 16; ++i) w[i] = keep * w[i] - rate * acc[a + (i >> 3)][b + (i >> 2 & 1)][i & 3];
+			set_weights(s, at, w, in);
 		}
 }
+
+// ---- a matrix in one workgroup ---------------------------------------------------------------------------------------------------------------
+//
+// Short side at most 64, long side at most 256 (the matrices of the framework's own networks): X^T, A and B stay in LDS in the same split layout, and the whole step is one launch
+// whose time is the latency of its chain: 3 products an iteration, four barriers.  Five 64 x 64 matrices: 76 us as 17 launches of the kernels above.
+struct TinyJobs { NgpMuonMatrix m[128]; };
+constexpr uint32_t TINY_N = 64, TINY_K = 256;
+constexpr int TINY_PITCH = 64 * 4 + 16;   // bytes of a row of 64 columns in two halves
+
+__device__ __forceinline__ i32x4 tiny_along(const lds_char* p, int row0, int col0, int half, int lane) {   // 16 rows, 32 k along them from col0 (a multiple of 32)
+	return *(const __attribute__((address_space(3))) i32x4*)(p + (row0 + (lane & 15)) * TINY_PITCH + col0 * 4 + half * 64 + (lane >> 4) * 16);
+}
+__device__ __forceinline__ i32x4 tiny_turned(const lds_char* p, int row0, int k0, int half, int lane) {    // 16 columns from row0, 32 k: the LDS rows from k0
+	const lds_char* q = p + (k0 + 8 * (lane >> 4) + ((lane & 15) >> 2)) * TINY_PITCH + (row0 >> 5) * 128 + half * 64 + ((row0 & 31) + 4 * (lane & 3)) * 2;
+	const i32x2 a = __builtin_bit_cast(i32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)q));
+	const i32x2 b = __builtin_bit_cast(i32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(q + 4 * TINY_PITCH)));
+	return i32x4{a.x, a.y, b.x, b.y};
+}
+__device__ __forceinline__ void tiny_put(lds_char* p, int row, int col, const f32x4& v) {   // four columns
+	f16x4 hi, lo;
+#pragma unroll
+	for (int e = 0; e < 4; ++e) { f16 h, l; split2(v[e], h, l); hi[e] = h; lo[e] = l; }
+	lds_char* q = p + row * TINY_PITCH + (col >> 5) * 128 + (col & 31) * 2;
+	*(__attribute__((address_space(3))) f16x4*)q = hi;
+	*(__attribute__((address_space(3))) f16x4*)(q + 64) = lo;
+}
+__device__ __forceinline__ f32x4 tiny_get(const lds_char* p, int row, int col) {
+	const lds_char* q = p + row * TINY_PITCH + (col >> 5) * 128 + (col & 31) * 2;
+	return __builtin_convertvector(*(const __attribute__((address_space(3))) f16x4*)q, f32x4) + __builtin_convertvector(*(const __attribute__((address_space(3))) f16x4*)(q + 64), f32x4);
+}
+__device__ __forceinline__ f32x4 mfma3(i32x4 nh, i32x4 nl, i32x4 mh, i32x4 ml, f32x4 c) {
+	c = mfma16<f16>(nl, mh, c);
+	c = mfma16<f16>(nh, ml, c);
+	return mfma16<f16>(nh, mh, c);
+}
+
+__global__ void __launch_bounds__(512) tiny_kernel(TinyJobs jobs, Step s, uint32_t iterations) {
+	__shared__ __attribute__((aligned(16))) char xt_[TINY_K * TINY_PITCH], a_[TINY_N * TINY_PITCH], b_[TINY_N * TINY_PITCH];
+	__shared__ double sums[8];
+	lds_char *const xt = lds_of(xt_), *const ma = lds_of(a_), *const mb = lds_of(b_);
+	const NgpMuonMatrix job = jobs.m[blockIdx.x];
+	const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+	const bool turn = job.rows > job.cols;                                    // the matrix lies as X^T
+	const uint32_t n = turn ? job.cols : job.rows, k = turn ? job.rows : job.cols, total = job.rows * job.cols;
+	const int k_steps = (int)((k + 31) / 32);
+	constexpr int EACH = TINY_N * TINY_K / 512;
+	float u[EACH];
+	double sum = 0.0;
+#pragma unroll
+	for (int c = 0; c < EACH; c += 8) {   // eight loads, then eight stores
+		if (c * 512 >= total) {
+#pragma unroll
+			for (int q = c; q < c + 8; ++q) u[q] = 0.0f;
+			continue;
+		}
+		float old[8], g[8];
+		uint64_t at[8];
+#pragma unroll
+		for (int q = 0; q < 8; ++q) {
+			at[q] = job.offset + min((uint32_t)((c + q) * 512 + tid), total - 1);
+			old[q] = s.buffer[at[q]];
+		}
+		load_grads(s, at, g);
+#pragma unroll
+		for (int q = 0; q < 8; ++q) {
+			const uint32_t i = (c + q) * 512 + tid;
+			const float m = s.momentum * old[q] + g[q];
+			if (i < total) s.buffer[at[q]] = m;
+			const double d = i < total ? (s.nesterov ? g[q] + s.momentum * m : m) : 0.0f;
+			u[c + q] = (float)d;
+			sum += d * d;
+		}
+	}
+	for (int i = tid; i < k_steps * 32 * (TINY_PITCH / 16); i += 512) *(__attribute__((address_space(3))) i32x4*)(xt + i * 16) = i32x4{0, 0, 0, 0};
+	for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
+	if (lane == 0) sums[wave] = sum;
+	__syncthreads();
+	sum = sums[0];
+	for (int i = 1; i < 8; ++i) sum += sums[i];
+	const double norm = sqrt(sum) + (double)s.eps, scale = norm == 0.0 ? 0.0 : (double)SX / norm;
+#pragma unroll
+	for (int q = 0; q < EACH; ++q) {
+		const uint32_t i = q * 512 + tid;
+		if (q * 512 < total && i < total) {
+			const uint32_t r = i / job.cols, c = i % job.cols, row = turn ? r : c, col = turn ? c : r;   // of X^T
+			f16 hi, lo;
+			split2((float)((double)u[q] * scale), hi, lo);
+			lds_char* p = xt + row * TINY_PITCH + (col >> 5) * 128 + (col & 31) * 2;
+			*(__attribute__((address_space(3))) f16*)p = hi;
+			*(__attribute__((address_space(3))) f16*)(p + 64) = lo;
+		}
+	}
+	__syncthreads();
+	const int m0 = wave / 2 * 16, n0 = wave % 2 * 32, lm = lane & 15, ln = 4 * (lane >> 4);   // of A and B: one row of blocks, two of its four
+	for (uint32_t it = 0; it < iterations; ++it) {
+		f32x4 acc[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+		for (int ks = 0; ks < k_steps; ++ks) {
+			const i32x4 mh = tiny_turned(xt, m0, ks * 32, 0, lane), ml = tiny_turned(xt, m0, ks * 32, 1, lane);
+#pragma unroll
+			for (int b = 0; b < 2; ++b) acc[b] = mfma3(tiny_turned(xt, n0 + b * 16, ks * 32, 0, lane), tiny_turned(xt, n0 + b * 16, ks * 32, 1, lane), mh, ml, acc[b]);
+		}
+#pragma unroll
+		for (int b = 0; b < 2; ++b) tiny_put(ma, m0 + lm, n0 + b * 16 + ln, acc[b] * (SA / (SX * SX)));
+		__syncthreads();
+		acc[0] = acc[1] = f32x4{0, 0, 0, 0};
+#pragma unroll
+		for (int ks = 0; ks < 2; ++ks) {
+			const i32x4 mh = tiny_along(ma, m0, ks * 32, 0, lane), ml = tiny_along(ma, m0, ks * 32, 1, lane);
+#pragma unroll
+			for (int b = 0; b < 2; ++b) acc[b] = mfma3(tiny_along(ma, n0 + b * 16, ks * 32, 0, lane), tiny_along(ma, n0 + b * 16, ks * 32, 1, lane), mh, ml, acc[b]);
+		}
+#pragma unroll
+		for (int b = 0; b < 2; ++b) {
+			const int row = m0 + lm, col = n0 + b * 16 + ln;
+			f32x4 v = NS_C / SA * acc[b] + NS_B * tiny_get(ma, row, col);
+#pragma unroll
+			for (int e = 0; e < 4; ++e)
+				if (row == col + e) v[e] += NS_A * SA;
+			tiny_put(mb, row, col, v);
+		}
+		__syncthreads();
+		f32x4 x[2][4];   // rows 16 wave .. and 128 + 16 wave .. of X^T B
+#pragma unroll
+		for (int h = 0; h < 2; ++h) {
+			const int r = h * 128 + wave * 16;
+			if (r >= k_steps * 32) break;
+#pragma unroll
+			for (int b = 0; b < 4; ++b) x[h][b] = f32x4{0, 0, 0, 0};
+#pragma unroll
+			for (int ks = 0; ks < 2; ++ks) {
+				const i32x4 mh = tiny_along(xt, r, ks * 32, 0, lane), ml = tiny_along(xt, r, ks * 32, 1, lane);
+#pragma unroll
+				for (int b = 0; b < 4; ++b) x[h][b] = mfma3(tiny_along(mb, b * 16, ks * 32, 0, lane), tiny_along(mb, b * 16, ks * 32, 1, lane), mh, ml, x[h][b]);
+			}
+		}
+		const bool last = it + 1 == iterations;   // a wave reads and writes its own rows of X^T alone: no barrier between
+		const float keep = 1.0f - s.lr * s.decay, rate = s.lr * sqrtf(fmaxf(1.0f, (float)job.rows / (float)job.cols)) / (SA * SX);
+#pragma unroll
+		for (int h = 0; h < 2; ++h) {
+			const int r = h * 128 + wave * 16 + lm;
+			if (h * 128 + wave * 16 >= k_steps * 32) break;
+			if (!last) {
+#pragma unroll
+				for (int b = 0; b < 4; ++b) tiny_put(xt, r, b * 16 + ln, x[h][b] * (1.0f / SA));
+				continue;
+			}
+			float w[16];
+			uint64_t at[16];
+			bool in[16];
+#pragma unroll
+			for (int i = 0; i < 16; ++i) {
+				const uint32_t c = (i >> 2) * 16 + ln + (i & 3);
+				in[i] = (uint32_t)r < k && c < n;
+				at[i] = job.offset + (in[i] ? (turn ? (uint64_t)r * job.cols + c : (uint64_t)c * job.cols + r) : 0);
+				w[i] = s.master[at[i]];
+			}
+#pragma unroll
+			for (int i = 0; i < 16; ++i) w[i] = keep * w[i] - rate * x[h][i >> 2][i & 3];
+			set_weights(s, at, w, in);
+		}
+		__syncthreads();
+	}
+}
+static bool is_tiny(const NgpMuonMatrix& m) { return std::min(m.rows, m.cols) <= TINY_N && std::max(m.rows, m.cols) <= TINY_K; }
 
 // ---- host ------------------------------------------------------------------------------------------------------------------------------
 
@@ -409,14 +592,24 @@ static const char* bad_matrices(uint32_t count, const NgpMuonMatrix* m) {
 	return nullptr;
 }
 
-// the buffers of matrices [first, first + jobs.count) in `base` (null: the size alone)
-static uint64_t lay_out(Jobs& jobs, const NgpMuonMatrix* m, char* base) {
+// the next MAX_JOBS matrices from `first` on that are too large for one workgroup
+static bool next_jobs(Jobs& jobs, uint32_t n, const NgpMuonMatrix* m, uint32_t& first) {
+	jobs.count = 0;
+	for (; first < n && jobs.count < MAX_JOBS; ++first) {
+		if (is_tiny(m[first])) continue;
+		Job& j = jobs.job[jobs.count++];
+		j.offset = m[first].offset; j.rows = m[first].rows; j.cols = m[first].cols;
+	}
+	return jobs.count != 0;
+}
+
+// their buffers in `base` (null: the size alone)
+static uint64_t lay_out(Jobs& jobs, char* base) {
 	uint64_t used = 0;
 	auto take = [&](uint64_t bytes) { char* p = base ? base + used : nullptr; used += up256(bytes); return p; };
 	for (int kind = 0; kind < N_STARTS; ++kind) jobs.start[kind][0] = 0;
 	for (uint32_t i = 0; i < jobs.count; ++i) {
 		Job& j = jobs.job[i];
-		j.offset = m[i].offset; j.rows = m[i].rows; j.cols = m[i].cols;
 		j.n = std::min(j.rows, j.cols); j.k = std::max(j.rows, j.cols);
 		j.np = (j.n + 31) & ~31u;
 		const uint32_t blocks = (uint32_t)std::min<uint64_t>(SUM_BLOCKS, ((uint64_t)j.rows * j.cols + 4095) / 4096);
@@ -463,10 +656,7 @@ uint64_t ngp_hip_muon_workspace_bytes(uint32_t n_matrices, const NgpMuonMatrix* 
 	if (const char* bad = bad_matrices(n_matrices, matrices_host)) { refuse(bad); return 0; }
 	uint64_t most = 0;
 	Jobs jobs;
-	for (uint32_t first = 0; first < n_matrices; first += MAX_JOBS) {
-		jobs.count = std::min(MAX_JOBS, n_matrices - first);
-		most = std::max(most, lay_out(jobs, matrices_host + first, nullptr));
-	}
+	for (uint32_t first = 0; next_jobs(jobs, n_matrices, matrices_host, first);) most = std::max(most, lay_out(jobs, nullptr));
 	return most;
 }
 
@@ -482,14 +672,22 @@ int ngp_hip_muon_step(void* stream, uint32_t n_matrices, const NgpMuonMatrix* ma
 	if (!bad && dtype == NGP_DTYPE_F32 && params) bad = "dtype F32 has no params: the master copy is the parameters";
 	if (!bad && n_matrices && (!grads || !master || !momentum_buffer)) bad = "null tensor";
 	if (!bad && ((((uintptr_t)master | (uintptr_t)momentum_buffer) & 3) || (((uintptr_t)grads | (uintptr_t)params) & (dtype == NGP_DTYPE_F32 ? 3 : 1)))) bad = "a tensor is not aligned to its elements";
-	if (!bad && n_matrices && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < ngp_hip_muon_workspace_bytes(n_matrices, matrices_host))) bad = "workspace null, not 16-byte aligned or too small (ngp_hip_muon_workspace_bytes)";
+	const uint64_t need = bad ? 0 : ngp_hip_muon_workspace_bytes(n_matrices, matrices_host);
+	if (!bad && need && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < need)) bad = "workspace null, not 16-byte aligned or too small (ngp_hip_muon_workspace_bytes)";
 	if (bad) { snprintf(msg, sizeof(msg), "ngp_hip_muon_step: %s", bad); return refuse(msg); }
 	hipStream_t st = (hipStream_t)stream;
 	const Step s{learning_rate, momentum, weight_decay, epsilon, 1.0f / loss_scale, nesterov, dtype, grads, master, params, momentum_buffer};
-	for (uint32_t first = 0; first < n_matrices; first += MAX_JOBS) {
-		Jobs jobs;
-		jobs.count = std::min(MAX_JOBS, n_matrices - first);
-		lay_out(jobs, matrices_host + first, (char*)workspace);
+	for (uint32_t first = 0; first < n_matrices;) {
+		TinyJobs tiny;
+		uint32_t count = 0;
+		for (; first < n_matrices && count < 128; ++first)
+			if (is_tiny(matrices_host[first])) tiny.m[count++] = matrices_host[first];
+		if (count) hipLaunchKernelGGL(tiny_kernel, dim3(count), dim3(512), 0, st, tiny, s, n_iterations);
+		NGP_LAUNCH_CHECK("tiny_kernel");
+	}
+	Jobs jobs;
+	for (uint32_t first = 0; next_jobs(jobs, n_matrices, matrices_host, first);) {
+		lay_out(jobs, (char*)workspace);
 		const uint32_t c = jobs.count;
 		hipLaunchKernelGGL(momentum_kernel, dim3(jobs.start[START_SUM][c]), dim3(256), 0, st, jobs, s);
 		hipLaunchKernelGGL(split_kernel, dim3(jobs.start[START_SPLIT][c]), dim3(256), 0, st, jobs, s);

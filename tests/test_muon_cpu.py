@@ -14,7 +14,7 @@ def matrices(*rows):
     return d
 
 
-GOOD = matrices((0, 64, 32), (2048, 16, 64))
+GOOD = matrices((0, 64, 32), (2048, 160, 64), (12288, 80, 100))
 
 
 def call(ngp, m=GOOD, count=None, **kw):
@@ -46,8 +46,16 @@ def test_null_list_and_too_many(ngp):
 
 
 def test_workspace(ngp):
-    n = ngp.ngp_hip_muon_workspace_bytes(2, GOOD.ctypes.data)
+    n = ngp.ngp_hip_muon_workspace_bytes(len(GOOD), GOOD.ctypes.data)
     assert n > 0 and call(ngp, n=n - 1) != 0 and b"workspace" in ngp.ngp_hip_last_error()
+
+
+def test_small_matrices_need_no_workspace(ngp):
+    m = matrices((0, 64, 32), (2048, 16, 64), (4096, 256, 64), (1 << 20, 1, 256))
+    assert ngp.ngp_hip_muon_workspace_bytes(len(m), m.ctypes.data) == 0
+    for big in ((1, 257), (257, 1), (65, 65)):
+        m = matrices((0, *big))
+        assert ngp.ngp_hip_muon_workspace_bytes(1, m.ctypes.data) > 0
 
 
 def test_no_matrices_is_no_work(ngp):

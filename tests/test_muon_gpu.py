@@ -81,7 +81,7 @@ def check_step(ngp, v, **kw):
             assert torch.equal(v.of(v.params, i), v.of(v.master, i).to(v.t))
 
 
-SHAPES = [(1, 1), (1, 7), (5, 1), (3, 2), (16, 64), (64, 32), (64, 64), (33, 65), (63, 200), (65, 64), (128, 128), (100, 300), (300, 100), (129, 257), (130, 1000), (1000, 127), (768, 520), (520, 2050)]
+SHAPES = [(1, 1), (1, 7), (5, 1), (3, 2), (16, 64), (64, 32), (64, 64), (33, 65), (63, 200), (64, 256), (256, 17), (257, 30), (65, 64), (128, 128), (100, 300), (300, 100), (129, 257), (130, 1000), (1000, 127), (768, 520), (520, 2050)]
 
 
 @pytest.mark.parametrize("shape", SHAPES, ids=lambda s: "%dx%d" % s)
@@ -101,6 +101,7 @@ def test_the_whole_step_on_matrices_of_many_shapes(ngp, cuda, dtype, nesterov):
 def test_more_matrices_than_one_launch_takes(ngp, cuda):
     check_step(ngp, Vector([(8 + 3 * i, 90 - i) for i in range(60)], "bf16", gap=1), iterations=5)
     check_step(ngp, Vector([(70 + i, 150 - i) for i in range(30)], "f16", gap=0), iterations=3)
+    check_step(ngp, Vector([(2 + i % 5, 3 + i % 7) if i % 3 else (66, 70) for i in range(160)], "f32", gap=2), iterations=2)
 
 
 @pytest.mark.parametrize("iterations", [1, 2, 3, 6])
