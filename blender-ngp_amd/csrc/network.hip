@@ -2864,6 +2864,43 @@ int ngp_hip_grid_backward_unordered(void* stream, uint32_t n_dims, const NgpNetD
 	return grid_backward_entry(stream, n_dims, desc_dev, pos, pos_stride_floats, n, dL_dx_planes, grid_grad, scratch, scratch_bytes, false);
 }
 
+// ---- the encoding alone, in rows of 32 features: what a network that is not one of the fused kernels reads and sends gradients back to.  The encoder and the hash-grid backward work
+// on level planes [16][n] x 2 features; these two turn 32 samples x 16 levels through LDS (64 bytes a row on one side, 128 a plane on the other: bound by memory).
+__global__ void __launch_bounds__(256) planes_to_rows_kernel(const uint32_t* __restrict__ planes, uint32_t n_pad, uint32_t n, uint32_t* __restrict__ rows) {
+	__shared__ uint32_t t[64][17];
+	const uint32_t s0 = blockIdx.x * 64;
+	for (uint32_t i = threadIdx.x; i < 1024; i += 256) t[i & 63][i >> 6] = s0 + (i & 63) < n ? planes[(size_t)(i >> 6) * n_pad + s0 + (i & 63)] : 0u;
+	__syncthreads();
+	for (uint32_t i = threadIdx.x; i < 1024; i += 256) if (s0 + (i >> 4) < n) rows[(size_t)(s0 + (i >> 4)) * 16 + (i & 15)] = t[i >> 4][i & 15];
+}
+__global__ void __launch_bounds__(256) rows_to_planes_kernel(const uint32_t* __restrict__ rows, uint32_t n, uint32_t* __restrict__ planes) {
+	__shared__ uint32_t t[64][17];
+	const uint32_t s0 = blockIdx.x * 64;
+	for (uint32_t i = threadIdx.x; i < 1024; i += 256) t[i >> 4][i & 15] = s0 + (i >> 4) < n ? rows[(size_t)(s0 + (i >> 4)) * 16 + (i & 15)] : 0u;
+	__syncthreads();
+	for (uint32_t i = threadIdx.x; i < 1024; i += 256) if (s0 + (i & 63) < n) planes[(size_t)(i >> 6) * n + s0 + (i & 63)] = t[i & 63][i >> 6];
+}
+int ngp_hip_grid_encode(void* stream, uint32_t n_dims, const NgpNetDesc* desc_dev, const uint16_t* grid, const float* pos, uint32_t pos_stride_floats, uint32_t n, uint16_t* features,
+                        void* workspace, uint64_t workspace_bytes) {
+	if (n_dims != 2 && n_dims != 3) { set_last_error("ngp_hip_grid_encode: n_dims must be 2 or 3", hipErrorInvalidValue); return -1; }
+	if (!n) return 0;
+	if (!desc_dev || !grid || !pos || !features || ((uintptr_t)grid & 3) || ((uintptr_t)features & 3)) { set_last_error("ngp_hip_grid_encode: null or unaligned buffer (feature pairs are read and written as 4 bytes)", hipErrorInvalidValue); return -1; }
+	const h2* planes; uint32_t n_pad;
+	if (launch_encode(stream, desc_dev, grid, pos, pos_stride_floats, n, workspace, workspace_bytes, &planes, &n_pad, "ngp_hip_grid_encode: workspace too small (ngp_hip_nerf_encode_workspace_bytes)", nullptr, 0u, n_dims)) return -1;
+	hipLaunchKernelGGL(planes_to_rows_kernel, dim3(div_up(n, 64)), dim3(256), 0, (hipStream_t)stream, (const uint32_t*)planes, n_pad, n, (uint32_t*)features);
+	NGP_LAUNCH_CHECK("planes_to_rows_kernel");
+	return 0;
+}
+uint64_t ngp_hip_grid_gradient_scratch_bytes(uint32_t n) { return (uint64_t)16 * n * 4u + ngp_hip_grid_backward_scratch_bytes(n); }
+int ngp_hip_grid_gradient(void* stream, uint32_t n_dims, const NgpNetDesc* desc_dev, const float* pos, uint32_t pos_stride_floats, uint32_t n, const uint16_t* dL_dfeatures, int ordered,
+                          uint16_t* grid_grad, void* scratch, uint64_t scratch_bytes) {
+	if (n == 0 || (n % 256) != 0) { set_last_error("ngp_hip_grid_gradient: n must be a positive multiple of 256", hipErrorInvalidValue); return -1; }
+	if (!dL_dfeatures || ((uintptr_t)dL_dfeatures & 3) || !scratch || scratch_bytes < ngp_hip_grid_gradient_scratch_bytes(n)) { set_last_error("ngp_hip_grid_gradient: null or unaligned buffer, or scratch too small (ngp_hip_grid_gradient_scratch_bytes)", hipErrorInvalidValue); return -1; }
+	hipLaunchKernelGGL(rows_to_planes_kernel, dim3(div_up(n, 64)), dim3(256), 0, (hipStream_t)stream, (const uint32_t*)dL_dfeatures, n, (uint32_t*)scratch);
+	NGP_LAUNCH_CHECK("rows_to_planes_kernel");
+	return grid_backward_entry(stream, n_dims, desc_dev, pos, pos_stride_floats, n, (const uint16_t*)scratch, grid_grad, (char*)scratch + (uint64_t)16 * n * 4u, scratch_bytes - (uint64_t)16 * n * 4u, ordered != 0);
+}
+
 // ---- plumbing configs: grid encoding -> one MLP (P1 image, P2 sdf)
 int ngp_hip_gridmlp_make_desc_host(uint32_t n_dims, uint32_t n_levels, uint32_t log2_hashmap_size, uint32_t base_resolution, float per_level_scale, NgpNetDesc* d) {
 	if (n_levels != 16 || !d || (n_dims != 2 && n_dims != 3)) { set_last_error("ngp_hip_gridmlp_make_desc_host: n_levels must be 16 and n_dims 2 or 3", hipErrorInvalidValue); return -1; }

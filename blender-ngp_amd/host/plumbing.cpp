@@ -16,7 +16,6 @@
 namespace ngp {
 
 #define HIP_TRY(x) do { hipError_t e_ = (x); if (e_ != hipSuccess) throw std::runtime_error(std::string(#x) + ": " + hipGetErrorString(e_)); } while (0)
-static constexpr uint32_t GM_OUT_STRIDE = 4;
 static constexpr float LOSS_SCALE = 128.0f;                 // testbed.h:272, optimizer_step(stream, 128)
 static constexpr uint32_t BATCH_SIZE_GRANULARITY = 128;     // tcnn::batch_size_granularity
 static inline uint32_t next_multiple(uint32_t v, uint32_t m) { return (v + m - 1) / m * m; }
@@ -33,7 +32,19 @@ void Testbed::reset_network_gridmlp() {  // testbed.cu:2249-2470, Image / Sdf br
 	std::string enc_type = enc.value("otype", "HashGrid"); std::transform(enc_type.begin(), enc_type.end(), enc_type.begin(), ::tolower);
 	require(enc_type == "hashgrid", "encoding.otype must be HashGrid");
 	require((uint32_t)enc.value("n_features_per_level", 2) == 2 && (uint32_t)enc.value("n_levels", 16) == 16, "HashGrid must have 16 levels x 2 features");
-	if (config.contains("network")) require(config["network"].value("n_neurons", 64) == 64 && config["network"].value("n_hidden_layers", 2) == 2, "network must be 64 neurons x 2 hidden layers");
+	std::string net_type = config.contains("network") ? config["network"].value("otype", "FullyFusedMLP") : std::string("FullyFusedMLP"); std::transform(net_type.begin(), net_type.end(), net_type.begin(), ::tolower);
+	m_gated = net_type == "gatedmlp";
+	if (m_gated) {
+		const Json& net = config["network"];
+		const int width = (int)net.value("n_neurons", 64);
+		require(width >= 8 && width <= 65536 && width % 8 == 0, "GatedMLP: n_neurons must be a multiple of 8 up to 65536");
+		std::string act = net.value("activation", "SiLU"); std::transform(act.begin(), act.end(), act.begin(), ::tolower);
+		m_gated_block.activation = act == "silu" ? NGP_ACT_SILU : act == "gelu" ? NGP_ACT_GELU : act == "relu" ? NGP_ACT_RELU : act == "sigmoid" || act == "logistic" ? NGP_ACT_LOGISTIC : act == "none" ? NGP_ACT_NONE : -1;
+		require(m_gated_block.activation >= 0, "GatedMLP: activation must be SiLU, GELU, ReLU, Sigmoid or None");
+		std::string out_act = net.value("output_activation", "None"); std::transform(out_act.begin(), out_act.end(), out_act.begin(), ::tolower);
+		require(out_act == "none", "GatedMLP: output_activation must be None");
+		m_gated_block.n_in = 32; m_gated_block.n_hidden = (uint32_t)width; m_gated_block.n_out = 16; m_gated_block.dtype = NGP_DTYPE_F16;
+	} else if (config.contains("network")) require(config["network"].value("n_neurons", 64) == 64 && config["network"].value("n_hidden_layers", 2) == 2, "network must be 64 neurons x 2 hidden layers");
 	m_num_levels = 16;
 	const uint32_t n_dims = gridmlp_n_dims();
 	const uint32_t log2_hashmap_size = (uint32_t)enc.value("log2_hashmap_size", 15);
@@ -46,6 +57,13 @@ void Testbed::reset_network_gridmlp() {  // testbed.cu:2249-2470, Image / Sdf br
 	check(ngp_hip_gridmlp_make_desc_host(n_dims, m_num_levels, log2_hashmap_size, m_base_grid_resolution, m_per_level_scale, &m_desc), "ngp_hip_gridmlp_make_desc_host");
 	m_n_params = ngp_hip_gridmlp_n_params_host(&m_desc);
 	m_n_matrix_params = NGP_GRIDMLP_N_PARAMS;
+	m_matrices.clear();
+	if (m_gated) {   // gate, up, down, grid
+		const uint32_t f = m_gated_block.n_hidden;
+		add_matrix(f, 32); add_matrix(f, 32); add_matrix(16, f);
+		m_n_matrix_params = 80u * f;
+		m_n_params = (size_t)m_n_matrix_params + 2u * (size_t)m_desc.n_grid_entries;
+	} else { add_matrix(64, 32); add_matrix(64, 64); add_matrix(16, 64); }
 	m_desc_gpu.resize(sizeof(NgpNetDesc));
 	m_desc_gpu.copy_from_host(&m_desc, sizeof(NgpNetDesc));
 	std::string loss = config.contains("loss") ? config["loss"].value("otype", "L2") : std::string("L2");
@@ -60,34 +78,82 @@ void Testbed::reset_network_gridmlp() {  // testbed.cu:2249-2470, Image / Sdf br
 	m_params.resize(m_n_params * 2); m_inference_params.resize(m_n_params * 2); m_grads.resize(m_n_params * 2);
 	m_master.resize(m_n_params * 4); m_first_moments.resize(m_n_params * 4); m_second_moments.resize(m_n_params * 4); m_ema.resize(m_n_params * 4);
 	m_first_moments.memset(0, m_stream); m_second_moments.memset(0, m_stream); m_ema.memset(0, m_stream); m_grads.memset(0, m_stream);
-	check(ngp_hip_gridmlp_init_params(m_stream, &m_desc, m_seed, m_master.as<float>(), m_params.as<uint16_t>(), m_inference_params.as<uint16_t>()), "ngp_hip_gridmlp_init_params");
+	if (m_gated) gated_init_params();
+	else check(ngp_hip_gridmlp_init_params(m_stream, &m_desc, m_seed, m_master.as<float>(), m_params.as<uint16_t>(), m_inference_params.as<uint16_t>()), "ngp_hip_gridmlp_init_params");
+	if (m_gated && m_dloss.bytes()) m_dloss.memset(0, m_stream);
 	m_loss_scalar_gpu.resize(4);
 	m_training_step = 0;
 	m_loss_scalar = 0.f;
 	sync();
 }
 
+// as the fused MLP's parameters start: uniform within sqrt(6 / (rows + columns)) per matrix (a down projection's 16 padded outputs counted), the grid within 1e-4, one number of the
+// stream per parameter
+void Testbed::gated_init_params() {
+	std::vector<float> w(m_n_params);
+	std::vector<uint16_t> h(m_n_params);
+	Pcg32 rng(m_seed);
+	size_t i = 0;
+	auto fill = [&](size_t end, float scale) { for (; i < end; ++i) { w[i] = rng.next_float() * (2.0f * scale) - scale; h[i] = float_to_half_bits(w[i]); } };
+	for (const NgpMuonMatrix& m : m_matrices) fill((size_t)m.offset + (size_t)m.rows * m.cols, std::sqrt(6.0f / (float)(m.rows + m.cols)));
+	fill(m_n_params, 1e-4f);
+	m_master.copy_from_host(w.data(), w.size() * 4);
+	m_params.copy_from_host(h.data(), h.size() * 2);
+	m_inference_params.copy_from_host(h.data(), h.size() * 2);
+}
+
+// the network's outputs (rows of gm_out_stride()); x_saved (may be null: rendering): the encoded features for the backward pass
+void Testbed::gridmlp_inference(const uint16_t* params, const float* pos, uint32_t n_dims, uint32_t n, uint16_t* out, uint16_t* x_saved, const char* who) {
+	const NgpNetDesc* desc = m_desc_gpu.as<NgpNetDesc>();
+	if (!m_gated) {
+		check(ngp_hip_gridmlp_forward(m_stream, n_dims, desc, params, pos, n_dims, n, out, gm_out_stride(), x_saved), who);
+		return;
+	}
+	if (!x_saved) { m_x_saved.enlarge((size_t)n * 32 * 2); x_saved = m_x_saved.as<uint16_t>(); }
+	m_enc_ws.enlarge(ngp_hip_nerf_encode_workspace_bytes(n));
+	m_gated_ws.enlarge(std::max<uint64_t>(16, ngp_hip_gated_ffn_workspace_bytes(&m_gated_block, n, 0)));
+	const uint32_t f = m_gated_block.n_hidden;
+	check(ngp_hip_grid_encode(m_stream, n_dims, desc, params + m_n_matrix_params, pos, n_dims, n, x_saved, m_enc_ws.data(), m_enc_ws.bytes()), who);
+	check(ngp_hip_gated_ffn_forward(m_stream, &m_gated_block, n, x_saved, 32, params, params + 32 * f, params + 64 * f, out, gm_out_stride(), m_gated_ws.data(), m_gated_ws.bytes()), who);
+}
+
 // Trainer::training_step (forward, loss, backward) + optimizer_step(128) + Trainer::loss (sum of the per-element values)
 void Testbed::gridmlp_training_step(const float* pos, uint32_t n_dims, const float* targets, uint32_t dims, uint32_t n, bool get_loss_scalar) {
 	if (n % 256) throw std::runtime_error{"training batch size must be a multiple of 256"};
-	m_gm_out.enlarge((size_t)n * GM_OUT_STRIDE * 2); m_x_saved.enlarge((size_t)n * 32 * 2); m_dloss.enlarge((size_t)n * GM_OUT_STRIDE * 2);
+	m_gm_out.enlarge((size_t)n * gm_out_stride() * 2); m_x_saved.enlarge((size_t)n * 32 * 2);
+	const size_t dloss_bytes = (size_t)n * gm_out_stride() * 2;
+	const bool grown = m_dloss.bytes() < dloss_bytes;
+	m_dloss.enlarge(dloss_bytes);
+	if (m_gated && grown) m_dloss.memset(0, m_stream);   // the loss writes channels 0..3 of the block's 16
 	m_gm_values.enlarge((size_t)n * dims * 4);
 	m_bwd_scratch.enlarge(ngp_hip_gridmlp_backward_scratch_bytes(n));
 	const NgpNetDesc* desc = m_desc_gpu.as<NgpNetDesc>();
 	profile_begin(PK_FORWARD);
 	// fused or encode + MLP kernel: measured on this workload (testbed.h ENetworkPass) — random SDF points want the two-kernel pass, stratified image batches the fused one
-	if (tuner_pick(m_stream)) {
+	if (m_gated) gridmlp_inference(m_params.as<uint16_t>(), pos, n_dims, n, m_gm_out.as<uint16_t>(), m_x_saved.as<uint16_t>(), "gated forward");
+	else if (tuner_pick(m_stream)) {
 		m_enc_ws.enlarge(ngp_hip_nerf_encode_workspace_bytes(n));
-		check(ngp_hip_gridmlp_forward_ws(m_stream, n_dims, desc, m_params.as<uint16_t>(), pos, n_dims, n, m_gm_out.as<uint16_t>(), GM_OUT_STRIDE, m_x_saved.as<uint16_t>(), m_enc_ws.data(), m_enc_ws.bytes()), "gridmlp_forward (two kernels)");
+		check(ngp_hip_gridmlp_forward_ws(m_stream, n_dims, desc, m_params.as<uint16_t>(), pos, n_dims, n, m_gm_out.as<uint16_t>(), gm_out_stride(), m_x_saved.as<uint16_t>(), m_enc_ws.data(), m_enc_ws.bytes()), "gridmlp_forward (two kernels)");
 	} else {
-		check(ngp_hip_gridmlp_forward(m_stream, n_dims, desc, m_params.as<uint16_t>(), pos, n_dims, n, m_gm_out.as<uint16_t>(), GM_OUT_STRIDE, m_x_saved.as<uint16_t>()), "gridmlp_forward");
+		check(ngp_hip_gridmlp_forward(m_stream, n_dims, desc, m_params.as<uint16_t>(), pos, n_dims, n, m_gm_out.as<uint16_t>(), gm_out_stride(), m_x_saved.as<uint16_t>()), "gridmlp_forward");
 	}
-	tuner_done(m_stream);
+	if (!m_gated) tuner_done(m_stream);
 	profile_end(PK_FORWARD, n);
-	check(ngp_hip_loss_and_gradient(m_stream, (int)m_nerf.training.loss_type, n, dims, LOSS_SCALE, m_gm_out.as<uint16_t>(), GM_OUT_STRIDE, targets, m_gm_values.as<float>(), m_dloss.as<uint16_t>(),
-	                                GM_OUT_STRIDE), "loss_and_gradient");
+	check(ngp_hip_loss_and_gradient(m_stream, (int)m_nerf.training.loss_type, n, dims, LOSS_SCALE, m_gm_out.as<uint16_t>(), gm_out_stride(), targets, m_gm_values.as<float>(), m_dloss.as<uint16_t>(),
+	                                gm_out_stride()), "loss_and_gradient");
 	profile_begin(PK_BACKWARD);
-	check(ngp_hip_gridmlp_backward(m_stream, n_dims, desc, m_params.as<uint16_t>(), pos, n_dims, n, m_x_saved.as<uint16_t>(), m_dloss.as<uint16_t>(), GM_OUT_STRIDE, m_grads.as<uint16_t>(),
+	if (m_gated) {
+		const uint32_t f = m_gated_block.n_hidden;
+		uint16_t *const w = m_params.as<uint16_t>(), *const g = m_grads.as<uint16_t>();
+		m_gated_dx.enlarge((size_t)n * 32 * 2);
+		m_gated_ws.enlarge(std::max<uint64_t>(16, ngp_hip_gated_ffn_workspace_bytes(&m_gated_block, n, NGP_FFN_BACKWARD)));
+		check(ngp_hip_gated_ffn_backward(m_stream, &m_gated_block, n, m_x_saved.as<uint16_t>(), 32, w, w + 32 * f, w + 64 * f, m_dloss.as<uint16_t>(), gm_out_stride(), m_gated_dx.as<uint16_t>(), 32, g,
+		                                 g + 32 * f, g + 64 * f, m_gated_ws.data(), m_gated_ws.bytes()), "gated_ffn_backward");
+		m_bwd_scratch.enlarge(ngp_hip_grid_gradient_scratch_bytes(n));
+		// as ngp_hip_gridmlp_backward: the stratified image batch runs along x, SDF samples have no order
+		check(ngp_hip_grid_gradient(m_stream, n_dims, desc, pos, n_dims, n, m_gated_dx.as<uint16_t>(), n_dims == 2, g + m_n_matrix_params, m_bwd_scratch.data(), m_bwd_scratch.bytes()), "grid_gradient");
+	} else
+	check(ngp_hip_gridmlp_backward(m_stream, n_dims, desc, m_params.as<uint16_t>(), pos, n_dims, n, m_x_saved.as<uint16_t>(), m_dloss.as<uint16_t>(), gm_out_stride(), m_grads.as<uint16_t>(),
 	                               m_bwd_scratch.data(), m_bwd_scratch.bytes()), "gridmlp_backward");
 	profile_end(PK_BACKWARD, n);
 	if (get_loss_scalar) {
@@ -170,14 +236,13 @@ void Testbed::train_image(uint32_t batch_size, bool get_loss_scalar) {  // testb
 void Testbed::render_image(RenderBuffer& rb) {  // testbed_image.cu:293-360 (no activation visualisation)
 	const uint32_t n_pixels = (uint32_t)rb.res[0] * (uint32_t)rb.res[1];
 	const uint32_t n_elements = next_multiple(n_pixels, BATCH_SIZE_GRANULARITY);
-	m_image.render_coords.enlarge((size_t)n_elements * 8); m_image.render_out.enlarge((size_t)n_elements * GM_OUT_STRIDE * 2);
+	m_image.render_coords.enlarge((size_t)n_elements * 8); m_image.render_out.enlarge((size_t)n_elements * gm_out_stride() * 2);
 	const float sc[2] = {m_screen_center[0] - 0.5f, m_screen_center[1] - 0.5f};
 	HIP_TRY(hipMemsetAsync(m_image.render_coords.data(), 0, (size_t)n_elements * 8, (hipStream_t)m_stream));
 	check(ngp_hip_image_init_coords(m_stream, m_image.render_coords.as<float>(), rb.res, m_image.resolution, m_scale, m_image.pos, sc, m_snap_to_pixel_centers, rb.spp), "image_init_coords");
 	join_side_ema();
-	check(ngp_hip_gridmlp_forward(m_stream, 2, m_desc_gpu.as<NgpNetDesc>(), m_inference_params.as<uint16_t>(), m_image.render_coords.as<float>(), 2, n_elements, m_image.render_out.as<uint16_t>(),
-	                              GM_OUT_STRIDE, nullptr), "gridmlp_forward (render)");
-	check(ngp_hip_image_shade(m_stream, rb.res, m_image.render_coords.as<float>(), m_image.render_out.as<uint16_t>(), GM_OUT_STRIDE, rb.frame_buffer.as<float>(), rb.depth_buffer.as<float>(),
+	gridmlp_inference(m_inference_params.as<uint16_t>(), m_image.render_coords.as<float>(), 2, n_elements, m_image.render_out.as<uint16_t>(), nullptr, "gridmlp_forward (render)");
+	check(ngp_hip_image_shade(m_stream, rb.res, m_image.render_coords.as<float>(), m_image.render_out.as<uint16_t>(), gm_out_stride(), rb.frame_buffer.as<float>(), rb.depth_buffer.as<float>(),
 	                          m_image.linear_colors), "image_shade");
 }
 
@@ -187,15 +252,15 @@ float Testbed::compute_image_mse(bool quantize_to_byte) {  // testbed_image.cu:4
 	const uint32_t max_batch = 1u << 20;
 	m_image.se.enlarge((size_t)(n_elements + 256) * 4);
 	DeviceBuffer pos, targets, pred;
-	pos.resize((size_t)max_batch * 8); targets.resize((size_t)max_batch * 12); pred.resize((size_t)max_batch * GM_OUT_STRIDE * 2);
+	pos.resize((size_t)max_batch * 8); targets.resize((size_t)max_batch * 12); pred.resize((size_t)max_batch * gm_out_stride() * 2);
 	for (uint32_t offset = 0; offset < n_elements; offset += max_batch) {
 		const uint32_t count = std::min(max_batch, n_elements - offset);
 		const uint32_t batch = (count + 255u) & ~255u;
 		check(ngp_hip_image_coords_from_idx(m_stream, batch, offset, pos.as<float>(), m_image.resolution), "image_coords_from_idx");
 		check(ngp_hip_image_eval_and_snap(m_stream, batch, m_image.data.data(), m_image.type, pos.as<float>(), m_image.resolution, targets.as<float>(), 3, 1, m_image.linear_colors), "eval_image_and_snap");
 		join_side_ema();
-		check(ngp_hip_gridmlp_forward(m_stream, 2, m_desc_gpu.as<NgpNetDesc>(), m_inference_params.as<uint16_t>(), pos.as<float>(), 2, batch, pred.as<uint16_t>(), GM_OUT_STRIDE, nullptr), "gridmlp_forward (mse)");
-		check(ngp_hip_image_mse(m_stream, count, targets.as<float>(), pred.as<uint16_t>(), GM_OUT_STRIDE, m_image.se.as<float>() + offset, quantize_to_byte), "image_mse");
+		gridmlp_inference(m_inference_params.as<uint16_t>(), pos.as<float>(), 2, batch, pred.as<uint16_t>(), nullptr, "gridmlp_forward (mse)");
+		check(ngp_hip_image_mse(m_stream, count, targets.as<float>(), pred.as<uint16_t>(), gm_out_stride(), m_image.se.as<float>() + offset, quantize_to_byte), "image_mse");
 	}
 	check(ngp_hip_reduce_sum_f32(m_stream, m_image.se.as<float>(), n_elements, m_loss_scalar_gpu.as<float>()), "reduce_sum");
 	sync();

@@ -441,16 +441,16 @@ PYBIND11_MODULE(pyngp, m) {
 				if (b.ndim != 2 || (uint32_t)b.shape[1] != n_dims) throw std::runtime_error{"positions must be (N, n_dims)"};
 				const uint32_t n = (uint32_t)b.shape[0];
 				DeviceBuffer d_pos, d_out;
-				d_pos.resize((size_t)n * n_dims * 4); d_out.resize((size_t)n * 8);
+				const uint32_t stride = t.gm_out_stride();
+				d_pos.resize((size_t)n * n_dims * 4); d_out.resize((size_t)n * stride * 2);
 				d_pos.copy_from_host(b.ptr, (size_t)n * n_dims * 4);
 				t.join_side_ema();
-				if (ngp_hip_gridmlp_forward(t.stream(), n_dims, t.m_desc_gpu.as<NgpNetDesc>(), t.m_inference_params.as<uint16_t>(), d_pos.as<float>(), n_dims, n, d_out.as<uint16_t>(), 4, nullptr))
-					throw std::runtime_error{ngp_hip_last_error()};
+				t.gridmlp_inference(t.m_inference_params.as<uint16_t>(), d_pos.as<float>(), n_dims, n, d_out.as<uint16_t>(), nullptr, "gridmlp_inference");
 				t.sync();
-				std::vector<uint16_t> h((size_t)n * 4);
+				std::vector<uint16_t> h((size_t)n * stride);
 				d_out.copy_to_host(h.data(), h.size() * 2);
 				py::array_t<float> out({(py::ssize_t)n, (py::ssize_t)4});
-				for (size_t i = 0; i < h.size(); ++i) out.mutable_data()[i] = half_bits_to_float(h[i]);
+				for (size_t i = 0; i < (size_t)n * 4; ++i) out.mutable_data()[i] = half_bits_to_float(h[i / 4 * stride + i % 4]);
 				return out;
 			}, py::arg("positions"))
 		.def_property_readonly("image_resolution", [](Testbed& t) { return std::vector<int>{t.m_image.resolution[0], t.m_image.resolution[1]}; })

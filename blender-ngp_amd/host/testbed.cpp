@@ -704,6 +704,7 @@ static ELossType string_to_loss_type(std::string s) {  // testbed.cu:2220-2240
 void Testbed::parse_optimizer_config(const Json& opt_in) {
 	// configs/nerf/base.json:5-22: Ema{decay} o ExponentialDecay{decay_start, decay_interval, decay_base} o Adam{...}; any subset of the wrappers
 	m_use_ema = false; m_has_decay = false;
+	m_muon = Muon();
 	m_ema_decay = 0.95f; m_decay_start = 0; m_decay_interval = 1; m_decay_end = 0; m_decay_base = 1.0f;
 	const Json* o = &opt_in;
 	while (true) {
@@ -719,8 +720,16 @@ void Testbed::parse_optimizer_config(const Json& opt_in) {
 			m_beta1 = (float)o->value("beta1", 0.9); m_beta2 = (float)o->value("beta2", 0.999);
 			m_epsilon = (float)o->value("epsilon", 1e-8); m_l2_reg = (float)o->value("l2_reg", 1e-8);
 			break;
+		} else if (lower == "muon") {   // Muon{...; nested: Adam}: the matrices by Muon, the encoding by the nested Adam
+			m_muon.enabled = true;
+			m_muon.learning_rate = (float)o->value("learning_rate", 0.02); m_muon.momentum = (float)o->value("momentum", 0.95);
+			m_muon.weight_decay = (float)o->value("weight_decay", 0.0); m_muon.epsilon = (float)o->value("epsilon", 1e-7);
+			m_muon.nesterov = o->value("nesterov", true);
+			const int it = (int)o->value("n_iterations", 5);
+			if (it < 1 || it > 32) throw std::runtime_error{"optimizer Muon: n_iterations must be 1 .. 32"};
+			m_muon.n_iterations = (uint32_t)it;
 		} else {
-			throw std::runtime_error{"optimizer otype '" + otype + "' is not part of the NeRF hot path (Ema / ExponentialDecay / Adam are)"};
+			throw std::runtime_error{"optimizer otype '" + otype + "' is not part of the NeRF hot path (Ema / ExponentialDecay / Muon / Adam are)"};
 		}
 		if (!o->contains("nested")) throw std::runtime_error{"optimizer '" + otype + "' needs a nested optimizer"};
 		o = &o->at("nested");
@@ -743,7 +752,8 @@ void TrainableBuffer::reset(int w, int h, uint32_t dims, const Json& optimizer_c
 		} else if (lower == "adam") {
 			base_learning_rate = (float)o->value("learning_rate", 1e-3); beta1 = (float)o->value("beta1", 0.9); beta2 = (float)o->value("beta2", 0.999); epsilon = (float)o->value("epsilon", 1e-8);
 			break;
-		} else throw std::runtime_error{"optimizer otype '" + lower + "' of a trainable buffer: Ema / ExponentialDecay / Adam are built"};
+		} else if (lower != "muon")   // a buffer has no matrices: the Adam nested in Muon
+			throw std::runtime_error{"optimizer otype '" + lower + "' of a trainable buffer: Ema / ExponentialDecay / Adam are built"};
 		o = o->contains("nested") ? &o->at("nested") : nullptr;
 	}
 	learning_rate = base_learning_rate;
@@ -767,6 +777,13 @@ void TrainableBuffer::optimizer_step(void* stream, float loss_scale) {
 	                                           params.as<float>(), first_moments.as<float>(), second_moments.as<float>(), use_ema ? ema.as<float>() : nullptr);
 	if (rc != 0) throw std::runtime_error{std::string("ngp_hip_optimizer_step_f32: ") + ngp_hip_last_error()};
 	if (has_decay && step >= decay_start && (decay_end == 0 || step < decay_end) && decay_interval && step % decay_interval == 0) learning_rate *= decay_base;   // as Testbed::optimizer_step
+}
+
+void Testbed::add_matrix(uint32_t rows, uint32_t cols) {   // behind the last one
+	NgpMuonMatrix m;
+	m.offset = m_matrices.empty() ? 0 : m_matrices.back().offset + (uint64_t)m_matrices.back().rows * m_matrices.back().cols;
+	m.rows = rows; m.cols = cols;
+	m_matrices.push_back(m);
 }
 
 void Testbed::reset_network(bool clear_density_grid) {  // testbed.cu:2249-2470
@@ -826,6 +843,15 @@ void Testbed::reset_network(bool clear_density_grid) {  // testbed.cu:2249-2470
 	NgpNetVariant nv;
 	m_n_matrix_params = ngp_hip_net_mlp_params_host(net_variant(nv));
 	m_n_params = (size_t)m_n_matrix_params + 2u * (size_t)m_desc.n_grid_entries;
+	m_matrices.clear();   // density network, colour network: the parameter order of ngp_hip_nerf_init_params
+	add_matrix(64, 32); add_matrix(16, 64);
+	const uint32_t rgb_in = m_n_extra_dims ? 48 : 32;
+	if (m_n_rgb_hidden_layers == 0) add_matrix(16, rgb_in);
+	else {
+		add_matrix(64, rgb_in);
+		for (uint32_t l = 1; l < m_n_rgb_hidden_layers; ++l) add_matrix(64, 64);
+		add_matrix(16, 64);
+	}
 	tr.reset_extra_dims(m_rng);   // testbed.cu:2347
 	m_desc_gpu.resize(sizeof(NgpNetDesc));
 	m_desc_gpu.copy_from_host(&m_desc, sizeof(NgpNetDesc));
@@ -1075,7 +1101,7 @@ void Testbed::dp_gather_optimizer_state() {
 	// this rank's shard.  What rebuilds the whole state clears the flag instead: reset_network, load_snapshot.
 	if (m_dp_state_stale && !m_dp_comm)
 		throw std::runtime_error{"dp_gather_optimizer_state: the fp32 optimizer state is stale outside this rank's shard and the data-parallel communicator is gone — gather on ALL ranks BEFORE shutdown_data_parallel(); now only reset_network() / load_snapshot() rebuild the state"};
-	if (m_dp_comm && m_world_size >= 2 && m_dp_sharded_optimizer && m_n_params != 0) {
+	if (m_dp_comm && m_world_size >= 2 && dp_sharded_step() && m_n_params != 0) {
 		const uint32_t shard = next_multiple(((uint32_t)m_n_params + m_world_size - 1) / m_world_size, 8u);
 		check(ngp_rccl_allgather_f32(m_dp_comm, m_stream, m_master.as<float>(), shard), "ngp_rccl_allgather_f32 (master weights)");
 		check(ngp_rccl_allgather_f32(m_dp_comm, m_stream, m_first_moments.as<float>(), shard), "ngp_rccl_allgather_f32 (first moments)");
@@ -1125,7 +1151,7 @@ void Testbed::train_nerf(uint32_t target_batch_size, bool get_loss_scalar) {  //
 		double sum[3];
 		m_dp_shm->all_sum(m_dp_exchange_step++, mine, sum);
 		train_nerf_dp_backward(B, (uint32_t)sum[0], (uint32_t)sum[1], get_loss_scalar, (float)sum[2]);
-		if (!m_dp_sharded_optimizer) {   // the round-1 / round-2 exchange: fp16 all-reduce of the whole gradient vector, the optimizer step replicated on every rank
+		if (!dp_sharded_step()) {   // the round-1 / round-2 exchange: fp16 all-reduce of the whole gradient vector, the optimizer step replicated on every rank
 			profile_begin(PK_GRAD_EXCHANGE);
 			check(ngp_rccl_allreduce_grads(m_dp_comm, m_stream, m_grads.as<uint16_t>(), m_n_params), "ngp_rccl_allreduce_grads");
 			profile_end(PK_GRAD_EXCHANGE, m_n_params);
@@ -1738,11 +1764,20 @@ void Testbed::require_inference_params(const char* who, bool collective) {
 }
 
 void Testbed::optimizer_step() {  // Trainer::optimizer_step(stream, LOSS_SCALE) (testbed_nerf.cu:2950)
-	if (m_dp_comm && m_dp_sharded_optimizer) { optimizer_step_sharded(); return; }
+	if (m_dp_comm && dp_sharded_step()) { optimizer_step_sharded(); return; }
 	if (m_dp_state_stale) throw std::runtime_error{"optimizer step on fp32 state that sharded data-parallel steps left stale outside this rank's shard: call dp_gather_optimizer_state() on all ranks before shutdown_data_parallel()"};
 	++m_optimizer_step;
-	const uint32_t mask = (m_train_network ? 1u : 0u) | (m_train_encoding ? 2u : 0u);
+	uint32_t mask = (m_train_network ? 1u : 0u) | (m_train_encoding ? 2u : 0u);
 	const float ema_decay = m_use_ema ? m_ema_decay : 0.0f;
+	if (m_muon.enabled && m_train_network) {   // the matrices; the launch below then steps the encoding and the Ema copy of both
+		join_side_ema();
+		const uint32_t n = (uint32_t)m_matrices.size();
+		m_muon_workspace.enlarge(std::max<uint64_t>(16, ngp_hip_muon_workspace_bytes(n, m_matrices.data())));
+		check(ngp_hip_muon_step(m_stream, n, m_matrices.data(), m_muon.learning_rate * (m_base_learning_rate > 0.0f ? m_learning_rate / m_base_learning_rate : 1.0f), m_muon.momentum, m_muon.weight_decay,
+		                        m_muon.epsilon, m_muon.nesterov, m_muon.n_iterations, LOSS_SCALE, NGP_DTYPE_F16, m_grads.as<uint16_t>(), m_master.as<float>(), m_params.as<uint16_t>(),
+		                        m_first_moments.as<float>(), m_muon_workspace.data(), m_muon_workspace.bytes()), "muon_step");
+		mask &= ~1u;
+	}
 	// The Ema stage (12 of the step's 36 bytes per parameter: read the new fp16 weight and the fp32 average, write the average and the fp16 inference weight) feeds renderers
 	// and snapshots, not the next training step: `ema_on_side_stream` runs it on stream B beside the next step's network pass instead of in front of it.  Element for element the
 	// arithmetic of the one-launch step (NGP_OPT_NO_EMA / NGP_OPT_EMA_ONLY: the split of the data-parallel path, tests/test_dp_gpu.py).  OFF by default — measured
@@ -2431,7 +2466,12 @@ void Testbed::save_snapshot(const std::string& path, bool include_optimizer_stat
 		Json decay = Json::object();
 		decay["otype"] = Json("ExponentialDecay");
 		decay["learning_rate"] = Json((double)m_learning_rate);
-		decay["nested"] = adam;
+		if (m_muon.enabled) {
+			Json muon = Json::object();
+			muon["otype"] = Json("Muon");
+			muon["nested"] = adam;
+			decay["nested"] = muon;
+		} else decay["nested"] = adam;
 		Json ema = Json::object();
 		ema["otype"] = Json("Ema");
 		ema["ema_step"] = Json(m_optimizer_step);
@@ -2558,6 +2598,7 @@ void Testbed::load_snapshot(const std::string& path) {
 				m_optimizer_step = (uint32_t)o->value("current_step", 0);
 				take(*o, "first_moments_binary", m_first_moments);
 				take(*o, "second_moments_binary", m_second_moments);
+			} else if (otype == "Muon") {   // its momentum is in the nested Adam's first moments
 			} else {
 				fprintf(stderr, "load_snapshot: optimizer block of type '%s' is not understood: skipped\n", otype.c_str());
 			}

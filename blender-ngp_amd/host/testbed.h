@@ -376,6 +376,13 @@ public:
 	void train_sdf(uint32_t batch_size, bool get_loss_scalar);                        // testbed_sdf.cu:1229-1252 on user-provided (pos, distance) pairs
 	void render_image(RenderBuffer& rb);                                              // testbed_image.cu:293-360
 	float compute_image_mse(bool quantize_to_byte);                                   // testbed_image.cu:461-523
+	// network.otype "GatedMLP" of the Image / Sdf configs: encoding -> ngp_hip_gated_ffn (n_neurons hidden columns) -> 16 outputs, in place of the 64 x 64 MLP
+	bool m_gated = false;
+	NgpGatedFfn m_gated_block{};
+	DeviceBuffer m_gated_ws, m_gated_dx;
+	uint32_t gm_out_stride() const { return m_gated ? 16u : 4u; }
+	void gated_init_params();
+	void gridmlp_inference(const uint16_t* params, const float* pos, uint32_t n_dims, uint32_t n, uint16_t* out, uint16_t* x_saved, const char* who);
 	uint32_t gridmlp_n_dims() const { return m_testbed_mode == ETestbedMode::Image ? 2u : 3u; }
 	void gridmlp_training_step(const float* pos, uint32_t n_dims, const float* targets, uint32_t dims, uint32_t n, bool get_loss_scalar);
 	uint32_t m_n_matrix_params = NGP_MLP_N_PARAMS;     // parameters that get weight decay (the MLPs): 10240 NeRF (base family), 7168 grid -> MLP
@@ -586,6 +593,17 @@ public:
 	size_t m_n_params = 0;
 	uint32_t m_optimizer_step = 0;
 	float m_learning_rate = 1e-2f, m_base_learning_rate = 1e-2f, m_beta1 = 0.9f, m_beta2 = 0.99f, m_epsilon = 1e-15f, m_l2_reg = 1e-6f;
+	// optimizer.otype "Muon": the network's matrices take ngp_hip_muon_step, everything else (the encoding) the Adam nested in it.  The momentum lives where Adam keeps the
+	// matrices' first moments; its learning rate decays with Adam's.
+	struct Muon {
+		bool enabled = false, nesterov = true;
+		float learning_rate = 0.02f, momentum = 0.95f, weight_decay = 0.0f, epsilon = 1e-7f;
+		uint32_t n_iterations = 5;
+	} m_muon;
+	std::vector<NgpMuonMatrix> m_matrices;       // the network's weight matrices in the parameter vector (reset_network)
+	DeviceBuffer m_muon_workspace;
+	void add_matrix(uint32_t rows, uint32_t cols);
+	bool dp_sharded_step() const { return m_dp_sharded_optimizer && !m_muon.enabled; }   // an update needs its whole matrix: Muon steps run replicated
 	float m_ema_decay = 0.95f;
 	bool m_use_ema = true;
 	uint32_t m_decay_start = 20000, m_decay_interval = 10000, m_decay_end = 0;

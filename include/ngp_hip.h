@@ -472,6 +472,14 @@ int ngp_hip_grid_backward(void* stream, uint32_t n_dims, const NgpNetDesc* desc_
 int ngp_hip_grid_backward_unordered(void* stream, uint32_t n_dims, const NgpNetDesc* desc_dev, const float* pos, uint32_t pos_stride_floats, uint32_t n,
                           const uint16_t* dL_dx_planes, uint16_t* grid_grad, void* scratch, uint64_t scratch_bytes);
 
+/* The encoding alone, for networks that are not one of the fused kernels (the gated block below): features [n][32] fp16 from positions, and the table's gradient from the features'
+ * gradient.  grid: the table, [n_grid_entries][2] fp16; workspace: ngp_hip_nerf_encode_workspace_bytes(n).  ordered: see ngp_hip_grid_backward (1) / _unordered (0); n a multiple of 256. */
+int ngp_hip_grid_encode(void* stream, uint32_t n_dims, const NgpNetDesc* desc_dev, const uint16_t* grid, const float* pos, uint32_t pos_stride_floats, uint32_t n, uint16_t* features,
+                        void* workspace, uint64_t workspace_bytes);
+uint64_t ngp_hip_grid_gradient_scratch_bytes(uint32_t n);
+int ngp_hip_grid_gradient(void* stream, uint32_t n_dims, const NgpNetDesc* desc_dev, const float* pos, uint32_t pos_stride_floats, uint32_t n, const uint16_t* dL_dfeatures, int ordered,
+                          uint16_t* grid_grad, void* scratch, uint64_t scratch_bytes);
+
 /* ============================ Muon ============================
  * The optimizer step of matrix parameters next to Adam (ngp_hip_optimizer_step; no reference counterpart): momentum, the update orthogonalised by Newton-Schulz products, the weights.
  *   g = grads / loss_scale;  m <- momentum m + g;  u = nesterov ? g + momentum m : m;  X = u / (|u|_F + epsilon)

@@ -1,0 +1,270 @@
+"""The gated block and the Muon step where the framework calls them: behind the hash grid through the C ABI (encode, block, loss, block backward, table gradient, Muon and Adam), and
+through `pyngp` (network.otype "GatedMLP" of the Image / Sdf configs, optimizer.otype "Muon" of all modes)."""
+import json
+import os
+import sys
+
+import numpy as np
+import pytest
+import torch
+
+import capi
+import ffn_reference as F
+import helpers as H
+import muon_reference as M
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+sys.path[:0] = [os.path.join(ROOT, "blender-ngp_amd")]
+pytestmark = pytest.mark.gpu
+CFG = os.path.join(ROOT, "blender-ngp_amd", "configs")
+
+
+def make_desc(ngp, n_dims, log2=12, base=16, pls=1.5):
+    d = np.zeros(1, capi.NET_DESC)
+    capi.check(ngp.ngp_hip_gridmlp_make_desc_host(n_dims, 16, log2, base, H.f32(pls), d.ctypes.data))
+    return d
+
+
+def random_grid(desc, seed=0, scale=0.5):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (torch.rand(int(desc["n_grid_entries"][0]) * 2, generator=g, device="cuda") * 2 - 1).mul(scale).half()
+
+
+def positions(n, n_dims, seed=1):
+    return torch.rand(n, n_dims, generator=torch.Generator(device="cuda").manual_seed(seed), device="cuda")
+
+
+def view(ptr, n, typestr="<f2"):
+    """n elements at a device address the library owns"""
+    class Holder:
+        __cuda_array_interface__ = {"shape": (n,), "typestr": typestr, "data": (ptr, False), "version": 3}
+    return torch.as_tensor(Holder(), device="cuda")
+
+
+@pytest.mark.parametrize("n_dims", [2, 3])
+@pytest.mark.parametrize("n", [1, 65, 1000, 40000])
+def test_encode_alone_gives_the_fused_pass_its_features(ngp, cuda, n_dims, n):
+    desc = make_desc(ngp, n_dims)
+    d_desc, grid, pos = H.to_dev(desc, cuda), random_grid(desc), positions(n, n_dims)
+    params = torch.cat([torch.zeros(7168, dtype=torch.float16, device="cuda"), grid])
+    out, saved = torch.empty(n, 4, dtype=torch.float16, device="cuda"), torch.empty(n, 32, dtype=torch.float16, device="cuda")
+    capi.check(ngp.ngp_hip_gridmlp_forward(None, n_dims, d_desc.data_ptr(), params.data_ptr(), pos.data_ptr(), n_dims, n, out.data_ptr(), 4, saved.data_ptr()))
+    size = ngp.ngp_hip_nerf_encode_workspace_bytes(n)
+    ws = torch.empty(size, dtype=torch.uint8, device="cuda")
+    rows = torch.full((n + 4, 32), 9.0, dtype=torch.float16, device="cuda")
+    capi.check(ngp.ngp_hip_grid_encode(None, n_dims, d_desc.data_ptr(), grid.data_ptr(), pos.data_ptr(), n_dims, n, rows.data_ptr(), ws.data_ptr(), size))
+    torch.cuda.synchronize()
+    assert torch.equal(rows[:n], saved) and (rows[n:] == 9.0).all()
+
+
+@pytest.mark.parametrize("n_dims,ordered", [(2, 1), (3, 0)])
+def test_table_gradient_from_rows(ngp, cuda, n_dims, ordered):
+    n, desc = 2048, make_desc(ngp, n_dims)
+    d_desc, pos = H.to_dev(desc, cuda), positions(n, n_dims)
+    rows = torch.randn(n, 32, generator=torch.Generator(device="cuda").manual_seed(3), device="cuda").mul(0.05).half()
+    planes = rows.view(n, 16, 2).permute(1, 0, 2).contiguous()
+    size = int(desc["n_grid_entries"][0]) * 2
+    got, want = (torch.full((size,), 7.0, dtype=torch.float16, device="cuda") for _ in range(2))
+    sb = ngp.ngp_hip_grid_backward_scratch_bytes(n)
+    s1 = torch.empty(sb, dtype=torch.uint8, device="cuda")
+    fn = ngp.ngp_hip_grid_backward if ordered else ngp.ngp_hip_grid_backward_unordered
+    capi.check(fn(None, n_dims, d_desc.data_ptr(), pos.data_ptr(), n_dims, n, planes.data_ptr(), want.data_ptr(), s1.data_ptr(), sb))
+    sg = ngp.ngp_hip_grid_gradient_scratch_bytes(n)
+    s2 = torch.empty(sg, dtype=torch.uint8, device="cuda")
+    capi.check(ngp.ngp_hip_grid_gradient(None, n_dims, d_desc.data_ptr(), pos.data_ptr(), n_dims, n, rows.data_ptr(), ordered, got.data_ptr(), s2.data_ptr(), sg))
+    torch.cuda.synchronize()
+    assert torch.equal(got, want) and got.abs().sum() > 0
+    assert ngp.ngp_hip_grid_gradient(None, n_dims, d_desc.data_ptr(), pos.data_ptr(), n_dims, n, rows.data_ptr(), ordered, got.data_ptr(), s2.data_ptr(), sg - 1) != 0
+    assert ngp.ngp_hip_grid_gradient(None, n_dims, d_desc.data_ptr(), pos.data_ptr(), n_dims, n - 1, rows.data_ptr(), ordered, got.data_ptr(), s2.data_ptr(), sg) != 0
+    assert ngp.ngp_hip_grid_encode(None, 4, d_desc.data_ptr(), rows.data_ptr(), pos.data_ptr(), n_dims, n, rows.data_ptr(), s2.data_ptr(), sg) != 0
+
+
+def test_a_training_step_of_the_parts_together(ngp, cuda):
+    """encode -> block -> loss -> block backward -> table gradient -> Muon (matrices) + Adam and Ema (table), three steps; every product of a step against 64 bits"""
+    n, f, n_dims = 4096, 64, 3
+    desc = make_desc(ngp, n_dims)
+    d_desc, grid_entries = H.to_dev(desc, cuda), int(desc["n_grid_entries"][0])
+    n_mlp = 80 * f
+    total = n_mlp + 2 * grid_entries
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    master = torch.cat([torch.randn(n_mlp, generator=gen, device="cuda") * 0.2, (torch.rand(2 * grid_entries, generator=gen, device="cuda") - 0.5)])
+    params, inference, ema = master.half(), master.half(), torch.zeros(total, device="cuda")
+    m1, m2, grads = torch.zeros(total, device="cuda"), torch.zeros(total, device="cuda"), torch.zeros(total, dtype=torch.float16, device="cuda")
+    block = np.zeros(1, capi.GATED_FFN)
+    block["n_in"], block["n_hidden"], block["n_out"], block["dtype"], block["activation"] = 32, f, 16, 0, capi.ACT_SILU
+    mats = np.zeros(3, capi.MUON_MATRIX)
+    mats["offset"], mats["rows"], mats["cols"] = [0, 32 * f, 64 * f], [f, f, 16], [32, 32, f]
+    sizes = [ngp.ngp_hip_nerf_encode_workspace_bytes(n), ngp.ngp_hip_gated_ffn_workspace_bytes(block.ctypes.data, n, capi.FFN_BACKWARD), ngp.ngp_hip_grid_gradient_scratch_bytes(n),
+             max(16, ngp.ngp_hip_muon_workspace_bytes(3, mats.ctypes.data))]
+    ws = [torch.empty(s, dtype=torch.uint8, device="cuda") for s in sizes]
+    x, dx = (torch.empty(n, 32, dtype=torch.float16, device="cuda") for _ in range(2))
+    y, dy, values = torch.empty(n, 16, dtype=torch.float16, device="cuda"), torch.zeros(n, 16, dtype=torch.float16, device="cuda"), torch.empty(n, 3, device="cuda")
+    w = lambda v: (v[:32 * f].view(f, 32), v[32 * f:64 * f].view(f, 32), v[64 * f:80 * f].view(16, f))   # noqa: E731
+    for step in range(1, 4):
+        pos, targets = positions(n, n_dims, 10 + step), torch.rand(n, 3, generator=gen, device="cuda")
+        p_before, w_before, m_before = params.clone(), master.clone(), m1.clone()
+        pp, gp = params.data_ptr(), grads.data_ptr()
+        capi.check(ngp.ngp_hip_grid_encode(None, n_dims, d_desc.data_ptr(), pp + 2 * n_mlp, pos.data_ptr(), n_dims, n, x.data_ptr(), ws[0].data_ptr(), sizes[0]))
+        capi.check(ngp.ngp_hip_gated_ffn_forward(None, block.ctypes.data, n, x.data_ptr(), 32, pp, pp + 64 * f, pp + 128 * f, y.data_ptr(), 16, ws[1].data_ptr(), sizes[1]))
+        capi.check(ngp.ngp_hip_loss_and_gradient(None, 0, n, 3, 128.0, y.data_ptr(), 16, targets.data_ptr(), values.data_ptr(), dy.data_ptr(), 16))
+        capi.check(ngp.ngp_hip_gated_ffn_backward(None, block.ctypes.data, n, x.data_ptr(), 32, pp, pp + 64 * f, pp + 128 * f, dy.data_ptr(), 16, dx.data_ptr(), 32, gp, gp + 64 * f, gp + 128 * f,
+                                                  ws[1].data_ptr(), sizes[1]))
+        capi.check(ngp.ngp_hip_grid_gradient(None, n_dims, d_desc.data_ptr(), pos.data_ptr(), n_dims, n, dx.data_ptr(), 0, gp + 2 * n_mlp, ws[2].data_ptr(), sizes[2]))
+        capi.check(ngp.ngp_hip_muon_step(None, 3, mats.ctypes.data, 0.02, 0.95, 0.0, 1e-7, 1, 5, 128.0, 0, gp, master.data_ptr(), pp, m1.data_ptr(), ws[3].data_ptr(), sizes[3]))
+        capi.check(ngp.ngp_hip_optimizer_step(None, total, n_mlp, step, 1e-2, 0.9, 0.99, 1e-15, 1e-6, 128.0, 0.95, gp, master.data_ptr(), pp, m1.data_ptr(), m2.data_ptr(), ema.data_ptr(),
+                                              inference.data_ptr(), 2))
+        torch.cuda.synchronize()
+        ref = F.Block("silu", x, *w(p_before), dy)
+        F.check("y", y, ref.y, ref.ey)
+        F.check("dx", dx, ref.dx, ref.edx)
+        for got, want, bound in zip(w(grads), (ref.dwg, ref.dwu, ref.dwd), (ref.edwg, ref.edwu, ref.edwd)):
+            F.check("gradient", got, want, bound)
+        for i, (g, w0, b0, w1, b1) in enumerate(zip(w(grads), w(w_before), w(m_before), w(master), w(m1))):
+            mom, new, exact, u = M.step(g, w0, b0, 0.02, 0.95, 0.0, 1e-7, 1, 5, 128.0)
+            assert ((b1.double() - mom).abs() <= 4 * 2.0 ** -24 * (0.95 * b0.double().abs() + g.double().abs() / 128)).all()
+            rate = 0.02 * max(1.0, g.shape[0] / g.shape[1]) ** 0.5
+            spread = 3 * 2.0 ** -24 * (new.norm() + w0.double().norm()).item()
+            assert (w1.double() - new).norm().item() <= rate * M.bound(u, 1e-7, 5, exact) + spread, "matrix %d" % i
+        assert torch.equal(params[:n_mlp], master[:n_mlp].half())
+        # the table moved by Adam where it has a gradient and only there; the Ema copy of both is of the new weights
+        moved = master[n_mlp:] != w_before[n_mlp:]
+        assert moved.any() and not (moved & (grads[n_mlp:] == 0)).any()
+        if step == 1:   # a debiased average of one value is that value: within a rounding of fp32 and one of fp16
+            assert (inference.double() - params.double()).abs().max().item() <= (2.0 ** -10 * params.double().abs().max()).item()
+
+
+def _image(w=96, h=64):
+    y, x = np.mgrid[0:h, 0:w].astype(np.float32)
+    img = np.ones((h, w, 4), np.float32)
+    img[..., 0], img[..., 1], img[..., 2] = 0.5 + 0.4 * np.sin(9 * x / w), (x / w) * (y / h), 0.3
+    return img
+
+
+def _config(tmp_path, name, **changes):
+    c = json.load(open(os.path.join(CFG, *name.split("/"))))
+    for key, value in changes.items():
+        c[key] = {**c[key], **value} if isinstance(value, dict) and key != "optimizer" else value
+    p = str(tmp_path / ("%s.json" % abs(hash(json.dumps(c)))))
+    json.dump(c, open(p, "w"))
+    return p
+
+
+def _muon_moved(before, after, grads, shapes, lr):
+    """the fp16 weights' change against the update that the step's own gradients give (first step: the momentum is the gradient, its direction the update's)"""
+    at = 0
+    for r, c in shapes:
+        p0, p1, g = (t[at:at + r * c].double().view(r, c) for t in (before, after, grads))
+        at += r * c
+        x = M.orthogonalise(1.95 * g / 128, 1e-7, 5)
+        rate = lr * max(1.0, r / c) ** 0.5
+        # both weights are the master's rounded to fp16: half a step each
+        limit = 2.0 ** -11 * (p0.abs() + p1.abs()) + 2.0 ** -24 + rate * 1e-4
+        off = (p0 - p1 - rate * x).abs()
+        assert (off <= limit).all(), "matrix %d x %d: off by up to %.3g of what it may" % (r, c, (off / limit).max().item())
+
+
+def test_image_config_with_gated_network_and_muon(ngp, cuda, tmp_path):
+    import pyngp
+    img = _image()
+    tb = pyngp.Testbed(pyngp.TestbedMode.Image)
+    tb.set_image_data(img)
+    tb.reload_network_from_file(_config(tmp_path, "image/gated.json", encoding=dict(log2_hashmap_size=14)))
+    assert tb.n_mlp_params == 80 * 64 and tb.n_params() == 80 * 64 + tb.n_encoding_params()
+    before = torch.from_numpy(tb.debug_params("training").view(np.float16).copy()).cuda()
+    bound = (6.0 / 96) ** 0.5
+    assert before[:32 * 64].abs().max() <= bound and before[:32 * 64].abs().max() > 0.98 * bound and before[80 * 64:].abs().max() <= 1.001e-4
+    tb.shall_train = True
+    tb.train(1 << 12)
+    tb.sync()
+    grads = view(tb.gradients_ptr(), tb.n_params()).clone()
+    after = torch.from_numpy(tb.debug_params("training").view(np.float16).copy()).cuda()
+    _muon_moved(before, after, grads, [(64, 32), (64, 32), (16, 64)], 1e-2)
+    assert torch.isfinite(after).all() and (after[80 * 64:] != before[80 * 64:]).any()
+    for batch in (1 << 10, 1 << 13, 1 << 12):   # other batch sizes through the same buffers
+        tb.train(batch)
+    assert tb.training_step == 4 and np.isfinite(tb.loss) and np.isfinite(tb.compute_image_mse(False))
+    tb.scale = 1.0
+    assert np.isfinite(tb.render(96, 64, 1, True)).all()
+    # what gridmlp_inference answers is the chain of the entry points on the inference weights
+    pos = positions(333, 2, 4)
+    out = tb.gridmlp_inference(pos.cpu().numpy())
+    p = torch.from_numpy(tb.debug_params("inference").view(np.float16).copy()).cuda()
+    desc = make_desc(ngp, 2, 14, 16, float(np.exp(np.log(np.float32(48.0) / np.float32(16)) / np.float32(15))))
+    size = ngp.ngp_hip_nerf_encode_workspace_bytes(333)
+    ws, x, y = torch.empty(size, dtype=torch.uint8, device="cuda"), torch.empty(333, 32, dtype=torch.float16, device="cuda"), torch.empty(333, 16, dtype=torch.float16, device="cuda")
+    grid = p[80 * 64:].clone()
+    capi.check(ngp.ngp_hip_grid_encode(None, 2, H.to_dev(desc, cuda).data_ptr(), grid.data_ptr(), pos.data_ptr(), 2, 333, x.data_ptr(), ws.data_ptr(), size))
+    torch.cuda.synchronize()
+    ref = F.Block("silu", x, p[:2048].view(64, 32), p[2048:4096].view(64, 32), p[4096:5120].view(16, 64))
+    F.check("inference", torch.from_numpy(out).cuda(), ref.y[:, :4], ref.ey[:, :4])
+
+
+@pytest.mark.parametrize("width,act", [(8, "GELU"), (136, "ReLU"), (256, "Sigmoid")])
+def test_sdf_config_with_gated_network(cuda, tmp_path, width, act):
+    import pyngp
+    rs = np.random.RandomState(0)
+    n = 1 << 13
+    pts = rs.rand(n, 3).astype(np.float32)
+    tb = pyngp.Testbed(pyngp.TestbedMode.Sdf)
+    tb.override_sdf_training_data(pts, (np.linalg.norm(pts - 0.5, axis=1) - 0.3).astype(np.float32))
+    tb.reload_network_from_file(_config(tmp_path, "sdf/gated.json", network=dict(n_neurons=width, activation=act), encoding=dict(log2_hashmap_size=12)))
+    assert tb.n_mlp_params == 80 * width
+    tb.shall_train = True
+    before = tb.debug_params("training").copy()
+    for _ in range(3):
+        tb.train(1 << 12)
+    after = tb.debug_params("training")
+    assert np.isfinite(tb.loss) and np.isfinite(after.view(np.float16)).all() and (after[:80 * width] != before[:80 * width]).mean() > 0.2
+    assert np.isfinite(tb.gridmlp_inference(pts[:100])).all()
+
+
+def test_muon_on_the_fused_networks(cuda, tmp_path):
+    """the 64-neuron MLP of the image config, and the NeRF networks, by Muon: the matrices in the fused kernels' parameter order"""
+    import pyngp
+    import scene
+    tb = pyngp.Testbed(pyngp.TestbedMode.Image)
+    tb.set_image_data(_image())
+    tb.reload_network_from_file(_config(tmp_path, "image/base.json", encoding=dict(log2_hashmap_size=12), optimizer={"otype": "Muon", "learning_rate": 5e-3, "nested": {"otype": "Adam", "learning_rate": 1e-2}}))
+    before = torch.from_numpy(tb.debug_params("training").view(np.float16).copy()).cuda()
+    tb.shall_train = True
+    tb.train(1 << 12)
+    tb.sync()
+    after = torch.from_numpy(tb.debug_params("training").view(np.float16).copy()).cuda()
+    _muon_moved(before, after, view(tb.gradients_ptr(), tb.n_params()).clone(), [(64, 32), (64, 64), (16, 64)], 5e-3)
+    ds = scene.make_dataset(n_train=4, n_test=1, res=48, device=torch.device("cuda:0"))
+    nerf = scene.build_testbed(ds, os.path.join(CFG, "nerf", "muon.json"))
+    before = torch.from_numpy(nerf.debug_params("training").view(np.float16).copy()).cuda()
+    scene.train(nerf, 1)
+    nerf.sync()
+    after = torch.from_numpy(nerf.debug_params("training").view(np.float16).copy()).cuda()
+    _muon_moved(before, after, view(nerf.gradients_ptr(), nerf.n_params()).clone(), [(64, 32), (16, 64), (64, 32), (64, 64), (16, 64)], 1e-2)
+    # a network that is switched off keeps its weights and its momentum
+    nerf.shall_train_network = False
+    scene.train(nerf, 2)
+    kept = torch.from_numpy(nerf.debug_params("training").view(np.float16).copy()).cuda()
+    assert torch.equal(kept[:10240], after[:10240]) and not torch.equal(kept[10240:], after[10240:])
+    # the optimizer's state goes through a snapshot
+    nerf.shall_train_network = True
+    path = str(tmp_path / "muon.msgpack")
+    nerf.save_snapshot(path, True)
+    other = scene.build_testbed(ds, os.path.join(CFG, "nerf", "muon.json"))
+    other.load_snapshot(path)
+    again = str(tmp_path / "again.msgpack")
+    other.save_snapshot(again, True)
+    import msgpack
+    a, b = (msgpack.unpackb(open(p, "rb").read(), raw=False)["snapshot"]["optimizer"] for p in (path, again))
+    assert a["nested"]["nested"]["otype"] == "Muon" and a["nested"]["nested"]["nested"]["first_moments_binary"] == b["nested"]["nested"]["nested"]["first_moments_binary"]
+    assert np.frombuffer(a["nested"]["nested"]["nested"]["first_moments_binary"], np.float32)[:10240].any()
+    scene.train(other, 5)
+    assert np.isfinite(other.loss)
+
+
+@pytest.mark.parametrize("change,words", [
+    (dict(network=dict(n_neurons=12)), "n_neurons"), (dict(network=dict(n_neurons=0)), "n_neurons"), (dict(network=dict(activation="Tanh")), "activation"),
+    (dict(network=dict(output_activation="ReLU")), "output_activation"), (dict(optimizer={"otype": "Muon"}), "nested"), (dict(optimizer={"otype": "Muon", "n_iterations": 0, "nested": {"otype": "Adam"}}), "n_iterations")])
+def test_configs_that_are_refused(cuda, tmp_path, change, words):
+    import pyngp
+    tb = pyngp.Testbed(pyngp.TestbedMode.Image)
+    tb.set_image_data(_image())
+    with pytest.raises(RuntimeError, match=words):
+        tb.reload_network_from_file(_config(tmp_path, "image/gated.json", **change))
