@@ -99,6 +99,16 @@ __global__ void __launch_bounds__(Shape<BIG>::THREADS, Shape<BIG>::RESIDENT) gat
 struct Pair { Mat n, m; };                        // one product's operands
 template <class T> struct Rows2 { Out<T> a, b; uint32_t a_rows; };   // rows 0 .. a_rows - 1 of the result go to a, the rest to b (b starts at row a_rows)
 
+// One result: the sum of up to two products of the same k (dx = dg Wg + du Wu), each in `splits` parts of k_split.  partials: splits over all products, 0: none, straight to `out`.
+template <class T> struct Item {
+	Pair p[2];
+	Rows2<T> out;
+	float* partial;
+	uint32_t n_products, tiles_n, tiles_m, splits, k_split, partials, turned;   // turned: the M side has k as its rows too
+	uint32_t first, count;   // workgroups; first is a multiple of 8, so that a workgroup's number within the item still says which XCD it runs on
+};
+template <class T> struct Group { Item<T> item[3]; uint32_t n; };
+
 template <class T, int NB, int MB>
 __device__ __forceinline__ void store_tile(f32x4 (&acc)[1][NB][MB], const Rows2<T>& o, uint32_t n0, uint32_t m0, lds_char* lds, int lane) {
 #pragma unroll
@@ -112,37 +122,49 @@ __device__ __forceinline__ void store_tile(f32x4 (&acc)[1][NB][MB], const Rows2<
 	}
 }
 
-// C = sum of up to two products of the same k (dx = dg Wg + du Wu), all of it or one split.  With splits, a workgroup leaves its accumulators in `partial` as they lie in the registers,
-// and split_sum_kernel adds the splits in their order: the result does not depend on which workgroup ends first.
 template <class T, int NLAY, int MLAY, bool BIG>
-__global__ void __launch_bounds__(Shape<BIG>::THREADS, Shape<BIG>::RESIDENT) product_kernel(Pair p0, Pair p1, int n_products, Rows2<T> out, uint32_t tiles_n, uint32_t tiles_m, uint32_t splits, uint32_t k_split, float* partial) {
+__device__ __forceinline__ void one_tile(const Item<T>& it, uint32_t pid, lds_char* lds) {
 	using S = Shape<BIG>;
 	using P = Product<T, NLAY, MLAY, 1, S::N, S::M, S::WN, S::WM>;
-	__shared__ __attribute__((aligned(1024))) char lds[P::LDS_BYTES];
 	uint32_t tn, tm, split;
-	tile_of(blockIdx.x, gridDim.x, tiles_n, tiles_m, tn, tm, split);
+	tile_of(pid, it.count, it.tiles_n, it.tiles_m, tn, tm, split);
 	f32x4 acc[1][P::NB][P::MB];
 	clear(acc);
 	const uint32_t n0 = tn * S::N, m0 = tm * S::M;
-	if (partial) {   // split s of product s / splits
-		const bool second = split >= splits;
-		const Pair& p = second ? p1 : p0;
-		const uint32_t k0 = (second ? split - splits : split) * k_split;
-		P::run(acc, &p.n, p.m, n0, m0, k0, p.n.k - k0 < k_split ? p.n.k : k0 + k_split, lds_of(lds));
-	} else {
-		P::run(acc, &p0.n, p0.m, n0, m0, 0, p0.n.k, lds_of(lds));
-		if (n_products == 2) P::run(acc, &p1.n, p1.m, n0, m0, 0, p1.n.k, lds_of(lds));
+	const bool parts = it.partials != 0;   // part `split % splits` of product `split / splits`
+	const uint32_t from = parts ? split / it.splits : 0, to = parts ? from + 1 : it.n_products;
+	for (uint32_t q = from; q < to; ++q) {
+		const Pair& p = it.p[q];
+		const uint32_t k0 = parts ? split % it.splits * it.k_split : 0;
+		P::run(acc, &p.n, p.m, n0, m0, k0, p.n.k - k0 < it.k_split ? p.n.k : k0 + it.k_split, lds);
 	}
 	const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wn = wave % S::WN, wm = wave / S::WN;
-	if (partial) {
-		float* q = partial + ((uint64_t)split * tiles_n * tiles_m + (uint64_t)tm * tiles_n + tn) * (S::N * S::M) + threadIdx.x * 4;
+	if (parts) {
+		float* q = it.partial + ((uint64_t)split * it.tiles_n * it.tiles_m + (uint64_t)tm * it.tiles_n + tn) * (S::N * S::M) + threadIdx.x * 4;
 #pragma unroll
 		for (int b = 0; b < P::NB; ++b)
 #pragma unroll
 			for (int c = 0; c < P::MB; ++c) *(f32x4*)(q + (b * P::MB + c) * (S::THREADS * 4)) = acc[0][b][c];
 		return;
 	}
-	store_tile<T, P::NB, P::MB>(acc, out, n0 + wn * (P::NB * 16), m0 + wm * (P::MB * 16), lds_of(lds) + wave * Rows<P::NB>::BYTES, lane);
+	store_tile<T, P::NB, P::MB>(acc, it.out, n0 + wn * (P::NB * 16), m0 + wm * (P::MB * 16), lds + wave * Rows<P::NB>::BYTES, lane);
+}
+
+// All results that are ready to be computed at one point in one launch: y (FORWARD), or dx and the three weight gradients, whose tiles fill the chip together where each alone would
+// leave a part of it idle.  With splits, a workgroup leaves its accumulators in `partial` as they lie in the registers, and group_sum_kernel adds the splits in their order: the
+// result does not depend on which workgroup ends first.
+template <class T, bool BIG, bool FORWARD>
+__global__ void __launch_bounds__(Shape<BIG>::THREADS, Shape<BIG>::RESIDENT) group_kernel(Group<T> g) {
+	using S = Shape<BIG>;
+	__shared__ __attribute__((aligned(1024))) char lds[Product<T, KC, KC, 1, S::N, S::M, S::WN, S::WM>::LDS_BYTES];
+	uint32_t i = 0;
+	while (i + 1 < g.n && blockIdx.x >= g.item[i + 1].first) ++i;
+	const Item<T>& it = g.item[i];
+	const uint32_t pid = blockIdx.x - it.first;
+	if (pid >= it.count) return;
+	if (FORWARD) one_tile<T, KC, KC, BIG>(it, pid, lds_of(lds));
+	else if (it.turned) one_tile<T, RC, RC, BIG>(it, pid, lds_of(lds));
+	else one_tile<T, RC, KC, BIG>(it, pid, lds_of(lds));
 }
 
 // `splits` partials -> ceil(splits / SUM_FAN) in the first of them, sixteen neighbours in their order: a long list of splits would otherwise be one workgroup's serial work
@@ -156,15 +178,19 @@ __global__ void __launch_bounds__(256) split_fold_kernel(float* partial, uint32_
 	*(f32x4*)(partial + first * floats + at) = v;
 }
 
-// the splits of a tile (every `every`-th of them), added in order, rounded once
-template <class T, bool BIG>
-__global__ void __launch_bounds__(Shape<BIG>::THREADS) split_sum_kernel(const float* partial, uint32_t splits, uint32_t every, Rows2<T> out, uint32_t tiles_n, uint32_t tiles_m) {
-	using S = Shape<BIG>;
+// the splits of the tiles (every `every`-th of them, where they have been folded), added in order, rounded once; items without splits have no tiles here
+template <class T>
+__global__ void __launch_bounds__(256) group_sum_kernel(Group<T> g) {
+	using S = Shape<false>;
 	constexpr int NB = S::N / S::WN / 16, MB = S::M / S::WM / 16;
 	__shared__ __attribute__((aligned(16))) char lds[S::WN * S::WM * Rows<NB>::BYTES];
-	const uint32_t tn = blockIdx.x % tiles_n, tm = blockIdx.x / tiles_n;
-	const float* q = partial + (uint64_t)blockIdx.x * (S::N * S::M) + threadIdx.x * 4;
-	const uint64_t stride = (uint64_t)every * tiles_n * tiles_m * (S::N * S::M);
+	uint32_t i = 0;
+	while (i + 1 < g.n && blockIdx.x >= g.item[i + 1].first) ++i;
+	const Item<T>& it = g.item[i];
+	const uint32_t t = blockIdx.x - it.first, tiles = it.tiles_n * it.tiles_m, tn = t % it.tiles_n, tm = t / it.tiles_n;
+	const uint32_t every = it.partials > SUM_FAN ? SUM_FAN : 1, splits = (it.partials + every - 1) / every;
+	const float* q = it.partial + (uint64_t)t * (S::N * S::M) + threadIdx.x * 4;
+	const uint64_t stride = (uint64_t)every * tiles * (S::N * S::M);
 	const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wn = wave % S::WN, wm = wave / S::WN;
 	f32x4 acc[1][NB][MB];
 	clear(acc);
@@ -173,7 +199,7 @@ __global__ void __launch_bounds__(Shape<BIG>::THREADS) split_sum_kernel(const fl
 		for (int b = 0; b < NB; ++b)
 #pragma unroll
 			for (int c = 0; c < MB; ++c) acc[0][b][c] += *(const f32x4*)(q + (b * MB + c) * (S::THREADS * 4));
-	store_tile<T, NB, MB>(acc, out, tn * S::N + wn * (NB * 16), tm * S::M + wm * (MB * 16), lds_of(lds) + wave * Rows<NB>::BYTES, lane);
+	store_tile<T, NB, MB>(acc, it.out, tn * S::N + wn * (NB * 16), tm * S::M + wm * (MB * 16), lds_of(lds) + wave * Rows<NB>::BYTES, lane);
 }
 
 // g, u and dh of a tile in one set of registers; from them dg, du (next to each other: d[m][0 .. f8) and d[m][f8 .. 2 f8)) and h
@@ -224,19 +250,28 @@ __global__ void __launch_bounds__(Shape<BIG>::THREADS, Shape<BIG>::RESIDENT) hid
 	}
 }
 
-// rows of any width, stride and alignment -> rows of a multiple of 8 elements, 16-byte aligned, zeros behind the width
-__global__ void __launch_bounds__(256) pad_rows_kernel(const uint16_t* __restrict__ src, uint64_t src_ld, uint64_t rows, uint32_t cols, uint16_t* __restrict__ dst, uint32_t dst_ld) {
-	const uint64_t n = rows * (dst_ld / 8);
-	for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (uint64_t)gridDim.x * 256) {
-		const uint64_t r = i / (dst_ld / 8);
-		const uint32_t c = (uint32_t)(i % (dst_ld / 8)) * 8;
-		uint32_t w[4];
+// rows of any width, stride and alignment -> rows of a multiple of 8 elements, 16-byte aligned, zeros behind the width; all of a call's tensors in one launch
+struct PadJob { const uint16_t* src; uint16_t* dst; uint64_t src_ld, pieces; uint32_t cols, dst_ld, first; };   // pieces: rows x dst_ld / 8; first: of its workgroups
+struct PadJobs { PadJob job[5]; uint32_t n; };
+constexpr uint32_t PAD_BLOCK = 1024;   // pieces of a workgroup
+__global__ void __launch_bounds__(256) pad_rows_kernel(PadJobs jobs) {
+	uint32_t j = 0;
+	while (j + 1 < jobs.n && blockIdx.x >= jobs.job[j + 1].first) ++j;
+	const PadJob& p = jobs.job[j];
+	const uint32_t per_row = p.dst_ld / 8;
 #pragma unroll
-		for (int e = 0; e < 4; ++e) {
-			const uint32_t a = c + 2 * e < cols ? src[r * src_ld + c + 2 * e] : 0, b = c + 2 * e + 1 < cols ? src[r * src_ld + c + 2 * e + 1] : 0;
-			w[e] = a | b << 16;
-		}
-		*(uint4*)(dst + r * dst_ld + c) = make_uint4(w[0], w[1], w[2], w[3]);
+	for (int q = 0; q < 4; ++q) {
+		const uint64_t i = (uint64_t)(blockIdx.x - p.first) * PAD_BLOCK + q * 256 + threadIdx.x;
+		if (i >= p.pieces) continue;
+		const uint64_t r = i / per_row;
+		const uint32_t c = (uint32_t)(i % per_row) * 8;
+		const uint16_t* row = p.src + r * p.src_ld;
+		uint32_t v[8];
+#pragma unroll
+		for (int e = 0; e < 8; ++e) v[e] = row[min(c + e, p.cols - 1)];
+#pragma unroll
+		for (int e = 0; e < 8; ++e) v[e] = c + e < p.cols ? v[e] : 0u;
+		*(uint4*)(p.dst + r * p.dst_ld + c) = make_uint4(v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16);
 	}
 }
 
@@ -274,27 +309,38 @@ struct Arena {
 	void* take(uint64_t bytes) { void* p = base ? base + used : nullptr; used += up256(bytes); return p; }
 };
 
-struct Plan { bool big; uint32_t tiles_n, tiles_m, splits, k_split, partials; };
-
-// Tile and splits of one product.  256 x 256 tiles need the least LDS and memory traffic per multiplication and win wherever they fill the 256 CUs; below that, 128 x 128 tiles
-// (two workgroups a CU), and where even those are few and k is long, k is split until about 512 workgroups run, with at least 8 steps of 64 each.
-static Plan plan_product(uint64_t n, uint64_t m, uint64_t k, uint32_t n_products) {
-	Plan p;
-	const uint64_t t256 = ceil_div(n, 256) * ceil_div(m, 256);
-	p.big = t256 >= 192;
-	const uint32_t t = p.big ? 256 : 128;
-	p.tiles_n = (uint32_t)ceil_div(n, t); p.tiles_m = (uint32_t)ceil_div(m, t);
-	const uint64_t tiles = (uint64_t)p.tiles_n * p.tiles_m;
-	uint64_t splits = 1;
-	if (!p.big && tiles < 256) splits = std::max<uint64_t>(1, std::min<uint64_t>(512 / (tiles * n_products), k / 512));
-	p.k_split = (uint32_t)(ceil_div(ceil_div(k, 64), splits) * 64);
-	p.splits = (uint32_t)std::max<uint64_t>(1, ceil_div(k, p.k_split));
-	p.partials = p.splits > 1 ? p.splits * n_products : 0;
-	return p;
+// The sizes of one result before it has pointers, and how a group of them is cut.  256 x 256 tiles need the least LDS and memory traffic per multiplication and win wherever the group
+// fills three quarters of the 256 CUs with them; below that, 128 x 128 tiles (two workgroups a CU), with k in parts of at least 512 where the group has fewer than 512 tiles.
+struct Size { uint64_t n, m, k; uint32_t n_products; };
+struct Plan { uint32_t tiles_n, tiles_m, splits, k_split, partials; };
+static bool plan_group(const Size* s, int count, Plan* plan) {
+	uint64_t big_tiles = 0;
+	for (int i = 0; i < count; ++i) big_tiles += ceil_div(s[i].n, 256) * ceil_div(s[i].m, 256);
+	const bool big = big_tiles >= 192;
+	uint64_t part = 512;
+	auto splits_of = [&](const Size& z) { return std::max<uint64_t>(1, std::min<uint64_t>(ceil_div(z.k, part), z.k / 512)); };
+	for (; !big; part *= 2) {
+		uint64_t groups = 0;
+		for (int i = 0; i < count; ++i) groups += ceil_div(s[i].n, 128) * ceil_div(s[i].m, 128) * (splits_of(s[i]) > 1 ? s[i].n_products * splits_of(s[i]) : 1);
+		if (groups <= 512 || part > (1ull << 31)) break;
+	}
+	for (int i = 0; i < count; ++i) {
+		const uint32_t t = big ? 256 : 128;
+		Plan& p = plan[i];
+		p.tiles_n = (uint32_t)ceil_div(s[i].n, t); p.tiles_m = (uint32_t)ceil_div(s[i].m, t);
+		const uint64_t splits = big ? 1 : splits_of(s[i]);
+		p.k_split = (uint32_t)(ceil_div(ceil_div(s[i].k, 64), splits) * 64);
+		p.splits = (uint32_t)std::max<uint64_t>(1, ceil_div(s[i].k, p.k_split));
+		p.partials = p.splits > 1 ? p.splits * s[i].n_products : 0;
+	}
+	return big;
 }
-// room for its splits, never less than any smaller batch of the same block takes: the splits' tiles are at most 512, and at most k / 512 for each tile and product
-static uint64_t partial_room(uint64_t n, uint64_t m, uint64_t k, uint32_t n_products) {
-	return k >= 1024 ? std::min<uint64_t>(512, ceil_div(n, 128) * ceil_div(m, 128) * n_products * (k / 512)) * (128 * 128 * 4) : 0;
+// room for a group's splits, never less than any smaller batch of the same block takes: at most 512 tiles' worth, and at most k / 512 for each tile and product
+static uint64_t partial_room(const Size* s, int count) {
+	uint64_t parts = 0;
+	for (int i = 0; i < count; ++i)
+		if (s[i].k >= 1024) parts += ceil_div(s[i].n, 128) * ceil_div(s[i].m, 128) * s[i].n_products * (s[i].k / 512);
+	return std::min<uint64_t>(512, parts) * (128 * 128 * 4);
 }
 
 struct Tensor { const void* p; uint64_t ld; uint64_t rows; uint32_t cols; };
@@ -387,7 +433,7 @@ struct Space {
 	uint32_t d8, f8, o8, fp;                                   // widths as the copies have them; fp: row pitch of h, dg and du
 	void *x = nullptr, *wg = nullptr, *wu = nullptr, *wd = nullptr, *dy = nullptr, *h = nullptr, *d = nullptr;
 	float* partial = nullptr;
-	Plan y, dx, dwgu, dwd;
+	Size size[3];
 	uint64_t bytes;
 	bool has_copies(uint32_t width, bool any) const { return any || width % 8; }
 	Space(char* base, const NgpGatedFfn& b, uint64_t rows, bool backward, bool any) {
@@ -408,18 +454,16 @@ struct Space {
 		if (has_copies(b.n_hidden, any)) wd = a.take((uint64_t)b.n_out * f8 * 2);
 		if (backward && has_copies(b.n_out, any)) dy = a.take(rows * o8 * 2);
 		h = a.take(rows * fp * 2);
-		uint64_t part = 0;
 		if (backward) {
 			d = a.take(rows * fp * 4);
-			dx = plan_product(b.n_in, rows, b.n_hidden, 2);
-			dwgu = plan_product(b.n_in, 2 * (uint64_t)fp, rows, 1);
-			dwd = plan_product(b.n_hidden, b.n_out, rows, 1);
-			part = std::max(partial_room(b.n_in, rows, b.n_hidden, 2), std::max(partial_room(b.n_in, 2 * (uint64_t)fp, rows, 1), partial_room(b.n_hidden, b.n_out, rows, 1)));
+			size[0] = {b.n_in, rows, b.n_hidden, 2};                       // dx
+			size[1] = {b.n_in, 2 * (uint64_t)fp, rows, 1};                 // dw_gate over dw_up
+			size[2] = {b.n_hidden, b.n_out, rows, 1};                      // dw_down
+			partial = (float*)a.take(partial_room(size, 3));
 		} else {
-			y = plan_product(b.n_out, rows, f8, 1);
-			part = partial_room(b.n_out, rows, f8, 1);
+			size[0] = {b.n_out, rows, f8, 1};
+			partial = (float*)a.take(partial_room(size, 1));
 		}
-		partial = (float*)a.take(part);   // one after the other on one stream: they share it
 		bytes = a.used;
 	}
 };
@@ -433,31 +477,60 @@ struct Launch {
 		if (e != hipSuccess) { set_last_error(what, e); rc = (int)e; }
 		return rc == 0;
 	}
-	// `t` as the DMA takes it, through `copy` where it is not ready (copy null: not reserved)
+	PadJobs pads{};
+	uint32_t pad_groups = 0;
+	// `t` as the DMA takes it, through `copy` where it is not ready (copy null: not reserved); pad() runs the copies
 	Tensor ready(const Tensor& t, void* copy, uint32_t width8) {
 		if (rc || dma_ready(t)) return t;
 		if (!copy) { rc = refuse("ngp_hip_gated_ffn: a row that is not 16-byte aligned needs the workspace of NGP_FFN_ANY_LAYOUT"); return t; }
-		hipLaunchKernelGGL(pad_rows_kernel, dim3(copy_grid(t.rows * (width8 / 8))), dim3(256), 0, st, (const uint16_t*)t.p, t.ld, t.rows, t.cols, (uint16_t*)copy, width8);
-		ok("pad_rows_kernel");
+		PadJob& j = pads.job[pads.n++];
+		j = PadJob{(const uint16_t*)t.p, (uint16_t*)copy, t.ld, t.rows * (width8 / 8), t.cols, width8, pad_groups};
+		pad_groups += (uint32_t)ceil_div(j.pieces, PAD_BLOCK);
 		return Tensor{copy, width8, t.rows, width8};
 	}
-	template <class T, int NLAY, int MLAY> void product(const Plan& p, const Pair& p0, const Pair* p1, const Rows2<T>& out, float* partial) {
-		if (rc) return;
-		const uint32_t tiles = p.tiles_n * p.tiles_m;
-		float* part = p.partials ? partial : nullptr;
-		const dim3 grid(tiles * std::max(1u, p.partials));
-		if (p.big) hipLaunchKernelGGL((product_kernel<T, NLAY, MLAY, true>), grid, dim3(Shape<true>::THREADS), 0, st, p0, p1 ? *p1 : p0, p1 ? 2 : 1, out, p.tiles_n, p.tiles_m, p.splits, p.k_split, part);
-		else hipLaunchKernelGGL((product_kernel<T, NLAY, MLAY, false>), grid, dim3(256), 0, st, p0, p1 ? *p1 : p0, p1 ? 2 : 1, out, p.tiles_n, p.tiles_m, p.splits, p.k_split, part);
-		if (!ok("product_kernel") || !part) return;
-		uint32_t splits = p.partials, every = 1;
-		if (splits > SUM_FAN) {
-			const uint64_t floats = (uint64_t)tiles * 128 * 128;
-			hipLaunchKernelGGL(split_fold_kernel, dim3((uint32_t)(floats / 1024 * ceil_div(splits, SUM_FAN))), dim3(256), 0, st, part, splits, floats);
-			splits = (uint32_t)ceil_div(splits, SUM_FAN);
-			every = SUM_FAN;
+	void pad() {
+		if (rc || !pads.n) return;
+		hipLaunchKernelGGL(pad_rows_kernel, dim3(pad_groups), dim3(256), 0, st, pads);
+		ok("pad_rows_kernel");
+	}
+	// The group's products, item i of size sizes[which[i]]; `partial`: the room of partial_room.  The plan is made for all `count` sizes, whichever of them are asked for: a result's bits
+	// do not depend on the others being wanted too.
+	template <class T, bool FORWARD> void products(Group<T>& g, const int* which, const Size* sizes, int count, float* partial) {
+		if (rc || !g.n) return;
+		Plan plans[3];
+		const bool big = plan_group(sizes, count, plans);
+		uint32_t groups = 0, sum_groups = 0;
+		bool sums = false;
+		for (uint32_t i = 0; i < g.n; ++i) {
+			Item<T>& it = g.item[i];
+			const Plan& plan = plans[which[i]];
+			it.n_products = sizes[which[i]].n_products;
+			it.tiles_n = plan.tiles_n; it.tiles_m = plan.tiles_m; it.splits = plan.splits; it.k_split = plan.k_split; it.partials = plan.partials;
+			it.partial = partial;
+			partial += (uint64_t)it.partials * it.tiles_n * it.tiles_m * (128 * 128);
+			it.first = groups;
+			it.count = it.tiles_n * it.tiles_m * std::max(1u, it.partials);
+			groups += (it.count + 7) & ~7u;
+			sums |= it.partials != 0;
 		}
-		hipLaunchKernelGGL((split_sum_kernel<T, false>), dim3(tiles), dim3(256), 0, st, (const float*)part, splits, every, out, p.tiles_n, p.tiles_m);
-		ok("split_sum_kernel");
+		if (big) hipLaunchKernelGGL((group_kernel<T, true, FORWARD>), dim3(groups), dim3(Shape<true>::THREADS), 0, st, g);
+		else hipLaunchKernelGGL((group_kernel<T, false, FORWARD>), dim3(groups), dim3(Shape<false>::THREADS), 0, st, g);
+		if (!ok("group_kernel") || !sums) return;
+		Group<T> s;
+		s.n = 0;
+		for (uint32_t i = 0; i < g.n; ++i) {
+			if (!g.item[i].partials) continue;
+			Item<T>& it = s.item[s.n++] = g.item[i];
+			const uint32_t tiles = it.tiles_n * it.tiles_m;
+			it.first = sum_groups;
+			sum_groups += tiles;
+			if (it.partials > SUM_FAN) {
+				const uint64_t floats = (uint64_t)tiles * 128 * 128;
+				hipLaunchKernelGGL(split_fold_kernel, dim3((uint32_t)(floats / 1024 * ceil_div(it.partials, SUM_FAN))), dim3(256), 0, st, it.partial, it.partials, floats);
+			}
+		}
+		hipLaunchKernelGGL((group_sum_kernel<T>), dim3(sum_groups), dim3(256), 0, st, s);
+		ok("group_sum_kernel");
 	}
 };
 
@@ -469,6 +542,7 @@ template <class T>
 static int forward(hipStream_t st, const NgpGatedFfn& b, const Space& s, Tensor x, Tensor wg, Tensor wu, Tensor wd, void* y, uint64_t y_ld) {
 	Launch l{st};
 	x = l.ready(x, s.x, s.d8); wg = l.ready(wg, s.wg, s.d8); wu = l.ready(wu, s.wu, s.d8); wd = l.ready(wd, s.wd, s.f8);
+	l.pad();
 	if (l.rc) return l.rc;
 	const Out<T> h{(T*)s.h, s.fp, (uint32_t)x.rows, s.fp};
 	const bool big = ceil_div(s.fp, 128) * ceil_div(x.rows, 256) >= 192;
@@ -477,7 +551,12 @@ static int forward(hipStream_t st, const NgpGatedFfn& b, const Space& s, Tensor 
 	else hipLaunchKernelGGL((gate_up_kernel<T, false>), dim3(tn * tm), dim3(256), 0, st, kc(x), kc(wg), kc(wu), h, b.activation, tn, tm);
 	l.ok("gate_up_kernel");
 	const Tensor th{s.h, s.fp, x.rows, s.f8};
-	l.product<T, KC, KC>(s.y, Pair{kc(wd), kc(th)}, nullptr, whole<T>(y, y_ld, x.rows, b.n_out), s.partial);
+	Group<T> g;
+	g.n = 1;
+	g.item[0].p[0] = Pair{kc(wd), kc(th)};
+	g.item[0].out = whole<T>(y, y_ld, x.rows, b.n_out);
+	const int which[1] = {0};
+	l.products<T, true>(g, which, s.size, 1, s.partial);
 	return l.rc;
 }
 
@@ -485,6 +564,7 @@ template <class T>
 static int backward(hipStream_t st, const NgpGatedFfn& b, const Space& s, Tensor x, Tensor wg, Tensor wu, Tensor wd, Tensor dy, void* dx, uint64_t dx_ld, void* dwg, void* dwu, void* dwd) {
 	Launch l{st};
 	x = l.ready(x, s.x, s.d8); wg = l.ready(wg, s.wg, s.d8); wu = l.ready(wu, s.wu, s.d8); wd = l.ready(wd, s.wd, s.f8); dy = l.ready(dy, s.dy, s.o8);
+	l.pad();
 	if (l.rc) return l.rc;
 	const uint32_t rows = (uint32_t)x.rows;
 	T* const d = (T*)s.d;
@@ -495,15 +575,22 @@ static int backward(hipStream_t st, const NgpGatedFfn& b, const Space& s, Tensor
 	else hipLaunchKernelGGL((hidden_backward_kernel<T, false>), dim3(tn * tm), dim3(256), 0, st, kc(x), kc(wg), kc(wu), kc(dy), rc(wd), dg, du, h, b.activation, tn, tm);
 	l.ok("hidden_backward_kernel");
 	const Tensor tdg{dg.p, dg.ld, rows, s.f8}, tdu{du.p, du.ld, rows, s.f8}, tboth{d, 2ull * s.fp, rows, 2 * s.fp}, th{s.h, s.fp, rows, s.fp};
-	if (dx) {
-		const Pair up{rc(wu), kc(tdu)};
-		l.product<T, RC, KC>(s.dx, Pair{rc(wg), kc(tdg)}, &up, whole<T>(dx, dx_ld, rows, b.n_in), s.partial);
-	}
+	Group<T> g;
+	int which[3];
+	g.n = 0;
+	auto add = [&](int size, const Pair& p0, const Pair& p1, const Rows2<T>& out, bool turned) {
+		Item<T>& it = g.item[g.n];
+		it.p[0] = p0; it.p[1] = p1; it.out = out; it.turned = turned;
+		which[g.n++] = size;
+	};
+	if (dx) add(0, Pair{rc(wg), kc(tdg)}, Pair{rc(wu), kc(tdu)}, whole<T>(dx, dx_ld, rows, b.n_in), false);
 	if (dwg) {
-		const Rows2<T> out{Out<T>{(T*)dwg, b.n_in, b.n_hidden, b.n_in}, Out<T>{(T*)dwu, b.n_in, b.n_hidden, b.n_in}, s.fp};
-		l.product<T, RC, RC>(s.dwgu, Pair{rc(x), rc(tboth)}, nullptr, out, s.partial);
-		l.product<T, RC, RC>(s.dwd, Pair{rc(th), rc(dy)}, nullptr, whole<T>(dwd, b.n_hidden, b.n_out, b.n_hidden), s.partial);
+		const Out<T> og{(T*)dwg, b.n_in, b.n_hidden, b.n_in}, ou{(T*)dwu, b.n_in, b.n_hidden, b.n_in};
+		const Pair gu{rc(x), rc(tboth)}, down{rc(th), rc(dy)};
+		add(1, gu, gu, Rows2<T>{og, ou, s.fp}, true);
+		add(2, down, down, whole<T>(dwd, b.n_hidden, b.n_out, b.n_hidden), true);
 	}
+	l.products<T, false>(g, which, s.size, 3, s.partial);
 	return l.rc;
 }
 

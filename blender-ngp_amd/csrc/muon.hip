@@ -52,12 +52,6 @@ __device__ __forceinline__ uint32_t job_of(const Jobs& j, int kind, uint32_t& pi
 	pid -= j.start[kind][i];
 	return i;
 }
-// workgroups in the order of the XCDs they run on (see matmul_mfma.cuh tile_of)
-__device__ __forceinline__ uint32_t xcd_order(uint32_t pid, uint32_t total) {
-	const uint32_t xcd = pid & 7, per = total >> 3, rem = total & 7;
-	return xcd * per + (xcd < rem ? xcd : rem) + (pid >> 3);
-}
-
 __device__ __forceinline__ float load_grad(const Step& s, uint64_t i) {
 	const float g = s.dtype == NGP_DTYPE_F32 ? ((const float*)s.grads)[i] : s.dtype == NGP_DTYPE_F16 ? (float)((const f16*)s.grads)[i] : (float)((const b16*)s.grads)[i];
 	return g * s.inv_loss_scale;
