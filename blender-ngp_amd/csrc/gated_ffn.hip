@@ -282,7 +282,7 @@ __global__ void __launch_bounds__(256) zero_kernel(uint16_t* p, uint64_t n) {
 // ---- host ------------------------------------------------------------------------------------------------------------------------------
 
 constexpr uint32_t MAX_WIDTH = 1u << 20;
-constexpr uint64_t MAX_ROWS = 1ull << 31, MAX_DMA_LD = 1u << 21;   // a tile's 256 rows stay within the 2 GiB of a buffer descriptor
+constexpr uint64_t MAX_ROWS = 1ull << 30, MAX_DMA_LD = 1u << 21;   // a tile's 256 rows stay within the 2 GiB of a buffer descriptor
 
 static inline uint64_t up8(uint64_t v) { return (v + 7) & ~7ull; }
 static inline uint64_t up256(uint64_t v) { return (v + 255) & ~255ull; }
@@ -610,7 +610,7 @@ int ngp_hip_gated_ffn_forward(void* stream, const NgpGatedFfn* b, uint64_t n_row
                               void* y, uint64_t y_stride, void* workspace, uint64_t workspace_bytes) {
 	using namespace ffn;
 	if (check_block(b, "ngp_hip_gated_ffn_forward")) return -1;
-	if (n_rows > MAX_ROWS) return refuse("ngp_hip_gated_ffn_forward: more than 2^31 rows");
+	if (n_rows > MAX_ROWS) return refuse("ngp_hip_gated_ffn_forward: more than 2^30 rows");
 	if (n_rows == 0) return 0;
 	if (!x || !w_gate || !w_up || !w_down || !y) return refuse("ngp_hip_gated_ffn_forward: null tensor");
 	if (x_stride < b->n_in || y_stride < b->n_out) return refuse("ngp_hip_gated_ffn_forward: a row stride is smaller than its row");
@@ -634,7 +634,7 @@ int ngp_hip_gated_ffn_backward(void* stream, const NgpGatedFfn* b, uint64_t n_ro
                                const void* dy, uint64_t dy_stride, void* dx, uint64_t dx_stride, void* dw_gate, void* dw_up, void* dw_down, void* workspace, uint64_t workspace_bytes) {
 	using namespace ffn;
 	if (check_block(b, "ngp_hip_gated_ffn_backward")) return -1;
-	if (n_rows > MAX_ROWS) return refuse("ngp_hip_gated_ffn_backward: more than 2^31 rows");
+	if (n_rows > MAX_ROWS) return refuse("ngp_hip_gated_ffn_backward: more than 2^30 rows");
 	if ((dw_gate == nullptr) != (dw_up == nullptr) || (dw_gate == nullptr) != (dw_down == nullptr)) return refuse("ngp_hip_gated_ffn_backward: the three weight gradients go together");
 	if (!dx && !dw_gate) return refuse("ngp_hip_gated_ffn_backward: nothing to compute");
 	if (((uintptr_t)dw_gate | (uintptr_t)dw_up | (uintptr_t)dw_down | (uintptr_t)dx) & 1) return refuse("ngp_hip_gated_ffn_backward: a tensor is not aligned to its elements");

@@ -71,41 +71,48 @@ struct Tile {
 		return CHUNKS >= 16 ? (r & 3) << 1 | (r & 8) : (r & 2) | (r & 8) >> 1;
 	}
 
-	const char* base;        // of this step (uniform)
-	int64_t left;            // bytes from base to the operand's end
+	// All but k_here, k_past and voff are uniform and 32 bits where the loop touches them: the next descriptor is five scalar instructions (worked out in 64 bits, with a compare on the
+	// vector unit, it was a quarter of a small tile's step).
+	const char* base;        // of this step
 	int64_t step_bytes;
-	int k_here;              // KC: k of this thread's chunk in the step; beyond `k_left` it reads zero
+	int row_bytes, end_bytes;   // KC: bytes to the last row of the tile, 0.  RC: bytes from row to row (of k), bytes of the operand in a row from here on
 	int k_left;
+	int k_here;              // KC: k of this thread's chunk in the step; beyond `k_left` it reads zero
 	bool k_past;
 	int voff[LOADS];
 
-	__device__ __forceinline__ void init(const Mat& m, uint32_t row0, int tid) {
+	// steps of BK from k0 on (a multiple of BK)
+	__device__ __forceinline__ void init(const Mat& m, uint32_t row0, uint32_t k0, int tid) {
+		const int ld2 = (int)((uint32_t)m.ld * 2u);
+		const bool any = row0 < m.rows;   // a tile without rows reads nothing
 		if (LAY == KC) {
-			base = (const char*)m.p + (uint64_t)row0 * m.ld * 2;
-			left = row0 < m.rows ? (int64_t)(((uint64_t)(m.rows - row0 - 1) * m.ld + m.k) * 2) : 0;
+			base = (const char*)m.p + ((uint64_t)row0 * m.ld + k0) * 2;
 			step_bytes = BK * 2;
+			const uint32_t rows = any ? m.rows - row0 : 0;
+			row_bytes = any ? (int)((rows < BR ? rows : BR) - 1) * ld2 : -0x40000000;
+			end_bytes = 0;
 		} else {
-			base = (const char*)m.p + (uint64_t)row0 * 2;
-			left = row0 < m.rows ? (int64_t)(((uint64_t)(m.k - 1) * m.ld + m.rows - row0) * 2) : 0;
+			base = (const char*)m.p + ((uint64_t)k0 * m.ld + row0) * 2;
 			step_bytes = (int64_t)m.ld * BK * 2;
+			row_bytes = any ? ld2 : 0;
+			end_bytes = any ? (int)((m.rows - row0) * 2u) : -0x40000000;
 		}
-		k_left = (int)m.k;
+		k_left = (int)(m.k - k0);
 #pragma unroll
 		for (int i = 0; i < LOADS; ++i) {
 			const int slot = i * THREADS + tid, r = slot / CHUNKS, c = (slot % CHUNKS) ^ swizzle(r);
 			voff[i] = (int)((uint32_t)r * (uint32_t)m.ld * 2u) + c * 16;
 			if (LAY == KC && i == 0) k_here = c * 8;   // the same for every i: a thread's rows differ by a multiple of 16
 		}
+		asm volatile("s_nop 4");   // a word of the descriptors below that came from the vector unit must be five wait states old when a memory instruction reads it
 	}
-	// descriptor of the current step (what lies behind the operand's end reads as zero), then on to the next
+	// descriptor of the current step (it ends where the operand does: what lies behind reads as zero), then on to the next
 	__device__ __forceinline__ i32x4 next() {
 		const uint64_t b = (uint64_t)base;
-		const int records = left > 0x7fffffff ? 0x7fffffff : left < 0 ? 0 : (int)left;
-		i32x4 r = {(int)(uint32_t)b, (int)((uint32_t)(b >> 32) & 0xffffu), records, 0x00020000};
-		asm volatile("s_nop 4" : "+s"(r));   // a descriptor word that came from the VALU must be five wait states old when a memory instruction reads it
+		const int here = k_left < BK ? k_left : BK, end = LAY == KC ? row_bytes + 2 * k_left : (here - 1) * row_bytes + end_bytes;
+		const i32x4 r = {(int)(uint32_t)b, (int)((uint32_t)(b >> 32) & 0xffffu), end > 0 ? end : 0, 0x00020000};
 		k_past = LAY == KC && k_here >= k_left;
 		base += step_bytes;
-		left -= step_bytes;
 		k_left -= BK;
 		return r;
 	}
@@ -152,14 +159,8 @@ struct Product {
 		NT nt[NM];
 		MT mt;
 #pragma unroll
-		for (int j = 0; j < NM; ++j) nt[j].init(n[j], n0, tid);
-		mt.init(m, m0, tid);
-		if (k0) {
-			const int64_t skip = k0 / BK;
-#pragma unroll
-			for (int j = 0; j < NM; ++j) { nt[j].base += skip * nt[j].step_bytes; nt[j].left -= skip * nt[j].step_bytes; nt[j].k_left -= (int)k0; }
-			mt.base += skip * mt.step_bytes; mt.left -= skip * mt.step_bytes; mt.k_left -= (int)k0;
-		}
+		for (int j = 0; j < NM; ++j) nt[j].init(n[j], n0, k0, tid);
+		mt.init(m, m0, k0, tid);
 		const int steps = (int)((k1 - k0 + BK - 1) / BK);
 		// Steps are issued without end (those behind the last one would bring the next split's or, behind the operand, zeros: nothing reads them), so that the count of DMA in flight is
 		// the same in every step and the waits can be counted.

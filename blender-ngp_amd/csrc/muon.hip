@@ -210,8 +210,8 @@ struct SplitProduct {
 			for (int b = 0; b < MB; ++b) acc[a][b] = f32x4{0, 0, 0, 0};
 		NT nt;
 		MT mt;
-		nt.init(n, LAY == KC ? n0 : 2 * n0, tid);
-		mt.init(m, LAY == KC ? m0 : 2 * m0, tid);
+		nt.init(n, LAY == KC ? n0 : 2 * n0, 0, tid);
+		mt.init(m, LAY == KC ? m0 : 2 * m0, 0, tid);
 		const int steps = (int)(LAY == KC ? n.k / 64 : (n.k + 31) / 32);
 		i32x4 rn, rm;
 		int slot = 0;

@@ -499,7 +499,7 @@ int ngp_hip_muon_step(void* stream, uint32_t n_matrices, const NgpMuonMatrix* ma
  *   x [n_rows][n_in], y [n_rows][n_out] with a row stride in elements; w_gate, w_up [n_hidden][n_in] and w_down [n_out][n_hidden] row-major and contiguous, as every matrix
  *   of a parameter vector here.  All tensors are of `dtype` (F16 or BF16); products accumulate in fp32, the hidden row is rounded once, every output is rounded once.
  *   activation: NGP_ACT_NONE (bilinear), RELU, LOGISTIC, SILU or GELU (the exact one, with erf); applied to x Wg^T.
- * Widths 1 .. 2^20 and rows 0 .. 2^31 of any remainder.  Rows whose width, stride and base are multiples of 8 elements / 16 bytes are read in place; others cost one padded copy.
+ * Widths 1 .. 2^20 and rows 0 .. 2^30 of any remainder.  Rows whose width, stride and base are multiples of 8 elements / 16 bytes are read in place; others cost one padded copy.
  * Nothing outside y, dx, the gradients and the workspace is written; bytes between rows of a strided output stay as they are.  No atomics: the same inputs give the same bits.
  * A call only enqueues (capturable); two calls that may overlap need workspaces of their own. */
 typedef struct { uint32_t n_in, n_hidden, n_out; int32_t dtype, activation; } NgpGatedFfn;   /* host struct */

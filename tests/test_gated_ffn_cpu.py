@@ -42,7 +42,7 @@ def test_null_tensors(ngp, call, bad):
 @pytest.mark.parametrize("call,kw,word", [
     (fwd, dict(xs=135), b"stride"), (fwd, dict(ys=135), b"stride"), (bwd, dict(xs=135), b"stride"), (bwd, dict(dys=135), b"stride"), (bwd, dict(dxs=135), b"stride"),
     (fwd, dict(x=P + 1), b"aligned"), (fwd, dict(y=P + 1), b"aligned"), (bwd, dict(dy=P + 1), b"aligned"), (bwd, dict(u=P + 1), b"aligned"), (fwd, dict(ws=P + 8), b"workspace"),
-    (fwd, dict(rows=(1 << 31) + 1), b"rows"), (bwd, dict(rows=(1 << 31) + 1), b"rows"), (bwd, dict(g=None), b"together"), (bwd, dict(d=None), b"together"),
+    (fwd, dict(rows=(1 << 30) + 1), b"rows"), (bwd, dict(rows=(1 << 30) + 1), b"rows"), (bwd, dict(g=None), b"together"), (bwd, dict(d=None), b"together"),
     (bwd, dict(dx=None, g=None, u=None, d=None), b"nothing")])
 def test_arguments_that_are_refused(ngp, call, kw, word):
     assert call(ngp, block(), **kw) != 0 and word in ngp.ngp_hip_last_error(), ngp.ngp_hip_last_error()
