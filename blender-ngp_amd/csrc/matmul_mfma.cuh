@@ -179,19 +179,13 @@ struct Product {
 			else mt.issue(rm, i - NM * NT::LOADS, to + NM * NT::BYTES, wave);
 		};
 		i32x4 fm[2][MB], fn[2][HALF];   // M side of this step and the next; N side of this half and the next
-		auto read_m = [&](int set, const lds_char* p) {
-#pragma unroll
-			for (int b = 0; b < MB; ++b) fm[set][b] = MT::frag(p + NM * NT::BYTES, wm * (BM / WM) + b * 16, lane);
+		auto read_m = [&](int set, int b, const lds_char* p) { fm[set][b] = MT::frag(p + NM * NT::BYTES, wm * (BM / WM) + b * 16, lane); };
+		auto read_n = [&](int half, int i, const lds_char* p) {
+			const int u = half * HALF + i;
+			fn[half][i] = NT::frag(p + u / NB * NT::BYTES, wn * (BN / WN) + u % NB * 16, lane);
 		};
-		auto read_n = [&](int half, const lds_char* p) {
-#pragma unroll
-			for (int i = 0; i < HALF; ++i) {
-				const int u = half * HALF + i;
-				fn[half][i] = NT::frag(p + u / NB * NT::BYTES, wn * (BN / WN) + u % NB * 16, lane);
-			}
-		};
-		// half a step's MFMAs, with DMA first .. last - 1 spread between them
-		auto multiply = [&](int half, int set, int first, int last) {
+		// half a step's MFMAs, with `count` other instructions (DMA, LDS reads) spread between them: other(0) .. other(count - 1)
+		auto multiply = [&](int half, int set, int count, auto other) {
 			constexpr int COUNT = HALF * MB;
 			__builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -199,10 +193,10 @@ struct Product {
 				const int u = half * HALF + i / MB, c = i % MB;
 				acc[u / NB][u % NB][c] = mfma16<T>(fn[half][i / MB], fm[set][c], acc[u / NB][u % NB][c]);
 #pragma unroll
-				for (int d = first; d < last; ++d)
-					if ((d - first) * COUNT / (last - first) + 1 == i) {
+				for (int d = 0; d < count; ++d)
+					if (d * COUNT / count == i) {
 						__builtin_amdgcn_sched_barrier(0);
-						issue(d);
+						other(d);
 						__builtin_amdgcn_sched_barrier(0);
 					}
 			}
@@ -215,16 +209,17 @@ struct Product {
 			for (int i = 0; i < LOADS; ++i) issue(i);
 		}
 		wait_and_sync<(STAGES - 2) * LOADS>();
-		read_m(0, lds);
-		read_n(0, lds);
+#pragma unroll
+		for (int b = 0; b < MB; ++b) read_m(0, b, lds);
+#pragma unroll
+		for (int i = 0; i < HALF; ++i) read_n(0, i, lds);
 		auto step = [&](int s, int set) {   // set: s & 1, a constant
 			next_step();
-			read_n(1, lds + (s & (STAGES - 1)) * STAGE_BYTES);
-			multiply(0, set, 0, EARLY);
+			const lds_char* p = lds + (s & (STAGES - 1)) * STAGE_BYTES;
+			multiply(0, set, HALF + EARLY, [&](int d) { if (d < HALF) read_n(1, d, p); else issue(d - HALF); });
 			wait_and_sync<(STAGES - 3) * LOADS + EARLY>();   // the next step has landed, this one has been read: its buffer is the next to be filled
-			read_m(set ^ 1, lds + ((s + 1) & (STAGES - 1)) * STAGE_BYTES);   // behind the last step: not used
-			read_n(0, lds + ((s + 1) & (STAGES - 1)) * STAGE_BYTES);
-			multiply(1, set, EARLY, LOADS);
+			const lds_char* q = lds + ((s + 1) & (STAGES - 1)) * STAGE_BYTES;   // behind the last step: not used
+			multiply(1, set, MB + HALF + LOADS - EARLY, [&](int d) { if (d < MB) read_m(set ^ 1, d, q); else if (d < MB + HALF) read_n(0, d - MB, q); else issue(EARLY + d - MB - HALF); });
 		};
 		int s = 0;
 		for (; s + 1 < steps; s += 2) {

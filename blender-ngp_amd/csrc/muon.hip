@@ -226,43 +226,51 @@ struct SplitProduct {
 			if (i < NT::LOADS) nt.issue(rn, i, to, wave);
 			else mt.issue(rm, i - NT::LOADS, to + NT::BYTES, wave);
 		};
+		// Fragments are read a step ahead of the MFMAs that take them, and between MFMAs, as the DMA is issued: a burst of reads behind the barrier holds up every wave's MFMAs at once.
+		i32x4 fm[2][2][MB], fn[2][2][NB];   // of two steps: hi, lo
+		constexpr int READS = 2 * (MB + NB), COUNT = 3 * NB * MB;
+		auto read = [&](int set, int d, const lds_char* p) {
+			const int half = d / (MB + NB), i = d % (MB + NB);
+			if (i < MB) fm[set][half][i] = frag<MT>(p + NT::BYTES, wm * (BM / WM) + i * 16, half, lane);
+			else fn[set][half][i - MB] = frag<NT>(p, wn * (BN / WN) + (i - MB) * 16, half, lane);
+		};
+		int at = 0;
+		auto step = [&](int set) {
+			wait_and_sync<(STAGES - 2) * LOADS>();   // the next step has landed; this one is in registers everywhere, and its buffer free
+			next_step();
+			at = at + 1 == STAGES ? 0 : at + 1;
+			const lds_char* p = lds + at * STAGE_BYTES;   // behind the last step: not used
+			__builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-		for (int s = 0; s < STAGES - 1; ++s) {   // the steps behind the last one read zeros
+			for (int i = 0; i < COUNT; ++i) {
+				const int part = i / (NB * MB), a = i % (NB * MB) / MB, b = i % MB;
+				acc[a][b] = mfma16<f16>(fn[set][part == 2][a], fm[set][part == 1][b], acc[a][b]);   // hi hi, hi lo, lo hi
+#pragma unroll
+				for (int d = 0; d < READS + LOADS; ++d)
+					if (d * (COUNT - 2) / (READS + LOADS) == i) {
+						__builtin_amdgcn_sched_barrier(0);
+						if (d < READS) read(set ^ 1, d, p);
+						else issue(d - READS);
+						__builtin_amdgcn_sched_barrier(0);
+					}
+			}
+			__builtin_amdgcn_sched_barrier(0);
+		};
+#pragma unroll
+		for (int s = 0; s < STAGES; ++s) {   // the steps behind the last one read zeros
 			next_step();
 #pragma unroll
 			for (int i = 0; i < LOADS; ++i) issue(i);
 		}
-		int at = 0;
-		for (int s = 0; s < steps; ++s) {
-			wait_and_sync<(STAGES - 2) * LOADS>();   // this step has landed; the one before has been read
-			const lds_char* p = lds + at * STAGE_BYTES;
-			at = at + 1 == STAGES ? 0 : at + 1;
-			next_step();
-			i32x4 mh[MB], ml[MB], nh[NB], nl[NB];
+		wait_and_sync<(STAGES - 1) * LOADS>();
 #pragma unroll
-			for (int b = 0; b < MB; ++b) mh[b] = frag<MT>(p + NT::BYTES, wm * (BM / WM) + b * 16, 0, lane);
-#pragma unroll
-			for (int b = 0; b < NB; ++b) nh[b] = frag<NT>(p, wn * (BN / WN) + b * 16, 0, lane);
-#pragma unroll
-			for (int b = 0; b < MB; ++b) ml[b] = frag<MT>(p + NT::BYTES, wm * (BM / WM) + b * 16, 1, lane);
-#pragma unroll
-			for (int b = 0; b < NB; ++b) nl[b] = frag<NT>(p, wn * (BN / WN) + b * 16, 1, lane);
-			constexpr int COUNT = NB * MB;
-#pragma unroll
-			for (int part = 0; part < 3; ++part)
-#pragma unroll
-				for (int i = 0; i < COUNT; ++i) {
-					const int a = i / MB, b = i % MB;
-					acc[a][b] = part == 0 ? mfma16<f16>(nh[a], mh[b], acc[a][b]) : part == 1 ? mfma16<f16>(nh[a], ml[b], acc[a][b]) : mfma16<f16>(nl[a], mh[b], acc[a][b]);
-#pragma unroll
-					for (int d = 0; d < LOADS; ++d)
-						if (d * (2 * COUNT) / LOADS == part * COUNT + i) {   // within the first two thirds
-							__builtin_amdgcn_sched_barrier(0);
-							issue(d);
-							__builtin_amdgcn_sched_barrier(0);
-						}
-				}
+		for (int d = 0; d < READS; ++d) read(0, d, lds);
+		int s = 0;
+		for (; s + 1 < steps; s += 2) {
+			step(0);
+			step(1);
 		}
+		if (s < steps) step(0);
 		wait_and_sync();   // the DMA behind the last step too
 	}
 };
