@@ -36,8 +36,10 @@ struct Job {
 	uint32_t np;                        // n up to a multiple of 32
 	f16 *xt[2], *a, *b;                 // X^T [k][2 np] (two: an iteration reads one and writes the other), A and B [n][2 np]
 	double* sums;
+	float* partial;                     // the parts' sums of the tiles of A
+	uint32_t parts;                     // of k, in the products that give A
 };
-enum { START_SUM, START_SPLIT, START_SYM, START_APPLY, N_STARTS };
+enum { START_SUM, START_SPLIT, START_GRAM, START_SYM, START_APPLY, N_STARTS };
 struct Jobs {
 	Job job[MAX_JOBS];
 	uint32_t start[N_STARTS][MAX_JOBS + 1];   // first workgroup of each job, per kind of kernel (the products': of the tile chosen by use_tile)
@@ -307,35 +309,23 @@ __device__ __forceinline__ void write_split(f16* p, uint32_t pitch, uint32_t row
 	}
 }
 
-// Tiles that hold an element on or below the diagonal, by rows of tiles; a tile row's last tiles (M / N of them) are its square on the diagonal, whole, the others are written twice.
+// Square tiles on and below the diagonal, by rows; those below are written twice.
 template <class G> inline uint32_t symmetric_tiles(uint32_t n) {
-	const uint32_t tm = (n + G::BM - 1) / G::BM, tn = (n + G::BN - 1) / G::BN, r = G::BM / G::BN;
-	uint32_t t = 0;
-	for (uint32_t i = 0; i < tm; ++i) t += r * (i + 1) < tn ? r * (i + 1) : tn;
-	return t;
+	static_assert(G::BN == G::BM, "square");
+	const uint32_t t = (n + G::BM - 1) / G::BM;
+	return t * (t + 1) / 2;
+}
+__device__ __forceinline__ void symmetric_tile(uint32_t pid, uint32_t& tm, uint32_t& tn) {
+	for (tm = 0; pid > tm; ++tm) pid -= tm + 1;
+	tn = pid;
 }
 
-// A = X X^T (POLY 0), or B = a I + b A + c A^2 (POLY 1)
-template <class G, int POLY>
-__global__ void __launch_bounds__(G::THREADS, (SplitProduct<G, KC>::LDS_BYTES <= 80 * 1024 ? 2 : 1)) symmetric_kernel(Jobs jobs, int from) {
-	using P = SplitProduct<G, POLY ? KC : RC>;
-	__shared__ __attribute__((aligned(1024))) char lds[P::LDS_BYTES];
-	uint32_t pid = xcd_order(blockIdx.x, gridDim.x);
-	const Job& j = jobs.job[job_of(jobs, START_SYM, pid)];
-	constexpr uint32_t R = P::M / P::N;
-	uint32_t tm = 0;
-	for (uint32_t t = pid;; ++tm) {   // tile rows of R, 2 R, 3 R ... tiles
-		if (t < R * (tm + 1)) { pid = t; break; }
-		t -= R * (tm + 1);
-	}
-	const uint32_t tn = pid;
-	const Mat mat = POLY ? Mat{j.a, 2ull * j.np, j.n, 2 * j.np} : Mat{j.xt[from], 2ull * j.np, 2 * j.np, j.k};
-	f32x4 acc[P::NB][P::MB];
-	P::run(acc, mat, mat, tn * P::N, tm * P::M, lds_of(lds));
+// one tile of A = X X^T (POLY 0), or of B = a I + b A + c A^2 (POLY 1), from the sums in `acc`
+template <class P, int POLY>
+__device__ __forceinline__ void store_symmetric(const f32x4 (&acc)[P::NB][P::MB], const Job& j, uint32_t tm, uint32_t tn, lds_char* lds) {
 	const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wn = wave % P::WAVES_N, wm = wave / P::WAVES_N;
-	lds_char* mine = lds_of(lds) + wave * (32 * 144);
+	lds_char* mine = lds + wave * (32 * 144);
 	f16* const out = POLY ? j.b : j.a;
-	const bool twice = tn < tm * R;
 #pragma unroll
 	for (int a = 0; a < P::NB; a += 2)
 #pragma unroll
@@ -360,13 +350,64 @@ __global__ void __launch_bounds__(G::THREADS, (SplitProduct<G, KC>::LDS_BYTES <=
 					put_split(v[x][y], false, x, y, mine, lane);
 				}
 			write_split(out, 2 * j.np, j.n, j.np, m0, n0, mine, lane);
-			if (!twice) continue;
+			if (tn == tm) continue;
 #pragma unroll
 			for (int x = 0; x < 2; ++x)
 #pragma unroll
 				for (int y = 0; y < 2; ++y) put_split(v[x][y], true, x, y, mine, lane);
 			write_split(out, 2 * j.np, j.n, j.np, n0, m0, mine, lane);
 		}
+}
+
+// A, all of k or (a long, narrow X has few tiles) a part of it: then the sums are left as they lie in the registers, and gram_sum_kernel adds the parts in their order
+template <class G>
+__global__ void __launch_bounds__(G::THREADS, (SplitProduct<G, RC>::LDS_BYTES <= 80 * 1024 ? 2 : 1)) gram_kernel(Jobs jobs, int from) {
+	using P = SplitProduct<G, RC>;
+	__shared__ __attribute__((aligned(1024))) char lds[P::LDS_BYTES];
+	uint32_t pid = xcd_order(blockIdx.x, gridDim.x), tm, tn;
+	const Job& j = jobs.job[job_of(jobs, START_GRAM, pid)];
+	const uint32_t part = pid % j.parts, tile = pid / j.parts;
+	symmetric_tile(tile, tm, tn);
+	const uint32_t per = ((j.k + 31) / 32 + j.parts - 1) / j.parts * 32, k0 = part * per;
+	const Mat mat{j.xt[from] + (uint64_t)k0 * 2 * j.np, 2ull * j.np, 2 * j.np, min(per, j.k - k0)};
+	f32x4 acc[P::NB][P::MB];
+	P::run(acc, mat, mat, tn * P::N, tm * P::M, lds_of(lds));
+	if (j.parts == 1) { store_symmetric<P, 0>(acc, j, tm, tn, lds_of(lds)); return; }
+	f32x4* q = (f32x4*)j.partial + (uint64_t)pid * (G::BN * G::BM / 4) + threadIdx.x;
+#pragma unroll
+	for (int i = 0; i < P::NB * P::MB; ++i) q[i * G::THREADS] = acc[i / P::MB][i % P::MB];
+}
+template <class G>
+__global__ void __launch_bounds__(G::THREADS) gram_sum_kernel(Jobs jobs) {
+	using P = SplitProduct<G, RC>;
+	__shared__ __attribute__((aligned(16))) char lds[G::WN * G::WM * 32 * 144];
+	uint32_t pid = blockIdx.x, tm, tn;
+	const Job& j = jobs.job[job_of(jobs, START_SYM, pid)];
+	if (j.parts == 1) return;
+	symmetric_tile(pid, tm, tn);
+	const f32x4* q = (const f32x4*)j.partial + (uint64_t)pid * j.parts * (G::BN * G::BM / 4) + threadIdx.x;
+	f32x4 acc[P::NB][P::MB];
+#pragma unroll
+	for (int i = 0; i < P::NB * P::MB; ++i) acc[i / P::MB][i % P::MB] = q[i * G::THREADS];
+#pragma unroll 4
+	for (uint32_t part = 1; part < j.parts; ++part)
+#pragma unroll
+		for (int i = 0; i < P::NB * P::MB; ++i) acc[i / P::MB][i % P::MB] += q[part * (G::BN * G::BM / 4) + i * G::THREADS];
+	store_symmetric<P, 0>(acc, j, tm, tn, lds_of(lds));
+}
+
+// B
+template <class G>
+__global__ void __launch_bounds__(G::THREADS, (SplitProduct<G, KC>::LDS_BYTES <= 80 * 1024 ? 2 : 1)) poly_kernel(Jobs jobs) {
+	using P = SplitProduct<G, KC>;
+	__shared__ __attribute__((aligned(1024))) char lds[P::LDS_BYTES];
+	uint32_t pid = xcd_order(blockIdx.x, gridDim.x), tm, tn;
+	const Job& j = jobs.job[job_of(jobs, START_SYM, pid)];
+	symmetric_tile(pid, tm, tn);
+	const Mat mat{j.a, 2ull * j.np, j.n, 2 * j.np};
+	f32x4 acc[P::NB][P::MB];
+	P::run(acc, mat, mat, tn * P::N, tm * P::M, lds_of(lds));
+	store_symmetric<P, 1>(acc, j, tm, tn, lds_of(lds));
 }
 
 // X^T <- X^T B, or (LAST) straight into the weights
@@ -610,6 +651,8 @@ static uint64_t lay_out(Jobs& jobs, char* base) {
 	uint64_t used = 0;
 	auto take = [&](uint64_t bytes) { char* p = base ? base + used : nullptr; used += up256(bytes); return p; };
 	for (int kind = 0; kind < N_STARTS; ++kind) jobs.start[kind][0] = 0;
+	uint32_t tiles = 0;
+	for (uint32_t i = 0; i < jobs.count; ++i) tiles += symmetric_tiles<Little>(std::min(jobs.job[i].rows, jobs.job[i].cols));
 	for (uint32_t i = 0; i < jobs.count; ++i) {
 		Job& j = jobs.job[i];
 		j.n = std::min(j.rows, j.cols); j.k = std::max(j.rows, j.cols);
@@ -620,30 +663,45 @@ static uint64_t lay_out(Jobs& jobs, char* base) {
 		j.a = (f16*)take((uint64_t)j.n * j.np * 4);
 		j.b = (f16*)take((uint64_t)j.n * j.np * 4);
 		j.sums = (double*)take(blocks * 8);
+		// Few tiles: k in parts of at least 8 steps, two workgroups a CU (each holds 64 KiB of LDS).  The step of one 96 x 8192 373 -> 149 us, 256 x 4096 251 -> 152 us, 700 x 6000 (66
+		// tiles) 455 -> 363 us; with 136 tiles, 1531 x 1000, it costs: 244 -> 250 us.
+		j.parts = tiles >= 128 ? 1 : std::max(1u, std::min(512 / tiles, (j.k + 31) / 32 / 8));
+		const uint32_t steps = (j.k + 31) / 32, per = (steps + j.parts - 1) / j.parts;
+		j.parts = (steps + per - 1) / per;
+		j.partial = (float*)take(j.parts > 1 ? (uint64_t)j.parts * symmetric_tiles<Little>(j.n) * (Little::BN * Little::BM * 4) : 0);
 		jobs.start[START_SUM][i + 1] = jobs.start[START_SUM][i] + blocks;
 		jobs.start[START_SPLIT][i + 1] = jobs.start[START_SPLIT][i] + ((j.np + 63) / 64) * ((j.k + 63) / 64);
 	}
 	return used;
 }
 
-template <class P> static void use_tile(Jobs& jobs) {
+template <class G> static uint32_t count_symmetric(Jobs& jobs) {
+	for (uint32_t i = 0; i < jobs.count; ++i) {
+		const uint32_t tiles = symmetric_tiles<G>(jobs.job[i].n);
+		jobs.start[START_SYM][i + 1] = jobs.start[START_SYM][i] + tiles;
+		jobs.start[START_GRAM][i + 1] = jobs.start[START_GRAM][i] + tiles * jobs.job[i].parts;
+	}
+	return jobs.start[START_SYM][jobs.count];
+}
+template <class G> static uint32_t count_apply(Jobs& jobs) {
 	for (uint32_t i = 0; i < jobs.count; ++i) {
 		const Job& j = jobs.job[i];
-		jobs.start[START_SYM][i + 1] = jobs.start[START_SYM][i] + symmetric_tiles<P>(j.n);
-		jobs.start[START_APPLY][i + 1] = jobs.start[START_APPLY][i] + ((j.n + P::BN - 1) / P::BN) * ((j.k + P::BM - 1) / P::BM);
+		jobs.start[START_APPLY][i + 1] = jobs.start[START_APPLY][i] + ((j.n + G::BN - 1) / G::BN) * ((j.k + G::BM - 1) / G::BM);
 	}
+	return jobs.start[START_APPLY][jobs.count];
 }
 
-template <class P> static void iterate(hipStream_t st, Jobs& jobs, const Step& s, uint32_t n_iterations) {
-	use_tile<P>(jobs);
-	const uint32_t c = jobs.count;
-	const dim3 block(P::THREADS), sym(jobs.start[START_SYM][c]), apply(jobs.start[START_APPLY][c]);
-	for (uint32_t i = 0; i < n_iterations; ++i) {
-		hipLaunchKernelGGL((symmetric_kernel<P, 0>), sym, block, 0, st, jobs, (int)(i & 1));
-		hipLaunchKernelGGL((symmetric_kernel<P, 1>), sym, block, 0, st, jobs, 0);
-		if (i + 1 < n_iterations) hipLaunchKernelGGL((apply_kernel<P, 0>), apply, block, 0, st, jobs, s, (int)(i & 1));
-		else hipLaunchKernelGGL((apply_kernel<P, 1>), apply, block, 0, st, jobs, s, (int)(i & 1));
-	}
+// B of the X that `from` names
+template <class G> static void symmetric_products(hipStream_t st, Jobs& jobs, int from) {
+	const uint32_t tiles = count_symmetric<G>(jobs), groups = jobs.start[START_GRAM][jobs.count];
+	hipLaunchKernelGGL(gram_kernel<G>, dim3(groups), dim3(G::THREADS), 0, st, jobs, from);
+	if (groups > tiles) hipLaunchKernelGGL(gram_sum_kernel<G>, dim3(tiles), dim3(G::THREADS), 0, st, jobs);
+	hipLaunchKernelGGL(poly_kernel<G>, dim3(tiles), dim3(G::THREADS), 0, st, jobs);
+}
+template <class G> static void apply(hipStream_t st, Jobs& jobs, const Step& s, int from, bool last) {
+	const dim3 groups(count_apply<G>(jobs));
+	if (last) hipLaunchKernelGGL((apply_kernel<G, 1>), groups, dim3(G::THREADS), 0, st, jobs, s, from);
+	else hipLaunchKernelGGL((apply_kernel<G, 0>), groups, dim3(G::THREADS), 0, st, jobs, s, from);
 }
 
 } // namespace muon
@@ -693,12 +751,18 @@ int ngp_hip_muon_step(void* stream, uint32_t n_matrices, const NgpMuonMatrix* ma
 		const uint32_t c = jobs.count;
 		hipLaunchKernelGGL(momentum_kernel, dim3(jobs.start[START_SUM][c]), dim3(256), 0, st, jobs, s);
 		hipLaunchKernelGGL(split_kernel, dim3(jobs.start[START_SPLIT][c]), dim3(256), 0, st, jobs, s);
-		use_tile<Middle>(jobs);
-		const uint32_t middle = jobs.start[START_SYM][c];
-		use_tile<Large>(jobs);
-		if (jobs.start[START_SYM][c] >= 512) iterate<Large>(st, jobs, s, n_iterations);
-		else if (middle >= 200) iterate<Middle>(st, jobs, s, n_iterations);
-		else iterate<Little>(st, jobs, s, n_iterations);
+		// The largest tile that fills the chip: 128 x 256 twice over (two 8192 x 4096: 1.25 ms where 128 x 128 take 1.7), 128 x 128 four fifths of it, else 64 x 64.  For the symmetric
+		// products 128 x 256 gave nothing over 128 x 128 (0.87 ms both: more of a larger tile lies above the diagonal).
+		const bool middle_symmetric = count_symmetric<Middle>(jobs) >= 200, large_apply = count_apply<Large>(jobs) >= 512, middle_apply = count_apply<Middle>(jobs) >= 200;
+		for (uint32_t i = 0; i < n_iterations; ++i) {
+			const int from = (int)(i & 1);
+			const bool last = i + 1 == n_iterations;
+			if (middle_symmetric) symmetric_products<Middle>(st, jobs, from);
+			else symmetric_products<Little>(st, jobs, from);
+			if (large_apply) apply<Large>(st, jobs, s, from, last);
+			else if (middle_apply) apply<Middle>(st, jobs, s, from, last);
+			else apply<Little>(st, jobs, s, from, last);
+		}
 		NGP_LAUNCH_CHECK("ngp_hip_muon_step");
 	}
 	return 0;

@@ -98,6 +98,20 @@ def test_the_whole_step_on_matrices_of_many_shapes(ngp, cuda, dtype, nesterov):
     check_step(ngp, Vector([(64, 32), (16, 64), (64, 32), (64, 64), (16, 64), (200, 136), (1, 9), (129, 128)], dtype, seed=nesterov), nesterov=nesterov, loss_scale=128.0, decay=0.1)
 
 
+@pytest.mark.parametrize("shapes", [[(500 - i, 530 + 3 * i) for i in range(24)], [(1130 + 5 * i, 1100 - i) for i in range(14)] + [(64, 2100), (700, 90)]], ids=["128x128", "128x256"])
+def test_larger_tiles(ngp, cuda, shapes):
+    """enough matrices at once for the products' tiles of 128 x 128 and of 128 x 256"""
+    check_step(ngp, Vector(shapes, "bf16", gap=1), iterations=5)
+
+
+@pytest.mark.parametrize("shapes", [[(65, 8200)], [(5000, 96)], [(100, 512), (66, 513), (300, 1111), (130, 131)]], ids=["wide", "tall", "several"])
+def test_sums_over_a_long_side_in_parts(ngp, cuda, shapes):
+    for dtype in ("f16", "f32"):
+        v = Vector(shapes, dtype, seed=5)
+        v.master.zero_()
+        check_step(ngp, v, lr=1.0, decay=0.0)
+
+
 def test_more_matrices_than_one_launch_takes(ngp, cuda):
     check_step(ngp, Vector([(8 + 3 * i, 90 - i) for i in range(60)], "bf16", gap=1), iterations=5)
     check_step(ngp, Vector([(70 + i, 150 - i) for i in range(30)], "f16", gap=0), iterations=3)
