@@ -178,29 +178,33 @@ __global__ void __launch_bounds__(256) split_fold_kernel(float* partial, uint32_
 	*(f32x4*)(partial + first * floats + at) = v;
 }
 
-// the splits of the tiles (every `every`-th of them, where they have been folded), added in order, rounded once; items without splits have no tiles here
+// The splits of the tiles (every `every`-th of them, where they have been folded), added in order, rounded once; a workgroup takes two of a tile's MB block rows, the 32 rows that
+// are stored together.  Items without splits have no tiles here.
 template <class T>
 __global__ void __launch_bounds__(256) group_sum_kernel(Group<T> g) {
 	using S = Shape<false>;
 	constexpr int NB = S::N / S::WN / 16, MB = S::M / S::WM / 16;
 	__shared__ __attribute__((aligned(16))) char lds[S::WN * S::WM * Rows<NB>::BYTES];
+	const uint32_t pid = blockIdx.x / (MB / 2), c0 = blockIdx.x % (MB / 2) * 2;
 	uint32_t i = 0;
-	while (i + 1 < g.n && blockIdx.x >= g.item[i + 1].first) ++i;
+	while (i + 1 < g.n && pid >= g.item[i + 1].first) ++i;
 	const Item<T>& it = g.item[i];
-	const uint32_t t = blockIdx.x - it.first, tiles = it.tiles_n * it.tiles_m, tn = t % it.tiles_n, tm = t / it.tiles_n;
+	const uint32_t t = pid - it.first, tiles = it.tiles_n * it.tiles_m, tn = t % it.tiles_n, tm = t / it.tiles_n;
 	const uint32_t every = it.partials > SUM_FAN ? SUM_FAN : 1, splits = (it.partials + every - 1) / every;
-	const float* q = it.partial + (uint64_t)t * (S::N * S::M) + threadIdx.x * 4;
+	const float* q = it.partial + (uint64_t)t * (S::N * S::M) + c0 * (S::THREADS * 4) + threadIdx.x * 4;
 	const uint64_t stride = (uint64_t)every * tiles * (S::N * S::M);
 	const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wn = wave % S::WN, wm = wave / S::WN;
-	f32x4 acc[1][NB][MB];
+	f32x4 acc[1][NB][2];
 	clear(acc);
-	for (uint32_t s = 0; s < splits; ++s, q += stride)
+#pragma unroll 4
+	for (uint32_t s = 0; s < splits; ++s)
 #pragma unroll
 		for (int b = 0; b < NB; ++b)
 #pragma unroll
-			for (int c = 0; c < MB; ++c) acc[0][b][c] += *(const f32x4*)(q + (b * MB + c) * (S::THREADS * 4));
-	store_tile<T, NB, MB>(acc, it.out, tn * S::N + wn * (NB * 16), tm * S::M + wm * (MB * 16), lds_of(lds) + wave * Rows<NB>::BYTES, lane);
+			for (int c = 0; c < 2; ++c) acc[0][b][c] += *(const f32x4*)(q + s * stride + (b * MB + c) * (S::THREADS * 4));
+	store_tile<T, NB, 2>(acc, it.out, tn * S::N + wn * (NB * 16), tm * S::M + wm * (MB * 16) + c0 * 16, lds_of(lds) + wave * Rows<NB>::BYTES, lane);
 }
+constexpr uint32_t SUM_GROUPS = Shape<false>::M / Shape<false>::WM / 16 / 2;   // workgroups to a tile
 
 // g, u and dh of a tile in one set of registers; from them dg, du (next to each other: d[m][0 .. f8) and d[m][f8 .. 2 f8)) and h
 template <class T, bool BIG>
@@ -406,22 +410,37 @@ template <class T> static int run_narrow_backward(hipStream_t st, const NarrowAr
 	NGP_LAUNCH_CHECK("narrow_backward_kernel");
 	return 0;
 }
-// ---- few rows: a launch for h and one for y.  Workgroups of 4 to 16 waves (8 for the pair of matrices, whose sums take twice the LDS): about 2048 waves, 8 a CU.
-template <class T, int NM, int MB> static void launch_few(hipStream_t st, const T* x, uint64_t x_ld, uint32_t rows, const T* w0, const T* w1, uint32_t n, uint32_t k, T* out, uint64_t out_ld, int act) {
-	const uint32_t groups = (n + 15) / 16;
+// ---- few rows: a launch for h and one for y, and one that packs x.  Workgroups of 4 to 16 waves (8 for the pair of matrices, whose sums take twice the LDS): about 2048 waves, 8 a CU.
+template <class T, int NM, int MB, bool PX, bool PO>
+static void launch_few(hipStream_t st, const void* x, uint64_t x_ld, uint32_t rows, const void* w0, const void* w1, uint32_t n, uint32_t k, void* out, uint64_t out_ld, int act) {
+	const uint32_t groups = PO ? (n + 31) / 32 * 2 : (n + 15) / 16;
 	uint32_t waves = 4;
 	while (waves < (NM == 2 ? 8 : 16) && groups * waves < 2048 && waves * (FEW_CHUNK * 32) < k) waves *= 2;
-	hipLaunchKernelGGL((few_rows_kernel<T, NM, MB>), dim3(groups), dim3(64 * waves), 0, st, x, x_ld, rows, w0, w1, n, k, out, out_ld, act);
+	hipLaunchKernelGGL((few_rows_kernel<T, NM, MB, PX, PO>), dim3(groups), dim3(64 * waves), 0, st, (const T*)x, x_ld, rows, (const T*)w0, (const T*)w1, n, k, (T*)out, out_ld, act);
 }
-template <class T, int NM> static void pick_few(hipStream_t st, const T* x, uint64_t x_ld, uint32_t rows, const T* w0, const T* w1, uint32_t n, uint32_t k, T* out, uint64_t out_ld, int act) {
-	if (rows <= 16) launch_few<T, NM, 1>(st, x, x_ld, rows, w0, w1, n, k, out, out_ld, act);
-	else if (rows <= 32) launch_few<T, NM, 2>(st, x, x_ld, rows, w0, w1, n, k, out, out_ld, act);
-	else launch_few<T, NM, 4>(st, x, x_ld, rows, w0, w1, n, k, out, out_ld, act);
+constexpr uint32_t FEW_PACK_H = 8, FEW_PACK_X = 5 << 16;
+// Which of the two products' rows are packed.  h where more than a few rows are read of it: 12 rows, 2048 - 8192 - 2048, 28.9 -> 27.9 us, one row 24 -> 26.5.  x where that saves more
+// than its launch takes: 32 rows of that block 33.4 us without and 34 with, 48 rows 41.9 and 39.4.
+static uint32_t few_pitch(uint32_t width) { return (width + 31) & ~31u; }
+static uint64_t few_padded(uint64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
+static bool few_pack_h(uint64_t rows) { return rows > FEW_PACK_H; }
+static bool few_pack_x(uint64_t rows, const NgpGatedFfn& b) { return few_pack_h(rows) && rows * ((uint64_t)b.n_in + b.n_hidden) >= FEW_PACK_X; }
+template <class T, int MB>
+static void launch_few_pair(hipStream_t st, const NgpGatedFfn& b, uint32_t rows, const void* x, uint64_t x_ld, const void* wg, const void* wu, const void* wd, void* y, uint64_t y_ld, void* h, void* packed) {
+	const uint32_t pitch = few_pitch(b.n_hidden), d = b.n_in, f = b.n_hidden;
+	if (few_pack_x(rows, b)) {
+		hipLaunchKernelGGL((pack_few_kernel<T, MB>), dim3((d + 127) / 128 * MB), dim3(256), 0, st, (const T*)x, x_ld, rows, d, (T*)packed);
+		launch_few<T, 2, MB, true, true>(st, packed, 0, rows, wg, wu, f, d, h, 0, b.activation);
+	} else if (few_pack_h(rows)) launch_few<T, 2, MB, false, true>(st, x, x_ld, rows, wg, wu, f, d, h, 0, b.activation);
+	else launch_few<T, 2, 1, false, false>(st, x, x_ld, rows, wg, wu, f, d, h, pitch, b.activation);
+	if (few_pack_h(rows)) launch_few<T, 1, MB, true, false>(st, h, 0, rows, wd, nullptr, b.n_out, f, y, y_ld, 0);
+	else launch_few<T, 1, 1, false, false>(st, h, pitch, rows, wd, nullptr, b.n_out, f, y, y_ld, 0);
 }
-template <class T> static int run_few(hipStream_t st, const NgpGatedFfn& b, uint32_t rows, const void* x, uint64_t x_ld, const void* wg, const void* wu, const void* wd, void* y, uint64_t y_ld, void* h) {
-	const uint32_t pitch = (b.n_hidden + 31) & ~31u;
-	pick_few<T, 2>(st, (const T*)x, x_ld, rows, (const T*)wg, (const T*)wu, b.n_hidden, b.n_in, (T*)h, pitch, b.activation);
-	pick_few<T, 1>(st, (const T*)h, pitch, rows, (const T*)wd, nullptr, b.n_out, b.n_hidden, (T*)y, y_ld, 0);
+template <class T>
+static int run_few(hipStream_t st, const NgpGatedFfn& b, uint32_t rows, const void* x, uint64_t x_ld, const void* wg, const void* wu, const void* wd, void* y, uint64_t y_ld, void* h, void* packed) {
+	if (rows <= 16) launch_few_pair<T, 1>(st, b, rows, x, x_ld, wg, wu, wd, y, y_ld, h, packed);
+	else if (rows <= 32) launch_few_pair<T, 2>(st, b, rows, x, x_ld, wg, wu, wd, y, y_ld, h, packed);
+	else launch_few_pair<T, 4>(st, b, rows, x, x_ld, wg, wu, wd, y, y_ld, h, packed);
 	NGP_LAUNCH_CHECK("few_rows_kernel");
 	return 0;
 }
@@ -446,7 +465,8 @@ struct Space {
 			return;
 		}
 		if (!backward && rows <= FEW_ROWS) {
-			h = a.take(rows * fp * 2);
+			h = a.take((few_pack_h(rows) ? few_padded(rows) : rows) * fp * 2);
+			if (few_pack_x(rows, b)) x = a.take(few_padded(rows) * few_pitch(b.n_in) * 2);
 			bytes = a.used;
 			return;
 		}
@@ -529,7 +549,7 @@ struct Launch {
 				hipLaunchKernelGGL(split_fold_kernel, dim3((uint32_t)(floats / 1024 * ceil_div(it.partials, SUM_FAN))), dim3(256), 0, st, it.partial, it.partials, floats);
 			}
 		}
-		hipLaunchKernelGGL((group_sum_kernel<T>), dim3(sum_groups), dim3(256), 0, st, s);
+		hipLaunchKernelGGL((group_sum_kernel<T>), dim3(sum_groups * SUM_GROUPS), dim3(256), 0, st, s);
 		ok("group_sum_kernel");
 	}
 };
@@ -624,8 +644,8 @@ int ngp_hip_gated_ffn_forward(void* stream, const NgpGatedFfn* b, uint64_t n_row
 	const bool plain = (b->n_in % 8 || (dma_ready(tx) && dma_ready(tg) && dma_ready(tu))) && (b->n_hidden % 8 || dma_ready(td));
 	const Space s((char*)workspace, *b, n_rows, false, !plain);
 	if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < s.bytes) return refuse("ngp_hip_gated_ffn_forward: workspace null, not 16-byte aligned or too small (ngp_hip_gated_ffn_workspace_bytes; rows that are not 16-byte aligned: NGP_FFN_ANY_LAYOUT)");
-	if (n_rows <= FEW_ROWS) return b->dtype == NGP_DTYPE_F16 ? run_few<f16>((hipStream_t)stream, *b, (uint32_t)n_rows, x, x_stride, w_gate, w_up, w_down, y, y_stride, s.h)
-	                                                         : run_few<b16>((hipStream_t)stream, *b, (uint32_t)n_rows, x, x_stride, w_gate, w_up, w_down, y, y_stride, s.h);
+	if (n_rows <= FEW_ROWS) return b->dtype == NGP_DTYPE_F16 ? run_few<f16>((hipStream_t)stream, *b, (uint32_t)n_rows, x, x_stride, w_gate, w_up, w_down, y, y_stride, s.h, s.x)
+	                                                         : run_few<b16>((hipStream_t)stream, *b, (uint32_t)n_rows, x, x_stride, w_gate, w_up, w_down, y, y_stride, s.h, s.x);
 	if (b->dtype == NGP_DTYPE_F16) return forward<f16>((hipStream_t)stream, *b, s, tx, tg, tu, td, y, y_stride);
 	return forward<b16>((hipStream_t)stream, *b, s, tx, tg, tu, td, y, y_stride);
 }
