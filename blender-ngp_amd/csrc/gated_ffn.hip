@@ -23,9 +23,16 @@ template <int ACT>
 __device__ __forceinline__ float2 activate(float g) {
 	if (ACT == NGP_ACT_NONE) return make_float2(g, 1.0f);
 	if (ACT == NGP_ACT_RELU) return g <= 0.0f ? make_float2(0.0f, 0.0f) : make_float2(g, 1.0f);   // a NaN stays one
-	if (ACT == NGP_ACT_GELU) {   // g Phi(g); erfc keeps the small tail's digits
-		const float phi = 0.5f * erfcf(g * -0.70710678f);
-		return make_float2(g * phi, phi + g * 0.39894228f * __expf(-0.5f * g * g));
+	if (ACT == NGP_ACT_GELU) {
+		// g Phi(g).  Phi(-a) = e^(-a^2/2) R(a) for a >= 0, R smooth: t P(t), t = 1 / (1 + 0.325 a), P the polynomial of degree 7 with the least relative error, 6.8e-7 (with the
+		// roundings here Phi(-a) is within 2e-6 of itself up to a = 6: its small tail keeps its digits).  One exponential serves the value and the derivative; with erfcf the
+		// backward pass of 4096 x 1024 - 2816 - 1024 took 222 us, SiLU's 202.
+		const float e = __expf(-0.5f * g * g), t = __builtin_amdgcn_rcpf(1.0f + 0.325f * fabsf(g));
+		float p = 0.0338170901f;
+		p = fmaf(p, t, -0.113520846f); p = fmaf(p, t, 0.0853101463f); p = fmaf(p, t, 0.0260451920f); p = fmaf(p, t, 0.0935166031f);
+		p = fmaf(p, t, 0.115503825f); p = fmaf(p, t, 0.129672095f); p = fmaf(p, t, 0.129656151f);
+		const float tail = p * t * e, phi = g < 0.0f ? tail : 1.0f - tail;
+		return make_float2(g * phi, fmaf(g * 0.39894228f, e, phi));
 	}
 	const float s = __builtin_amdgcn_rcpf(1.0f + __expf(-g));   // both within 2 ulp
 	if (ACT == NGP_ACT_LOGISTIC) return make_float2(s, s * (1.0f - s));
@@ -53,9 +60,11 @@ __device__ __forceinline__ void with_activation(int act, F f) {
 namespace ngp {
 namespace ffn {
 
-template <bool BIG> struct Shape;   // BIG: 256 x 256 in 8 waves, one workgroup a CU; else 128 x 128 in 4 waves, two a CU
-template <> struct Shape<true> { static constexpr int N = 256, M = 256, WN = 2, WM = 4, THREADS = 512, RESIDENT = 2; };
-template <> struct Shape<false> { static constexpr int N = 128, M = 128, WN = 2, WM = 2, THREADS = 256, RESIDENT = 2; };
+enum { SMALL, BIG, HALF };
+template <int SHAPE> struct Shape;   // BIG: 256 x 256 in 8 waves, one workgroup a CU; HALF: 256 x 128 in 8 waves; SMALL: 128 x 128 in 4 waves, two a CU
+template <> struct Shape<BIG> { static constexpr int N = 256, M = 256, WN = 2, WM = 4, THREADS = 512, RESIDENT = 2; };
+template <> struct Shape<HALF> { static constexpr int N = 256, M = 128, WN = 4, WM = 2, THREADS = 512, RESIDENT = 2; };
+template <> struct Shape<SMALL> { static constexpr int N = 128, M = 128, WN = 2, WM = 2, THREADS = 256, RESIDENT = 2; };
 
 template <int NM, int NB, int MB> __device__ __forceinline__ void clear(f32x4 (&acc)[NM][NB][MB]) {
 #pragma unroll
@@ -67,20 +76,22 @@ template <int NM, int NB, int MB> __device__ __forceinline__ void clear(f32x4 (&
 }
 
 // h = act(x Wg^T) * (x Wu^T): one tile of rows of x against N / 2 gate rows and the same N / 2 up rows, so that both factors of an h meet in one lane
-template <class T, bool BIG>
-__global__ void __launch_bounds__(Shape<BIG>::THREADS, Shape<BIG>::RESIDENT) gate_up_kernel(Mat x, Mat wg, Mat wu, Out<T> h, int act, uint32_t tiles_n, uint32_t tiles_m) {
-	using S = Shape<BIG>;
+template <class T, int SHAPE> struct HiddenProducts {
+	using S = Shape<SHAPE>;
 	using P = Product<T, KC, KC, 2, S::N / 2, S::M, S::WN, S::WM>;
-	__shared__ __attribute__((aligned(1024))) char lds[P::LDS_BYTES];
-	uint32_t tn, tm, split;
-	tile_of(blockIdx.x, gridDim.x, tiles_n, tiles_m, tn, tm, split);
+	using Q = Product<T, RC, KC, 1, S::N / 2, S::M, S::WN, S::WM>;
+	static_assert(Q::LDS_BYTES <= P::LDS_BYTES, "one buffer for both");
+};
+template <class T, int SHAPE>
+__device__ __forceinline__ void gate_up_tile(const Mat& x, const Mat& wg, const Mat& wu, const Out<T>& h, int act, uint32_t n0, uint32_t m0, lds_char* lds) {
+	using S = Shape<SHAPE>;
+	using P = typename HiddenProducts<T, SHAPE>::P;
 	f32x4 acc[2][P::NB][P::MB];
 	clear(acc);
 	const Mat w[2] = {wg, wu};
-	const uint32_t n0 = tn * (S::N / 2), m0 = tm * S::M;
-	P::run(acc, w, x, n0, m0, 0, x.k, lds_of(lds));
+	P::run(acc, w, x, n0, m0, 0, x.k, lds);
 	const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wn = wave % S::WN, wm = wave / S::WN;
-	lds_char* mine = lds_of(lds) + wave * Rows<P::NB>::BYTES;
+	lds_char* mine = lds + wave * Rows<P::NB>::BYTES;
 #pragma unroll
 	for (int c = 0; c < P::MB; ++c) {
 		with_activation(act, [&](auto a) {
@@ -94,6 +105,27 @@ __global__ void __launch_bounds__(Shape<BIG>::THREADS, Shape<BIG>::RESIDENT) gat
 		});
 		if (c & 1) store_rows<T, P::NB>(h, n0 + wn * (P::NB * 16), m0 + wm * (P::MB * 16) + (c - 1) * 16, mine, lane);
 	}
+}
+
+// The tiles of a launch over all of h: rows of BIG tiles and, behind them, rows of tiles half as high, where those spare most of a round of the chip (cover_of)
+struct Cover { uint32_t tiles_n, tiles_m, half_first, half_tiles_m; };   // half_first: the first workgroup with a half tile, a multiple of 8
+// f(Constant<shape>, n0, m0) for this workgroup's tile
+template <int SHAPE, bool HALVES, class F>
+__device__ __forceinline__ void with_tile(const Cover& c, F f) {
+	uint32_t tn, tm, split;
+	if (!HALVES || blockIdx.x < c.half_first) {
+		if (HALVES && blockIdx.x >= c.tiles_n * c.tiles_m) return;
+		tile_of(blockIdx.x, c.tiles_n * c.tiles_m, c.tiles_n, c.tiles_m, tn, tm, split);
+		f(Constant<SHAPE>(), tn * (Shape<SHAPE>::N / 2), tm * Shape<SHAPE>::M);
+	} else {
+		tile_of(blockIdx.x - c.half_first, c.tiles_n * c.half_tiles_m, c.tiles_n, c.half_tiles_m, tn, tm, split);
+		f(Constant<HALF>(), tn * (Shape<HALF>::N / 2), c.tiles_m * Shape<BIG>::M + tm * Shape<HALF>::M);
+	}
+}
+template <class T, int SHAPE, bool HALVES>
+__global__ void __launch_bounds__(Shape<SHAPE>::THREADS, Shape<SHAPE>::RESIDENT) gate_up_kernel(Mat x, Mat wg, Mat wu, Out<T> h, int act, Cover cover) {
+	__shared__ __attribute__((aligned(1024))) char lds[HiddenProducts<T, SHAPE>::P::LDS_BYTES];
+	with_tile<SHAPE, HALVES>(cover, [&](auto shape, uint32_t n0, uint32_t m0) { gate_up_tile<T, decltype(shape)::value>(x, wg, wu, h, act, n0, m0, lds_of(lds)); });
 }
 
 struct Pair { Mat n, m; };                        // one product's operands
@@ -122,9 +154,9 @@ __device__ __forceinline__ void store_tile(f32x4 (&acc)[1][NB][MB], const Rows2<
 	}
 }
 
-template <class T, int NLAY, int MLAY, bool BIG>
+template <class T, int NLAY, int MLAY, int SHAPE>
 __device__ __forceinline__ void one_tile(const Item<T>& it, uint32_t pid, lds_char* lds) {
-	using S = Shape<BIG>;
+	using S = Shape<SHAPE>;
 	using P = Product<T, NLAY, MLAY, 1, S::N, S::M, S::WN, S::WM>;
 	uint32_t tn, tm, split;
 	tile_of(pid, it.count, it.tiles_n, it.tiles_m, tn, tm, split);
@@ -153,18 +185,18 @@ __device__ __forceinline__ void one_tile(const Item<T>& it, uint32_t pid, lds_ch
 // All results that are ready to be computed at one point in one launch: y (FORWARD), or dx and the three weight gradients, whose tiles fill the chip together where each alone would
 // leave a part of it idle.  With splits, a workgroup leaves its accumulators in `partial` as they lie in the registers, and group_sum_kernel adds the splits in their order: the
 // result does not depend on which workgroup ends first.
-template <class T, bool BIG, bool FORWARD>
-__global__ void __launch_bounds__(Shape<BIG>::THREADS, Shape<BIG>::RESIDENT) group_kernel(Group<T> g) {
-	using S = Shape<BIG>;
+template <class T, int SHAPE, bool FORWARD>
+__global__ void __launch_bounds__(Shape<SHAPE>::THREADS, Shape<SHAPE>::RESIDENT) group_kernel(Group<T> g) {
+	using S = Shape<SHAPE>;
 	__shared__ __attribute__((aligned(1024))) char lds[Product<T, KC, KC, 1, S::N, S::M, S::WN, S::WM>::LDS_BYTES];
 	uint32_t i = 0;
 	while (i + 1 < g.n && blockIdx.x >= g.item[i + 1].first) ++i;
 	const Item<T>& it = g.item[i];
 	const uint32_t pid = blockIdx.x - it.first;
 	if (pid >= it.count) return;
-	if (FORWARD) one_tile<T, KC, KC, BIG>(it, pid, lds_of(lds));
-	else if (it.turned) one_tile<T, RC, RC, BIG>(it, pid, lds_of(lds));
-	else one_tile<T, RC, KC, BIG>(it, pid, lds_of(lds));
+	if (FORWARD) one_tile<T, KC, KC, SHAPE>(it, pid, lds_of(lds));
+	else if (it.turned) one_tile<T, RC, RC, SHAPE>(it, pid, lds_of(lds));
+	else one_tile<T, RC, KC, SHAPE>(it, pid, lds_of(lds));
 }
 
 // `splits` partials -> ceil(splits / SUM_FAN) in the first of them, sixteen neighbours in their order: a long list of splits would otherwise be one workgroup's serial work
@@ -182,7 +214,7 @@ __global__ void __launch_bounds__(256) split_fold_kernel(float* partial, uint32_
 // are stored together.  Items without splits have no tiles here.
 template <class T>
 __global__ void __launch_bounds__(256) group_sum_kernel(Group<T> g) {
-	using S = Shape<false>;
+	using S = Shape<SMALL>;
 	constexpr int NB = S::N / S::WN / 16, MB = S::M / S::WM / 16;
 	__shared__ __attribute__((aligned(16))) char lds[S::WN * S::WM * Rows<NB>::BYTES];
 	const uint32_t pid = blockIdx.x / (MB / 2), c0 = blockIdx.x % (MB / 2) * 2;
@@ -204,27 +236,23 @@ __global__ void __launch_bounds__(256) group_sum_kernel(Group<T> g) {
 			for (int c = 0; c < 2; ++c) acc[0][b][c] += *(const f32x4*)(q + s * stride + (b * MB + c) * (S::THREADS * 4));
 	store_tile<T, NB, 2>(acc, it.out, tn * S::N + wn * (NB * 16), tm * S::M + wm * (MB * 16) + c0 * 16, lds_of(lds) + wave * Rows<NB>::BYTES, lane);
 }
-constexpr uint32_t SUM_GROUPS = Shape<false>::M / Shape<false>::WM / 16 / 2;   // workgroups to a tile
+constexpr uint32_t SUM_GROUPS = Shape<SMALL>::M / Shape<SMALL>::WM / 16 / 2;   // workgroups to a tile
 
 // g, u and dh of a tile in one set of registers; from them dg, du (next to each other: d[m][0 .. f8) and d[m][f8 .. 2 f8)) and h
-template <class T, bool BIG>
-__global__ void __launch_bounds__(Shape<BIG>::THREADS, Shape<BIG>::RESIDENT) hidden_backward_kernel(Mat x, Mat wg, Mat wu, Mat dy, Mat wd, Out<T> dg, Out<T> du, Out<T> h, int act, uint32_t tiles_n, uint32_t tiles_m) {
-	using S = Shape<BIG>;
-	using P = Product<T, KC, KC, 2, S::N / 2, S::M, S::WN, S::WM>;
-	using Q = Product<T, RC, KC, 1, S::N / 2, S::M, S::WN, S::WM>;
-	__shared__ __attribute__((aligned(1024))) char lds[P::LDS_BYTES];
-	static_assert(Q::LDS_BYTES <= P::LDS_BYTES, "one buffer for both");
-	uint32_t tn, tm, split;
-	tile_of(blockIdx.x, gridDim.x, tiles_n, tiles_m, tn, tm, split);
+template <class T, int SHAPE>
+__device__ __forceinline__ void hidden_backward_tile(const Mat& x, const Mat& wg, const Mat& wu, const Mat& dy, const Mat& wd, const Out<T>& dg, const Out<T>& du, const Out<T>& h, int act, uint32_t n0, uint32_t m0,
+                                                     lds_char* lds) {
+	using S = Shape<SHAPE>;
+	using P = typename HiddenProducts<T, SHAPE>::P;
+	using Q = typename HiddenProducts<T, SHAPE>::Q;
 	f32x4 gu[2][P::NB][P::MB], dh[1][P::NB][P::MB];
 	clear(gu);
 	const Mat w[2] = {wg, wu};
-	const uint32_t n0 = tn * (S::N / 2), m0 = tm * S::M;
-	P::run(gu, w, x, n0, m0, 0, x.k, lds_of(lds));
+	P::run(gu, w, x, n0, m0, 0, x.k, lds);
 	clear(dh);
-	Q::run(dh, &wd, dy, n0, m0, 0, dy.k, lds_of(lds));
+	Q::run(dh, &wd, dy, n0, m0, 0, dy.k, lds);
 	const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wn = wave % S::WN, wm = wave / S::WN;
-	lds_char* mine = lds_of(lds) + wave * (3 * Rows<P::NB>::BYTES);
+	lds_char* mine = lds + wave * (3 * Rows<P::NB>::BYTES);
 	static_assert(S::WN * S::WM * 3 * Rows<P::NB>::BYTES <= P::LDS_BYTES, "three results of every wave at once");
 	const uint32_t n = n0 + wn * (P::NB * 16);
 #pragma unroll
@@ -252,6 +280,12 @@ __global__ void __launch_bounds__(Shape<BIG>::THREADS, Shape<BIG>::RESIDENT) hid
 		store_rows<T, P::NB>(dg, n, m, mine + Rows<P::NB>::BYTES, lane);
 		store_rows<T, P::NB>(du, n, m, mine + 2 * Rows<P::NB>::BYTES, lane);
 	}
+}
+
+template <class T, int SHAPE, bool HALVES>
+__global__ void __launch_bounds__(Shape<SHAPE>::THREADS, Shape<SHAPE>::RESIDENT) hidden_backward_kernel(Mat x, Mat wg, Mat wu, Mat dy, Mat wd, Out<T> dg, Out<T> du, Out<T> h, int act, Cover cover) {
+	__shared__ __attribute__((aligned(1024))) char lds[HiddenProducts<T, SHAPE>::P::LDS_BYTES];
+	with_tile<SHAPE, HALVES>(cover, [&](auto shape, uint32_t n0, uint32_t m0) { hidden_backward_tile<T, decltype(shape)::value>(x, wg, wu, dy, wd, dg, du, h, act, n0, m0, lds_of(lds)); });
 }
 
 // rows of any width, stride and alignment -> rows of a multiple of 8 elements, 16-byte aligned, zeros behind the width; all of a call's tensors in one launch
@@ -345,6 +379,24 @@ static uint64_t partial_room(const Size* s, int count) {
 	for (int i = 0; i < count; ++i)
 		if (s[i].k >= 1024) parts += ceil_div(s[i].n, 128) * ceil_div(s[i].m, 128) * s[i].n_products * (s[i].k / 512);
 	return std::min<uint64_t>(512, parts) * (128 * 128 * 4);
+}
+
+// The tiles of h: BIG where they fill three quarters of the 256 CUs.  A round of BIG tiles that would leave half of the chip idle or more is made of half tiles instead: such a round
+// takes 0.7 of the other.
+static bool cover_of(uint32_t width, uint64_t rows, Cover& c, uint32_t& groups) {
+	const bool big = ceil_div(width, 128) * ceil_div(rows, 256) >= 192;
+	c.tiles_n = (uint32_t)ceil_div(width, big ? 128 : 64); c.tiles_m = (uint32_t)ceil_div(rows, big ? 256 : 128);
+	c.half_tiles_m = 0;
+	const uint64_t tiles = (uint64_t)c.tiles_n * c.tiles_m;
+	c.half_first = groups = (uint32_t)tiles;
+	if (!big || tiles < 256) return big;
+	const uint32_t whole = (uint32_t)(tiles / 256 * 256 / c.tiles_n);   // rows of tiles in the full rounds
+	const uint64_t halves = ceil_div(rows - std::min<uint64_t>(rows, whole * 256ull), 128);
+	if (halves == 0 || halves * c.tiles_n > 256) return big;
+	c.tiles_m = whole; c.half_tiles_m = (uint32_t)halves;
+	c.half_first = (c.tiles_n * whole + 7) & ~7u;
+	groups = c.half_first + c.tiles_n * c.half_tiles_m;
+	return big;
 }
 
 struct Tensor { const void* p; uint64_t ld; uint64_t rows; uint32_t cols; };
@@ -533,8 +585,8 @@ struct Launch {
 			groups += (it.count + 7) & ~7u;
 			sums |= it.partials != 0;
 		}
-		if (big) hipLaunchKernelGGL((group_kernel<T, true, FORWARD>), dim3(groups), dim3(Shape<true>::THREADS), 0, st, g);
-		else hipLaunchKernelGGL((group_kernel<T, false, FORWARD>), dim3(groups), dim3(Shape<false>::THREADS), 0, st, g);
+		if (big) hipLaunchKernelGGL((group_kernel<T, BIG, FORWARD>), dim3(groups), dim3(Shape<BIG>::THREADS), 0, st, g);
+		else hipLaunchKernelGGL((group_kernel<T, SMALL, FORWARD>), dim3(groups), dim3(Shape<SMALL>::THREADS), 0, st, g);
 		if (!ok("group_kernel") || !sums) return;
 		Group<T> s;
 		s.n = 0;
@@ -565,10 +617,12 @@ static int forward(hipStream_t st, const NgpGatedFfn& b, const Space& s, Tensor 
 	l.pad();
 	if (l.rc) return l.rc;
 	const Out<T> h{(T*)s.h, s.fp, (uint32_t)x.rows, s.fp};
-	const bool big = ceil_div(s.fp, 128) * ceil_div(x.rows, 256) >= 192;
-	const uint32_t tn = (uint32_t)ceil_div(s.fp, big ? 128 : 64), tm = (uint32_t)ceil_div(x.rows, big ? 256 : 128);
-	if (big) hipLaunchKernelGGL((gate_up_kernel<T, true>), dim3(tn * tm), dim3(Shape<true>::THREADS), 0, st, kc(x), kc(wg), kc(wu), h, b.activation, tn, tm);
-	else hipLaunchKernelGGL((gate_up_kernel<T, false>), dim3(tn * tm), dim3(256), 0, st, kc(x), kc(wg), kc(wu), h, b.activation, tn, tm);
+	uint32_t groups;
+	Cover cover;
+	const bool big = cover_of(s.fp, x.rows, cover, groups);
+	if (cover.half_tiles_m) hipLaunchKernelGGL((gate_up_kernel<T, BIG, true>), dim3(groups), dim3(Shape<BIG>::THREADS), 0, st, kc(x), kc(wg), kc(wu), h, b.activation, cover);
+	else if (big) hipLaunchKernelGGL((gate_up_kernel<T, BIG, false>), dim3(groups), dim3(Shape<BIG>::THREADS), 0, st, kc(x), kc(wg), kc(wu), h, b.activation, cover);
+	else hipLaunchKernelGGL((gate_up_kernel<T, SMALL, false>), dim3(groups), dim3(Shape<SMALL>::THREADS), 0, st, kc(x), kc(wg), kc(wu), h, b.activation, cover);
 	l.ok("gate_up_kernel");
 	const Tensor th{s.h, s.fp, x.rows, s.f8};
 	Group<T> g;
@@ -589,10 +643,12 @@ static int backward(hipStream_t st, const NgpGatedFfn& b, const Space& s, Tensor
 	const uint32_t rows = (uint32_t)x.rows;
 	T* const d = (T*)s.d;
 	const Out<T> h{(T*)s.h, s.fp, rows, s.fp}, dg{d, 2ull * s.fp, rows, s.fp}, du{d + s.fp, 2ull * s.fp, rows, s.fp};
-	const bool big = ceil_div(s.fp, 128) * ceil_div(rows, 256) >= 192;
-	const uint32_t tn = (uint32_t)ceil_div(s.fp, big ? 128 : 64), tm = (uint32_t)ceil_div(rows, big ? 256 : 128);
-	if (big) hipLaunchKernelGGL((hidden_backward_kernel<T, true>), dim3(tn * tm), dim3(Shape<true>::THREADS), 0, st, kc(x), kc(wg), kc(wu), kc(dy), rc(wd), dg, du, h, b.activation, tn, tm);
-	else hipLaunchKernelGGL((hidden_backward_kernel<T, false>), dim3(tn * tm), dim3(256), 0, st, kc(x), kc(wg), kc(wu), kc(dy), rc(wd), dg, du, h, b.activation, tn, tm);
+	uint32_t groups;
+	Cover cover;
+	const bool big = cover_of(s.fp, rows, cover, groups);
+	if (cover.half_tiles_m) hipLaunchKernelGGL((hidden_backward_kernel<T, BIG, true>), dim3(groups), dim3(Shape<BIG>::THREADS), 0, st, kc(x), kc(wg), kc(wu), kc(dy), rc(wd), dg, du, h, b.activation, cover);
+	else if (big) hipLaunchKernelGGL((hidden_backward_kernel<T, BIG, false>), dim3(groups), dim3(Shape<BIG>::THREADS), 0, st, kc(x), kc(wg), kc(wu), kc(dy), rc(wd), dg, du, h, b.activation, cover);
+	else hipLaunchKernelGGL((hidden_backward_kernel<T, SMALL, false>), dim3(groups), dim3(Shape<SMALL>::THREADS), 0, st, kc(x), kc(wg), kc(wu), kc(dy), rc(wd), dg, du, h, b.activation, cover);
 	l.ok("hidden_backward_kernel");
 	const Tensor tdg{dg.p, dg.ld, rows, s.f8}, tdu{du.p, du.ld, rows, s.f8}, tboth{d, 2ull * s.fp, rows, 2 * s.fp}, th{s.h, s.fp, rows, s.fp};
 	Group<T> g;

@@ -65,7 +65,7 @@ def backward(ngp, b, x, wg, wu, wd, dy, dx, grads, ws, n, stream=None):
 # few rows (the row-streaming kernels), narrow blocks over many rows, and sizes whose tiles fill the chip for each product
 SHAPES = [(1, 1, 1, 1), (1, 8, 8, 8), (1, 64, 128, 64), (1, 520, 1032, 264), (3, 7, 5, 9), (2, 333, 77, 130), (16, 72, 264, 40), (17, 256, 96, 48), (1, 136, 264, 136), (33, 129, 130, 131), (64, 300, 500, 200), (65, 300, 500, 200), (24, 1024, 2056, 520), (33, 64, 64, 64),
           (64, 32, 64, 16), (65, 33, 65, 17), (129, 128, 96, 257), (300, 40, 200, 3), (513, 264, 328, 136), (4097, 32, 64, 16), (5000, 16, 32, 8), (3000, 64, 128, 64),
-          (2500, 96, 160, 32), (4500, 8, 64, 16), (6200, 136, 1000, 2056), (200, 1600, 4104, 3000)]
+          (2500, 96, 160, 32), (4500, 8, 64, 16), (6200, 136, 1000, 2056), (6200, 136, 1400, 72), (200, 1600, 4104, 3000)]
 
 
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
@@ -273,3 +273,19 @@ def test_rows_whose_offsets_pass_32_bits(ngp, cuda, widths):
     R.check("y", y, ref.y, ref.ey)
     for v, want, bound in zip(outs, (ref.dx, ref.dwg, ref.dwu, ref.dwd), (ref.edx, ref.edwg, ref.edwu, ref.edwd)):
         R.check("gradient", v, want, bound)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_gelu_far_out(ngp, cuda, dtype):
+    """g = u = x up to where Phi(-x) is 1e-9: one column of everything, the weights 1.  h and y are rounded once each, the activation itself within 1e-5 of its value."""
+    t = TYPES[dtype][0]
+    x = torch.linspace(-6, 6, 4099, device="cuda").to(t).view(-1, 1)
+    one = torch.ones(1, 1, device="cuda", dtype=t)
+    b = block(1, 1, 1, dtype, "gelu")
+    ws, n = workspace(ngp, b, len(x), 0)
+    y = torch.empty_like(x)
+    forward(ngp, b, x, one, one, one, y, ws, n)
+    torch.cuda.synchronize()
+    want = (x.double() ** 2 * torch.special.ndtr(x.double()))
+    smallest = torch.finfo(t).tiny * torch.finfo(t).eps   # half a step of f16's subnormal values, twice
+    assert ((y.double() - want).abs() <= (torch.finfo(t).eps + 1.1e-5) * want.abs() + smallest).all()
