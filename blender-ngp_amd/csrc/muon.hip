@@ -277,7 +277,8 @@ struct SplitProduct {
 	}
 };
 using Large = Geometry<128, 256, 2, 4, 3>;   // 144 KB of LDS
-using Middle = Geometry<128, 128, 4, 2, 4>;  // 128 KB
+using Middle = Geometry<128, 128, 2, 2, 2>;  // 64 KB: two workgroups a CU, one's MFMAs beside the other's loads and stores
+using Lone = Geometry<128, 128, 4, 2, 4>;    // 128 KB: where there is one tile a CU
 using Little = Geometry<64, 64, 2, 2, 4>;    // 64 KB: two workgroups a CU
 
 // A wave's 32 x 32 block (2 x 2 of 16) of a split matrix, through LDS of its own (32 rows of 144 bytes) into rows of 64 hi and 64 lo bytes: as it lies (rows m), or transposed (rows n)
@@ -751,16 +752,20 @@ int ngp_hip_muon_step(void* stream, uint32_t n_matrices, const NgpMuonMatrix* ma
 		const uint32_t c = jobs.count;
 		hipLaunchKernelGGL(momentum_kernel, dim3(jobs.start[START_SUM][c]), dim3(256), 0, st, jobs, s);
 		hipLaunchKernelGGL(split_kernel, dim3(jobs.start[START_SPLIT][c]), dim3(256), 0, st, jobs, s);
-		// The largest tile that fills the chip: 128 x 256 twice over (two 8192 x 4096: 1.25 ms where 128 x 128 take 1.7), 128 x 128 four fifths of it, else 64 x 64.  For the symmetric
-		// products 128 x 256 gave nothing over 128 x 128 (0.87 ms both: more of a larger tile lies above the diagonal).
-		const bool middle_symmetric = count_symmetric<Middle>(jobs) >= 200, large_apply = count_apply<Large>(jobs) >= 512, middle_apply = count_apply<Middle>(jobs) >= 200;
+		// 128 x 128 where that fills four fifths of the chip, else 64 x 64; 128 x 256 where it fills the chip twice over (two 8192 x 4096: 1.25 ms a launch where 128 x 128 take 1.7; not
+		// for the symmetric products: 0.87 ms both, more of a larger tile lies above the diagonal).  More than one 128 x 128 tile a CU: two workgroups of four waves at a time, 24 of
+		// 768 x 768 957 -> 845 us; up to one: eight waves, 6 of 768 x 768 336 -> 299 us.
+		auto tile_for = [](uint32_t tiles) { return tiles < 200 ? 0 : tiles <= 256 ? 1 : 2; };
+		const int symmetric_tile = tile_for(count_symmetric<Middle>(jobs)), apply_tile = count_apply<Large>(jobs) >= 512 ? 3 : tile_for(count_apply<Middle>(jobs));
 		for (uint32_t i = 0; i < n_iterations; ++i) {
 			const int from = (int)(i & 1);
 			const bool last = i + 1 == n_iterations;
-			if (middle_symmetric) symmetric_products<Middle>(st, jobs, from);
+			if (symmetric_tile == 2) symmetric_products<Middle>(st, jobs, from);
+			else if (symmetric_tile == 1) symmetric_products<Lone>(st, jobs, from);
 			else symmetric_products<Little>(st, jobs, from);
-			if (large_apply) apply<Large>(st, jobs, s, from, last);
-			else if (middle_apply) apply<Middle>(st, jobs, s, from, last);
+			if (apply_tile == 3) apply<Large>(st, jobs, s, from, last);
+			else if (apply_tile == 2) apply<Middle>(st, jobs, s, from, last);
+			else if (apply_tile == 1) apply<Lone>(st, jobs, s, from, last);
 			else apply<Little>(st, jobs, s, from, last);
 		}
 		NGP_LAUNCH_CHECK("ngp_hip_muon_step");
