@@ -53,12 +53,30 @@ __device__ __forceinline__ void store_transposed(const f32x16& v, T* row, uint32
 	}
 }
 
-// fragment `rows r0 .., k k0 ..` of a row-major weight matrix in A-operand order, element by element (once per workgroup); PERM: k in the order of as_operand
+// Fragment `rows r0 .., k k0 ..` of a row-major weight matrix in A-operand order, once per workgroup; perm: k in the order of as_operand.  By 16 (perm: 8) bytes where no piece ends
+// inside a row's last one, else by elements: these are eight times the requests, and all workgroups make them of the same lines at once.
 template <class T>
 __device__ __forceinline__ void stage_fragment(lds_char* dst, const T* w, uint32_t rows, uint32_t cols, uint32_t r0, uint32_t k0, bool turned, bool perm, int lane) {
 	typedef T t8 __attribute__((ext_vector_type(8)));
 	t8 v;
 	const uint32_t r = r0 + (lane & 31);
+	if (!turned && cols % 8 == 0) {
+		typedef i32x4 i32x4_any __attribute__((aligned(2)));
+		typedef i32x2 i32x2_any __attribute__((aligned(2)));
+		const T* row = w + (uint64_t)min(r, rows - 1) * cols;
+		const uint32_t k = k0 + (perm ? 4 : 8) * (lane >> 5);
+		i32x4 q = {0, 0, 0, 0};
+		if (!perm) {
+			if (r < rows && k < cols) q = *(const i32x4_any*)(row + k);
+		} else {
+			i32x2 lo = {0, 0}, hi = {0, 0};
+			if (r < rows && k < cols) lo = *(const i32x2_any*)(row + k);
+			if (r < rows && k + 8 < cols) hi = *(const i32x2_any*)(row + k + 8);
+			q = i32x4{lo.x, lo.y, hi.x, hi.y};
+		}
+		*(__attribute__((address_space(3))) i32x4*)(dst + lane * 16) = q;
+		return;
+	}
 #pragma unroll
 	for (int j = 0; j < 8; ++j) {
 		const uint32_t k = k0 + (perm ? 8 * (j >> 2) + 4 * (lane >> 5) + (j & 3) : 8 * (lane >> 5) + j);
