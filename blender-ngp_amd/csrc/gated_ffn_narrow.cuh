@@ -165,8 +165,8 @@ template <int DB, int FB, int OB> struct NarrowBackward {
 	static constexpr int ROWS = 64, BLOCKS = 2 * FB * DB + FB * OB, OWN = (BLOCKS + 3) / 4;
 	static constexpr int PX = DB * 64 + 16, PY = OB * 64 + 16, PF = FB * 64 + 16;                       // LDS row pitches in bytes
 	static constexpr int OFF_X = 0, OFF_Y = OFF_X + ROWS * PX, OFF_G = OFF_Y + ROWS * PY, OFF_U = OFF_G + ROWS * PF, OFF_H = OFF_U + ROWS * PF, OFF_W = (OFF_H + ROWS * PF + 1023) / 1024 * 1024;
-	static constexpr int W_GU = FB * 2 * DB, W_D = FB * 2 * OB, W_T = DB * 2 * FB;                      // fragments: gate (the same again: up), down^T, gate^T (again: up^T)
-	static constexpr int LDS_BYTES = OFF_W + (2 * W_GU + W_D + 2 * W_T) * 1024;
+	static constexpr int W_GU = FB * 2 * DB, W_D = FB * 2 * OB;                                         // fragments: gate (the same again: up), down^T
+	static constexpr int LDS_BYTES = OFF_W + (2 * W_GU + W_D) * 1024, RESIDENT = LDS_BYTES <= 80 * 1024 ? 2 : 1;
 };
 static_assert(NarrowBackward<2, 4, 2>::LDS_BYTES <= 160 * 1024, "the largest instance fits into a CU's LDS");
 
@@ -179,7 +179,7 @@ __device__ __forceinline__ i32x4 turned_fragment(const lds_char* tile, int pitch
 }
 
 template <class T, int DB, int FB, int OB, bool VEC>
-__global__ void __launch_bounds__(256, (NarrowBackward<DB, FB, OB>::LDS_BYTES <= 80 * 1024 ? 2 : 1)) narrow_backward_kernel(NarrowArgs a) {
+__global__ void __launch_bounds__(256, (NarrowBackward<DB, FB, OB>::RESIDENT)) narrow_backward_kernel(NarrowArgs a) {
 	using S = NarrowBackward<DB, FB, OB>;
 	__shared__ __attribute__((aligned(1024))) char smem[S::LDS_BYTES];
 	lds_char* const lds = lds_of(smem);
@@ -205,18 +205,23 @@ __global__ void __launch_bounds__(256, (NarrowBackward<DB, FB, OB>::LDS_BYTES <=
 	};
 	uint32_t tile = blockIdx.x;
 	if (tile < tiles) load(tile);
-	for (int i = wave; i < 2 * S::W_GU + S::W_D + 2 * S::W_T; i += 4) {
+	for (int i = wave; i < 2 * S::W_GU + S::W_D; i += 4) {
 		if (i < 2 * S::W_GU) {
 			const int c = i % S::W_GU;
 			stage_fragment<T>(w + i * 1024, (const T*)(i < S::W_GU ? a.wg : a.wu), a.f, a.d, c / (2 * DB) * 32, c % (2 * DB) * 16, false, false, lane);
-		} else if (i < 2 * S::W_GU + S::W_D) {
+		} else {
 			const int c = i - 2 * S::W_GU;
 			stage_fragment<T>(w + i * 1024, (const T*)a.wd, a.o, a.f, c / (2 * OB) * 32, c % (2 * OB) * 16, true, false, lane);
-		} else {
-			const int c = i - 2 * S::W_GU - S::W_D;
-			stage_fragment<T>(w + i * 1024, (const T*)(c < S::W_T ? a.wg : a.wu), a.f, a.d, (c % S::W_T) / (2 * FB) * 32, c % (2 * FB) * 16, true, false, lane);
 		}
 	}
+	// the 32 input columns of block db as rows, k hidden columns 16 c ..: the transpose of gate's (up's) fragments by transposed reads
+	auto weight_turned = [&](int up, int db, int c) {
+		const int f = c * 16 + 8 * (lane >> 5) + ((lane & 15) >> 2), d = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);   // of the block; four f by four d a lane's group
+		const lds_char* p = w + (up * S::W_GU + (f >> 5) * 2 * DB + db * 2 + (d >> 4)) * 1024 + ((d >> 3) & 1) * 512 + (f & 31) * 16 + (d & 7) * 2;
+		const i32x2 lo = __builtin_bit_cast(i32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p));
+		const i32x2 hi = __builtin_bit_cast(i32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(p + 64)));   // f + 4
+		return i32x4{lo.x, lo.y, hi.x, hi.y};
+	};
 	for (; tile < tiles; tile += gridDim.x) {
 		__syncthreads();   // phase 2 of the rows before has been read (first time: the weights are there)
 		i32x4 x[2 * DB], y[2 * OB];
@@ -280,14 +285,14 @@ __global__ void __launch_bounds__(256, (NarrowBackward<DB, FB, OB>::LDS_BYTES <=
 		if (a.dx) {
 #pragma unroll
 			for (int i = 0; i < (2 * DB + 3) / 4; ++i) {
-				const int c = wave + 4 * i, rt = c & 1, db = c >> 1;   // rows rt * 32 .., input block db
+				const int c = 3 - wave + 4 * i, rt = c & 1, db = c >> 1;   // rows rt * 32 .., input block db; first to the waves with fewer blocks of the gradients
 				if (db >= DB) break;
 				f32x16 v = zero16();
 #pragma unroll
 				for (int k = 0; k < 2 * FB; ++k) {
 					const int at = (rt * 32 + (lane & 31)) * S::PF + k * 32 + (lane >> 5) * 16;
-					v = mfma<T>(weight(2 * S::W_GU + S::W_D + db * 2 * FB + k), *(const __attribute__((address_space(3))) i32x4*)(lds + S::OFF_G + at), v);
-					v = mfma<T>(weight(2 * S::W_GU + S::W_D + S::W_T + db * 2 * FB + k), *(const __attribute__((address_space(3))) i32x4*)(lds + S::OFF_U + at), v);
+					v = mfma<T>(weight_turned(0, db, k), *(const __attribute__((address_space(3))) i32x4*)(lds + S::OFF_G + at), v);
+					v = mfma<T>(weight_turned(1, db, k), *(const __attribute__((address_space(3))) i32x4*)(lds + S::OFF_U + at), v);
 				}
 				const uint64_t m = (uint64_t)tile * 64 + rt * 32 + (lane & 31);
 				store_transposed<T>(v, m < a.rows ? (T*)a.dx + m * a.dx_ld : nullptr, db * 32, a.d, wide, lane);
