@@ -517,8 +517,7 @@ struct Space {
 			return;
 		}
 		if (!backward && rows <= FEW_ROWS) {
-			h = a.take((few_pack_h(rows) ? few_padded(rows) : rows) * fp * 2);
-			if (few_pack_x(rows, b)) x = a.take(few_padded(rows) * few_pitch(b.n_in) * 2);
+			take_few(a, b, rows);
 			bytes = a.used;
 			return;
 		}
@@ -537,6 +536,16 @@ struct Space {
 			partial = (float*)a.take(partial_room(size, 1));
 		}
 		bytes = a.used;
+		if (!backward) {   // never less than any smaller batch takes
+			Arena few{nullptr};
+			Space unused = *this;
+			unused.take_few(few, b, FEW_ROWS);
+			bytes = std::max(bytes, few.used);
+		}
+	}
+	void take_few(Arena& a, const NgpGatedFfn& b, uint64_t rows) {
+		h = a.take((few_pack_h(rows) ? few_padded(rows) : rows) * fp * 2);
+		if (few_pack_x(rows, b)) x = a.take(few_padded(rows) * few_pitch(b.n_in) * 2);
 	}
 };
 

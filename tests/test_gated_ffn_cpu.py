@@ -70,7 +70,7 @@ def test_workspace_of_a_narrow_block(ngp):
 
 def test_workspace_holds_fewer_rows(ngp):
     """the size never falls with the number of rows, across every change of kernel and tile"""
-    for d, f, o in ((32, 64, 16), (64, 128, 64), (33, 65, 17), (1024, 2816, 1024), (4096, 10240, 4096)):
+    for d, f, o in ((32, 64, 16), (64, 128, 64), (33, 65, 17), (1024, 2816, 1024), (4096, 10240, 4096), (8192, 1000, 64)):
         for flags in range(4):
             last = 0
             for rows in [*range(0, 300), *range(300, 20000, 371), 1 << 17, 1 << 18]:

@@ -63,7 +63,7 @@ def backward(ngp, b, x, wg, wu, wd, dy, dx, grads, ws, n, stream=None):
 
 # (rows, n_in, n_hidden, n_out): single rows and columns, widths around the vector and tile sizes, k that ends inside a step, rows that end inside a tile, split sums,
 # few rows (the row-streaming kernels), narrow blocks over many rows, and sizes whose tiles fill the chip for each product
-SHAPES = [(1, 1, 1, 1), (1, 8, 8, 8), (1, 64, 128, 64), (1, 520, 1032, 264), (3, 7, 5, 9), (2, 333, 77, 130), (16, 72, 264, 40), (17, 256, 96, 48), (1, 136, 264, 136), (33, 129, 130, 131), (64, 300, 500, 200), (65, 300, 500, 200), (24, 1024, 2056, 520), (33, 64, 64, 64),
+SHAPES = [(1, 1, 1, 1), (1, 8, 8, 8), (1, 64, 128, 64), (1, 520, 1032, 264), (3, 7, 5, 9), (2, 333, 77, 130), (16, 72, 264, 40), (17, 256, 96, 48), (1, 136, 264, 136), (33, 129, 130, 131), (64, 300, 500, 200), (65, 300, 500, 200), (24, 1024, 2056, 520), (9, 2000, 130, 24), (33, 64, 64, 64), (20, 8200, 8200, 40), (33, 2001, 8011, 131), (64, 1030, 4100, 72),
           (64, 32, 64, 16), (65, 33, 65, 17), (129, 128, 96, 257), (300, 40, 200, 3), (513, 264, 328, 136), (4097, 32, 64, 16), (5000, 16, 32, 8), (3000, 64, 128, 64),
           (2500, 96, 160, 32), (4500, 8, 64, 16), (6200, 136, 1000, 2056), (6200, 136, 1400, 72), (200, 1600, 4104, 3000)]
 
@@ -94,7 +94,7 @@ def test_against_64_bits(ngp, cuda, shape, dtype):
 
 
 @pytest.mark.parametrize("rows", [1, 5, 40, 300])
-@pytest.mark.parametrize("widths", [(64, 96, 48), (33, 65, 17), (32, 64, 16), (136, 200, 144), (133, 161, 139)], ids=lambda w: "x".join(map(str, w)))
+@pytest.mark.parametrize("widths", [(64, 96, 48), (33, 65, 17), (32, 64, 16), (136, 200, 144), (133, 161, 139), (2051, 6205, 24)], ids=lambda w: "x".join(map(str, w)))
 @pytest.mark.parametrize("layout", ["aligned stride", "odd stride", "odd base"])
 def test_strides_and_alignment(ngp, cuda, rows, widths, layout):
     d, f, o = widths
