@@ -42,7 +42,7 @@ struct Job {
 enum { START_SUM, START_SPLIT, START_GRAM, START_SYM, START_APPLY, N_STARTS };
 struct Jobs {
 	Job job[MAX_JOBS];
-	uint32_t start[N_STARTS][MAX_JOBS + 1];   // first workgroup of each job, per kind of kernel (the products': of the tile chosen by use_tile)
+	uint32_t start[N_STARTS][MAX_JOBS + 1];   // first workgroup of each job, per kind of kernel (the products: of the tile of the launch)
 	uint32_t count;
 };
 

@@ -2880,11 +2880,19 @@ __global__ void __launch_bounds__(256) rows_to_planes_kernel(const uint32_t* __r
 	__syncthreads();
 	for (uint32_t i = threadIdx.x; i < 1024; i += 256) if (s0 + (i & 63) < n) planes[(size_t)(i >> 6) * n + s0 + (i & 63)] = t[i & 63][i >> 6];
 }
+// the encoder and the binning pass clear their counters with memset nodes, which replay wrongly
+static bool refuse_capture(void* stream, const char* what) {
+	hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+	if (hipStreamIsCapturing((hipStream_t)stream, &status) == hipSuccess && status == hipStreamCaptureStatusNone) return false;
+	set_last_error(what, hipErrorStreamCaptureUnsupported);
+	return true;
+}
 int ngp_hip_grid_encode(void* stream, uint32_t n_dims, const NgpNetDesc* desc_dev, const uint16_t* grid, const float* pos, uint32_t pos_stride_floats, uint32_t n, uint16_t* features,
                         void* workspace, uint64_t workspace_bytes) {
 	if (n_dims != 2 && n_dims != 3) { set_last_error("ngp_hip_grid_encode: n_dims must be 2 or 3", hipErrorInvalidValue); return -1; }
 	if (!n) return 0;
 	if (!desc_dev || !grid || !pos || !features || ((uintptr_t)grid & 3) || ((uintptr_t)features & 3)) { set_last_error("ngp_hip_grid_encode: null or unaligned buffer (feature pairs are read and written as 4 bytes)", hipErrorInvalidValue); return -1; }
+	if (refuse_capture(stream, "ngp_hip_grid_encode: the stream is being captured")) return -1;
 	const h2* planes; uint32_t n_pad;
 	if (launch_encode(stream, desc_dev, grid, pos, pos_stride_floats, n, workspace, workspace_bytes, &planes, &n_pad, "ngp_hip_grid_encode: workspace too small (ngp_hip_nerf_encode_workspace_bytes)", nullptr, 0u, n_dims)) return -1;
 	hipLaunchKernelGGL(planes_to_rows_kernel, dim3(div_up(n, 64)), dim3(256), 0, (hipStream_t)stream, (const uint32_t*)planes, n_pad, n, (uint32_t*)features);
@@ -2896,6 +2904,7 @@ int ngp_hip_grid_gradient(void* stream, uint32_t n_dims, const NgpNetDesc* desc_
                           uint16_t* grid_grad, void* scratch, uint64_t scratch_bytes) {
 	if (n == 0 || (n % 256) != 0) { set_last_error("ngp_hip_grid_gradient: n must be a positive multiple of 256", hipErrorInvalidValue); return -1; }
 	if (!dL_dfeatures || ((uintptr_t)dL_dfeatures & 3) || !scratch || scratch_bytes < ngp_hip_grid_gradient_scratch_bytes(n)) { set_last_error("ngp_hip_grid_gradient: null or unaligned buffer, or scratch too small (ngp_hip_grid_gradient_scratch_bytes)", hipErrorInvalidValue); return -1; }
+	if (refuse_capture(stream, "ngp_hip_grid_gradient: the stream is being captured")) return -1;
 	hipLaunchKernelGGL(rows_to_planes_kernel, dim3(div_up(n, 64)), dim3(256), 0, (hipStream_t)stream, (const uint32_t*)dL_dfeatures, n, (uint32_t*)scratch);
 	NGP_LAUNCH_CHECK("rows_to_planes_kernel");
 	return grid_backward_entry(stream, n_dims, desc_dev, pos, pos_stride_floats, n, (const uint16_t*)scratch, grid_grad, (char*)scratch + (uint64_t)16 * n * 4u, scratch_bytes - (uint64_t)16 * n * 4u, ordered != 0);

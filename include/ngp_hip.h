@@ -473,7 +473,8 @@ int ngp_hip_grid_backward_unordered(void* stream, uint32_t n_dims, const NgpNetD
                           const uint16_t* dL_dx_planes, uint16_t* grid_grad, void* scratch, uint64_t scratch_bytes);
 
 /* The encoding alone, for networks that are not one of the fused kernels (the gated block below): features [n][32] fp16 from positions, and the table's gradient from the features'
- * gradient.  grid: the table, [n_grid_entries][2] fp16; workspace: ngp_hip_nerf_encode_workspace_bytes(n).  ordered: see ngp_hip_grid_backward (1) / _unordered (0); n a multiple of 256. */
+ * gradient.  grid: the table, [n_grid_entries][2] fp16; workspace: ngp_hip_nerf_encode_workspace_bytes(n).  ordered: see ngp_hip_grid_backward (1) / _unordered (0); n a multiple of 256.
+ * Neither is for a stream that is being captured: such a call is refused (their counters are cleared by memsets, which do not replay). */
 int ngp_hip_grid_encode(void* stream, uint32_t n_dims, const NgpNetDesc* desc_dev, const uint16_t* grid, const float* pos, uint32_t pos_stride_floats, uint32_t n, uint16_t* features,
                         void* workspace, uint64_t workspace_bytes);
 uint64_t ngp_hip_grid_gradient_scratch_bytes(uint32_t n);
@@ -488,7 +489,8 @@ int ngp_hip_grid_gradient(void* stream, uint32_t n_dims, const NgpNetDesc* desc_
  * grads, master, params and momentum_buffer are whole parameter vectors; matrices_host names the row-major matrices in them, in ascending order and without overlap (nothing else is
  * read or written: the encoding behind the matrices belongs to Adam).  dtype: of grads and params (F16, BF16; F32: grads alone, params NULL); params may be NULL.
  * Products run on pairs of fp16 halves (22 bits) with fp32 sums, norms in 64 bits: X agrees with 64-bit arithmetic to about 1e-6 of its norm.  No atomics: the same inputs give the
- * same bits.  A gradient that is not finite makes its matrix not finite, no other.  A zero update leaves X = 0.  Enqueues only (capturable: matrices_host is read during the call). */
+ * same bits (of the same list: the split of the sums depends on the matrices beside).  A gradient that is not finite makes its matrix not finite, no other.  A zero update leaves X = 0.
+ * Enqueues only (capturable: matrices_host is read during the call); two calls that may overlap need workspaces of their own. */
 typedef struct { uint64_t offset; uint32_t rows, cols; } NgpMuonMatrix;   /* offset in elements from the start of the vectors; rows, cols 1 .. 65536 */
 uint64_t ngp_hip_muon_workspace_bytes(uint32_t n_matrices, const NgpMuonMatrix* matrices_host);   /* Host only; 0 for a list that is refused */
 int ngp_hip_muon_step(void* stream, uint32_t n_matrices, const NgpMuonMatrix* matrices_host, float learning_rate, float momentum, float weight_decay, float epsilon, int nesterov,
@@ -500,11 +502,12 @@ int ngp_hip_muon_step(void* stream, uint32_t n_matrices, const NgpMuonMatrix* ma
  *   of a parameter vector here.  All tensors are of `dtype` (F16 or BF16); products accumulate in fp32, the hidden row is rounded once, every output is rounded once.
  *   activation: NGP_ACT_NONE (bilinear), RELU, LOGISTIC, SILU or GELU (the exact one, with erf); applied to x Wg^T.
  * Widths 1 .. 2^20 and rows 0 .. 2^30 of any remainder.  Rows whose width, stride and base are multiples of 8 elements / 16 bytes are read in place; others cost one padded copy.
- * Nothing outside y, dx, the gradients and the workspace is written; bytes between rows of a strided output stay as they are.  No atomics: the same inputs give the same bits.
+ * Nothing outside y, dx, the gradients and the workspace is written; bytes between rows of a strided output stay as they are.  Outputs must not overlap inputs or each other.
+ * No atomics: the same inputs give the same bits.
  * A call only enqueues (capturable); two calls that may overlap need workspaces of their own. */
 typedef struct { uint32_t n_in, n_hidden, n_out; int32_t dtype, activation; } NgpGatedFfn;   /* host struct */
 enum { NGP_FFN_BACKWARD = 1,     /* the workspace of the backward call */
-       NGP_FFN_ANY_LAYOUT = 2 }; /* ... where a base address or a row stride is no multiple of 16 bytes although its width is */
+       NGP_FFN_ANY_LAYOUT = 2 }; /* ... where a base address or a row stride is no multiple of 16 bytes although its width is, or a stride passes 2^21 elements */
 /* bytes of workspace a call of n_rows rows needs (it may be used for fewer rows of the same block); 0 for a block that is refused.  Host only. */
 uint64_t ngp_hip_gated_ffn_workspace_bytes(const NgpGatedFfn* block_host, uint64_t n_rows, uint32_t flags);
 int ngp_hip_gated_ffn_forward(void* stream, const NgpGatedFfn* block_host, uint64_t n_rows, const void* x, uint64_t x_stride, const void* w_gate, const void* w_up,

@@ -79,6 +79,28 @@ def test_table_gradient_from_rows(ngp, cuda, n_dims, ordered):
     assert ngp.ngp_hip_grid_encode(None, 4, d_desc.data_ptr(), rows.data_ptr(), pos.data_ptr(), n_dims, n, rows.data_ptr(), s2.data_ptr(), sg) != 0
 
 
+def test_encoding_is_not_captured(ngp, cuda):
+    """the encoder's counters are cleared by memsets, which do not replay: a stream that is being captured is refused, and the graph stays as it was"""
+    n, desc = 512, make_desc(ngp, 3)
+    d_desc, grid, pos = H.to_dev(desc, cuda), random_grid(desc), positions(n, 3)
+    size, sg = ngp.ngp_hip_nerf_encode_workspace_bytes(n), ngp.ngp_hip_grid_gradient_scratch_bytes(n)
+    ws = torch.empty(max(size, sg), dtype=torch.uint8, device="cuda")
+    rows, seven = torch.zeros(n, 32, dtype=torch.float16, device="cuda"), torch.zeros(4, device="cuda")
+    table = torch.zeros(int(desc["n_grid_entries"][0]) * 2, dtype=torch.float16, device="cuda")
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        s = torch.cuda.current_stream().cuda_stream
+        assert ngp.ngp_hip_grid_encode(s, 3, d_desc.data_ptr(), grid.data_ptr(), pos.data_ptr(), 3, n, rows.data_ptr(), ws.data_ptr(), size) != 0
+        assert b"captured" in ngp.ngp_hip_last_error()
+        assert ngp.ngp_hip_grid_gradient(s, 3, d_desc.data_ptr(), pos.data_ptr(), 3, n, rows.data_ptr(), 0, table.data_ptr(), ws.data_ptr(), sg) != 0
+        assert b"captured" in ngp.ngp_hip_last_error()
+        seven.fill_(7.0)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert (seven == 7.0).all() and (rows == 0).all()
+
+
 def test_a_training_step_of_the_parts_together(ngp, cuda):
     """encode -> block -> loss -> block backward -> table gradient -> Muon (matrices) + Adam and Ema (table), three steps; every product of a step against 64 bits"""
     n, f, n_dims = 4096, 64, 3
