@@ -120,12 +120,6 @@ struct Tile {
 	__device__ __forceinline__ void issue(const i32x4& r, int i, lds_char* lds, int wave) const {
 		dma16(r, lds + (i * THREADS + wave * 64) * 16, k_past ? (int)0x80000000 : voff[i]);
 	}
-	// fragment of rows row0 .. row0 + 31, k-block ks of 16 (KC): lane l has row l & 31 and k = 8 (l >> 5) .. + 7
-	static __device__ __forceinline__ i32x4 frag32(const lds_char* lds, int row0, int ks, int lane) {
-		static_assert(LAY == KC, "the 32-row fragments are read along k");
-		const int r = row0 + (lane & 31), c = (ks * 2 + (lane >> 5)) ^ swizzle(lane & 31);
-		return *(const __attribute__((address_space(3))) i32x4*)(lds + r * (BK * 2) + c * 16);
-	}
 	// fragment of rows row0 .. row0 + 15, all 32 k: lane l has row l & 15 and k = 8 (l >> 4) .. + 7
 	static __device__ __forceinline__ i32x4 frag(const lds_char* lds, int row0, int lane) {
 		static_assert(BK == 32, "one k-block a step");
