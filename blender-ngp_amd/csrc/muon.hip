@@ -327,10 +327,25 @@ __device__ __forceinline__ void store_symmetric(const f32x4 (&acc)[P::NB][P::MB]
 	const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wn = wave % P::WAVES_N, wm = wave / P::WAVES_N;
 	lds_char* mine = lds + wave * (32 * 144);
 	f16* const out = POLY ? j.b : j.a;
+	i32x4 old[POLY ? P::NB / 2 : 1][POLY ? P::MB / 2 : 1][4];   // POLY: the tile of A, in whole rows of 32 columns, all of it under way at once
+	if (POLY)
+#pragma unroll
+		for (int a = 0; a < P::NB; a += 2)
+#pragma unroll
+			for (int b = 0; b < P::MB; b += 2)
+#pragma unroll
+				for (int r = 0; r < 4; ++r) {
+					const uint32_t n0 = tn * P::N + wn * (P::NB * 16) + a * 16, m = tm * P::M + wm * (P::MB * 16) + b * 16 + r * 8 + (lane >> 3);
+					old[a / 2][b / 2][r] = i32x4{0, 0, 0, 0};
+					if (m < j.n && n0 < j.np) old[a / 2][b / 2][r] = *(const i32x4*)(j.a + (uint64_t)m * 2 * j.np + (uint64_t)n0 * 2 + (lane & 7) * 8);
+				}
 #pragma unroll
 	for (int a = 0; a < P::NB; a += 2)
 #pragma unroll
 		for (int b = 0; b < P::MB; b += 2) {
+			if (POLY)
+#pragma unroll
+				for (int r = 0; r < 4; ++r) *(__attribute__((address_space(3))) i32x4*)(mine + (r * 8 + (lane >> 3)) * 144 + (lane & 7) * 16) = old[a / 2][b / 2][r];
 			const uint32_t n0 = tn * P::N + wn * (P::NB * 16) + a * 16, m0 = tm * P::M + wm * (P::MB * 16) + b * 16;
 			f32x4 v[2][2];
 #pragma unroll
@@ -340,11 +355,8 @@ __device__ __forceinline__ void store_symmetric(const f32x4 (&acc)[P::NB][P::MB]
 					v[x][y] = acc[a + x][b + y];
 					if (POLY) {
 						const uint32_t m = m0 + y * 16 + (lane & 15), n = n0 + x * 16 + 4 * (lane >> 4);
-						f16x4 hi = {0, 0, 0, 0}, lo = {0, 0, 0, 0};
-						if (m < j.n && n < j.np) {
-							const f16* d = j.a + (uint64_t)m * 2 * j.np + split_col(n);
-							hi = *(const f16x4*)d; lo = *(const f16x4*)(d + 32);
-						}
+						const lds_char* d = mine + (y * 16 + (lane & 15)) * 144 + (x * 16 + 4 * (lane >> 4)) * 2;
+						const f16x4 hi = *(const __attribute__((address_space(3))) f16x4*)d, lo = *(const __attribute__((address_space(3))) f16x4*)(d + 64);
 #pragma unroll
 						for (int e = 0; e < 4; ++e) v[x][y][e] = NS_C / SA * v[x][y][e] + NS_B * ((float)hi[e] + (float)lo[e]) + (m == n + e && m < j.n ? NS_A * SA : 0.0f);
 					} else v[x][y] *= SA / (SX * SX);
