@@ -467,12 +467,23 @@ template <class T> static int run_narrow_backward(hipStream_t st, const NarrowAr
 	return 0;
 }
 // ---- few rows: a launch for h and one for y, and one that packs x.  Workgroups of 4 to 16 waves (8 for the pair of matrices, whose sums take twice the LDS): about 2048 waves, 8 a CU.
-template <class T, int NM, int MB, bool PX, bool PO>
-static void launch_few(hipStream_t st, const void* x, uint64_t x_ld, uint32_t rows, const void* w0, const void* w1, uint32_t n, uint32_t k, void* out, uint64_t out_ld, int act) {
-	const uint32_t groups = PO ? (n + 31) / 32 * 2 : (n + 15) / 16;
+template <class T, int NM, int NB, int MB, bool PX, bool PO>
+static void launch_few(hipStream_t st, const void* x, uint64_t x_ld, uint32_t rows, const void* w0, const void* w1, uint32_t n, uint32_t k, uint32_t per, void* out, uint64_t out_ld, int act) {
+	const uint32_t groups = (uint32_t)ceil_div(PO ? (n + 31) & ~31u : n, per);
 	uint32_t waves = 4;
-	while (waves < (NM == 2 ? 8 : 16) && groups * waves < 2048 && waves * (FEW_CHUNK * 32) < k) waves *= 2;
-	hipLaunchKernelGGL((few_rows_kernel<T, NM, MB, PX, PO>), dim3(groups), dim3(64 * waves), 0, st, (const T*)x, x_ld, rows, (const T*)w0, (const T*)w1, n, k, (T*)out, out_ld, act);
+	while (waves < (uint32_t)few_waves(NM, NB) && groups * waves < 2048 && waves * 256 < k) waves *= 2;
+	hipLaunchKernelGGL((few_rows_kernel<T, NM, NB, MB, PX, PO>), dim3(groups), dim3(64 * waves), 0, st, (const T*)x, x_ld, rows, (const T*)w0, (const T*)w1, n, k, per, (T*)out, out_ld, act);
+}
+// Rows of the weights to a workgroup: 16, or, where that gives some CUs a workgroup more than others, the same for every CU in as few rounds of the chip as 48 rows (MB = 4, whose
+// sums would not fit: 32) leave, in steps of 8.  24 rows through 4096 - 10240 - 4096 (640 workgroups of 16 rows, 256 of 40) 77.4 -> 72.9 us, through 1500 - 5000 - 1500 36.3 -> 30.6;
+// 2048 - 8192 - 2048, which 16 divide, 32.4 with 16 and 31.6 with 32, one row 23.7 and 24.8.
+template <class T, int NM, int MB, bool PX, bool PO>
+static void pick_few(hipStream_t st, const void* x, uint64_t x_ld, uint32_t rows, const void* w0, const void* w1, uint32_t n, uint32_t k, void* out, uint64_t out_ld, int act) {
+	const uint64_t rounds = ceil_div(n, 256 * (MB == 4 ? 32 : 48)), even = up8(ceil_div(n, 256 * rounds));
+	const uint32_t per = even * rounds < ceil_div(n, 256 * 16) * 16 ? (uint32_t)std::max<uint64_t>(even, 16) : 16;
+	if (per <= 16) launch_few<T, NM, 1, MB, PX, PO>(st, x, x_ld, rows, w0, w1, n, k, per, out, out_ld, act);
+	else if (per <= 32) launch_few<T, NM, 2, MB, PX, PO>(st, x, x_ld, rows, w0, w1, n, k, per, out, out_ld, act);
+	else if constexpr (MB < 4) launch_few<T, NM, 3, MB, PX, PO>(st, x, x_ld, rows, w0, w1, n, k, per, out, out_ld, act);
 }
 constexpr uint32_t FEW_PACK_H = 8, FEW_PACK_X = 5 << 16;
 // Which of the two products' rows are packed.  h where more than a few rows are read of it: 12 rows, 2048 - 8192 - 2048, 28.9 -> 27.9 us, one row 24 -> 26.5.  x where that saves more
@@ -486,11 +497,11 @@ static void launch_few_pair(hipStream_t st, const NgpGatedFfn& b, uint32_t rows,
 	const uint32_t pitch = few_pitch(b.n_hidden), d = b.n_in, f = b.n_hidden;
 	if (few_pack_x(rows, b)) {
 		hipLaunchKernelGGL((pack_few_kernel<T, MB>), dim3((d + 127) / 128 * MB), dim3(256), 0, st, (const T*)x, x_ld, rows, d, (T*)packed);
-		launch_few<T, 2, MB, true, true>(st, packed, 0, rows, wg, wu, f, d, h, 0, b.activation);
-	} else if (few_pack_h(rows)) launch_few<T, 2, MB, false, true>(st, x, x_ld, rows, wg, wu, f, d, h, 0, b.activation);
-	else launch_few<T, 2, 1, false, false>(st, x, x_ld, rows, wg, wu, f, d, h, pitch, b.activation);
-	if (few_pack_h(rows)) launch_few<T, 1, MB, true, false>(st, h, 0, rows, wd, nullptr, b.n_out, f, y, y_ld, 0);
-	else launch_few<T, 1, 1, false, false>(st, h, pitch, rows, wd, nullptr, b.n_out, f, y, y_ld, 0);
+		pick_few<T, 2, MB, true, true>(st, packed, 0, rows, wg, wu, f, d, h, 0, b.activation);
+	} else if (few_pack_h(rows)) pick_few<T, 2, MB, false, true>(st, x, x_ld, rows, wg, wu, f, d, h, 0, b.activation);
+	else pick_few<T, 2, 1, false, false>(st, x, x_ld, rows, wg, wu, f, d, h, pitch, b.activation);
+	if (few_pack_h(rows)) pick_few<T, 1, MB, true, false>(st, h, 0, rows, wd, nullptr, b.n_out, f, y, y_ld, 0);
+	else pick_few<T, 1, 1, false, false>(st, h, pitch, rows, wd, nullptr, b.n_out, f, y, y_ld, 0);
 }
 template <class T>
 static int run_few(hipStream_t st, const NgpGatedFfn& b, uint32_t rows, const void* x, uint64_t x_ld, const void* wg, const void* wu, const void* wd, void* y, uint64_t y_ld, void* h, void* packed) {

@@ -289,3 +289,21 @@ def test_gelu_far_out(ngp, cuda, dtype):
     want = (x.double() ** 2 * torch.special.ndtr(x.double()))
     smallest = torch.finfo(t).tiny * torch.finfo(t).eps   # half a step of f16's subnormal values, twice
     assert ((y.double() - want).abs() <= (torch.finfo(t).eps + 1.1e-5) * want.abs() + smallest).all()
+
+
+# 24 to 48 rows of the weights to a workgroup, for h and for y; x packed or not
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("shape", [(3, 40, 4500, 10001), (3, 41, 10001, 4500), (12, 40, 4500, 10001), (12, 41, 10001, 4500), (24, 40, 4500, 10001), (24, 41, 10001, 4500), (50, 40, 4500, 5001),
+                                   (16, 16000, 4500, 40), (16, 12000, 10001, 40), (24, 9500, 4500, 40), (24, 4001, 10001, 40), (50, 4001, 4500, 40), (2, 30, 17000, 21000)], ids=lambda s: "x".join(map(str, s)))
+def test_few_rows_through_many_columns(ngp, cuda, shape, dtype):
+    rows, d, f, o = shape
+    b = block(d, f, o, dtype, "silu")
+    x, wg, wu, wd, dy = inputs(rows, d, f, o, dtype, seed=rows + f)
+    ref = R.Block("silu", x, wg, wu, wd, dy)
+    ybuf, y = guarded(rows, o, o, x.dtype)
+    ws, n = workspace(ngp, b, rows, 0)
+    forward(ngp, b, x, wg, wu, wd, y, ws, n)
+    torch.cuda.synchronize()
+    R.check("y", y, ref.y, ref.ey)
+    untouched(ybuf, y)
+    assert (ws[n:] == 0xff).all()
