@@ -65,7 +65,7 @@ def backward(ngp, b, x, wg, wu, wd, dy, dx, grads, ws, n, stream=None):
 # few rows (the row-streaming kernels), narrow blocks over many rows, and sizes whose tiles fill the chip for each product
 SHAPES = [(1, 1, 1, 1), (1, 8, 8, 8), (1, 64, 128, 64), (1, 520, 1032, 264), (3, 7, 5, 9), (2, 333, 77, 130), (16, 72, 264, 40), (17, 256, 96, 48), (1, 136, 264, 136), (33, 129, 130, 131), (64, 300, 500, 200), (65, 300, 500, 200), (24, 1024, 2056, 520), (9, 2000, 130, 24), (33, 64, 64, 64), (20, 8200, 8200, 40), (33, 2001, 8011, 131), (64, 1030, 4100, 72),
           (64, 32, 64, 16), (65, 33, 65, 17), (129, 128, 96, 257), (300, 40, 200, 3), (513, 264, 328, 136), (4097, 32, 64, 16), (5000, 16, 32, 8), (3000, 64, 128, 64),
-          (2500, 96, 160, 32), (4500, 8, 64, 16), (6200, 136, 1000, 2056), (6200, 136, 1400, 72), (200, 1600, 4104, 3000)]
+          (2500, 96, 160, 32), (4500, 8, 64, 16), (6200, 136, 1000, 2056), (6200, 136, 1400, 72), (3000, 1200, 2600, 1100), (40000, 72, 136, 72), (200, 1600, 4104, 3000)]
 
 
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
