@@ -406,22 +406,23 @@ static uint64_t partial_room(const Size* s, int count) {
 	return std::min<uint64_t>(MAX_PARTIAL_TILES, parts) * (128 * 128 * 4);
 }
 
-// The tiles of h: BIG where they fill three quarters of the 256 CUs.  A round of BIG tiles that would leave half of the chip idle or more is made of half tiles instead: such a round
-// takes 0.7 of the other (352 BIG tiles, 4096 x 1024 - 2816: hidden_backward_kernel 114 us, with 242 and 220 half tiles 87; half tiles alone 111).
+// The tiles of h.  A round of BIG tiles that would leave half of the chip idle or more is made of half tiles instead: such a round takes 0.7 of the other (352 BIG tiles, 4096 x 1024 -
+// 2816: hidden_backward_kernel 114 us, with 242 and 220 half tiles 87; half tiles alone 111).  A round of SMALL tiles takes 0.6 of a round of BIG ones: 500 rows forward 4096 - 10240 -
+// 4096 194 us with SMALL tiles (2 rounds of 512), 157 with BIG ones (160, one round); 700 rows backward 1024 - 2816 - 1024 (264 and 66) 63 and 75.
 static bool cover_of(uint32_t width, uint64_t rows, Cover& c, uint32_t& groups) {
-	const bool big = ceil_div(width, 128) * ceil_div(rows, 256) >= 192;
-	c.tiles_n = (uint32_t)ceil_div(width, big ? 128 : 64); c.tiles_m = (uint32_t)ceil_div(rows, big ? 256 : 128);
-	c.half_tiles_m = 0;
-	const uint64_t tiles = (uint64_t)c.tiles_n * c.tiles_m;
-	c.half_first = groups = (uint32_t)tiles;
-	if (!big || tiles < 256) return big;
-	const uint32_t whole = (uint32_t)(tiles / 256 * 256 / c.tiles_n);   // rows of tiles in the full rounds
+	const uint32_t bn = (uint32_t)ceil_div(width, 128), bm = (uint32_t)ceil_div(rows, 256), sn = (uint32_t)ceil_div(width, 64), sm = (uint32_t)ceil_div(rows, 128);
+	const uint64_t tiles = (uint64_t)bn * bm;
+	const uint32_t whole = (uint32_t)(tiles / 256 * 256 / bn);   // rows of BIG tiles in the full rounds
 	const uint64_t halves = ceil_div(rows - std::min<uint64_t>(rows, whole * 256ull), 128);
-	if (halves == 0 || halves * c.tiles_n > 256) return big;
-	c.tiles_m = whole; c.half_tiles_m = (uint32_t)halves;
-	c.half_first = (c.tiles_n * whole + 7) & ~7u;
-	groups = c.half_first + c.tiles_n * c.half_tiles_m;
-	return big;
+	const bool mixed = tiles >= 256 && halves && halves * bn <= 256;
+	const double big = mixed ? tiles / 256 + 0.7 : ceil_div(tiles, 256), small = 0.6 * ceil_div((uint64_t)sn * sm, 512);
+	c = big <= small ? Cover{bn, mixed ? whole : bm, 0, 0} : Cover{sn, sm, 0, 0};
+	groups = c.half_first = c.tiles_n * c.tiles_m;
+	if (big > small || !mixed) return big <= small;
+	c.half_tiles_m = (uint32_t)halves;
+	c.half_first = (groups + 7) & ~7u;
+	groups = c.half_first + bn * c.half_tiles_m;
+	return true;
 }
 
 struct Tensor { const void* p; uint64_t ld; uint64_t rows; uint32_t cols; };

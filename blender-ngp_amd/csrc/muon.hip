@@ -769,11 +769,21 @@ int ngp_hip_muon_step(void* stream, uint32_t n_matrices, const NgpMuonMatrix* ma
 		const uint32_t c = jobs.count;
 		hipLaunchKernelGGL(momentum_kernel, dim3(jobs.start[START_SUM][c]), dim3(256), 0, st, jobs, s);
 		hipLaunchKernelGGL(split_kernel, dim3(jobs.start[START_SPLIT][c]), dim3(256), 0, st, jobs, s);
-		// 128 x 128 where that fills four fifths of the chip, else 64 x 64; 128 x 256 where it fills the chip twice over (two 8192 x 4096: 1.25 ms a launch where 128 x 128 take 1.7; not
-		// for the symmetric products: 0.87 ms both, more of a larger tile lies above the diagonal).  More than one 128 x 128 tile a CU: two workgroups of four waves at a time, 24 of
-		// 768 x 768 957 -> 845 us; up to one: eight waves, 6 of 768 x 768 336 -> 299 us.
-		auto tile_for = [](uint32_t tiles) { return tiles < 200 ? 0 : tiles <= 256 ? 1 : 2; };
-		const int symmetric_tile = tile_for(count_symmetric<Middle>(jobs)), apply_tile = count_apply<Large>(jobs) >= 512 ? 3 : tile_for(count_apply<Middle>(jobs));
+		// The tile whose rounds of the chip cost least.  A round, in units of one 128 x 128 tile a CU in eight waves: two of four waves (24 of 768 x 768: 957 -> 845 us) 1.7, one 128 x 256
+		// 1.68 (two 8192 x 4096: 1.25 ms a launch where 128 x 128 take 1.7; not for the symmetric products: 0.87 ms both, more of a larger tile lies above the diagonal), two 64 x 64
+		// 0.8.  In a sweep of 16 shapes this is within 3 % of the best of the four; a step of 2000 x 2000 723 -> 657 us, 1500 x 1500 425 -> 390, 4000 x 8000 6.92 -> 6.56 ms against
+		// fixed bounds on the number of tiles.
+		auto rounds = [](uint32_t tiles, uint32_t slots) { return (double)((tiles + slots - 1) / slots); };
+		auto tile_for = [&](uint32_t little, uint32_t middle, double large) {
+			const double cost[4] = {0.8 * rounds(little, 512), rounds(middle, 256), 1.7 * rounds(middle, 512), large};
+			return (int)(std::min_element(cost, cost + 4) - cost);
+		};
+		const uint32_t little_symmetric = count_symmetric<Little>(jobs), middle_symmetric = count_symmetric<Middle>(jobs);
+		const uint32_t little_apply = count_apply<Little>(jobs), middle_apply = count_apply<Middle>(jobs), large_apply = count_apply<Large>(jobs);
+		const int apply_tile = tile_for(little_apply, middle_apply, 1.68 * rounds(large_apply, 256));
+		int symmetric_tile = tile_for(little_symmetric, middle_symmetric, HUGE_VAL);
+		for (uint32_t i = 0; i < jobs.count; ++i)
+			if (jobs.job[i].parts > 1) symmetric_tile = 0;   // the parts are laid out for it
 		for (uint32_t i = 0; i < n_iterations; ++i) {
 			const int from = (int)(i & 1);
 			const bool last = i + 1 == n_iterations;

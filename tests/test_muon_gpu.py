@@ -98,9 +98,9 @@ def test_the_whole_step_on_matrices_of_many_shapes(ngp, cuda, dtype, nesterov):
     check_step(ngp, Vector([(64, 32), (16, 64), (64, 32), (64, 64), (16, 64), (200, 136), (1, 9), (129, 128)], dtype, seed=nesterov), nesterov=nesterov, loss_scale=128.0, decay=0.1)
 
 
-@pytest.mark.parametrize("shapes", [[(500 - i, 530 + 3 * i) for i in range(22)], [(390 - i, 520 + i) for i in range(14)], [(640 - i, 650 + 3 * i) for i in range(20)], [(1130 + 5 * i, 1100 - i) for i in range(14)] + [(64, 2100), (700, 90)]], ids=["one symmetric tile a CU", "one tile a CU", "128x128", "128x256"])
+@pytest.mark.parametrize("shapes", [[(500 - i, 530 + 3 * i) for i in range(22)], [(390 - i, 520 + i) for i in range(14)], [(640 - i, 650 + 3 * i) for i in range(20)], [(1130 + 5 * i, 1100 - i) for i in range(14)] + [(64, 2100), (700, 90)]], ids=["eight waves and 128x128", "64x64 and eight waves", "128x128 and 128x256", "eight waves twice"])
 def test_larger_tiles(ngp, cuda, shapes):
-    """enough matrices at once for the products' tiles of 128 x 128 and of 128 x 256"""
+    """enough matrices at once for each of the tiles of the symmetric products and of X B"""
     check_step(ngp, Vector(shapes, "bf16", gap=1), iterations=5)
 
 
