@@ -34,10 +34,10 @@ struct Job {
 	uint64_t offset;                    // of the matrix in the parameter vector, in elements
 	uint32_t rows, cols, n, k;          // n = min, k = max of rows and cols
 	uint32_t np;                        // n up to a multiple of 32
-	f16 *xt[2], *a, *b;                 // X^T [k][2 np] (two: an iteration reads one and writes the other), A and B [n][2 np]
+	f16 *xt[2], *a, *b;                 // X^T [k][2 np] (in slabs: one, [k][128]; two: an iteration reads one and writes the other), A and B [n][2 np]
 	double* sums;
 	float* partial;                     // the parts' sums of the tiles of A
-	uint32_t parts;                     // of k, in the products that give A
+	uint32_t parts;                     // of k, in the products that give A; of a matrix in slabs: the rows of one
 };
 enum { START_SUM, START_SPLIT, START_GRAM, START_SYM, START_APPLY, N_STARTS };
 struct Jobs {
@@ -506,6 +506,73 @@ __device__ __forceinline__ f32x4 mfma3(i32x4 nh, i32x4 nl, i32x4 mh, i32x4 ml, f
 	return mfma16<f16>(nh, mh, c);
 }
 
+struct TinyBlocks {   // of A and B: a wave's row of blocks and two of its four; a lane's row and first column in a block
+	int m0, n0, lm, ln;
+	__device__ __forceinline__ TinyBlocks(int wave, int lane) : m0(wave / 2 * 16), n0(wave % 2 * 32), lm(lane & 15), ln(4 * (lane >> 4)) {}
+};
+// the wave's blocks of X X^T, from 32 k_steps rows of X^T
+__device__ __forceinline__ void tiny_gram(const lds_char* xt, int k_steps, const TinyBlocks& o, int lane, f32x4 (&acc)[2]) {
+	acc[0] = acc[1] = f32x4{0, 0, 0, 0};
+	for (int ks = 0; ks < k_steps; ++ks) {
+		const i32x4 mh = tiny_turned(xt, o.m0, ks * 32, 0, lane), ml = tiny_turned(xt, o.m0, ks * 32, 1, lane);
+#pragma unroll
+		for (int b = 0; b < 2; ++b) acc[b] = mfma3(tiny_turned(xt, o.n0 + b * 16, ks * 32, 0, lane), tiny_turned(xt, o.n0 + b * 16, ks * 32, 1, lane), mh, ml, acc[b]);
+	}
+}
+// A from the blocks of X X^T into `ma`, then B into `mb`; every wave of the workgroup calls it
+__device__ __forceinline__ void tiny_polynomial(lds_char* ma, lds_char* mb, const TinyBlocks& o, int lane, f32x4 (&acc)[2]) {
+#pragma unroll
+	for (int b = 0; b < 2; ++b) tiny_put(ma, o.m0 + o.lm, o.n0 + b * 16 + o.ln, acc[b] * (SA / (SX * SX)));
+	__syncthreads();
+	acc[0] = acc[1] = f32x4{0, 0, 0, 0};
+#pragma unroll
+	for (int ks = 0; ks < 2; ++ks) {
+		const i32x4 mh = tiny_along(ma, o.m0, ks * 32, 0, lane), ml = tiny_along(ma, o.m0, ks * 32, 1, lane);
+#pragma unroll
+		for (int b = 0; b < 2; ++b) acc[b] = mfma3(tiny_along(ma, o.n0 + b * 16, ks * 32, 0, lane), tiny_along(ma, o.n0 + b * 16, ks * 32, 1, lane), mh, ml, acc[b]);
+	}
+#pragma unroll
+	for (int b = 0; b < 2; ++b) {
+		const int row = o.m0 + o.lm, col = o.n0 + b * 16 + o.ln;
+		f32x4 v = NS_C / SA * acc[b] + NS_B * tiny_get(ma, row, col);
+#pragma unroll
+		for (int e = 0; e < 4; ++e)
+			if (row == col + e) v[e] += NS_A * SA;
+		tiny_put(mb, row, col, v);
+	}
+	__syncthreads();
+}
+// rows r .. r + 15 of X^T B
+__device__ __forceinline__ void tiny_apply(const lds_char* xt, const lds_char* mb, int r, int lane, f32x4 (&x)[4]) {
+#pragma unroll
+	for (int b = 0; b < 4; ++b) x[b] = f32x4{0, 0, 0, 0};
+#pragma unroll
+	for (int ks = 0; ks < 2; ++ks) {
+		const i32x4 mh = tiny_along(xt, r, ks * 32, 0, lane), ml = tiny_along(xt, r, ks * 32, 1, lane);
+#pragma unroll
+		for (int b = 0; b < 4; ++b) x[b] = mfma3(tiny_along(mb, b * 16, ks * 32, 0, lane), tiny_along(mb, b * 16, ks * 32, 1, lane), mh, ml, x[b]);
+	}
+}
+// the weights of those rows, r counted from the matrix's first
+__device__ __forceinline__ void tiny_weights(const Step& s, uint64_t offset, uint32_t rows, uint32_t cols, uint32_t r, const TinyBlocks& o, const f32x4 (&x)[4]) {
+	const bool turn = rows > cols;
+	const uint32_t n = turn ? cols : rows, k = turn ? rows : cols, row = r + o.lm;
+	const float keep = 1.0f - s.lr * s.decay, rate = s.lr * sqrtf(fmaxf(1.0f, (float)rows / (float)cols)) / (SA * SX);
+	float w[16];
+	uint64_t at[16];
+	bool in[16];
+#pragma unroll
+	for (int i = 0; i < 16; ++i) {
+		const uint32_t c = (i >> 2) * 16 + o.ln + (i & 3);
+		in[i] = row < k && c < n;
+		at[i] = offset + (in[i] ? (turn ? (uint64_t)row * cols + c : (uint64_t)c * cols + row) : 0);
+		w[i] = s.master[at[i]];
+	}
+#pragma unroll
+	for (int i = 0; i < 16; ++i) w[i] = keep * w[i] - rate * x[i >> 2][i & 3];
+	set_weights(s, at, w, in);
+}
+
 __global__ void __launch_bounds__(512) tiny_kernel(TinyJobs jobs, Step s, uint32_t iterations) {
 	__shared__ __attribute__((aligned(16))) char xt_[TINY_K * TINY_PITCH], a_[TINY_N * TINY_PITCH], b_[TINY_N * TINY_PITCH];
 	__shared__ double sums[8];
@@ -563,77 +630,116 @@ __global__ void __launch_bounds__(512) tiny_kernel(TinyJobs jobs, Step s, uint32
 		}
 	}
 	__syncthreads();
-	const int m0 = wave / 2 * 16, n0 = wave % 2 * 32, lm = lane & 15, ln = 4 * (lane >> 4);   // of A and B: one row of blocks, two of its four
+	const TinyBlocks own(wave, lane);
 	for (uint32_t it = 0; it < iterations; ++it) {
-		f32x4 acc[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
-		for (int ks = 0; ks < k_steps; ++ks) {
-			const i32x4 mh = tiny_turned(xt, m0, ks * 32, 0, lane), ml = tiny_turned(xt, m0, ks * 32, 1, lane);
-#pragma unroll
-			for (int b = 0; b < 2; ++b) acc[b] = mfma3(tiny_turned(xt, n0 + b * 16, ks * 32, 0, lane), tiny_turned(xt, n0 + b * 16, ks * 32, 1, lane), mh, ml, acc[b]);
-		}
-#pragma unroll
-		for (int b = 0; b < 2; ++b) tiny_put(ma, m0 + lm, n0 + b * 16 + ln, acc[b] * (SA / (SX * SX)));
-		__syncthreads();
-		acc[0] = acc[1] = f32x4{0, 0, 0, 0};
-#pragma unroll
-		for (int ks = 0; ks < 2; ++ks) {
-			const i32x4 mh = tiny_along(ma, m0, ks * 32, 0, lane), ml = tiny_along(ma, m0, ks * 32, 1, lane);
-#pragma unroll
-			for (int b = 0; b < 2; ++b) acc[b] = mfma3(tiny_along(ma, n0 + b * 16, ks * 32, 0, lane), tiny_along(ma, n0 + b * 16, ks * 32, 1, lane), mh, ml, acc[b]);
-		}
-#pragma unroll
-		for (int b = 0; b < 2; ++b) {
-			const int row = m0 + lm, col = n0 + b * 16 + ln;
-			f32x4 v = NS_C / SA * acc[b] + NS_B * tiny_get(ma, row, col);
-#pragma unroll
-			for (int e = 0; e < 4; ++e)
-				if (row == col + e) v[e] += NS_A * SA;
-			tiny_put(mb, row, col, v);
-		}
-		__syncthreads();
+		f32x4 acc[2];
+		tiny_gram(xt, k_steps, own, lane, acc);
+		tiny_polynomial(ma, mb, own, lane, acc);
 		f32x4 x[2][4];   // rows 16 wave .. and 128 + 16 wave .. of X^T B
+#pragma unroll
+		for (int h = 0; h < 2; ++h) {
+			if (h * 128 + wave * 16 >= k_steps * 32) break;
+			tiny_apply(xt, mb, h * 128 + wave * 16, lane, x[h]);
+		}
+		const bool last = it + 1 == iterations;   // a wave reads and writes its own rows of X^T alone: no barrier between
 #pragma unroll
 		for (int h = 0; h < 2; ++h) {
 			const int r = h * 128 + wave * 16;
 			if (r >= k_steps * 32) break;
+			if (last) tiny_weights(s, job.offset, job.rows, job.cols, r, own, x[h]);
+			else
 #pragma unroll
-			for (int b = 0; b < 4; ++b) x[h][b] = f32x4{0, 0, 0, 0};
-#pragma unroll
-			for (int ks = 0; ks < 2; ++ks) {
-				const i32x4 mh = tiny_along(xt, r, ks * 32, 0, lane), ml = tiny_along(xt, r, ks * 32, 1, lane);
-#pragma unroll
-				for (int b = 0; b < 4; ++b) x[h][b] = mfma3(tiny_along(mb, b * 16, ks * 32, 0, lane), tiny_along(mb, b * 16, ks * 32, 1, lane), mh, ml, x[h][b]);
-			}
-		}
-		const bool last = it + 1 == iterations;   // a wave reads and writes its own rows of X^T alone: no barrier between
-		const float keep = 1.0f - s.lr * s.decay, rate = s.lr * sqrtf(fmaxf(1.0f, (float)job.rows / (float)job.cols)) / (SA * SX);
-#pragma unroll
-		for (int h = 0; h < 2; ++h) {
-			const int r = h * 128 + wave * 16 + lm;
-			if (h * 128 + wave * 16 >= k_steps * 32) break;
-			if (!last) {
-#pragma unroll
-				for (int b = 0; b < 4; ++b) tiny_put(xt, r, b * 16 + ln, x[h][b] * (1.0f / SA));
-				continue;
-			}
-			float w[16];
-			uint64_t at[16];
-			bool in[16];
-#pragma unroll
-			for (int i = 0; i < 16; ++i) {
-				const uint32_t c = (i >> 2) * 16 + ln + (i & 3);
-				in[i] = (uint32_t)r < k && c < n;
-				at[i] = job.offset + (in[i] ? (turn ? (uint64_t)r * job.cols + c : (uint64_t)c * job.cols + r) : 0);
-				w[i] = s.master[at[i]];
-			}
-#pragma unroll
-			for (int i = 0; i < 16; ++i) w[i] = keep * w[i] - rate * x[h][i >> 2][i & 3];
-			set_weights(s, at, w, in);
+				for (int b = 0; b < 4; ++b) tiny_put(xt, r + own.lm, b * 16 + own.ln, x[h][b] * (1.0f / SA));
 		}
 		__syncthreads();
 	}
 }
 static bool is_tiny(const NgpMuonMatrix& m) { return std::min(m.rows, m.cols) <= TINY_N && std::max(m.rows, m.cols) <= TINY_K; }
+
+// ---- a matrix of a short side up to 64, in slabs of its long one -------------------------------------------------------------------------------
+//
+// Between two iterations only A, 64 x 64, has to be known to all: a launch to an iteration, in which every workgroup adds the slabs' parts of A in their order, works out B for itself,
+// multiplies its 128 or 256 rows of X^T and leaves their part of the next A.  Bound by the launches: one 1640 x 24 64 us, 98 by the kernels above.
+constexpr uint32_t MAX_SLABS = 32, BATCH_SLABS = 256, PART_FLOATS = TINY_N * TINY_N;
+static uint32_t slab_rows(uint32_t k) { return k <= TINY_K / 2 * MAX_SLABS ? TINY_K / 2 : TINY_K; }
+static uint32_t slabs_of(const NgpMuonMatrix& m) {   // 0: not in slabs
+	const uint32_t k = std::max(m.rows, m.cols);
+	return std::min(m.rows, m.cols) > TINY_N || k <= TINY_K || k > TINY_K * MAX_SLABS ? 0 : (k + slab_rows(k) - 1) / slab_rows(k);
+}
+// Only as many as a round of the chip takes, or short ones: twelve 6264 x 48 in slabs are two batches, 245 us, and 191 by the kernels above.
+static bool in_slabs(uint32_t n, const NgpMuonMatrix* m) {
+	uint32_t slabs = 0, most = 0;
+	for (uint32_t i = 0; i < n && slabs <= BATCH_SLABS; ++i) { slabs += slabs_of(m[i]); most = std::max(most, slabs_of(m[i])); }
+	return slabs <= BATCH_SLABS || most <= MAX_SLABS / 2;
+}
+
+// it 0: X_0 and its A; it 1 ..: an iteration; the last: into the weights
+__global__ void __launch_bounds__(512) slim_kernel(Jobs jobs, Step s, uint32_t it, int last) {
+	__shared__ __attribute__((aligned(16))) char xt_[TINY_K * TINY_PITCH], a_[TINY_N * TINY_PITCH], b_[TINY_N * TINY_PITCH];
+	__shared__ double sums[8];
+	lds_char *const xt = lds_of(xt_), *const ma = lds_of(a_), *const mb = lds_of(b_);
+	const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+	uint32_t slab = blockIdx.x;
+	const uint32_t ji = job_of(jobs, START_GRAM, slab);
+	const Job& j = jobs.job[ji];
+	const uint32_t height = j.parts, r0 = slab * height, here = min(height, j.k - r0), slabs = (j.k + height - 1) / height;
+	const int k_steps = (int)((here + 31) / 32);
+	char* const x = (char*)j.xt[0] + (uint64_t)r0 * 256;
+	f32x4* const part = (f32x4*)(j.partial + ((uint64_t)(it & 1) * slabs + slab) * PART_FLOATS) + tid;
+	const TinyBlocks own(wave, lane);
+	f32x4 acc[2];
+	if (it == 0) {
+		const uint32_t blocks = jobs.start[START_SUM][ji + 1] - jobs.start[START_SUM][ji];
+		double sum = 0.0;
+		for (uint32_t i = tid; i < blocks; i += 512) sum += j.sums[i];
+		for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
+		if (lane == 0) sums[wave] = sum;
+		for (int i = tid; i < k_steps * 32 * (TINY_PITCH / 16); i += 512) *(__attribute__((address_space(3))) i32x4*)(xt + i * 16) = i32x4{0, 0, 0, 0};
+		__syncthreads();
+		sum = sums[0];
+		for (int i = 1; i < 8; ++i) sum += sums[i];
+		const double norm = sqrt(sum) + (double)s.eps, scale = norm == 0.0 ? 0.0 : (double)SX / norm;
+		const bool turn = j.rows > j.cols;   // the matrix lies as X^T
+#pragma unroll 8
+		for (uint32_t e = tid; e < here * j.n; e += 512) {   // along the matrix's rows
+			const uint32_t row = turn ? e / j.n : e % here, col = turn ? e % j.n : e / here;
+			const uint64_t i = j.offset + (turn ? (uint64_t)(r0 + row) * j.cols + col : (uint64_t)col * j.cols + r0 + row);
+			const float m = s.buffer[i], g = s.nesterov ? load_grad(s, i) : 0.0f;
+			f16 hi, lo;
+			split2((float)((double)(s.nesterov ? g + s.momentum * m : m) * scale), hi, lo);
+			lds_char* p = xt + row * TINY_PITCH + (col >> 5) * 128 + (col & 31) * 2;
+			*(__attribute__((address_space(3))) f16*)p = hi;
+			*(__attribute__((address_space(3))) f16*)(p + 64) = lo;
+		}
+		__syncthreads();
+	} else {
+		for (int i = tid; i < k_steps * 32 * 16; i += 512) *(__attribute__((address_space(3))) i32x4*)(xt + (i >> 4) * TINY_PITCH + (i & 15) * 16) = *(const i32x4*)(x + i * 16);
+		const f32x4* q = (const f32x4*)(j.partial + (uint64_t)(~it & 1) * slabs * PART_FLOATS) + tid;   // the parts that the launch before left
+		acc[0] = acc[1] = f32x4{0, 0, 0, 0};
+#pragma unroll 16
+		for (uint32_t i = 0; i < slabs; ++i)
+#pragma unroll
+			for (int b = 0; b < 2; ++b) acc[b] += q[i * (PART_FLOATS / 4) + b * 512];
+		tiny_polynomial(ma, mb, own, lane, acc);
+#pragma unroll
+		for (int h = 0; h < 2; ++h) {   // a wave reads and writes its own rows of X^T alone: no barrier between
+			const int r = h * 128 + wave * 16;
+			if (r >= k_steps * 32) break;
+			f32x4 y[4];
+			tiny_apply(xt, mb, r, lane, y);
+			if (last) tiny_weights(s, j.offset, j.rows, j.cols, r0 + r, own, y);
+			else
+#pragma unroll
+				for (int b = 0; b < 4; ++b) tiny_put(xt, r + own.lm, b * 16 + own.ln, y[b] * (1.0f / SA));
+		}
+		if (last) return;
+		__syncthreads();
+	}
+	for (int i = tid; i < k_steps * 32 * 16; i += 512) *(i32x4*)(x + i * 16) = *(const __attribute__((address_space(3))) i32x4*)(xt + (i >> 4) * TINY_PITCH + (i & 15) * 16);
+	tiny_gram(xt, k_steps, own, lane, acc);
+#pragma unroll
+	for (int b = 0; b < 2; ++b) part[b * 512] = acc[b];
+}
 
 // ---- host ------------------------------------------------------------------------------------------------------------------------------
 
@@ -653,11 +759,15 @@ static const char* bad_matrices(uint32_t count, const NgpMuonMatrix* m) {
 	return nullptr;
 }
 
-// the next MAX_JOBS matrices from `first` on that are too large for one workgroup
-static bool next_jobs(Jobs& jobs, uint32_t n, const NgpMuonMatrix* m, uint32_t& first) {
+// the next matrices from `first` on that are too large for one workgroup, at most MAX_JOBS: those in slabs (`slim`, at most BATCH_SLABS: more would be a second round of the chip), or the
+// others; slabs: in_slabs of the list
+static bool next_jobs(Jobs& jobs, uint32_t n, const NgpMuonMatrix* m, bool slabs, bool slim, uint32_t& first) {
 	jobs.count = 0;
-	for (; first < n && jobs.count < MAX_JOBS; ++first) {
-		if (is_tiny(m[first])) continue;
+	if (slim && !slabs) return false;
+	for (uint32_t total = 0; first < n && jobs.count < MAX_JOBS; ++first) {
+		const uint32_t mine = slabs ? slabs_of(m[first]) : 0;
+		if (is_tiny(m[first]) || (mine != 0) != slim) continue;
+		if ((total += mine) > BATCH_SLABS) break;
 		Job& j = jobs.job[jobs.count++];
 		j.offset = m[first].offset; j.rows = m[first].rows; j.cols = m[first].cols;
 	}
@@ -665,7 +775,7 @@ static bool next_jobs(Jobs& jobs, uint32_t n, const NgpMuonMatrix* m, uint32_t& 
 }
 
 // their buffers in `base` (null: the size alone)
-static uint64_t lay_out(Jobs& jobs, char* base) {
+static uint64_t lay_out(Jobs& jobs, bool slim, char* base) {
 	uint64_t used = 0;
 	auto take = [&](uint64_t bytes) { char* p = base ? base + used : nullptr; used += up256(bytes); return p; };
 	for (int kind = 0; kind < N_STARTS; ++kind) jobs.start[kind][0] = 0;
@@ -676,6 +786,16 @@ static uint64_t lay_out(Jobs& jobs, char* base) {
 		j.n = std::min(j.rows, j.cols); j.k = std::max(j.rows, j.cols);
 		j.np = (j.n + 31) & ~31u;
 		const uint32_t blocks = (uint32_t)std::min<uint64_t>(SUM_BLOCKS, ((uint64_t)j.rows * j.cols + 4095) / 4096);
+		jobs.start[START_SUM][i + 1] = jobs.start[START_SUM][i] + blocks;
+		if (slim) {
+			j.parts = slab_rows(j.k);
+			const uint32_t slabs = (j.k + j.parts - 1) / j.parts;
+			j.xt[0] = (f16*)take((uint64_t)slabs * j.parts * 256);
+			j.partial = (float*)take((uint64_t)2 * slabs * PART_FLOATS * 4);
+			j.sums = (double*)take(blocks * 8);
+			jobs.start[START_GRAM][i + 1] = jobs.start[START_GRAM][i] + slabs;
+			continue;
+		}
 		j.xt[0] = (f16*)take((uint64_t)j.k * j.np * 4);
 		j.xt[1] = (f16*)take((uint64_t)j.k * j.np * 4);
 		j.a = (f16*)take((uint64_t)j.n * j.np * 4);
@@ -687,7 +807,6 @@ static uint64_t lay_out(Jobs& jobs, char* base) {
 		const uint32_t steps = (j.k + 31) / 32, per = (steps + j.parts - 1) / j.parts;
 		j.parts = (steps + per - 1) / per;
 		j.partial = (float*)take(j.parts > 1 ? (uint64_t)j.parts * symmetric_tiles<Little>(j.n) * (Little::BN * Little::BM * 4) : 0);
-		jobs.start[START_SUM][i + 1] = jobs.start[START_SUM][i] + blocks;
 		jobs.start[START_SPLIT][i + 1] = jobs.start[START_SPLIT][i] + ((j.np + 63) / 64) * ((j.k + 63) / 64);
 	}
 	return used;
@@ -733,8 +852,10 @@ uint64_t ngp_hip_muon_workspace_bytes(uint32_t n_matrices, const NgpMuonMatrix* 
 	using namespace muon;
 	if (const char* bad = bad_matrices(n_matrices, matrices_host)) { refuse(bad); return 0; }
 	uint64_t most = 0;
+	const bool slabs = in_slabs(n_matrices, matrices_host);
 	Jobs jobs;
-	for (uint32_t first = 0; next_jobs(jobs, n_matrices, matrices_host, first);) most = std::max(most, lay_out(jobs, nullptr));
+	for (const bool slim : {false, true})
+		for (uint32_t first = 0; next_jobs(jobs, n_matrices, matrices_host, slabs, slim, first);) most = std::max(most, lay_out(jobs, slim, nullptr));
 	return most;
 }
 
@@ -763,9 +884,17 @@ int ngp_hip_muon_step(void* stream, uint32_t n_matrices, const NgpMuonMatrix* ma
 		if (count) hipLaunchKernelGGL(tiny_kernel, dim3(count), dim3(512), 0, st, tiny, s, n_iterations);
 		NGP_LAUNCH_CHECK("tiny_kernel");
 	}
+	const bool slabs = in_slabs(n_matrices, matrices_host);
 	Jobs jobs;
-	for (uint32_t first = 0; next_jobs(jobs, n_matrices, matrices_host, first);) {
-		lay_out(jobs, (char*)workspace);
+	for (uint32_t first = 0; next_jobs(jobs, n_matrices, matrices_host, slabs, true, first);) {
+		lay_out(jobs, true, (char*)workspace);
+		const uint32_t c = jobs.count;
+		hipLaunchKernelGGL(momentum_kernel, dim3(jobs.start[START_SUM][c]), dim3(256), 0, st, jobs, s);
+		for (uint32_t it = 0; it <= n_iterations; ++it) hipLaunchKernelGGL(slim_kernel, dim3(jobs.start[START_GRAM][c]), dim3(512), 0, st, jobs, s, it, (int)(it == n_iterations));
+		NGP_LAUNCH_CHECK("slim_kernel");
+	}
+	for (uint32_t first = 0; next_jobs(jobs, n_matrices, matrices_host, slabs, false, first);) {
+		lay_out(jobs, false, (char*)workspace);
 		const uint32_t c = jobs.count;
 		hipLaunchKernelGGL(momentum_kernel, dim3(jobs.start[START_SUM][c]), dim3(256), 0, st, jobs, s);
 		hipLaunchKernelGGL(split_kernel, dim3(jobs.start[START_SPLIT][c]), dim3(256), 0, st, jobs, s);

@@ -81,7 +81,7 @@ def check_step(ngp, v, **kw):
             assert torch.equal(v.of(v.params, i), v.of(v.master, i).to(v.t))
 
 
-SHAPES = [(1, 1), (1, 7), (5, 1), (3, 2), (16, 64), (64, 32), (64, 64), (33, 65), (63, 200), (64, 256), (256, 17), (257, 30), (65, 64), (128, 128), (100, 300), (300, 100), (129, 257), (130, 1000), (1000, 127), (768, 520), (520, 2050)]
+SHAPES = [(1, 1), (1, 7), (5, 1), (3, 2), (16, 64), (64, 32), (64, 64), (33, 65), (63, 200), (64, 256), (256, 17), (257, 30), (65, 64), (128, 128), (100, 300), (300, 100), (129, 257), (130, 1000), (1000, 127), (768, 520), (520, 2050), (30, 5000), (1640, 24), (64, 8192), (8191, 64), (63, 8193), (513, 1), (2, 300)]
 
 
 @pytest.mark.parametrize("shape", SHAPES, ids=lambda s: "%dx%d" % s)
@@ -104,7 +104,7 @@ def test_larger_tiles(ngp, cuda, shapes):
     check_step(ngp, Vector(shapes, "bf16", gap=1), iterations=5)
 
 
-@pytest.mark.parametrize("shapes", [[(65, 8200)], [(5000, 96)], [(100, 512), (66, 513), (300, 1111), (130, 131)]], ids=["wide", "tall", "several"])
+@pytest.mark.parametrize("shapes", [[(65, 8200)], [(5000, 96)], [(100, 512), (66, 513), (300, 1111), (130, 131)], [(40, 3000), (64, 300), (5000, 17), (33, 257), (60, 60)] * 4, [(40, 2000), (64, 300), (150, 200)] * 15, [(40, 3000), (64, 300)] * 12], ids=["wide", "tall", "several", "slabs", "two batches of slabs", "too many slabs"])
 def test_sums_over_a_long_side_in_parts(ngp, cuda, shapes):
     for dtype in ("f16", "f32"):
         v = Vector(shapes, dtype, seed=5)
