@@ -184,7 +184,7 @@ __device__ __forceinline__ void one_tile(const Item<T>& it, uint32_t pid, lds_ch
 }
 
 // All results that are ready to be computed at one point in one launch: y (FORWARD), or dx and the three weight gradients, whose tiles fill the chip together where each alone would
-// leave a part of it idle.  Bound by the matrix pipes: the five products behind 8192 x 4096 - 8192 - 4096 in f16 2.06 ms, 1.33 PFLOP/s; those of 4096 x 1024 - 2816 - 1024 122 us,
+// leave a part of it idle.  Bound by the matrix pipes: the five products behind 8192 x 4096 - 8192 - 4096 in f16 2.06 ms, 1.33 PFLOP/s; those of 4096 x 1024 - 2816 - 1024 125 us,
 // 0.97 (196 tiles for 256 CUs, a third of them with 5632 of k to the others' 4096).  With splits, a workgroup leaves its accumulators in `partial` as they lie in the registers, and group_sum_kernel adds the splits in their order: the
 // result does not depend on which workgroup ends first.
 template <class T, int SHAPE, bool FORWARD>
@@ -213,7 +213,7 @@ __global__ void __launch_bounds__(256) split_fold_kernel(float* partial, uint32_
 }
 
 // The splits of the tiles (every `every`-th of them, where they have been folded), added in order, rounded once; a workgroup takes two of a tile's MB block rows, the 32 rows that
-// are stored together.  Items without splits have no tiles here.  Bound by memory and, at these sizes, by starting up: 32 MB of 1537 x 387 - 1061 - 259 in 11 us.
+// are stored together.  Items without splits have no tiles here.  Bound by memory and by starting up: 32 MB of sums 11 us, 5 MB 5 us.
 template <class T>
 __global__ void __launch_bounds__(256) group_sum_kernel(Group<T> g) {
 	using S = Shape<SMALL>;

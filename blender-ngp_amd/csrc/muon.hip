@@ -375,7 +375,7 @@ __device__ __forceinline__ void store_symmetric(const f32x4 (&acc)[P::NB][P::MB]
 }
 
 // A, all of k or (a long, narrow X has few tiles) a part of it: then the sums are left as they lie in the registers, and gram_sum_kernel adds the parts in their order.
-// Bound by the matrix pipes where the tiles fill the chip (two 8192 x 4096: 0.88 ms, 0.97 PFLOP/s of fp16 products, 0.97 of the tiles' work being needed), else by the latency of the
+// Bound by the matrix pipes where the tiles fill the chip (two 8192 x 4096: 0.86 ms, 0.99 PFLOP/s of fp16 products, 0.97 of the tiles' work being needed), else by the latency of the
 // DMA: one 1531 x 1000, 136 tiles of 64 x 64 and 48 steps, 16 us.
 template <class G>
 __global__ void __launch_bounds__(G::THREADS, (SplitProduct<G, RC>::LDS_BYTES <= 80 * 1024 ? 2 : 1)) gram_kernel(Jobs jobs, int from) {
@@ -413,7 +413,7 @@ __global__ void __launch_bounds__(G::THREADS) gram_sum_kernel(Jobs jobs) {
 	store_symmetric<P, 0>(acc, j, tm, tn, lds_of(lds));
 }
 
-// B.  As gram_kernel: 0.42 ms and 12 us there
+// B.  As gram_kernel: 0.43 ms and 13 us there
 template <class G>
 __global__ void __launch_bounds__(G::THREADS, (SplitProduct<G, KC>::LDS_BYTES <= 80 * 1024 ? 2 : 1)) poly_kernel(Jobs jobs) {
 	using P = SplitProduct<G, KC>;
@@ -474,7 +474,7 @@ __global__ void __launch_bounds__(G::THREADS, (SplitProduct<G, KC>::LDS_BYTES <=
 // ---- a matrix in one workgroup ---------------------------------------------------------------------------------------------------------------
 //
 // Short side at most 64, long side at most 256 (the matrices of the framework's own networks): X^T, A and B stay in LDS in the same split layout, and the whole step is one launch
-// whose time is the latency of its chain: 3 products an iteration, four barriers.  Five 64 x 64 matrices: 20 us; 76 as 17 launches of the kernels above.
+// whose time is the latency of its chain: 3 products an iteration, four barriers.  Five 64 x 64 matrices: 18 us; 76 as 17 launches of the kernels above.
 struct TinyJobs { NgpMuonMatrix m[128]; };
 constexpr uint32_t TINY_N = 64, TINY_K = 256;
 constexpr int TINY_PITCH = 64 * 4 + 16;   // bytes of a row of 64 columns in two halves
