@@ -307,3 +307,22 @@ def test_few_rows_through_many_columns(ngp, cuda, shape, dtype):
     R.check("y", y, ref.y, ref.ey)
     untouched(ybuf, y)
     assert (ws[n:] == 0xff).all()
+
+
+@pytest.mark.parametrize("shape", [(3, 5, 1 << 20, 2), (3, 1 << 20, 5, 2), (3, 2, 5, 1 << 20), (70, 5, 1 << 20, 2), (70, 1 << 20, 5, 2), (70, 2, 5, 1 << 20), (3000001, 8, 16, 4), (400003, 136, 72, 40)],
+                         ids=lambda s: "x".join(map(str, s)))
+def test_the_widest_and_longest(ngp, cuda, shape):
+    rows, d, f, o = shape
+    b = block(d, f, o, "f16", "relu")
+    x, wg, wu, wd, dy = inputs(rows, d, f, o, "f16", seed=rows)
+    ref = R.Block("relu", x, wg, wu, wd, dy)
+    y, outs = torch.empty(rows, o, dtype=x.dtype, device="cuda"), [torch.empty_like(t) for t in (x, wg, wu, wd)]
+    ws, n = workspace(ngp, b, rows, 0)
+    forward(ngp, b, x, wg, wu, wd, y, ws, n)
+    ws2, n2 = workspace(ngp, b, rows, capi.FFN_BACKWARD)
+    backward(ngp, b, x, wg, wu, wd, dy, outs[0], outs[1:], ws2, n2)
+    torch.cuda.synchronize()
+    R.check("y", y, ref.y, ref.ey)
+    for name, v, want, bound in zip(("dx", "dw_gate", "dw_up", "dw_down"), outs, (ref.dx, ref.dwg, ref.dwu, ref.dwd), (ref.edx, ref.edwg, ref.edwu, ref.edwd)):
+        R.check(name, v, want, bound)
+    assert (ws[n:] == 0xff).all() and (ws2[n2:] == 0xff).all()

@@ -81,7 +81,7 @@ def check_step(ngp, v, **kw):
             assert torch.equal(v.of(v.params, i), v.of(v.master, i).to(v.t))
 
 
-SHAPES = [(1, 1), (1, 7), (5, 1), (3, 2), (16, 64), (64, 32), (64, 64), (33, 65), (63, 200), (64, 256), (256, 17), (257, 30), (65, 64), (128, 128), (100, 300), (300, 100), (129, 257), (130, 1000), (1000, 127), (768, 520), (520, 2050), (30, 5000), (1640, 24), (64, 8192), (8191, 64), (63, 8193), (513, 1), (2, 300)]
+SHAPES = [(1, 1), (1, 7), (5, 1), (3, 2), (16, 64), (64, 32), (64, 64), (33, 65), (63, 200), (64, 256), (256, 17), (257, 30), (65, 64), (128, 128), (100, 300), (300, 100), (129, 257), (130, 1000), (1000, 127), (768, 520), (520, 2050), (30, 5000), (1640, 24), (64, 8192), (8191, 64), (63, 8193), (65536, 70), (3, 65536), (513, 1), (2, 300)]
 
 
 @pytest.mark.parametrize("shape", SHAPES, ids=lambda s: "%dx%d" % s)
