@@ -326,3 +326,44 @@ def test_the_widest_and_longest(ngp, cuda, shape):
     for name, v, want, bound in zip(("dx", "dw_gate", "dw_up", "dw_down"), outs, (ref.dx, ref.dwg, ref.dwu, ref.dwd), (ref.edx, ref.edwg, ref.edwu, ref.edwd)):
         R.check(name, v, want, bound)
     assert (ws[n:] == 0xff).all() and (ws2[n2:] == 0xff).all()
+
+
+@pytest.mark.parametrize("shape", [(24, 1024, 2056, 520), (700, 264, 520, 136), (3000, 32, 64, 16)], ids=lambda s: "x".join(map(str, s)))
+def test_two_streams_at_once_and_graphs_that_share_a_workspace(ngp, cuda, shape):
+    rows, d, f, o = shape
+    b = block(d, f, o, "f16", "gelu")
+    sets = [inputs(rows, d, f, o, "f16", seed=s) for s in (1, 2)]
+    n = max(ngp.ngp_hip_gated_ffn_workspace_bytes(b.ctypes.data, rows, k) for k in (0, capi.FFN_BACKWARD))
+
+    def fresh():
+        return torch.empty(max(n, 16), dtype=torch.uint8, device="cuda"), torch.empty(rows, o, dtype=torch.float16, device="cuda"), [torch.empty_like(t) for t in sets[0][:4]]
+
+    def both(i, ws, y, outs):
+        x, wg, wu, wd, dy = sets[i]
+        forward(ngp, b, x, wg, wu, wd, y, ws, n)
+        backward(ngp, b, x, wg, wu, wd, dy, outs[0], outs[1:], ws, n)
+
+    want, got, streams = [fresh(), fresh()], [fresh(), fresh()], [torch.cuda.Stream(), torch.cuda.Stream()]
+    for i in range(2):
+        both(i, *want[i])
+    torch.cuda.synchronize()
+    for _ in range(5):   # in turn, so that the two streams' kernels lie beside each other
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                both(i, *got[i])
+    torch.cuda.synchronize()
+    same = lambda a, c: torch.equal(a[1], c[1]) and all(torch.equal(u, v) for u, v in zip(a[2], c[2]))   # noqa: E731
+    assert all(same(want[i], got[i]) for i in range(2))
+    shared, graphs = fresh()[0], []
+    for i in range(2):
+        got[i][1].zero_()
+        torch.cuda.synchronize()
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[i]):
+            both(i, shared, *got[i][1:])
+    for _ in range(3):
+        for i in (0, 1, 0):
+            got[i][1].fill_(-1.0)
+            graphs[i].replay()
+        torch.cuda.synchronize()
+        assert all(same(want[i], got[i]) for i in range(2))

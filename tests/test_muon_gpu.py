@@ -238,3 +238,32 @@ def test_offsets_that_pass_32_bits(ngp, cuda):
         at, k = int(desc["offset"][i]), int(desc["rows"][i]) * int(desc["cols"][i])
         for big, t in zip(far[1:], (small.master, small.params, small.buf)):
             assert torch.equal(big[at:at + k], small.of(t, i).reshape(-1))
+
+
+def test_two_streams_at_once_and_graphs_that_share_a_workspace(ngp, cuda):
+    shapes = [(64, 32), (40, 900), (200, 136), (300, 513)]
+    runs = [Vector(shapes, "f16", seed=s) for s in (1, 2)]
+    want = [Vector(shapes, "f16", seed=s) for s in (1, 2)]
+    for v in want:
+        ws, n = v.workspace(ngp)
+        for _ in range(4):
+            v.step(ngp, ws, n)
+    torch.cuda.synchronize()
+    spaces, streams = [v.workspace(ngp) for v in runs], [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for _ in range(2):
+        for v, (ws, n), s in zip(runs, spaces, streams):
+            with torch.cuda.stream(s):
+                v.step(ngp, ws, n)
+    torch.cuda.synchronize()
+    graphs = []
+    for v in runs:   # one workspace for both
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            v.step(ngp, *spaces[0])
+    for _ in range(2):
+        for g in graphs:
+            g.replay()
+    torch.cuda.synchronize()
+    for v, w in zip(runs, want):
+        assert torch.equal(v.master, w.master) and torch.equal(v.buf, w.buf) and torch.equal(v.params, w.params)
