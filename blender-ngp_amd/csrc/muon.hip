@@ -802,8 +802,9 @@ static uint64_t lay_out(Jobs& jobs, bool slim, char* base) {
 		j.b = (f16*)take((uint64_t)j.n * j.np * 4);
 		j.sums = (double*)take(blocks * 8);
 		// Few tiles: k in parts of at least 8 steps, two workgroups a CU (each holds 64 KiB of LDS).  The step of one 96 x 8192 373 -> 149 us, 256 x 4096 251 -> 152 us, 700 x 6000 (66
-		// tiles) 455 -> 363 us; with 136 tiles, 1531 x 1000, it costs: 244 -> 250 us.
-		j.parts = tiles >= 128 ? 1 : std::max(1u, std::min(512 / tiles, (j.k + 31) / 32 / 8));
+		// tiles) 455 -> 363 us; with 136 tiles, 1531 x 1000, it costs: 244 -> 250 us, and with a
+		// short side to sum over, twenty 128 x 616: 128 -> 134 us.
+		j.parts = tiles >= 128 || j.k < 768 ? 1 : std::max(1u, std::min(512 / tiles, (j.k + 31) / 32 / 8));
 		const uint32_t steps = (j.k + 31) / 32, per = (steps + j.parts - 1) / j.parts;
 		j.parts = (steps + per - 1) / per;
 		j.partial = (float*)take(j.parts > 1 ? (uint64_t)j.parts * symmetric_tiles<Little>(j.n) * (Little::BN * Little::BM * 4) : 0);
