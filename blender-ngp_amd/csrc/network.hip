@@ -2884,6 +2884,7 @@ __global__ void __launch_bounds__(256) rows_to_planes_kernel(const uint32_t* __r
 static bool refuse_capture(void* stream, const char* what) {
 	hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
 	if (hipStreamIsCapturing((hipStream_t)stream, &status) == hipSuccess && status == hipStreamCaptureStatusNone) return false;
+	(void)hipGetLastError();   // the question's own error is not the next launch's
 	set_last_error(what, hipErrorStreamCaptureUnsupported);
 	return true;
 }
