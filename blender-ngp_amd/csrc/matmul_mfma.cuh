@@ -53,10 +53,14 @@ template <> __device__ __forceinline__ f32x16 mfma<b16>(i32x4 a, i32x4 b, f32x16
 __device__ __forceinline__ lds_char* lds_of(void* p) { return (lds_char*)(__attribute__((address_space(3))) void*)p; }
 
 // 16 bytes of every lane straight into LDS at `lds` + 16 lane.  The instruction returns nothing to a register, and the compiler, told of it as a builtin, would wait for ALL
-// DMA in flight before each LDS read; written here, the waits are the two below and stand where the buffers change hands.
+// DMA in flight before each LDS read; written here, the waits are the two below and stand where the buffers change hands.  m0 is the compiler's too (its own LDS DMA, messages):
+// without the clobber it keeps a value there across this one.  Its warning that m0 is not preserved is what the clobber says.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void dma16(i32x4 rsrc, lds_char* lds, int voff) {
-	asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"((uint32_t)(uintptr_t)lds), "v"(voff), "s"(rsrc) : "memory");
+	asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"((uint32_t)(uintptr_t)lds), "v"(voff), "s"(rsrc) : "m0", "memory");
 }
+#pragma clang diagnostic pop
 // every DMA of this wave but the last PENDING has landed, every LDS read of it has returned; then all waves
 template <int PENDING = 0> __device__ __forceinline__ void wait_and_sync() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(PENDING) : "memory"); }
 
