@@ -669,7 +669,7 @@ static uint32_t slabs_of(const NgpMuonMatrix& m) {   // 0: not in slabs
 // Only as many as a round of the chip takes, or short ones: twelve 6264 x 48 in slabs are two batches, 245 us, and 191 by the kernels above.
 static bool in_slabs(uint32_t n, const NgpMuonMatrix* m) {
 	uint32_t slabs = 0, most = 0;
-	for (uint32_t i = 0; i < n && slabs <= BATCH_SLABS; ++i) { slabs += slabs_of(m[i]); most = std::max(most, slabs_of(m[i])); }
+	for (uint32_t i = 0; i < n; ++i) { slabs += slabs_of(m[i]); most = std::max(most, slabs_of(m[i])); }   // of the whole list, in whatever order: at most 2^21
 	return slabs <= BATCH_SLABS || most <= MAX_SLABS / 2;
 }
 

@@ -60,3 +60,18 @@ def test_small_matrices_need_no_workspace(ngp):
 
 def test_no_matrices_is_no_work(ngp):
     assert call(ngp, count=0, g=None, w=None, p=None, b=None, ws=None, n=0) == 0
+
+
+def listed(*shapes):
+    at, rows = 0, []
+    for r, c in shapes:
+        rows.append((at, r, c))
+        at += r * c
+    return matrices(*rows)
+
+
+def test_the_choice_of_slabs_does_not_depend_on_the_order_of_the_list(ngp):
+    """seventeen of 16 slabs and three of 32 are more than one round of the chip either way round"""
+    short, long = [(16, 2048)] * 17, [(64, 8192)] * 3
+    size = [ngp.ngp_hip_muon_workspace_bytes(len(m), m.ctypes.data) for m in (listed(*short, *long), listed(*long, *short), listed(*short[:9], *long, *short[9:]))]
+    assert size[0] == size[1] == size[2] > 0
