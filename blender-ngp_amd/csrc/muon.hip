@@ -28,7 +28,7 @@ using namespace mm;
 
 constexpr float SX = 32768.0f, SA = 8192.0f;                      // scales of X and of A, B
 constexpr float NS_A = 3.4445f, NS_B = -4.7750f, NS_C = 2.0315f;
-constexpr uint32_t MAX_JOBS = 24, MAX_SIDE = 65536, SUM_BLOCKS = 1024;
+constexpr uint32_t MAX_SIDE = 65536, SUM_BLOCKS = 1024;
 
 struct Job {
 	uint64_t offset;                    // of the matrix in the parameter vector, in elements
@@ -40,13 +40,15 @@ struct Job {
 	uint32_t parts;                     // of k, in the products that give A; of a matrix in slabs: the rows of one
 };
 enum { START_SUM, START_SPLIT, START_GRAM, START_SYM, START_APPLY, N_STARTS };
+struct Step { float lr, momentum, decay, eps, inv_loss_scale; int nesterov, dtype; const void* grads; float* master; void* params; float* buffer; };
+// As many matrices to a launch as its arguments, 4 KiB, hold beside Step, two numbers and the count: a longer list is more than one chain of launches, each waiting for the one before.
+constexpr uint32_t ARGUMENT_BYTES = 4096, MAX_JOBS = (ARGUMENT_BYTES - sizeof(Step) - 32 - 4 * N_STARTS) / (sizeof(Job) + 4 * N_STARTS);
 struct Jobs {
 	Job job[MAX_JOBS];
 	uint32_t start[N_STARTS][MAX_JOBS + 1];   // first workgroup of each job, per kind of kernel (the products: of the tile of the launch)
 	uint32_t count;
 };
-
-struct Step { float lr, momentum, decay, eps, inv_loss_scale; int nesterov, dtype; const void* grads; float* master; void* params; float* buffer; };
+static_assert(sizeof(Jobs) + sizeof(Step) + 16 <= ARGUMENT_BYTES && MAX_JOBS < 64, "fits the arguments of a launch; job_of has a lane for every end");
 
 // the job of a workgroup, which becomes its number within the job: every lane compares one job's end
 __device__ __forceinline__ uint32_t job_of(const Jobs& j, int kind, uint32_t& pid) {
@@ -759,20 +761,80 @@ static const char* bad_matrices(uint32_t count, const NgpMuonMatrix* m) {
 	return nullptr;
 }
 
-// the next matrices from `first` on that are too large for one workgroup, at most MAX_JOBS: those in slabs (`slim`, at most BATCH_SLABS: more would be a second round of the chip), or the
-// others; slabs: in_slabs of the list
-static bool next_jobs(Jobs& jobs, uint32_t n, const NgpMuonMatrix* m, bool slabs, bool slim, uint32_t& first) {
-	jobs.count = 0;
-	if (slim && !slabs) return false;
-	for (uint32_t total = 0; first < n && jobs.count < MAX_JOBS; ++first) {
-		const uint32_t mine = slabs ? slabs_of(m[first]) : 0;
-		if (is_tiny(m[first]) || (mine != 0) != slim) continue;
-		if ((total += mine) > BATCH_SLABS) break;
-		Job& j = jobs.job[jobs.count++];
-		j.offset = m[first].offset; j.rows = m[first].rows; j.cols = m[first].cols;
-	}
-	return jobs.count != 0;
+// The tile whose rounds of the chip cost least.  A round, in units of one 128 x 128 tile a CU in eight waves: two of four waves (24 of 768 x 768: 957 -> 845 us) 1.7, one 128 x 256
+// 1.68 (two 8192 x 4096: 1.25 ms a launch where 128 x 128 take 1.7; not for the symmetric products: 0.87 ms both, more of a larger tile lies above the diagonal), two 64 x 64
+// 0.8.  In a sweep of 16 shapes this is within 3 % of the best of the four; a step of 2000 x 2000 723 -> 657 us, 1500 x 1500 425 -> 390, 4000 x 8000 6.92 -> 6.56 ms against
+// fixed bounds on the number of tiles.
+enum { LITTLE_TILE, LONE_TILE, MIDDLE_TILE, LARGE_TILE };
+static double rounds(uint32_t tiles, uint32_t slots) { return (double)((tiles + slots - 1) / slots); }
+static int tile_for(uint32_t little, uint32_t middle, double large, double* least = nullptr) {
+	const double cost[4] = {0.8 * rounds(little, 512), rounds(middle, 256), 1.7 * rounds(middle, 512), large};
+	const int tile = (int)(std::min_element(cost, cost + 4) - cost);
+	if (least) *least = tile == LITTLE_TILE && little <= 256 ? 0.4 : cost[tile];   // one workgroup a CU, for the estimate below
+	return tile;
 }
+template <class G> static uint32_t apply_tiles(uint32_t n, uint32_t k) { return ((n + G::BN - 1) / G::BN) * ((k + G::BM - 1) / G::BM); }
+
+// An iteration of a batch, estimated in microseconds: the rounds of its three products by their steps, and what starting them takes.  Within a tenth for 1 to 36 matrices of 768 x 768, 20
+// and 25 of 128 x 616, 25 and 32 of 300 x 500; one 1531 x 1000 takes a fifth less.
+struct Load {
+	uint32_t count = 0, little_sym = 0, middle_sym = 0, little_apply = 0, middle_apply = 0, large_apply = 0;
+	double long_steps = 0.0, short_steps = 0.0;   // of the symmetric tiles, summed
+	void add(const NgpMuonMatrix& m) {
+		const uint32_t n = std::min(m.rows, m.cols), k = std::max(m.rows, m.cols), sym = symmetric_tiles<Middle>(n);
+		++count;
+		little_sym += symmetric_tiles<Little>(n); middle_sym += sym;
+		little_apply += apply_tiles<Little>(n, k); middle_apply += apply_tiles<Middle>(n, k); large_apply += apply_tiles<Large>(n, k);
+		long_steps += (double)sym * ((k + 31) / 32); short_steps += (double)sym * ((n + 31) / 32);
+	}
+	double time() const {
+		if (!count) return 0.0;
+		double symmetric, apply;
+		tile_for(little_sym, middle_sym, HUGE_VAL, &symmetric);
+		tile_for(little_apply, middle_apply, 1.68 * rounds(large_apply, 256), &apply);
+		return 12.0 + 0.9 * (symmetric * (long_steps + short_steps) + apply * short_steps) / middle_sym;
+	}
+};
+
+// The matrices of a list that are too large for one workgroup, in batches of at most MAX_JOBS in their order: those in slabs (`slim`, at most BATCH_SLABS: more would be a second round
+// of the chip), or the others, `limit` to a batch: the limit of least estimated time.  Few matrices more than fill the rounds of the chip are better a batch of their own (37 of
+// 768 x 768: 24 and 13 take 1390 us, 19 and 18 1510, 36 and one 1529), few more small ones are not (25 of 128 x 616: 131 us at once, 238 as 24 and one; 32 of 300 x 500 245 and 351).
+struct Batches {
+	uint32_t n;
+	const NgpMuonMatrix* m;
+	bool slabs, slim;   // slabs: in_slabs of the list
+	uint32_t first = 0, limit = MAX_JOBS;
+	Batches(uint32_t n_, const NgpMuonMatrix* m_, bool slabs_, bool slim_) : n(n_), m(m_), slabs(slabs_), slim(slim_) {
+		if (slim || n <= MAX_JOBS / 2) return;
+		double least = HUGE_VAL;
+		for (uint32_t l = MAX_JOBS; l >= MAX_JOBS / 2; --l) {
+			double time = 0.0;
+			uint32_t count = 0;
+			Load load;
+			for (uint32_t i = 0; i < n; ++i) {
+				if (!mine(m[i])) continue;
+				if (load.count == l) { time += load.time(); load = Load(); }
+				load.add(m[i]);
+				++count;
+			}
+			time += load.time();
+			if (time < 1.02 * least) { least = std::min(least, time); limit = l; }   // the smaller one of two alike: the estimate is a little low for the largest batches
+			l = std::min(l, count);   // one batch from there up
+			if (l <= MAX_JOBS / 2) return;
+		}
+	}
+	bool mine(const NgpMuonMatrix& e) const { return !is_tiny(e) && (slabs && slabs_of(e) != 0) == slim; }
+	bool next(Jobs& jobs) {
+		jobs.count = 0;
+		for (uint32_t total = 0; first < n && jobs.count < limit; ++first) {
+			if (!mine(m[first])) continue;
+			if (slim && (total += slabs_of(m[first])) > BATCH_SLABS) break;
+			Job& j = jobs.job[jobs.count++];
+			j.offset = m[first].offset; j.rows = m[first].rows; j.cols = m[first].cols;
+		}
+		return jobs.count != 0;
+	}
+};
 
 // their buffers in `base` (null: the size alone)
 static uint64_t lay_out(Jobs& jobs, bool slim, char* base) {
@@ -813,6 +875,14 @@ static uint64_t lay_out(Jobs& jobs, bool slim, char* base) {
 	return used;
 }
 
+// of the largest batch: they run one behind the other
+static uint64_t workspace_of(Batches b) {
+	uint64_t most = 0;
+	Jobs jobs;
+	while (b.next(jobs)) most = std::max(most, lay_out(jobs, b.slim, nullptr));
+	return most;
+}
+
 template <class G> static uint32_t count_symmetric(Jobs& jobs) {
 	for (uint32_t i = 0; i < jobs.count; ++i) {
 		const uint32_t tiles = symmetric_tiles<G>(jobs.job[i].n);
@@ -824,7 +894,7 @@ template <class G> static uint32_t count_symmetric(Jobs& jobs) {
 template <class G> static uint32_t count_apply(Jobs& jobs) {
 	for (uint32_t i = 0; i < jobs.count; ++i) {
 		const Job& j = jobs.job[i];
-		jobs.start[START_APPLY][i + 1] = jobs.start[START_APPLY][i] + ((j.n + G::BN - 1) / G::BN) * ((j.k + G::BM - 1) / G::BM);
+		jobs.start[START_APPLY][i + 1] = jobs.start[START_APPLY][i] + apply_tiles<G>(j.n, j.k);
 	}
 	return jobs.start[START_APPLY][jobs.count];
 }
@@ -852,12 +922,8 @@ extern "C" {
 uint64_t ngp_hip_muon_workspace_bytes(uint32_t n_matrices, const NgpMuonMatrix* matrices_host) {
 	using namespace muon;
 	if (const char* bad = bad_matrices(n_matrices, matrices_host)) { refuse(bad); return 0; }
-	uint64_t most = 0;
 	const bool slabs = in_slabs(n_matrices, matrices_host);
-	Jobs jobs;
-	for (const bool slim : {false, true})
-		for (uint32_t first = 0; next_jobs(jobs, n_matrices, matrices_host, slabs, slim, first);) most = std::max(most, lay_out(jobs, slim, nullptr));
-	return most;
+	return std::max(workspace_of(Batches(n_matrices, matrices_host, slabs, true)), workspace_of(Batches(n_matrices, matrices_host, slabs, false)));
 }
 
 int ngp_hip_muon_step(void* stream, uint32_t n_matrices, const NgpMuonMatrix* matrices_host, float learning_rate, float momentum, float weight_decay, float epsilon, int nesterov,
@@ -872,7 +938,10 @@ int ngp_hip_muon_step(void* stream, uint32_t n_matrices, const NgpMuonMatrix* ma
 	if (!bad && dtype == NGP_DTYPE_F32 && params) bad = "dtype F32 has no params: the master copy is the parameters";
 	if (!bad && n_matrices && (!grads || !master || !momentum_buffer)) bad = "null tensor";
 	if (!bad && ((((uintptr_t)master | (uintptr_t)momentum_buffer) & 3) || (((uintptr_t)grads | (uintptr_t)params) & (dtype == NGP_DTYPE_F32 ? 3 : 1)))) bad = "a tensor is not aligned to its elements";
-	const uint64_t need = bad ? 0 : ngp_hip_muon_workspace_bytes(n_matrices, matrices_host);
+	const uint32_t n = bad ? 0 : n_matrices;
+	const bool slabs = in_slabs(n, matrices_host);
+	Batches slim(n, matrices_host, slabs, true), tiled(n, matrices_host, slabs, false);
+	const uint64_t need = std::max(workspace_of(slim), workspace_of(tiled));
 	if (!bad && need && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < need)) bad = "workspace null, not 16-byte aligned or too small (ngp_hip_muon_workspace_bytes)";
 	if (bad) { snprintf(msg, sizeof(msg), "ngp_hip_muon_step: %s", bad); return refuse(msg); }
 	hipStream_t st = (hipStream_t)stream;
@@ -885,44 +954,34 @@ int ngp_hip_muon_step(void* stream, uint32_t n_matrices, const NgpMuonMatrix* ma
 		if (count) hipLaunchKernelGGL(tiny_kernel, dim3(count), dim3(512), 0, st, tiny, s, n_iterations);
 		NGP_LAUNCH_CHECK("tiny_kernel");
 	}
-	const bool slabs = in_slabs(n_matrices, matrices_host);
 	Jobs jobs;
-	for (uint32_t first = 0; next_jobs(jobs, n_matrices, matrices_host, slabs, true, first);) {
+	while (slim.next(jobs)) {
 		lay_out(jobs, true, (char*)workspace);
 		const uint32_t c = jobs.count;
 		hipLaunchKernelGGL(momentum_kernel, dim3(jobs.start[START_SUM][c]), dim3(256), 0, st, jobs, s);
 		for (uint32_t it = 0; it <= n_iterations; ++it) hipLaunchKernelGGL(slim_kernel, dim3(jobs.start[START_GRAM][c]), dim3(512), 0, st, jobs, s, it, (int)(it == n_iterations));
 		NGP_LAUNCH_CHECK("slim_kernel");
 	}
-	for (uint32_t first = 0; next_jobs(jobs, n_matrices, matrices_host, slabs, false, first);) {
+	while (tiled.next(jobs)) {
 		lay_out(jobs, false, (char*)workspace);
 		const uint32_t c = jobs.count;
 		hipLaunchKernelGGL(momentum_kernel, dim3(jobs.start[START_SUM][c]), dim3(256), 0, st, jobs, s);
 		hipLaunchKernelGGL(split_kernel, dim3(jobs.start[START_SPLIT][c]), dim3(256), 0, st, jobs, s);
-		// The tile whose rounds of the chip cost least.  A round, in units of one 128 x 128 tile a CU in eight waves: two of four waves (24 of 768 x 768: 957 -> 845 us) 1.7, one 128 x 256
-		// 1.68 (two 8192 x 4096: 1.25 ms a launch where 128 x 128 take 1.7; not for the symmetric products: 0.87 ms both, more of a larger tile lies above the diagonal), two 64 x 64
-		// 0.8.  In a sweep of 16 shapes this is within 3 % of the best of the four; a step of 2000 x 2000 723 -> 657 us, 1500 x 1500 425 -> 390, 4000 x 8000 6.92 -> 6.56 ms against
-		// fixed bounds on the number of tiles.
-		auto rounds = [](uint32_t tiles, uint32_t slots) { return (double)((tiles + slots - 1) / slots); };
-		auto tile_for = [&](uint32_t little, uint32_t middle, double large) {
-			const double cost[4] = {0.8 * rounds(little, 512), rounds(middle, 256), 1.7 * rounds(middle, 512), large};
-			return (int)(std::min_element(cost, cost + 4) - cost);
-		};
 		const uint32_t little_symmetric = count_symmetric<Little>(jobs), middle_symmetric = count_symmetric<Middle>(jobs);
 		const uint32_t little_apply = count_apply<Little>(jobs), middle_apply = count_apply<Middle>(jobs), large_apply = count_apply<Large>(jobs);
 		const int apply_tile = tile_for(little_apply, middle_apply, 1.68 * rounds(large_apply, 256));
 		int symmetric_tile = tile_for(little_symmetric, middle_symmetric, HUGE_VAL);
 		for (uint32_t i = 0; i < jobs.count; ++i)
-			if (jobs.job[i].parts > 1) symmetric_tile = 0;   // the parts are laid out for it
+			if (jobs.job[i].parts > 1) symmetric_tile = LITTLE_TILE;   // the parts are laid out for it
 		for (uint32_t i = 0; i < n_iterations; ++i) {
 			const int from = (int)(i & 1);
 			const bool last = i + 1 == n_iterations;
-			if (symmetric_tile == 2) symmetric_products<Middle>(st, jobs, from);
-			else if (symmetric_tile == 1) symmetric_products<Lone>(st, jobs, from);
+			if (symmetric_tile == MIDDLE_TILE) symmetric_products<Middle>(st, jobs, from);
+			else if (symmetric_tile == LONE_TILE) symmetric_products<Lone>(st, jobs, from);
 			else symmetric_products<Little>(st, jobs, from);
-			if (apply_tile == 3) apply<Large>(st, jobs, s, from, last);
-			else if (apply_tile == 2) apply<Middle>(st, jobs, s, from, last);
-			else if (apply_tile == 1) apply<Lone>(st, jobs, s, from, last);
+			if (apply_tile == LARGE_TILE) apply<Large>(st, jobs, s, from, last);
+			else if (apply_tile == MIDDLE_TILE) apply<Middle>(st, jobs, s, from, last);
+			else if (apply_tile == LONE_TILE) apply<Lone>(st, jobs, s, from, last);
 			else apply<Little>(st, jobs, s, from, last);
 		}
 		NGP_LAUNCH_CHECK("ngp_hip_muon_step");

@@ -75,3 +75,16 @@ def test_the_choice_of_slabs_does_not_depend_on_the_order_of_the_list(ngp):
     short, long = [(16, 2048)] * 17, [(64, 8192)] * 3
     size = [ngp.ngp_hip_muon_workspace_bytes(len(m), m.ctypes.data) for m in (listed(*short, *long), listed(*long, *short), listed(*short[:9], *long, *short[9:]))]
     assert size[0] == size[1] == size[2] > 0
+
+
+def test_a_batch_is_as_many_small_matrices_as_the_arguments_of_a_launch_hold(ngp):
+    """the workspace is that of the largest batch: matrices of one size take the same each"""
+    def size(*shapes):
+        m = listed(*shapes)
+        return ngp.ngp_hip_muon_workspace_bytes(len(m), m.ctypes.data)
+
+    one = size((200, 300))
+    for together in (2, 24, 25, 32, 36):
+        assert size(*[(200, 300)] * together) == together * one
+    for count in (37, 60, 200):
+        assert one * 18 <= size(*[(200, 300)] * count) <= one * 36

@@ -267,3 +267,10 @@ def test_two_streams_at_once_and_graphs_that_share_a_workspace(ngp, cuda):
     torch.cuda.synchronize()
     for v, w in zip(runs, want):
         assert torch.equal(v.master, w.master) and torch.equal(v.buf, w.buf) and torch.equal(v.params, w.params)
+
+
+@pytest.mark.parametrize("count", [24, 25, 36, 37, 75])
+def test_lists_around_what_one_launch_takes(ngp, cuda, count):
+    """one batch, two and three; large matrices among small ones"""
+    check_step(ngp, Vector([(600, 420) if i % 9 == 4 else (70 + i, 130 - i % 50) for i in range(count)], "bf16", gap=1), iterations=3)
+    check_step(ngp, Vector([(390, 410)] * count, "f16", gap=0), iterations=2)
