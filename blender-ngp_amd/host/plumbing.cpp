@@ -102,19 +102,28 @@ void Testbed::gated_init_params() {
 	m_inference_params.copy_from_host(h.data(), h.size() * 2);
 }
 
-// the network's outputs (rows of gm_out_stride()); x_saved (may be null: rendering): the encoded features for the backward pass
-void Testbed::gridmlp_inference(const uint16_t* params, const float* pos, uint32_t n_dims, uint32_t n, uint16_t* out, uint16_t* x_saved, const char* who) {
-	const NgpNetDesc* desc = m_desc_gpu.as<NgpNetDesc>();
+// rows of a gated block to a call where nothing has to be kept: 2^20 at most, and a hidden row's share of 1 GiB each (8192 rows of 65536 neurons)
+uint32_t Testbed::gated_chunk() const { return std::min<uint32_t>(1u << 20, (1u << 29) / m_gated_block.n_hidden & ~255u); }
+
+// encoding and block on n positions; x: their encoded features
+void Testbed::gated_forward(const uint16_t* params, const float* pos, uint32_t n_dims, uint32_t n, uint16_t* out, uint16_t* x, DeviceBuffer& enc_ws, DeviceBuffer& gated_ws, const char* who) {
+	enc_ws.enlarge(ngp_hip_nerf_encode_workspace_bytes(n));
+	gated_ws.enlarge(std::max<uint64_t>(16, ngp_hip_gated_ffn_workspace_bytes(&m_gated_block, n, 0)));
+	const uint32_t f = m_gated_block.n_hidden;
+	check(ngp_hip_grid_encode(m_stream, n_dims, m_desc_gpu.as<NgpNetDesc>(), params + m_n_matrix_params, pos, n_dims, n, x, enc_ws.data(), enc_ws.bytes()), who);
+	check(ngp_hip_gated_ffn_forward(m_stream, &m_gated_block, n, x, 32, params, params + 32 * f, params + 64 * f, out, gm_out_stride(), gated_ws.data(), gated_ws.bytes()), who);
+}
+
+// the network's outputs (rows of gm_out_stride()), nothing kept for a backward pass: rendering, errors, queries
+void Testbed::gridmlp_inference(const uint16_t* params, const float* pos, uint32_t n_dims, uint32_t n, uint16_t* out, const char* who) {
 	if (!m_gated) {
-		check(ngp_hip_gridmlp_forward(m_stream, n_dims, desc, params, pos, n_dims, n, out, gm_out_stride(), x_saved), who);
+		check(ngp_hip_gridmlp_forward(m_stream, n_dims, m_desc_gpu.as<NgpNetDesc>(), params, pos, n_dims, n, out, gm_out_stride(), nullptr), who);
 		return;
 	}
-	if (!x_saved) { m_x_saved.enlarge((size_t)n * 32 * 2); x_saved = m_x_saved.as<uint16_t>(); }
-	m_enc_ws.enlarge(ngp_hip_nerf_encode_workspace_bytes(n));
-	m_gated_ws.enlarge(std::max<uint64_t>(16, ngp_hip_gated_ffn_workspace_bytes(&m_gated_block, n, 0)));
-	const uint32_t f = m_gated_block.n_hidden;
-	check(ngp_hip_grid_encode(m_stream, n_dims, desc, params + m_n_matrix_params, pos, n_dims, n, x_saved, m_enc_ws.data(), m_enc_ws.bytes()), who);
-	check(ngp_hip_gated_ffn_forward(m_stream, &m_gated_block, n, x_saved, 32, params, params + 32 * f, params + 64 * f, out, gm_out_stride(), m_gated_ws.data(), m_gated_ws.bytes()), who);
+	const uint32_t chunk = std::min(n, gated_chunk());
+	m_gated_x.enlarge((size_t)chunk * 32 * 2);
+	for (uint32_t first = 0; first < n; first += chunk)
+		gated_forward(params, pos + (size_t)first * n_dims, n_dims, std::min(chunk, n - first), out + (size_t)first * gm_out_stride(), m_gated_x.as<uint16_t>(), m_gated_enc_ws, m_gated_infer_ws, who);
 }
 
 // Trainer::training_step (forward, loss, backward) + optimizer_step(128) + Trainer::loss (sum of the per-element values)
@@ -130,7 +139,7 @@ void Testbed::gridmlp_training_step(const float* pos, uint32_t n_dims, const flo
 	const NgpNetDesc* desc = m_desc_gpu.as<NgpNetDesc>();
 	profile_begin(PK_FORWARD);
 	// fused or encode + MLP kernel: measured on this workload (testbed.h ENetworkPass) — random SDF points want the two-kernel pass, stratified image batches the fused one
-	if (m_gated) gridmlp_inference(m_params.as<uint16_t>(), pos, n_dims, n, m_gm_out.as<uint16_t>(), m_x_saved.as<uint16_t>(), "gated forward");
+	if (m_gated) gated_forward(m_params.as<uint16_t>(), pos, n_dims, n, m_gm_out.as<uint16_t>(), m_x_saved.as<uint16_t>(), m_enc_ws, m_gated_ws, "gated forward");
 	else if (tuner_pick(m_stream)) {
 		m_enc_ws.enlarge(ngp_hip_nerf_encode_workspace_bytes(n));
 		check(ngp_hip_gridmlp_forward_ws(m_stream, n_dims, desc, m_params.as<uint16_t>(), pos, n_dims, n, m_gm_out.as<uint16_t>(), gm_out_stride(), m_x_saved.as<uint16_t>(), m_enc_ws.data(), m_enc_ws.bytes()), "gridmlp_forward (two kernels)");
@@ -241,7 +250,7 @@ void Testbed::render_image(RenderBuffer& rb) {  // testbed_image.cu:293-360 (no 
 	HIP_TRY(hipMemsetAsync(m_image.render_coords.data(), 0, (size_t)n_elements * 8, (hipStream_t)m_stream));
 	check(ngp_hip_image_init_coords(m_stream, m_image.render_coords.as<float>(), rb.res, m_image.resolution, m_scale, m_image.pos, sc, m_snap_to_pixel_centers, rb.spp), "image_init_coords");
 	join_side_ema();
-	gridmlp_inference(m_inference_params.as<uint16_t>(), m_image.render_coords.as<float>(), 2, n_elements, m_image.render_out.as<uint16_t>(), nullptr, "gridmlp_forward (render)");
+	gridmlp_inference(m_inference_params.as<uint16_t>(), m_image.render_coords.as<float>(), 2, n_elements, m_image.render_out.as<uint16_t>(), "gridmlp_forward (render)");
 	check(ngp_hip_image_shade(m_stream, rb.res, m_image.render_coords.as<float>(), m_image.render_out.as<uint16_t>(), gm_out_stride(), rb.frame_buffer.as<float>(), rb.depth_buffer.as<float>(),
 	                          m_image.linear_colors), "image_shade");
 }
@@ -259,7 +268,7 @@ float Testbed::compute_image_mse(bool quantize_to_byte) {  // testbed_image.cu:4
 		check(ngp_hip_image_coords_from_idx(m_stream, batch, offset, pos.as<float>(), m_image.resolution), "image_coords_from_idx");
 		check(ngp_hip_image_eval_and_snap(m_stream, batch, m_image.data.data(), m_image.type, pos.as<float>(), m_image.resolution, targets.as<float>(), 3, 1, m_image.linear_colors), "eval_image_and_snap");
 		join_side_ema();
-		gridmlp_inference(m_inference_params.as<uint16_t>(), pos.as<float>(), 2, batch, pred.as<uint16_t>(), nullptr, "gridmlp_forward (mse)");
+		gridmlp_inference(m_inference_params.as<uint16_t>(), pos.as<float>(), 2, batch, pred.as<uint16_t>(), "gridmlp_forward (mse)");
 		check(ngp_hip_image_mse(m_stream, count, targets.as<float>(), pred.as<uint16_t>(), gm_out_stride(), m_image.se.as<float>() + offset, quantize_to_byte), "image_mse");
 	}
 	check(ngp_hip_reduce_sum_f32(m_stream, m_image.se.as<float>(), n_elements, m_loss_scalar_gpu.as<float>()), "reduce_sum");

@@ -445,7 +445,7 @@ PYBIND11_MODULE(pyngp, m) {
 				d_pos.resize((size_t)n * n_dims * 4); d_out.resize((size_t)n * stride * 2);
 				d_pos.copy_from_host(b.ptr, (size_t)n * n_dims * 4);
 				t.join_side_ema();
-				t.gridmlp_inference(t.m_inference_params.as<uint16_t>(), d_pos.as<float>(), n_dims, n, d_out.as<uint16_t>(), nullptr, "gridmlp_inference");
+				t.gridmlp_inference(t.m_inference_params.as<uint16_t>(), d_pos.as<float>(), n_dims, n, d_out.as<uint16_t>(), "gridmlp_inference");
 				t.sync();
 				std::vector<uint16_t> h((size_t)n * stride);
 				d_out.copy_to_host(h.data(), h.size() * 2);

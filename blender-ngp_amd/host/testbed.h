@@ -380,9 +380,12 @@ public:
 	bool m_gated = false;
 	NgpGatedFfn m_gated_block{};
 	DeviceBuffer m_gated_ws, m_gated_dx;
+	DeviceBuffer m_gated_x, m_gated_enc_ws, m_gated_infer_ws;   // of inference, which leaves a training step's buffers alone
 	uint32_t gm_out_stride() const { return m_gated ? 16u : 4u; }
 	void gated_init_params();
-	void gridmlp_inference(const uint16_t* params, const float* pos, uint32_t n_dims, uint32_t n, uint16_t* out, uint16_t* x_saved, const char* who);
+	uint32_t gated_chunk() const;
+	void gated_forward(const uint16_t* params, const float* pos, uint32_t n_dims, uint32_t n, uint16_t* out, uint16_t* x, DeviceBuffer& enc_ws, DeviceBuffer& gated_ws, const char* who);
+	void gridmlp_inference(const uint16_t* params, const float* pos, uint32_t n_dims, uint32_t n, uint16_t* out, const char* who);
 	uint32_t gridmlp_n_dims() const { return m_testbed_mode == ETestbedMode::Image ? 2u : 3u; }
 	void gridmlp_training_step(const float* pos, uint32_t n_dims, const float* targets, uint32_t dims, uint32_t n, bool get_loss_scalar);
 	uint32_t m_n_matrix_params = NGP_MLP_N_PARAMS;     // parameters that get weight decay (the MLPs): 10240 NeRF (base family), 7168 grid -> MLP

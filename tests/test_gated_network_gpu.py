@@ -290,3 +290,37 @@ def test_configs_that_are_refused(cuda, tmp_path, change, words):
     tb.set_image_data(_image())
     with pytest.raises(RuntimeError, match=words):
         tb.reload_network_from_file(_config(tmp_path, "image/gated.json", **change))
+
+
+@pytest.mark.parametrize("width", [1024, 8192])
+def test_inference_of_a_wide_block_over_many_rows_takes_bounded_memory(ngp, cuda, tmp_path, width):
+    """rows go through the block in parts whose hidden rows take 1 GiB at most (524288 rows of 1024 neurons, 65536 of 8192): outputs on both sides of every cut, and a render, against 64 bits"""
+    import pyngp
+    tb = pyngp.Testbed(pyngp.TestbedMode.Image)
+    tb.set_image_data(_image())
+    tb.reload_network_from_file(_config(tmp_path, "image/gated.json", encoding=dict(log2_hashmap_size=12), network=dict(n_neurons=width)))
+    chunk = (1 << 29) // width
+    n = 4 * chunk + 777 if width == 8192 else 2 * chunk + 777
+    pos = positions(n, 2, 7)
+    host = pos.cpu().numpy()
+    torch.cuda.synchronize()
+    free = torch.cuda.mem_get_info()[0]
+    out = tb.gridmlp_inference(host)
+    kept = free - torch.cuda.mem_get_info()[0]
+    # the hidden rows of one part, its features and the encoder's workspace (64 bytes a row each, the workspace up to twice), and what the allocator rounds up to
+    assert kept <= (1 << 30) + chunk * 64 * 3 + (256 << 20), "%.2f GiB are kept" % (kept / 2 ** 30)
+    at = sorted({k for c in range(0, n, chunk) for k in range(max(0, c - 40), min(n, c + 40))} | set(range(n - 40, n)))
+    p = torch.from_numpy(tb.debug_params("inference").view(np.float16).copy()).cuda()
+    desc = make_desc(ngp, 2, 12, 16, float(np.exp(np.log(np.float32(48.0) / np.float32(16)) / np.float32(15))))
+    size = ngp.ngp_hip_nerf_encode_workspace_bytes(len(at))
+    ws, x, sub = torch.empty(size, dtype=torch.uint8, device="cuda"), torch.empty(len(at), 32, dtype=torch.float16, device="cuda"), pos[at].contiguous()
+    grid = p[80 * width:].clone()
+    capi.check(ngp.ngp_hip_grid_encode(None, 2, H.to_dev(desc, cuda).data_ptr(), grid.data_ptr(), sub.data_ptr(), 2, len(at), x.data_ptr(), ws.data_ptr(), size))
+    torch.cuda.synchronize()
+    ref = F.Block("silu", x, p[:32 * width].view(width, 32), p[32 * width:64 * width].view(width, 32), p[64 * width:80 * width].view(16, width))
+    F.check("inference", torch.from_numpy(out[at]).cuda(), ref.y[:, :4], ref.ey[:, :4])
+    assert np.isfinite(out).all()
+    tb.scale = 1.0
+    free = torch.cuda.mem_get_info()[0]
+    frame = tb.render(640, 512, 1, True)
+    assert np.isfinite(frame).all() and frame.std() > 0 and free - torch.cuda.mem_get_info()[0] <= 256 << 20
