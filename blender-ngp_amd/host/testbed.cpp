@@ -789,6 +789,10 @@ void Testbed::add_matrix(uint32_t rows, uint32_t cols) {   // behind the last on
 void Testbed::reset_network(bool clear_density_grid) {  // testbed.cu:2249-2470
 	join_side_ema();
 	if (m_testbed_mode != ETestbedMode::Nerf) { reset_network_gridmlp(); return; }
+	for (const char* which : {"network", "rgb_network"}) {   // the otypes of the reference's configs all name the fused kernels here; this one names another network
+		std::string otype = m_network_config.contains(which) ? m_network_config[which].value("otype", "FullyFusedMLP") : std::string("FullyFusedMLP"); std::transform(otype.begin(), otype.end(), otype.begin(), ::tolower);
+		if (otype == "gatedmlp") throw std::runtime_error{std::string("network config not supported by the gfx950 fused kernels: ") + which + ".otype GatedMLP is for the image and SDF modes"};
+	}
 	drop_prefetch();
 	if (m_live_count.bytes()) { m_live_count.memset(0, m_stream); m_live_parity = 0; m_live_last_batch = 0; }   // (a step that threw between the compaction and the backward pass may have left its counter behind)
 	++m_state_version;

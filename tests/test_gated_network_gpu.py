@@ -324,3 +324,17 @@ def test_inference_of_a_wide_block_over_many_rows_takes_bounded_memory(ngp, cuda
     free = torch.cuda.mem_get_info()[0]
     frame = tb.render(640, 512, 1, True)
     assert np.isfinite(frame).all() and frame.std() > 0 and free - torch.cuda.mem_get_info()[0] <= 256 << 20
+
+
+@pytest.mark.parametrize("which", ["network", "rgb_network"])
+@pytest.mark.parametrize("otype", ["GatedMLP", "gatedmlp"])
+def test_nerf_mode_refuses_the_gated_network(cuda, tmp_path, which, otype):
+    """it has no such network: the fused ReLU MLPs would train in its place.  A refusal leaves the Testbed usable."""
+    import scene
+    ds = scene.make_dataset(n_train=4, n_test=1, res=48, device=torch.device("cuda:0"))
+    tb = scene.build_testbed(ds)
+    with pytest.raises(RuntimeError, match=which + ".otype GatedMLP"):
+        tb.reload_network_from_file(_config(tmp_path, "nerf/base.json", **{which: dict(otype=otype, activation="SiLU")}))
+    tb.reload_network_from_file(_config(tmp_path, "nerf/base.json", **{which: dict(otype="CutlassMLP")}))
+    scene.train(tb, 1)
+    assert np.isfinite(tb.loss)
