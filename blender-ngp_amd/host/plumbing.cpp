@@ -22,39 +22,58 @@ static inline uint32_t next_multiple(uint32_t v, uint32_t m) { return (v + m - 1
 
 void Testbed::reset_network_gridmlp() {  // testbed.cu:2249-2470, Image / Sdf branch (2397-2445)
 	join_side_ema();
-	tuner_reset();
-	m_rng = Pcg32(m_seed);
-	m_windowless_render_surface.reset_accumulation();
 	const Json& config = m_network_config;
 	const Json empty = Json::object();
 	const Json& enc = config.contains("encoding") ? config["encoding"] : empty;
+	// what may be refused is read first: a refusal leaves the network, and what says how its parameters lie, as they were
 	auto require = [](bool ok, const std::string& what) { if (!ok) throw std::runtime_error{"network config not supported by the gfx950 fused kernels: " + what}; };
 	std::string enc_type = enc.value("otype", "HashGrid"); std::transform(enc_type.begin(), enc_type.end(), enc_type.begin(), ::tolower);
 	require(enc_type == "hashgrid", "encoding.otype must be HashGrid");
 	require((uint32_t)enc.value("n_features_per_level", 2) == 2 && (uint32_t)enc.value("n_levels", 16) == 16, "HashGrid must have 16 levels x 2 features");
 	std::string net_type = config.contains("network") ? config["network"].value("otype", "FullyFusedMLP") : std::string("FullyFusedMLP"); std::transform(net_type.begin(), net_type.end(), net_type.begin(), ::tolower);
-	m_gated = net_type == "gatedmlp";
-	if (m_gated) {
+	const bool gated = net_type == "gatedmlp";
+	NgpGatedFfn block{};
+	if (gated) {
 		const Json& net = config["network"];
 		const int width = (int)net.value("n_neurons", 64);
 		require(width >= 8 && width <= 65536 && width % 8 == 0, "GatedMLP: n_neurons must be a multiple of 8 up to 65536");
 		std::string act = net.value("activation", "SiLU"); std::transform(act.begin(), act.end(), act.begin(), ::tolower);
-		m_gated_block.activation = act == "silu" ? NGP_ACT_SILU : act == "gelu" ? NGP_ACT_GELU : act == "relu" ? NGP_ACT_RELU : act == "sigmoid" || act == "logistic" ? NGP_ACT_LOGISTIC : act == "none" ? NGP_ACT_NONE : -1;
-		require(m_gated_block.activation >= 0, "GatedMLP: activation must be SiLU, GELU, ReLU, Sigmoid or None");
+		block.activation = act == "silu" ? NGP_ACT_SILU : act == "gelu" ? NGP_ACT_GELU : act == "relu" ? NGP_ACT_RELU : act == "sigmoid" || act == "logistic" ? NGP_ACT_LOGISTIC : act == "none" ? NGP_ACT_NONE : -1;
+		require(block.activation >= 0, "GatedMLP: activation must be SiLU, GELU, ReLU, Sigmoid or None");
 		std::string out_act = net.value("output_activation", "None"); std::transform(out_act.begin(), out_act.end(), out_act.begin(), ::tolower);
 		require(out_act == "none", "GatedMLP: output_activation must be None");
-		m_gated_block.n_in = 32; m_gated_block.n_hidden = (uint32_t)width; m_gated_block.n_out = 16; m_gated_block.dtype = NGP_DTYPE_F16;
+		block.n_in = 32; block.n_hidden = (uint32_t)width; block.n_out = 16; block.dtype = NGP_DTYPE_F16;
 	} else if (config.contains("network")) require(config["network"].value("n_neurons", 64) == 64 && config["network"].value("n_hidden_layers", 2) == 2, "network must be 64 neurons x 2 hidden layers");
-	m_num_levels = 16;
+	std::string loss = config.contains("loss") ? config["loss"].value("otype", "L2") : std::string("L2");
+	std::transform(loss.begin(), loss.end(), loss.begin(), ::tolower);
+	ELossType loss_type;
+	if (loss == "l2") loss_type = ELossType::L2;
+	else if (loss == "relativel2") loss_type = ELossType::RelativeL2;
+	else if (loss == "l1") loss_type = ELossType::L1;
+	else if (loss == "mape") loss_type = ELossType::Mape;
+	else throw std::runtime_error{"loss '" + loss + "' is not implemented for the grid -> MLP configs (L2, RelativeL2, L1, MAPE are)"};
 	const uint32_t n_dims = gridmlp_n_dims();
 	const uint32_t log2_hashmap_size = (uint32_t)enc.value("log2_hashmap_size", 15);
-	m_base_grid_resolution = (uint32_t)enc.value("base_resolution", 0);
-	if (!m_base_grid_resolution) m_base_grid_resolution = 1u << (log2_hashmap_size / n_dims);
+	uint32_t base_resolution = (uint32_t)enc.value("base_resolution", 0);
+	if (!base_resolution) base_resolution = 1u << (log2_hashmap_size / n_dims);
 	float desired_resolution = 2048.0f;   // finest level over the unit cube (2315); Image: half the image resolution (2317)
 	if (m_testbed_mode == ETestbedMode::Image) desired_resolution = (float)std::max(m_image.resolution[0], m_image.resolution[1]) / 2.0f;
-	m_per_level_scale = (float)enc.value("per_level_scale", 0.0);
-	if (m_per_level_scale <= 0.0f) m_per_level_scale = std::exp(std::log(desired_resolution * 1.0f / (float)m_base_grid_resolution) / (float)(m_num_levels - 1));
-	check(ngp_hip_gridmlp_make_desc_host(n_dims, m_num_levels, log2_hashmap_size, m_base_grid_resolution, m_per_level_scale, &m_desc), "ngp_hip_gridmlp_make_desc_host");
+	float per_level_scale = (float)enc.value("per_level_scale", 0.0);
+	if (per_level_scale <= 0.0f) per_level_scale = std::exp(std::log(desired_resolution * 1.0f / (float)base_resolution) / 15.0f);
+	NgpNetDesc desc{};
+	check(ngp_hip_gridmlp_make_desc_host(n_dims, 16, log2_hashmap_size, base_resolution, per_level_scale, &desc), "ngp_hip_gridmlp_make_desc_host");
+	if (config.contains("optimizer")) parse_optimizer_config(config["optimizer"]);
+
+	tuner_reset();
+	m_rng = Pcg32(m_seed);
+	m_windowless_render_surface.reset_accumulation();
+	m_nerf.training.loss_type = loss_type;
+	m_gated = gated;
+	m_gated_block = block;
+	m_num_levels = 16;
+	m_base_grid_resolution = base_resolution;
+	m_per_level_scale = per_level_scale;
+	m_desc = desc;
 	m_n_params = ngp_hip_gridmlp_n_params_host(&m_desc);
 	m_n_matrix_params = NGP_GRIDMLP_N_PARAMS;
 	m_matrices.clear();
@@ -66,14 +85,6 @@ void Testbed::reset_network_gridmlp() {  // testbed.cu:2249-2470, Image / Sdf br
 	} else { add_matrix(64, 32); add_matrix(64, 64); add_matrix(16, 64); }
 	m_desc_gpu.resize(sizeof(NgpNetDesc));
 	m_desc_gpu.copy_from_host(&m_desc, sizeof(NgpNetDesc));
-	std::string loss = config.contains("loss") ? config["loss"].value("otype", "L2") : std::string("L2");
-	std::transform(loss.begin(), loss.end(), loss.begin(), ::tolower);
-	if (loss == "l2") m_nerf.training.loss_type = ELossType::L2;
-	else if (loss == "relativel2") m_nerf.training.loss_type = ELossType::RelativeL2;
-	else if (loss == "l1") m_nerf.training.loss_type = ELossType::L1;
-	else if (loss == "mape") m_nerf.training.loss_type = ELossType::Mape;
-	else throw std::runtime_error{"loss '" + loss + "' is not implemented for the grid -> MLP configs (L2, RelativeL2, L1, MAPE are)"};
-	if (config.contains("optimizer")) parse_optimizer_config(config["optimizer"]);
 	m_optimizer_step = 0;
 	m_params.resize(m_n_params * 2); m_inference_params.resize(m_n_params * 2); m_grads.resize(m_n_params * 2);
 	m_master.resize(m_n_params * 4); m_first_moments.resize(m_n_params * 4); m_second_moments.resize(m_n_params * 4); m_ema.resize(m_n_params * 4);

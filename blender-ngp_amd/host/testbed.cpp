@@ -701,8 +701,24 @@ static ELossType string_to_loss_type(std::string s) {  // testbed.cu:2220-2240
 	throw std::runtime_error{"Unknown loss type."};
 }
 
+static void check_optimizer_config(const Json& opt_in) {   // throws before anything of the optimizer has changed
+	for (const Json* o = &opt_in;; o = &o->at("nested")) {
+		const std::string otype = o->value("otype", "Adam");
+		std::string lower = otype; std::transform(lower.begin(), lower.end(), lower.begin(), ::tolower);
+		if (lower == "adam") return;
+		if (lower == "muon") {
+			const int it = (int)o->value("n_iterations", 5);
+			if (it < 1 || it > 32) throw std::runtime_error{"optimizer Muon: n_iterations must be 1 .. 32"};
+			if (!((float)o->value("epsilon", 1e-7) >= 0.0f)) throw std::runtime_error{"optimizer Muon: epsilon must not be negative"};
+		} else if (lower != "ema" && lower != "exponentialdecay")
+			throw std::runtime_error{"optimizer otype '" + otype + "' is not part of the NeRF hot path (Ema / ExponentialDecay / Muon / Adam are)"};
+		if (!o->contains("nested")) throw std::runtime_error{"optimizer '" + otype + "' needs a nested optimizer"};
+	}
+}
+
 void Testbed::parse_optimizer_config(const Json& opt_in) {
 	// configs/nerf/base.json:5-22: Ema{decay} o ExponentialDecay{decay_start, decay_interval, decay_base} o Adam{...}; any subset of the wrappers
+	check_optimizer_config(opt_in);
 	m_use_ema = false; m_has_decay = false;
 	m_muon = Muon();
 	m_ema_decay = 0.95f; m_decay_start = 0; m_decay_interval = 1; m_decay_end = 0; m_decay_base = 1.0f;
@@ -725,13 +741,8 @@ void Testbed::parse_optimizer_config(const Json& opt_in) {
 			m_muon.learning_rate = (float)o->value("learning_rate", 0.02); m_muon.momentum = (float)o->value("momentum", 0.95);
 			m_muon.weight_decay = (float)o->value("weight_decay", 0.0); m_muon.epsilon = (float)o->value("epsilon", 1e-7);
 			m_muon.nesterov = o->value("nesterov", true);
-			const int it = (int)o->value("n_iterations", 5);
-			if (it < 1 || it > 32) throw std::runtime_error{"optimizer Muon: n_iterations must be 1 .. 32"};
-			m_muon.n_iterations = (uint32_t)it;
-		} else {
-			throw std::runtime_error{"optimizer otype '" + otype + "' is not part of the NeRF hot path (Ema / ExponentialDecay / Muon / Adam are)"};
+			m_muon.n_iterations = (uint32_t)o->value("n_iterations", 5);
 		}
-		if (!o->contains("nested")) throw std::runtime_error{"optimizer '" + otype + "' needs a nested optimizer"};
 		o = &o->at("nested");
 	}
 	m_learning_rate = m_base_learning_rate;
@@ -840,6 +851,7 @@ void Testbed::reset_network(bool clear_density_grid) {  // testbed.cu:2249-2470
 		require(h == 0 || config["rgb_network"].value("n_neurons", 64) == 64, "rgb_network must be 64 neurons wide");
 		m_n_rgb_hidden_layers = (uint32_t)h;
 	}
+	if (config.contains("optimizer")) parse_optimizer_config(config["optimizer"]);   // the last of the config that may be refused: behind it the parameters' sizes change
 	// per-image extra dims (testbed.cu:2353-2357): the dataset decides
 	m_n_extra_dims = tr.dataset.n_extra_dims();
 	require(m_n_extra_dims <= 16, "at most 16 extra dims (n_extra_learnable_dims, or 3 light-direction dims)");
@@ -860,7 +872,6 @@ void Testbed::reset_network(bool clear_density_grid) {  // testbed.cu:2249-2470
 	m_desc_gpu.resize(sizeof(NgpNetDesc));
 	m_desc_gpu.copy_from_host(&m_desc, sizeof(NgpNetDesc));
 
-	if (config.contains("optimizer")) parse_optimizer_config(config["optimizer"]);
 	m_optimizer_step = 0;
 	tuner_reset();
 	m_dp_inference_stale = false;

@@ -338,3 +338,44 @@ def test_nerf_mode_refuses_the_gated_network(cuda, tmp_path, which, otype):
     tb.reload_network_from_file(_config(tmp_path, "nerf/base.json", **{which: dict(otype="CutlassMLP")}))
     scene.train(tb, 1)
     assert np.isfinite(tb.loss)
+
+
+MUON = {"otype": "Muon", "nested": {"otype": "Adam", "learning_rate": 1e-2}}
+
+
+@pytest.mark.parametrize("first", ["image/base.json", "image/gated.json"])
+def test_a_refused_config_leaves_the_network_as_it_was(ngp, cuda, tmp_path, first):
+    """the other network's kind, size and table must not be taken over with the parameters of this one"""
+    import pyngp
+    tb = pyngp.Testbed(pyngp.TestbedMode.Image)
+    tb.set_image_data(_image())
+    tb.reload_network_from_file(_config(tmp_path, first, encoding=dict(log2_hashmap_size=12), optimizer=MUON))
+    tb.shall_train = True
+    tb.train(1 << 10)
+    pos = positions(500, 2).cpu().numpy()
+    size, params, out = tb.n_params(), tb.debug_params("training").copy(), tb.gridmlp_inference(pos)
+    big = dict(log2_hashmap_size=20)
+    for name, change in (("image/gated.json", dict(network=dict(n_neurons=12))), ("image/gated.json", dict(network=dict(n_neurons=4096, activation="Tanh"))),
+                         ("image/gated.json", dict(network=dict(n_neurons=512), loss=dict(otype="Huber"), encoding=big)),
+                         ("image/gated.json", dict(network=dict(n_neurons=8), encoding=big, optimizer={**MUON, "n_iterations": 99})),
+                         ("image/gated.json", dict(encoding=big, optimizer={**MUON, "epsilon": -1.0})), ("image/gated.json", dict(encoding=dict(log2_hashmap_size=12, n_levels=8))),
+                         ("image/base.json", dict(network=dict(n_hidden_layers=3), encoding=big)), ("image/base.json", dict(encoding=big, optimizer={"otype": "Lookahead", "nested": {"otype": "Adam"}}))):
+        with pytest.raises(RuntimeError):
+            tb.reload_network_from_file(_config(tmp_path, name, **change))
+        assert tb.n_params() == size and np.array_equal(tb.debug_params("training"), params) and np.array_equal(tb.gridmlp_inference(pos), out)
+    tb.train(1 << 10)
+    assert np.isfinite(tb.loss) and not np.array_equal(tb.debug_params("training"), params)
+
+
+def test_a_refused_optimizer_leaves_the_nerf_networks_as_they_were(cuda, tmp_path):
+    import scene
+    ds = scene.make_dataset(n_train=4, n_test=1, res=48, device=torch.device("cuda:0"))
+    tb = scene.build_testbed(ds, _config(tmp_path, "nerf/muon.json", encoding=dict(log2_hashmap_size=14)))
+    scene.train(tb, 2)
+    size, params = tb.n_params(), tb.debug_params("training").copy()
+    for bad in ({**MUON, "n_iterations": 0}, {"otype": "Muon"}, {"otype": "Ema", "nested": {"otype": "Shampoo"}}):
+        with pytest.raises(RuntimeError):
+            tb.reload_network_from_file(_config(tmp_path, "nerf/base.json", encoding=dict(log2_hashmap_size=19), optimizer=bad))
+        assert tb.n_params() == size and np.array_equal(tb.debug_params("training"), params)
+    scene.train(tb, 4)
+    assert np.isfinite(tb.loss) and not np.array_equal(tb.debug_params("training"), params)
