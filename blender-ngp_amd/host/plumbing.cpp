@@ -37,6 +37,7 @@ void Testbed::reset_network_gridmlp() {  // testbed.cu:2249-2470, Image / Sdf br
 		const Json& net = config["network"];
 		const int width = (int)net.value("n_neurons", 64);
 		require(width >= 8 && width <= 65536 && width % 8 == 0, "GatedMLP: n_neurons must be a multiple of 8 up to 65536");
+		require(net.value("n_hidden_layers", 1) == 1, "GatedMLP: n_hidden_layers must be 1");
 		std::string act = net.value("activation", "SiLU"); std::transform(act.begin(), act.end(), act.begin(), ::tolower);
 		block.activation = act == "silu" ? NGP_ACT_SILU : act == "gelu" ? NGP_ACT_GELU : act == "relu" ? NGP_ACT_RELU : act == "sigmoid" || act == "logistic" ? NGP_ACT_LOGISTIC : act == "none" ? NGP_ACT_NONE : -1;
 		require(block.activation >= 0, "GatedMLP: activation must be SiLU, GELU, ReLU, Sigmoid or None");

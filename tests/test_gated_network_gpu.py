@@ -379,3 +379,14 @@ def test_a_refused_optimizer_leaves_the_nerf_networks_as_they_were(cuda, tmp_pat
         assert tb.n_params() == size and np.array_equal(tb.debug_params("training"), params)
     scene.train(tb, 4)
     assert np.isfinite(tb.loss) and not np.array_equal(tb.debug_params("training"), params)
+
+
+def test_a_gated_network_has_one_hidden_layer(cuda, tmp_path):
+    import pyngp
+    tb = pyngp.Testbed(pyngp.TestbedMode.Image)
+    tb.set_image_data(_image())
+    for n in (0, 2):
+        with pytest.raises(RuntimeError, match="n_hidden_layers"):
+            tb.reload_network_from_file(_config(tmp_path, "image/gated.json", network=dict(n_hidden_layers=n)))
+    tb.reload_network_from_file(_config(tmp_path, "image/gated.json", network=dict(n_hidden_layers=1)))
+    assert tb.n_mlp_params == 80 * 64
