@@ -8,7 +8,8 @@
 // Precision.  The quintic's slope at zero is 3.44: five iterations magnify what an early rounding does to a small singular value up to 480 times, so the products cannot run on
 // operands of 11 (fp16) or 8 bits.  fp32 matrix instructions would do at 1/16 of the fp16 rate; instead every matrix is kept as two fp16 halves, v = hi + lo with
 // hi = fp16(v) and lo = fp16(v - hi): 22 bits, and a product is three fp16 ones (hi hi + hi lo + lo hi, fp32 accumulation; lo lo is below the last bit kept).  Powers of two keep both
-// halves inside fp16's normal range: X is held as 2^15 X (|X_ij| <= 1.21, typically 1 / sqrt(n k)), A and B as 2^13 of themselves (spectral norms at most 1.5 and 3.5).
+// halves inside fp16's normal range: X is held as 2^15 X (|X_ij| <= 1.21, typically 1 / sqrt(n k)), A and B as 2^13 of themselves (spectral norms at most 1.5 and 3.5).  fp32 arithmetic
+// is as far from 64 bits: of the norm of X after 5 iterations, random 64 x 64 9e-7 here and 1.2e-6 there, 768 x 768 1.7e-6 and 2.8e-6, 768 x 768 of rank 1 1.4e-4 and 2.3e-4.
 // Layout of such a matrix: row-major, per 32 columns 32 hi values and 32 lo values: 128 bytes of a row are both halves of 32 k.
 //
 // X is kept transposed, [k][n], and only so: A = X X^T reads it with k as the rows (transposed LDS reads on both sides), X^T <- X^T B with B, which is symmetric, along rows.  One

@@ -274,3 +274,22 @@ def test_lists_around_what_one_launch_takes(ngp, cuda, count):
     """one batch, two and three; large matrices among small ones"""
     check_step(ngp, Vector([(600, 420) if i % 9 == 4 else (70 + i, 130 - i % 50) for i in range(count)], "bf16", gap=1), iterations=3)
     check_step(ngp, Vector([(390, 410)] * count, "f16", gap=0), iterations=2)
+
+
+@pytest.mark.parametrize("iterations", [5, 8, 10])
+@pytest.mark.parametrize("rank", [1, 3])
+@pytest.mark.parametrize("shape", [(64, 64), (150, 200), (40, 900), (768, 768)], ids=lambda s: "%dx%d" % s)
+def test_rounding_noise_in_directions_that_the_update_lacks(ngp, cuda, shape, rank, iterations):
+    """The stated bound, 2^-20 3.4445^n of the norm of X: what is stored of an X is off by 2^-22 of it, an iteration multiplies that by 3.4445 where the singular value is zero, every iteration
+    adds as much again (a factor of 1 / (1 - 1 / 3.4445) = 1.41 in all), X is at most 1.21 times its last norm in between: 1.7 units of 2^-22.  The rest of the four is for the sums in fp32."""
+    gen = torch.Generator(device="cuda").manual_seed(rank)
+    p, q = (torch.linalg.qr(torch.randn(s, rank, generator=gen, device="cuda", dtype=torch.float64))[0] for s in shape)
+    v = Vector([shape], "f32")
+    v.buf.zero_()
+    v.master.zero_()
+    v.of(v.grads, 0).copy_(p @ q.T)
+    _, want, x, _ = R.step(v.of(v.grads, 0), v.of(v.master, 0), v.of(v.buf, 0), 1.0, 0.0, 0.0, 0.0, 0, iterations, 1.0)
+    ws, n = v.workspace(ngp)
+    v.step(ngp, ws, n, lr=1.0, beta=0.0, eps=0.0, nesterov=0, iterations=iterations)
+    torch.cuda.synchronize()
+    assert (v.of(v.master, 0).double() - want).norm().item() <= 2.0 ** -20 * 3.4445 ** iterations * want.norm().item()
