@@ -503,6 +503,9 @@ int ngp_hip_muon_step(void* stream, uint32_t n_matrices, const NgpMuonMatrix* ma
  *   x [n_rows][n_in], y [n_rows][n_out] with a row stride in elements; w_gate, w_up [n_hidden][n_in] and w_down [n_out][n_hidden] row-major and contiguous, as every matrix
  *   of a parameter vector here.  All tensors are of `dtype` (F16 or BF16); products accumulate in fp32, the hidden row is rounded once, every output is rounded once.
  *   activation: NGP_ACT_NONE (bilinear), RELU, LOGISTIC, SILU or GELU (the exact one, with erf); applied to x Wg^T.
+ * Between two products the hidden row (and in the backward pass dg, du, the gradients of x Wg^T and x Wu^T) is of `dtype`, so outputs are off by about 1.45 times the rounding of the result
+ * alone.  F16: a hidden value or gradient beyond 65504 is infinite there, and its row's outputs are infinite or NaN, whatever would cancel; below 2^-14 they are kept to 2^-25, which a
+ * loss scale is for.  BF16 has the range of fp32.  g, u and every sum are fp32.
  * Widths 1 .. 2^20 and rows 0 .. 2^30 of any remainder.  Rows whose width, stride and base are multiples of 8 elements / 16 bytes are read in place; others cost one padded copy.
  * Nothing outside y, dx, the gradients and the workspace is written; bytes between rows of a strided output stay as they are.  Outputs must not overlap inputs or each other.
  * No atomics: the same inputs give the same bits.

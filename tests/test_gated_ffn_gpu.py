@@ -367,3 +367,30 @@ def test_two_streams_at_once_and_graphs_that_share_a_workspace(ngp, cuda, shape)
             graphs[i].replay()
         torch.cuda.synchronize()
         assert all(same(want[i], got[i]) for i in range(2))
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("shape", [(3, 32, 64, 16), (3, 256, 512, 128), (20, 256, 512, 128), (24, 9500, 4500, 40), (300, 256, 512, 128), (700, 2048, 4096, 256)], ids=lambda s: "x".join(map(str, s)))
+def test_the_range_of_the_hidden_row(ngp, cuda, shape, dtype):
+    """h = g u with g and u single products of powers of two: in f16 exact down to 2^-24 and up to 65504, infinite beyond and in its own row only; in bf16 far beyond that"""
+    rows, d, f, o = shape
+    t = TYPES[dtype][0]
+    x, wg, wu, wd = (torch.zeros(s, device="cuda", dtype=t) for s in ((rows, d), (f, d), (f, d), (o, f)))
+    wg[:, 0], wu[:, 1], wd[:, f - 1] = 1.0, 1.0, 2.0 ** -3
+    x[0, 0], x[0, 1] = 2.0 ** 8, 255.0 + 0.875 if dtype == "f16" else 255.0    # f16: 65504, the largest
+    x[1, 0], x[1, 1] = 2.0 ** -12, 3 * 2.0 ** -12                              # 3 steps of f16's smallest
+    x[2, 0], x[2, 1] = 2.0 ** 10, -2.0 ** 10                                   # 2^20: beyond f16, and y would not be
+    b = block(d, f, o, dtype, "none")
+    ws, n = workspace(ngp, b, rows, 0)
+    y = torch.full((rows, o), SENTINEL, device="cuda", dtype=t)
+    forward(ngp, b, x, wg, wu, wd, y, ws, n)
+    torch.cuda.synchronize()
+    h = x[:, 0].double() * x[:, 1].double()
+    want = (h / 8).to(t)   # exact in both types but for the smallest in f16: 3 2^-27 is rounded to nothing
+    assert torch.equal(y[3:], torch.zeros_like(y[3:])) and (y[0] == want[0]).all() and (y[1] == want[1]).all()
+    # f16: every hidden value of that row is minus infinity, and all weights of y but one are zero: a sum of infinity times zero is a NaN
+    assert not torch.isfinite(y[2]).any() if dtype == "f16" else (y[2] == want[2]).all()
+    wd[:, f - 1] = 2.0 ** 6   # what f16 holds of the small ones is all there
+    forward(ngp, b, x, wg, wu, wd, y, ws, n)
+    torch.cuda.synchronize()
+    assert (y[1] == 3 * 2.0 ** -18).all()
