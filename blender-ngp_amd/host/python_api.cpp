@@ -520,7 +520,7 @@ PYBIND11_MODULE(pyngp, m) {
 		.def("set_render_shard", &Testbed::set_render_shard, py::arg("rank"), py::arg("world_size"),
 			"render() traces only the rows of shard `rank` of `world_size` (rows [rank * ceil(H / world), ...)); the rest of the returned frame is background. With init_data_parallel the split and the gather happen inside render().")
 		.def("render_shard_rows", [](Testbed& t, int height) { int a, b; t.render_shard_rows(height, a, b); return py::make_tuple(a, b); }, py::arg("height"))
-		.def_property("dp_sharded_optimizer", [](Testbed& t) { return t.m_dp_sharded_optimizer; }, &Testbed::set_dp_sharded_optimizer, "data-parallel step: reduce-scatter (fp32 sums) -> Adam on this rank's 1 / world of the parameters -> all-gather of the fp16 weights (default); False: fp16 all-reduce of the gradients, the whole optimizer step on every rank.  Settable only while no communicator is live (before init_data_parallel)")
+		.def_property("dp_sharded_optimizer", [](Testbed& t) { return t.m_dp_sharded_optimizer; }, &Testbed::set_dp_sharded_optimizer, "data-parallel step: reduce-scatter (fp32 sums) -> Adam on this rank's 1 / world of the parameters -> all-gather of the fp16 weights (default); False: fp16 all-reduce of the gradients, the whole optimizer step on every rank.  With optimizer.otype Muon the step is the latter whatever is set here: an update needs its whole matrix, so nothing is stale and no gather is needed.  Settable only while no communicator is live (before init_data_parallel)")
 		.def_property("dp_sharded_ema", [](Testbed& t) { return t.m_dp_sharded_ema; }, &Testbed::set_dp_sharded_ema, "sharded data-parallel step: the Ema stage runs on this rank's shard only (one launch with Adam) and the fp16 inference weights are gathered on demand — render() gathers by itself when it is a collective (render_sharded), otherwise call dp_gather_inference_params() on all ranks before render() / save_snapshot().  False: Ema over all parameters on every rank (rounds 3-4).  Settable only while no communicator is live")
 		.def_readwrite("dp_fp16_wire", &Testbed::m_dp_fp16_wire, "sharded data-parallel step: gradients cross the wire as fp16 slices (point to point, ngp_rccl_alltoall_f16) and are summed by their owner in rank order in fp32 with one fp16 rounding; False: widen -> fp32 reduce-scatter -> narrow (twice the bytes).  Set it alike on every rank, between two steps")
 		.def("dp_gather_inference_params", &Testbed::dp_gather_inference_params, py::call_guard<py::gil_scoped_release>(), "COLLECTIVE (every rank): all-gather of the fp16 inference (Ema) weights that sharded-Ema steps keep current only inside each rank's shard")
