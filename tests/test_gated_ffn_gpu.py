@@ -394,3 +394,43 @@ def test_the_range_of_the_hidden_row(ngp, cuda, shape, dtype):
     forward(ngp, b, x, wg, wu, wd, y, ws, n)
     torch.cuda.synchronize()
     assert (y[1] == 3 * 2.0 ** -18).all()
+
+
+@pytest.mark.parametrize("bad_value", [float("nan"), float("inf")], ids=["nan", "inf"])
+@pytest.mark.parametrize("shape", [(2, 256, 512, 128), (5, 256, 512, 128), (12, 256, 512, 128), (24, 9500, 4500, 40), (50, 9500, 4500, 40), (33, 2001, 8011, 131), (70, 300, 500, 200)], ids=lambda s: "x".join(map(str, s)))
+def test_non_finite_rows_among_few(ngp, cuda, shape, bad_value):
+    """the streaming kernels, rows packed and not (their packed rows behind the last are never written), and the tiles behind them; the first row, a middle one, the last"""
+    rows, d, f, o = shape
+    b = block(d, f, o, "f16", "silu")
+    x, wg, wu, wd, _ = inputs(rows, d, f, o, "f16", seed=7)
+    ws, n = workspace(ngp, b, rows, 0)
+    y0, y1 = (torch.empty(rows, o, dtype=x.dtype, device="cuda") for _ in range(2))
+    forward(ngp, b, x, wg, wu, wd, y0, ws, n)
+    for bad in {0, rows // 2, rows - 1}:
+        x1 = x.clone()
+        x1[bad, 3] = bad_value
+        ws.fill_(0xff)
+        forward(ngp, b, x1, wg, wu, wd, y1, ws, n)
+        torch.cuda.synchronize()
+        keep = torch.arange(rows, device="cuda") != bad
+        assert not torch.isfinite(y1[bad]).any() and torch.equal(y0[keep], y1[keep]) and torch.isfinite(y0).all()
+
+
+@pytest.mark.parametrize("shape", [(40, 32, 64, 16), (5, 256, 512, 128), (70, 300, 500, 200), (700, 264, 520, 136)], ids=lambda s: "x".join(map(str, s)))
+def test_a_non_finite_row_of_the_backward_pass_stays_in_its_row_of_dx(ngp, cuda, shape):
+    """the weights' gradients are sums over the rows: all of them have it"""
+    rows, d, f, o = shape
+    b = block(d, f, o, "bf16", "gelu")
+    x, wg, wu, wd, dy = inputs(rows, d, f, o, "bf16", seed=8)
+    ws, n = workspace(ngp, b, rows, capi.FFN_BACKWARD)
+    runs = [[torch.empty_like(t) for t in (x, wg, wu, wd)] for _ in range(2)]
+    backward(ngp, b, x, wg, wu, wd, dy, runs[0][0], runs[0][1:], ws, n)
+    bad = rows // 2
+    dy[bad, 1] = float("nan")
+    backward(ngp, b, x, wg, wu, wd, dy, runs[1][0], runs[1][1:], ws, n)
+    torch.cuda.synchronize()
+    keep = torch.arange(rows, device="cuda") != bad
+    assert torch.isnan(runs[1][0][bad]).all() and torch.equal(runs[0][0][keep], runs[1][0][keep])
+    assert torch.isnan(runs[1][1]).all() and torch.isnan(runs[1][2]).all()
+    other = torch.arange(o, device="cuda") != 1
+    assert torch.isnan(runs[1][3][1]).all() and torch.equal(runs[0][3][other], runs[1][3][other])   # dw_down: the row of that output alone

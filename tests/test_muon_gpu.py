@@ -293,3 +293,66 @@ def test_rounding_noise_in_directions_that_the_update_lacks(ngp, cuda, shape, ra
     v.step(ngp, ws, n, lr=1.0, beta=0.0, eps=0.0, nesterov=0, iterations=iterations)
     torch.cuda.synchronize()
     assert (v.of(v.master, 0).double() - want).norm().item() <= 2.0 ** -20 * 3.4445 ** iterations * want.norm().item()
+
+
+SLABS = [(40, 900), (3000, 24), (64, 8192)]   # a short side up to 64: a launch to an iteration, its own code for the norm
+
+
+@pytest.mark.parametrize("shape", SLABS, ids=lambda s: "%dx%d" % s)
+def test_zero_update_in_slabs(ngp, cuda, shape):
+    v = Vector([shape], "f16")
+    v.grads.zero_()
+    v.buf.zero_()
+    before = v.master.clone()
+    for eps in (1e-7, 0.0):
+        ws, n = v.workspace(ngp)
+        v.step(ngp, ws, n, decay=0.0, eps=eps)
+        torch.cuda.synchronize()
+        assert torch.equal(v.master, before) and (v.of(v.buf, 0) == 0).all()
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf")], ids=["nan", "inf"])
+def test_a_gradient_that_is_not_finite_stays_in_its_matrix_of_slabs(ngp, cuda, value):
+    shapes = SLABS + [(40, 64), (150, 140)]
+    for bad in range(len(shapes)):
+        v, w = Vector(shapes, "f16", seed=1), Vector(shapes, "f16", seed=1)
+        v.of(v.grads, bad)[-1, -1] = value
+        for t in (v, w):
+            ws, n = t.workspace(ngp)
+            t.step(ngp, ws, n)
+        torch.cuda.synchronize()
+        assert not torch.isfinite(v.of(v.master, bad)).any()
+        for i in range(len(shapes)):
+            if i != bad:
+                assert torch.equal(v.of(v.master, i), w.of(w.master, i))
+
+
+@pytest.mark.parametrize("shape", SLABS, ids=lambda s: "%dx%d" % s)
+@pytest.mark.parametrize("scale", [1e-30, 1e-9, 1.0, 1e30])
+def test_magnitudes_of_single_precision_in_slabs(ngp, cuda, shape, scale):
+    v = Vector([shape], "f32", seed=2, scale=scale)
+    v.master.zero_()
+    check_step(ngp, v, lr=1.0, decay=0.0, eps=0.0 if scale == 1e-30 else 1e-7)
+
+
+@pytest.mark.parametrize("shape", SLABS, ids=lambda s: "%dx%d" % s)
+@pytest.mark.parametrize("power", [0.0, 1.0, 3.0])
+def test_low_rank_and_spread_spectra_in_slabs(ngp, cuda, shape, power):
+    """singular values i^-power; power 0: rank 3"""
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    n = min(shape)
+    p, q = (torch.linalg.qr(torch.randn(s, n, generator=gen, device="cuda", dtype=torch.float64))[0] for s in shape)
+    s = torch.arange(1, n + 1, device="cuda", dtype=torch.float64) ** -power if power else (torch.arange(n, device="cuda") < 3).double()
+    v = Vector([shape], "f32")
+    v.buf.zero_()
+    v.master.zero_()
+    v.of(v.grads, 0).copy_((p * s) @ q.T)
+    check_step(ngp, v, lr=1.0, decay=0.0, nesterov=0)
+
+
+@pytest.mark.parametrize("shape", SLABS, ids=lambda s: "%dx%d" % s)
+@pytest.mark.parametrize("iterations", [1, 2, 6])
+def test_iterations_in_slabs(ngp, cuda, shape, iterations):
+    v = Vector([shape], "f32", seed=iterations)
+    v.master.zero_()
+    check_step(ngp, v, lr=1.0, decay=0.0, iterations=iterations)
