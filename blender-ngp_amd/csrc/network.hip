@@ -2865,7 +2865,7 @@ int ngp_hip_grid_backward_unordered(void* stream, uint32_t n_dims, const NgpNetD
 }
 
 // ---- the encoding alone, in rows of 32 features: what a network that is not one of the fused kernels reads and sends gradients back to.  The encoder and the hash-grid backward work
-// on level planes [16][n] x 2 features; these two turn 32 samples x 16 levels through LDS (64 bytes a row on one side, 128 a plane on the other: bound by memory).
+// on level planes [16][n] x 2 features; these two turn 64 samples x 16 levels through LDS (64 bytes a row on one side, 256 a plane on the other: bound by memory).
 __global__ void __launch_bounds__(256) planes_to_rows_kernel(const uint32_t* __restrict__ planes, uint32_t n_pad, uint32_t n, uint32_t* __restrict__ rows) {
 	__shared__ uint32_t t[64][17];
 	const uint32_t s0 = blockIdx.x * 64;

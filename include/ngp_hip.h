@@ -490,7 +490,8 @@ int ngp_hip_grid_gradient(void* stream, uint32_t n_dims, const NgpNetDesc* desc_
  * read or written: the encoding behind the matrices belongs to Adam).  dtype: of grads and params (F16, BF16; F32: grads alone, params NULL); params may be NULL.
  * Products run on pairs of fp16 halves (22 bits) with fp32 sums, norms in 64 bits.  X agrees with 64-bit arithmetic to a few 1e-6 of its norm where the update has full rank.  In the
  * directions that it lacks, or has below 1e-6 of its norm, rounding noise grows by 3.4445 an iteration, in this arithmetic as in fp32: at most 2^-20 3.4445^n_iterations of the norm of X
- * (rank 1, 768 x 768: 1.4e-4 at 5 iterations, 4e-2 at 10), and from about 13 iterations on those directions are as large as the others.  No atomics: the same inputs give the
+ * (rank 1, 768 x 768: 1.4e-4 at 5 iterations, 4e-2 at 10), and from about 13 iterations on those directions are as large as the others.  An entry of X is held to 2^-40,
+ * which counts where |u|_F is below 1e-3 of epsilon, and X as small.  No atomics: the same inputs give the
  * same bits (of the same list: the split of the sums depends on the matrices beside).  A gradient that is not finite makes its matrix not finite, no other.  A zero update leaves X = 0.
  * Enqueues only (capturable: matrices_host is read during the call); two calls that may overlap need workspaces of their own. */
 typedef struct { uint64_t offset; uint32_t rows, cols; } NgpMuonMatrix;   /* offset in elements from the start of the vectors; rows, cols 1 .. 65536 */

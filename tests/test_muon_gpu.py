@@ -356,3 +356,20 @@ def test_iterations_in_slabs(ngp, cuda, shape, iterations):
     v = Vector([shape], "f32", seed=iterations)
     v.master.zero_()
     check_step(ngp, v, lr=1.0, decay=0.0, iterations=iterations)
+
+
+@pytest.mark.parametrize("shape", [(48, 64), (40, 900), (260, 140), (768, 768)], ids=lambda s: "%dx%d" % s)
+@pytest.mark.parametrize("below", [1e-3, 1e-6, 1e-9])
+def test_updates_far_below_epsilon(ngp, cuda, shape, below):
+    """X is then as small, and its entries are held to 2^-40: half a step of the smallest fp16 over 2^15, which the iterations multiply by 3.4445 each and, new in every one, sum to 1.41 of that"""
+    v = Vector([shape], "f32", seed=9)
+    v.buf.zero_()
+    v.master.zero_()
+    u = v.of(v.grads, 0)
+    u.mul_(below * 1e-3 / u.norm())
+    _, want, _, _ = R.step(u, v.of(v.master, 0), v.of(v.buf, 0), 1.0, 0.0, 0.0, 1e-3, 0, 5, 1.0)
+    ws, n = v.workspace(ngp)
+    v.step(ngp, ws, n, lr=1.0, beta=0.0, eps=1e-3, nesterov=0)
+    torch.cuda.synchronize()
+    rate, grown = max(1.0, shape[0] / shape[1]) ** 0.5, 3.4445 ** 5
+    assert (v.of(v.master, 0).double() - want).norm().item() <= 1.41 * 2.0 ** -40 * (shape[0] * shape[1]) ** 0.5 * grown * rate + 2.0 ** -20 * want.norm().item()
