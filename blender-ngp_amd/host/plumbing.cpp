@@ -138,6 +138,17 @@ void Testbed::gridmlp_inference(const uint16_t* params, const float* pos, uint32
 		gated_forward(params, pos + (size_t)first * n_dims, n_dims, std::min(chunk, n - first), out + (size_t)first * gm_out_stride(), m_gated_x.as<uint16_t>(), m_gated_enc_ws, m_gated_infer_ws, who);
 }
 
+// What the loss is multiplied by, so that F16 holds the gradients: 128 as everywhere, per sample 1 / n of it.  A gated network needs more of it for a large batch: its features start
+// within 1e-4 and a gate's gradient is a product with another of them, 1e-9 of a batch of 2^18 and so zero in F16 (the smallest is 6e-8): the image config stood at 3.03 dB for 1000
+// steps, with 1024 or more it reaches 35 to 36.  From 2^14 samples on a sample's share stays what it is there, up to 2^20 (the weights' gradients, sums over the batch, grow with the
+// scale: 8192 leaves them 8).  Not for the relative losses: their gradients are up to 100 times as large, and SDF samples lie where they are.
+float Testbed::gridmlp_loss_scale(uint32_t n) const {
+	float scale = LOSS_SCALE;
+	if (!m_gated || (m_nerf.training.loss_type != ELossType::L2 && m_nerf.training.loss_type != ELossType::L1)) return scale;
+	for (uint32_t k = n >> 15; k && scale < 64.0f * LOSS_SCALE; k >>= 1) scale *= 2.0f;
+	return scale;
+}
+
 // Trainer::training_step (forward, loss, backward) + optimizer_step(128) + Trainer::loss (sum of the per-element values)
 void Testbed::gridmlp_training_step(const float* pos, uint32_t n_dims, const float* targets, uint32_t dims, uint32_t n, bool get_loss_scalar) {
 	if (n % 256) throw std::runtime_error{"training batch size must be a multiple of 256"};
@@ -160,7 +171,8 @@ void Testbed::gridmlp_training_step(const float* pos, uint32_t n_dims, const flo
 	}
 	if (!m_gated) tuner_done(m_stream);
 	profile_end(PK_FORWARD, n);
-	check(ngp_hip_loss_and_gradient(m_stream, (int)m_nerf.training.loss_type, n, dims, LOSS_SCALE, m_gm_out.as<uint16_t>(), gm_out_stride(), targets, m_gm_values.as<float>(), m_dloss.as<uint16_t>(),
+	m_gridmlp_loss_scale = gridmlp_loss_scale(n);
+	check(ngp_hip_loss_and_gradient(m_stream, (int)m_nerf.training.loss_type, n, dims, m_gridmlp_loss_scale, m_gm_out.as<uint16_t>(), gm_out_stride(), targets, m_gm_values.as<float>(), m_dloss.as<uint16_t>(),
 	                                gm_out_stride()), "loss_and_gradient");
 	profile_begin(PK_BACKWARD);
 	if (m_gated) {
@@ -182,7 +194,7 @@ void Testbed::gridmlp_training_step(const float* pos, uint32_t n_dims, const flo
 		sync();
 		m_loss_scalar_gpu.copy_to_host(&m_loss_scalar, 4);
 	}
-	optimizer_step();
+	optimizer_step(m_gridmlp_loss_scale);
 	++m_training_step;
 }
 

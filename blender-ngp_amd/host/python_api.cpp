@@ -572,6 +572,7 @@ PYBIND11_MODULE(pyngp, m) {
 		.def_readonly("grid_prefetch_hits", &Testbed::m_grid_prefetch_hits)
 		.def("training_prep_nerf", &Testbed::training_prep_nerf, py::call_guard<py::gil_scoped_release>(), py::arg("batch_size") = 0)
 		.def("local_loss_sum", &Testbed::local_loss_sum)
+		.def_property_readonly("gridmlp_loss_scale", [](Testbed& t) { return t.m_gridmlp_loss_scale; }, "image / SDF modes: what the gradients of the last step (gradients_ptr) are multiplied by")
 		.def("gradients_ptr", [](Testbed& t) { return (uintptr_t)t.gradients(); })
 		.def("params_ptr", [](Testbed& t) { return (uintptr_t)t.m_params.data(); })
 		.def("sync", &Testbed::sync)

@@ -1778,7 +1778,7 @@ void Testbed::require_inference_params(const char* who, bool collective) {
 	throw std::runtime_error{std::string(who) + ": the inference (Ema) weights are sharded over the data-parallel ranks (dp_sharded_ema) and stale outside this rank's shard — call dp_gather_inference_params() on ALL ranks first (a collective), or set render_sharded on every rank so that render() is a collective and gathers by itself"};
 }
 
-void Testbed::optimizer_step() {  // Trainer::optimizer_step(stream, LOSS_SCALE) (testbed_nerf.cu:2950)
+void Testbed::optimizer_step(float loss_scale) {  // Trainer::optimizer_step(stream, LOSS_SCALE) (testbed_nerf.cu:2950)
 	if (m_dp_comm && dp_sharded_step()) { optimizer_step_sharded(); return; }
 	if (m_dp_state_stale) throw std::runtime_error{"optimizer step on fp32 state that sharded data-parallel steps left stale outside this rank's shard: call dp_gather_optimizer_state() on all ranks before shutdown_data_parallel()"};
 	++m_optimizer_step;
@@ -1789,7 +1789,7 @@ void Testbed::optimizer_step() {  // Trainer::optimizer_step(stream, LOSS_SCALE)
 		const uint32_t n = (uint32_t)m_matrices.size();
 		m_muon_workspace.enlarge(std::max<uint64_t>(16, ngp_hip_muon_workspace_bytes(n, m_matrices.data())));
 		check(ngp_hip_muon_step(m_stream, n, m_matrices.data(), m_muon.learning_rate * (m_base_learning_rate > 0.0f ? m_learning_rate / m_base_learning_rate : 1.0f), m_muon.momentum, m_muon.weight_decay,
-		                        m_muon.epsilon, m_muon.nesterov, m_muon.n_iterations, LOSS_SCALE, NGP_DTYPE_F16, m_grads.as<uint16_t>(), m_master.as<float>(), m_params.as<uint16_t>(),
+		                        m_muon.epsilon, m_muon.nesterov, m_muon.n_iterations, loss_scale, NGP_DTYPE_F16, m_grads.as<uint16_t>(), m_master.as<float>(), m_params.as<uint16_t>(),
 		                        m_first_moments.as<float>(), m_muon_workspace.data(), m_muon_workspace.bytes()), "muon_step");
 		mask &= ~1u;
 	}
@@ -1802,12 +1802,12 @@ void Testbed::optimizer_step() {  // Trainer::optimizer_step(stream, LOSS_SCALE)
 	profile_begin(PK_OPTIMIZER);
 	if (side_ema) {
 		join_side_ema();   // the previous Ema stage read the weights this Adam stage overwrites
-		check(ngp_hip_optimizer_step(m_stream, (uint32_t)m_n_params, m_n_matrix_params, m_optimizer_step, m_learning_rate, m_beta1, m_beta2, m_epsilon, m_l2_reg, LOSS_SCALE, ema_decay,
+		check(ngp_hip_optimizer_step(m_stream, (uint32_t)m_n_params, m_n_matrix_params, m_optimizer_step, m_learning_rate, m_beta1, m_beta2, m_epsilon, m_l2_reg, loss_scale, ema_decay,
 		                                    m_grads.as<uint16_t>(), m_master.as<float>(), m_params.as<uint16_t>(), m_first_moments.as<float>(), m_second_moments.as<float>(), nullptr, nullptr,
 		                                    mask | NGP_OPT_NO_EMA), "optimizer_step (Adam stage)");
 	} else {
 		join_side_ema();
-		check(ngp_hip_optimizer_step(m_stream, (uint32_t)m_n_params, m_n_matrix_params, m_optimizer_step, m_learning_rate, m_beta1, m_beta2, m_epsilon, m_l2_reg, LOSS_SCALE, ema_decay,
+		check(ngp_hip_optimizer_step(m_stream, (uint32_t)m_n_params, m_n_matrix_params, m_optimizer_step, m_learning_rate, m_beta1, m_beta2, m_epsilon, m_l2_reg, loss_scale, ema_decay,
 		                                    m_grads.as<uint16_t>(), m_master.as<float>(), m_params.as<uint16_t>(), m_first_moments.as<float>(), m_second_moments.as<float>(), m_ema.as<float>(),
 		                                    m_inference_params.as<uint16_t>(), mask), "optimizer_step");
 	}
@@ -1817,7 +1817,7 @@ void Testbed::optimizer_step() {  // Trainer::optimizer_step(stream, LOSS_SCALE)
 		if (!m_ema_event) { hipEvent_t e; HIP_CHECK_THROW(hipEventCreateWithFlags(&e, STEP_EVENT_FLAGS)); m_ema_event = e; }
 		HIP_CHECK_THROW(hipEventRecord((hipEvent_t)m_adam_event, (hipStream_t)m_stream));
 		HIP_CHECK_THROW(hipStreamWaitEvent((hipStream_t)m_stream_b, (hipEvent_t)m_adam_event, 0));
-		check(ngp_hip_optimizer_step(m_stream_b, (uint32_t)m_n_params, m_n_matrix_params, m_optimizer_step, m_learning_rate, m_beta1, m_beta2, m_epsilon, m_l2_reg, LOSS_SCALE, ema_decay, nullptr, nullptr,
+		check(ngp_hip_optimizer_step(m_stream_b, (uint32_t)m_n_params, m_n_matrix_params, m_optimizer_step, m_learning_rate, m_beta1, m_beta2, m_epsilon, m_l2_reg, loss_scale, ema_decay, nullptr, nullptr,
 		                                    m_params.as<uint16_t>(), nullptr, nullptr, m_ema.as<float>(), m_inference_params.as<uint16_t>(), NGP_OPT_EMA_ONLY), "optimizer_step (Ema stage, stream B)");
 		std::lock_guard<std::mutex> lock(m_ema_mutex);
 		HIP_CHECK_THROW(hipEventRecord((hipEvent_t)m_ema_event, (hipStream_t)m_stream_b));
@@ -1831,7 +1831,7 @@ void Testbed::optimizer_step() {  // Trainer::optimizer_step(stream, LOSS_SCALE)
 
 void Testbed::train_nerf_dp_end() {
 	NerfTraining& tr = m_nerf.training;
-	optimizer_step();
+	optimizer_step(LOSS_SCALE);
 	++m_training_step;
 	if (tr.train_envmap && m_envmap.n_params() > 0) {   // 2954-2956
 		if (m_dp_comm) check(ngp_rccl_allreduce_f32(m_dp_comm, m_stream, m_envmap.gradients.as<float>(), m_envmap.n_params()), "ngp_rccl_allreduce_f32 (envmap gradients)");

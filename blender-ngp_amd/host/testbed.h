@@ -383,6 +383,8 @@ public:
 	DeviceBuffer m_gated_x, m_gated_enc_ws, m_gated_infer_ws;   // of inference, which leaves a training step's buffers alone
 	uint32_t gm_out_stride() const { return m_gated ? 16u : 4u; }
 	void gated_init_params();
+	float gridmlp_loss_scale(uint32_t n) const;
+	float m_gridmlp_loss_scale = 128.0f;     // of the last step: what its gradients are multiplied by
 	uint32_t gated_chunk() const;
 	void gated_forward(const uint16_t* params, const float* pos, uint32_t n_dims, uint32_t n, uint16_t* out, uint16_t* x, DeviceBuffer& enc_ws, DeviceBuffer& gated_ws, const char* who);
 	void gridmlp_inference(const uint16_t* params, const float* pos, uint32_t n_dims, uint32_t n, uint16_t* out, const char* who);
@@ -682,7 +684,7 @@ private:
 	std::vector<void*> m_prof_event_pool;
 	void* prof_event();
 	void check(int rc, const char* what);
-	void optimizer_step();
+	void optimizer_step(float loss_scale);
 	void update_after_training(uint32_t target_batch_size, uint32_t counter, uint32_t compacted_counter, bool get_loss_scalar, float loss_sum);
 	void parse_optimizer_config(const Json& opt);
 };

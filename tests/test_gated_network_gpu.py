@@ -390,3 +390,64 @@ def test_a_gated_network_has_one_hidden_layer(cuda, tmp_path):
             tb.reload_network_from_file(_config(tmp_path, "image/gated.json", network=dict(n_hidden_layers=n)))
     tb.reload_network_from_file(_config(tmp_path, "image/gated.json", network=dict(n_hidden_layers=1)))
     assert tb.n_mlp_params == 80 * 64
+
+
+@pytest.mark.parametrize("loss", ["L2", "L1"])
+def test_a_large_batch_leaves_the_gated_network_its_first_gradients(cuda, tmp_path, loss):
+    """features start within 1e-4, so the first gradients behind a gate are products of two small numbers, divided by the batch: of 2^16 samples and more F16 held none of them at a loss
+    scale of 128.  From 2^14 on a sample's share of the scaled loss is the same, and more samples meet every entry of the table: no fewer of its gradients are there."""
+    import pyngp
+
+    def first_gradients(name, n):
+        tb = pyngp.Testbed(pyngp.TestbedMode.Image)
+        tb.set_image_data(_image())
+        tb.reload_network_from_file(_config(tmp_path, name, encoding=dict(log2_hashmap_size=14), loss=dict(otype=loss)))
+        tb.shall_train = True
+        tb.train(n)
+        tb.sync()
+        g = view(tb.gradients_ptr(), tb.n_params())
+        assert torch.isfinite(g).all()
+        return (g[tb.n_mlp_params:] != 0).double().mean().item(), tb.gridmlp_loss_scale
+
+    at_2_14, scale = first_gradients("image/gated.json", 1 << 14)
+    assert at_2_14 > 0 and scale == 128
+    for k, want in ((12, 128), (15, 256), (16, 512), (18, 2048), (20, 8192)):
+        got, scale = first_gradients("image/gated.json", 1 << k)
+        assert scale == want and (k < 14 or got >= 0.9 * at_2_14), (k, got, at_2_14, scale)
+    assert first_gradients("image/gated.json", 3 << 14)[1] == 256 and first_gradients("image/gated.json", 1 << 21)[1] == 8192
+    assert first_gradients("image/base.json", 1 << 18)[1] == 128
+
+
+def test_the_loss_scale_of_relative_losses_and_of_the_optimizers(cuda, tmp_path):
+    """MAPE, whose gradients are up to 100 times as large, keeps 128; and the scale is taken out again: Muon's update of the matrices is that of the unscaled gradient and momentum"""
+    import pyngp
+    pts = np.random.RandomState(0).rand(1 << 16, 3).astype(np.float32)
+    tb = pyngp.Testbed(pyngp.TestbedMode.Sdf)
+    tb.override_sdf_training_data(pts, (np.linalg.norm(pts - 0.5, axis=1) - 0.3).astype(np.float32))
+    tb.reload_network_from_file(_config(tmp_path, "sdf/gated.json", encoding=dict(log2_hashmap_size=12)))
+    tb.shall_train = True
+    tb.train(1 << 16)
+    assert tb.gridmlp_loss_scale == 128
+    im = pyngp.Testbed(pyngp.TestbedMode.Image)
+    im.set_image_data(_image())
+    im.reload_network_from_file(_config(tmp_path, "image/gated.json", encoding=dict(log2_hashmap_size=12)))
+    im.shall_train = True
+    momentum = torch.zeros(80 * 64, dtype=torch.float64, device="cuda")
+    for step in range(12):   # batches of both scales in turn: momentum from each, the update from both
+        n, scale = ((1 << 12, 128), (1 << 16, 512))[step % 2]
+        before = torch.from_numpy(im.debug_params("training").view(np.float16).copy()).cuda()
+        im.train(n)
+        im.sync()
+        assert im.gridmlp_loss_scale == scale
+        after = torch.from_numpy(im.debug_params("training").view(np.float16).copy()).cuda()
+        g = view(im.gradients_ptr(), im.n_params())[:80 * 64].double() / scale
+        momentum = 0.95 * momentum + g
+        at = 0
+        for r, c in ((64, 32), (64, 32), (16, 64)):
+            p0, p1, u = (t[at:at + r * c].double().view(r, c) for t in (before, after, g + 0.95 * momentum))
+            at += r * c
+            rate = 1e-2 * max(1.0, r / c) ** 0.5
+            # both weights are the master's rounded to fp16, half a step each; X within 2^-20 3.4445^5 of its norm, at most 1.21 a direction
+            limit = 2.0 ** -11 * (p0.abs() + p1.abs()) + 2.0 ** -24 + rate * 2.0 ** -20 * 3.4445 ** 5 * 1.21 * min(r, c) ** 0.5
+            assert ((p0 - p1 - rate * M.orthogonalise(u, 1e-7, 5)).abs() <= limit).all(), (step, r, c)
+    assert momentum.abs().sum() > 0
