@@ -8,10 +8,10 @@
 //   KC   [rows][k], k contiguous:     LDS [row][k], a fragment (lane: one row, 8 k) is one ds_read_b128;
 //   RC   [k][rows], rows contiguous:  LDS [k][row], a fragment is two ds_read_b64_tr_b16 (the LDS unit transposes 4 x 16 blocks on the way out).
 // Bank conflicts: the DMA writes LDS linearly, so the 16-byte chunks of a row are permuted by which chunk each lane ASKS for, chunk ^ swizzle(row): for KC such that 16 rows of
-// one chunk column cover every bank once, for RC such that the four k rows of a transposed block and its neighbour fall on different 32-byte units.  (The KC order that repeats
-// every 8 rows instead cost half of the LDS cycles in conflicts.)
-// What bounds it.  The matrix pipes and, below them, power: at 8192 x 4096 x 8192 the clock falls to about 1.7 GHz and a product of that size runs at 1.3 PFLOP/s (y of the gated block,
-// 0.42 ms), where the library's runs at 1.25 to 1.55 by layout and type.  Three things keep the pipes fed: fragments are read half a step
+// one chunk column cover every bank once, for RC such that the four k rows of a transposed block and its neighbour fall on different 32-byte units.  Measured: no conflicts for rows of
+// 128 bytes (the Muon step's), a tenth of the LDS cycles for RC; but half of them for KC rows of 64 bytes (28 % of the CU's cycles at 8192 x 4096 - 8192, behind the MFMAs).
+// What bounds it.  The matrix pipes and, below them, power: at 8192 x 4096 x 8192 the clock falls to 1.4 GHz (1.6 to 1.8 in the Muon step's products), the pipes are busy for three
+// quarters of it and a product of that size runs at 1.3 PFLOP/s (y of the gated block, 0.42 ms), where the library's runs at 1.25 to 1.55 by layout and type.  Three things keep the pipes fed: fragments are read half a step
 // ahead of the MFMAs that take them; the DMA instructions stand between MFMAs, two to a half step (eight in a row block the wave's issue, and with it its MFMAs, until the memory
 // pipe has taken them); and the only waits are for data that was asked for two steps ago.
 // The N side is the A operand of the MFMA: a lane then holds four consecutive n of one m per register quad, which is the contiguous direction of the output.

@@ -379,7 +379,7 @@ __device__ __forceinline__ void store_symmetric(const f32x4 (&acc)[P::NB][P::MB]
 
 // A, all of k or (a long, narrow X has few tiles) a part of it: then the sums are left as they lie in the registers, and gram_sum_kernel adds the parts in their order.
 // Bound by the matrix pipes where the tiles fill the chip (two 8192 x 4096: 0.86 ms, 0.99 PFLOP/s of fp16 products, 0.97 of the tiles' work being needed), else by the latency of the
-// DMA: one 1531 x 1000, 136 tiles of 64 x 64 and 48 steps, 16 us.
+// DMA: one 1531 x 1000, 136 tiles of 64 x 64 and 48 steps, 16 us: 0.33 us a step with three of them on their way, 110 MB out of the L2s, of which 63 % is found there.
 template <class G>
 __global__ void __launch_bounds__(G::THREADS, (SplitProduct<G, RC>::LDS_BYTES <= 80 * 1024 ? 2 : 1)) gram_kernel(Jobs jobs, int from) {
 	using P = SplitProduct<G, RC>;
@@ -662,7 +662,8 @@ static bool is_tiny(const NgpMuonMatrix& m) { return std::min(m.rows, m.cols) <=
 // ---- a matrix of a short side up to 64, in slabs of its long one -------------------------------------------------------------------------------
 //
 // Between two iterations only A, 64 x 64, has to be known to all: a launch to an iteration, in which every workgroup adds the slabs' parts of A in their order, works out B for itself,
-// multiplies its 128 or 256 rows of X^T and leaves their part of the next A.  Bound by the launches: one 1640 x 24 64 us, 98 by the kernels above.
+// multiplies its 128 or 256 rows of X^T and leaves their part of the next A.  Bound by the chain inside a launch, 10 us from
+// the slab's and the parts' way in to the slab's way out, no gap between them: one 1640 x 24 64 us, 98 by the kernels above.
 constexpr uint32_t MAX_SLABS = 32, BATCH_SLABS = 256, PART_FLOATS = TINY_N * TINY_N;
 static uint32_t slab_rows(uint32_t k) { return k <= TINY_K / 2 * MAX_SLABS ? TINY_K / 2 : TINY_K; }
 static uint32_t slabs_of(const NgpMuonMatrix& m) {   // 0: not in slabs
@@ -764,7 +765,7 @@ static const char* bad_matrices(uint32_t count, const NgpMuonMatrix* m) {
 
 // The tile whose rounds of the chip cost least.  A round, in units of one 128 x 128 tile a CU in eight waves: two of four waves (24 of 768 x 768: 957 -> 845 us) 1.7, one 128 x 256
 // 1.68 (two 8192 x 4096: 1.25 ms a launch where 128 x 128 take 1.7; not for the symmetric products: 0.87 ms both, more of a larger tile lies above the diagonal), two 64 x 64
-// 0.8.  In a sweep of 16 shapes this is within 3 % of the best of the four; a step of 2000 x 2000 723 -> 657 us, 1500 x 1500 425 -> 390, 4000 x 8000 6.92 -> 6.56 ms against
+// 0.8.  In a sweep of 16 shapes this is within 2.5 % of the best of the four (profiles/muon_tiles.txt); a step of 2000 x 2000 723 -> 657 us, 1500 x 1500 425 -> 390, 4000 x 8000 6.92 -> 6.56 ms against
 // fixed bounds on the number of tiles.
 enum { LITTLE_TILE, LONE_TILE, MIDDLE_TILE, LARGE_TILE };
 static double rounds(uint32_t tiles, uint32_t slots) { return (double)((tiles + slots - 1) / slots); }
