@@ -1703,7 +1703,7 @@ void Testbed::train_nerf_dp_backward(uint32_t target_batch_size, uint32_t global
 //     runs it by itself when it is a collective anyway — render_sharded — and refuses otherwise).  The fp32 state (master weights, moments, Ema) stays sharded: rank r
 //     owns elements [r * shard, (r + 1) * shard); dp_gather_optimizer_state makes it whole.
 // Element for element the arithmetic of the replicated step: tests/test_dp_cpu.py (gloo, oracle; worlds of 2 and 3) and tests/test_dp_gpu.py (shards on one GPU) compare bit for bit.
-void Testbed::optimizer_step_sharded() {
+void Testbed::optimizer_step_sharded(float loss_scale) {
 	join_side_ema();
 	++m_optimizer_step;
 	const uint32_t world = m_world_size, rank = m_rank;
@@ -1730,12 +1730,12 @@ void Testbed::optimizer_step_sharded() {
 	profile_begin(PK_OPTIMIZER);
 	const uint32_t matrix_here = m_n_matrix_params > off ? m_n_matrix_params - off : 0u;
 	if (m_dp_sharded_ema) {
-		if (mine) check(ngp_hip_optimizer_step(m_stream, mine, matrix_here, m_optimizer_step, m_learning_rate, m_beta1, m_beta2, m_epsilon, m_l2_reg, LOSS_SCALE, ema_decay,
+		if (mine) check(ngp_hip_optimizer_step(m_stream, mine, matrix_here, m_optimizer_step, m_learning_rate, m_beta1, m_beta2, m_epsilon, m_l2_reg, loss_scale, ema_decay,
 		                                              m_grads.as<uint16_t>() + off, m_master.as<float>() + off, m_params.as<uint16_t>() + off, m_first_moments.as<float>() + off,
 		                                              m_second_moments.as<float>() + off, m_ema.as<float>() + off, m_inference_params.as<uint16_t>() + off, mask), "optimizer_step (Adam + Ema, this rank's shard)");
 		if (world > 1) m_dp_inference_stale = true;
 	} else if (mine) {
-		check(ngp_hip_optimizer_step(m_stream, mine, matrix_here, m_optimizer_step, m_learning_rate, m_beta1, m_beta2, m_epsilon, m_l2_reg, LOSS_SCALE, ema_decay,
+		check(ngp_hip_optimizer_step(m_stream, mine, matrix_here, m_optimizer_step, m_learning_rate, m_beta1, m_beta2, m_epsilon, m_l2_reg, loss_scale, ema_decay,
 		                                    m_grads.as<uint16_t>() + off, m_master.as<float>() + off, m_params.as<uint16_t>() + off, m_first_moments.as<float>() + off,
 		                                    m_second_moments.as<float>() + off, nullptr, nullptr, mask | NGP_OPT_NO_EMA), "optimizer_step (Adam, this rank's shard)");
 	}
@@ -1744,7 +1744,7 @@ void Testbed::optimizer_step_sharded() {
 	check(ngp_rccl_allgather_f16(m_dp_comm, m_stream, m_params.as<uint16_t>(), shard), "ngp_rccl_allgather_f16 (weights)");
 	profile_end(PK_PARAM_GATHER, m_n_params);
 	if (!m_dp_sharded_ema)
-		check(ngp_hip_optimizer_step(m_stream, (uint32_t)m_n_params, m_n_matrix_params, m_optimizer_step, m_learning_rate, m_beta1, m_beta2, m_epsilon, m_l2_reg, LOSS_SCALE, ema_decay, nullptr, nullptr,
+		check(ngp_hip_optimizer_step(m_stream, (uint32_t)m_n_params, m_n_matrix_params, m_optimizer_step, m_learning_rate, m_beta1, m_beta2, m_epsilon, m_l2_reg, loss_scale, ema_decay, nullptr, nullptr,
 		                                    m_params.as<uint16_t>(), nullptr, nullptr, m_ema.as<float>(), m_inference_params.as<uint16_t>(), NGP_OPT_EMA_ONLY), "optimizer_step (Ema, all parameters)");
 	if (m_has_decay && m_optimizer_step >= m_decay_start && (m_decay_end == 0 || m_optimizer_step < m_decay_end) && m_decay_interval && m_optimizer_step % m_decay_interval == 0) {
 		m_learning_rate *= m_decay_base;
@@ -1779,7 +1779,7 @@ void Testbed::require_inference_params(const char* who, bool collective) {
 }
 
 void Testbed::optimizer_step(float loss_scale) {  // Trainer::optimizer_step(stream, LOSS_SCALE) (testbed_nerf.cu:2950)
-	if (m_dp_comm && dp_sharded_step()) { optimizer_step_sharded(); return; }
+	if (m_dp_comm && dp_sharded_step()) { optimizer_step_sharded(loss_scale); return; }
 	if (m_dp_state_stale) throw std::runtime_error{"optimizer step on fp32 state that sharded data-parallel steps left stale outside this rank's shard: call dp_gather_optimizer_state() on all ranks before shutdown_data_parallel()"};
 	++m_optimizer_step;
 	uint32_t mask = (m_train_network ? 1u : 0u) | (m_train_encoding ? 2u : 0u);

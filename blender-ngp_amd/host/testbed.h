@@ -335,7 +335,7 @@ public:
 	bool render_is_collective() const { return m_dp_comm && m_render_sharded; }   // (a one-rank communicator runs the same path: split, gather buffer, RCCL call)
 	static constexpr size_t DP_PARAM_SLACK = 1024;   // elements behind the weights / gradients: world x shard (shard a multiple of 8) may exceed n_params by < 8 x world
 	DeviceBuffer m_dp_grads_f32, m_dp_shard_f32;
-	void optimizer_step_sharded();
+	void optimizer_step_sharded(float loss_scale);
 	void dp_gather_optimizer_state();   // collective: the whole fp32 optimizer state on every rank (before a snapshot with optimizer state / leaving data-parallel mode)
 	void shutdown_data_parallel();
 	bool m_dp_strong_scaling = false;

@@ -434,3 +434,47 @@ def test_a_non_finite_row_of_the_backward_pass_stays_in_its_row_of_dx(ngp, cuda,
     assert torch.isnan(runs[1][1]).all() and torch.isnan(runs[1][2]).all()
     other = torch.arange(o, device="cuda") != 1
     assert torch.isnan(runs[1][3][1]).all() and torch.equal(runs[0][3][other], runs[1][3][other])   # dw_down: the row of that output alone
+
+
+def test_the_most_rows(ngp, cuda):
+    """2^30 rows: positions, tiles and row offsets of the narrow kernels at their largest.  y and dx against 64 bits on rows from all over; the gradients against the sums in 64 bits, to the roundings
+    of partial sums in fp32 (2^30 terms of one sign would be lost in one accumulator: here they have both, and 512 workgroups' waves have their own)"""
+    rows, d, f, o = 1 << 30, 2, 3, 1
+    x = torch.empty(rows, d, dtype=torch.float16, device="cuda")
+    dy = torch.empty(rows, o, dtype=torch.float16, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(1)
+    part = 1 << 26
+    for i in range(0, rows, part):
+        x[i:i + part] = torch.randn(part, d, generator=g, device="cuda", dtype=torch.float32)
+        dy[i:i + part] = torch.randn(part, o, generator=g, device="cuda", dtype=torch.float32) * 0.5
+    wg, wu, wd = (torch.randn(s, generator=g, device="cuda").half() for s in ((f, d), (f, d), (o, f)))
+    b = block(d, f, o, "f16", "relu")
+    y, dx = torch.empty(rows, o, dtype=torch.float16, device="cuda"), torch.empty_like(x)
+    grads = [torch.empty_like(w) for w in (wg, wu, wd)]
+    ws, n = workspace(ngp, b, rows, 0)
+    forward(ngp, b, x, wg, wu, wd, y, ws, n)
+    ws2, n2 = workspace(ngp, b, rows, capi.FFN_BACKWARD)
+    backward(ngp, b, x, wg, wu, wd, dy, dx, grads, ws2, n2)
+    torch.cuda.synchronize()
+    for at in (0, rows // 2 - 1000, rows - 3001, rows - 1000):
+        ref = R.Block("relu", x[at:at + 1000], wg, wu, wd, dy[at:at + 1000])
+        R.check("y", y[at:at + 1000], ref.y, ref.ey)
+        R.check("dx", dx[at:at + 1000], ref.dx, ref.edx)
+    sums, magnitudes = [torch.zeros_like(w, dtype=torch.float64) for w in grads], [torch.zeros_like(w, dtype=torch.float64) for w in grads]
+    part = 1 << 24   # sums of elementwise products: the library's product of such a shape, three by two over 2^26, takes two seconds
+    for i in range(0, rows, part):
+        xs, ys = x[i:i + part].double(), dy[i:i + part].double()
+        gg, u = (sum(xs[:, j:j + 1] * w[:, j].double() for j in range(d)) for w in (wg, wu))
+        on = (gg > 0).double()
+        dh = ys * wd.double()
+        for k, (p, q) in enumerate(((dh * u * on, xs), (dh * gg * on, xs), (ys, gg * on * u))):
+            for c in range(q.shape[1]):
+                t = p * q[:, c:c + 1]
+                sums[k][:, c] += t.sum(0)
+                magnitudes[k][:, c] += t.abs().sum(0)
+    for v, want, size in zip(grads, sums, magnitudes):
+        # every term is rounded once or twice to f16 and enters sums of up to 2^21 rows in one accumulator (2^30 / 512 workgroups): the roundings' signs are as random as the terms',
+        # so sqrt(terms) of 2^-11 of a term, and sqrt(2^21) 2^-24 of a partial sum, which is itself of the order of sqrt(2^21) terms; 8 standard deviations, and the result's own rounding
+        term = size / rows
+        limit = 8 * (2.0 ** 15 * 2 * 2.0 ** -11 * term * 2 + 512 ** 0.5 * 2.0 ** 10.5 * 2.0 ** -24 * 2.0 ** 10.5 * term * 2) + 2.0 ** -11 * want.abs() + 2.0 ** -25
+        assert (torch.isinf(v.double()) & (want.abs() > 60000)).logical_or((v.double() - want).abs() <= limit).all(), (v, want, limit)

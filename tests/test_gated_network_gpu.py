@@ -451,3 +451,27 @@ def test_the_loss_scale_of_relative_losses_and_of_the_optimizers(cuda, tmp_path)
             limit = 2.0 ** -11 * (p0.abs() + p1.abs()) + 2.0 ** -24 + rate * 2.0 ** -20 * 3.4445 ** 5 * 1.21 * min(r, c) ** 0.5
             assert ((p0 - p1 - rate * M.orthogonalise(u, 1e-7, 5)).abs() <= limit).all(), (step, r, c)
     assert momentum.abs().sum() > 0
+
+
+def test_one_testbed_through_both_networks(cuda, tmp_path):
+    """base -> gated -> base -> gated in one Testbed, a render and an error between the steps: every one trains as in a fresh Testbed, whatever the buffers held before"""
+    import pyngp
+
+    def trained(tb, name):
+        tb.reload_network_from_file(_config(tmp_path, name, encoding=dict(log2_hashmap_size=12)))
+        tb.shall_train = True
+        for n in (1 << 14, 1 << 10, 1 << 13):
+            tb.train(n)
+            assert np.isfinite(tb.render(48, 32, 1, True)).all() and np.isfinite(tb.compute_image_mse(False))
+        return tb.debug_params("training").copy(), tb.debug_params("inference").copy()
+
+    def fresh():
+        tb = pyngp.Testbed(pyngp.TestbedMode.Image)
+        tb.set_image_data(_image())
+        return tb
+
+    want = {name: trained(fresh(), name) for name in ("image/base.json", "image/gated.json")}
+    tb = fresh()
+    for name in ("image/base.json", "image/gated.json", "image/base.json", "image/gated.json"):
+        for got, exp in zip(trained(tb, name), want[name]):
+            np.testing.assert_array_equal(got, exp)
