@@ -140,12 +140,15 @@ void Testbed::gridmlp_inference(const uint16_t* params, const float* pos, uint32
 
 // What the loss is multiplied by, so that F16 holds the gradients: 128 as everywhere, per sample 1 / n of it.  A gated network needs more of it for a large batch: its features start
 // within 1e-4 and a gate's gradient is a product with another of them, 1e-9 of a batch of 2^18 and so zero in F16 (the smallest is 6e-8): the image config stood at 3.03 dB for 1000
-// steps, with 1024 or more it reaches 35 to 36.  From 2^14 samples on a sample's share stays what it is there, up to 2^20 (the weights' gradients, sums over the batch, grow with the
-// scale: 8192 leaves them 8).  Not for the relative losses: their gradients are up to 100 times as large, and SDF samples lie where they are.
+// steps, with 1024 or more it reaches 35 to 36.  From 2^14 samples on a sample's share stays what it is there, up to 2^20.  The weights' gradients, sums over the batch, grow with the
+// scale: 8192 leaves them 8, so an L2 loss whose residuals are larger than one (its last value read; none before the first step, whose hidden values are 1e-9) gives that back, down
+// to 128.  The relative losses keep 128: their gradients are up to 100 times as large, and at 2^20 samples 12 % (MAPE) and more of the table's first gradients are there.
 float Testbed::gridmlp_loss_scale(uint32_t n) const {
 	float scale = LOSS_SCALE;
-	if (!m_gated || (m_nerf.training.loss_type != ELossType::L2 && m_nerf.training.loss_type != ELossType::L1)) return scale;
+	const bool l2 = m_nerf.training.loss_type == ELossType::L2;
+	if (!m_gated || (!l2 && m_nerf.training.loss_type != ELossType::L1)) return scale;
 	for (uint32_t k = n >> 15; k && scale < 64.0f * LOSS_SCALE; k >>= 1) scale *= 2.0f;
+	for (float squares = l2 ? m_loss_scalar : 0.0f; squares > 1.0f && scale > LOSS_SCALE; squares *= 0.25f) scale *= 0.5f;
 	return scale;
 }
 

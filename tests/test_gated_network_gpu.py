@@ -475,3 +475,27 @@ def test_one_testbed_through_both_networks(cuda, tmp_path):
     for name in ("image/base.json", "image/gated.json", "image/base.json", "image/gated.json"):
         for got, exp in zip(trained(tb, name), want[name]):
             np.testing.assert_array_equal(got, exp)
+
+
+def test_bright_images_give_the_loss_scale_back(cuda, tmp_path):
+    """residuals far above one: the scale of a large batch goes down with the loss that was last read, and everything stays finite"""
+    import pyngp
+    tb = pyngp.Testbed(pyngp.TestbedMode.Image)
+    img = _image()
+    img[..., :3] *= 3000.0
+    tb.set_image_data(img)
+    c = _config(tmp_path, "image/gated.json", encoding=dict(log2_hashmap_size=14))
+    tb.reload_network_from_file(c)
+    tb.shall_train = True
+    tb.train(1 << 18)
+    assert tb.gridmlp_loss_scale == 2048 and tb.loss > 16
+    for _ in range(200):
+        tb.train(1 << 18)
+        assert 128 <= tb.gridmlp_loss_scale <= 2048
+    assert np.isfinite(tb.debug_params("training").view(np.float16)).all() and np.isfinite(tb.loss)
+    tb.reload_network_from_file(c)   # a fresh network starts with the full scale again
+    tb.train(1 << 18)
+    assert tb.gridmlp_loss_scale == 2048
+    first = tb.loss
+    tb.train(1 << 18)
+    assert tb.gridmlp_loss_scale == max(128.0, 2048.0 / 2.0 ** np.ceil(np.log2(max(1.0, first)) / 2))
