@@ -678,16 +678,22 @@ void Testbed::load_nerf_post() {
 Json Testbed::load_network_config(const std::string& path) {  // testbed.cu:120-145
 	return load_config_or_snapshot(path);
 }
+// the config and its path are those of the network in use: a refused one does not stay (a snapshot would name it)
+void Testbed::take_network_config(Json config, std::string path) {
+	std::swap(m_network_config, config);
+	std::swap(m_network_config_path, path);
+	try { reset_network(); }
+	catch (...) {
+		std::swap(m_network_config, config);
+		std::swap(m_network_config_path, path);
+		throw;
+	}
+}
 void Testbed::reload_network_from_file(const std::string& path) {
-	if (!path.empty()) m_network_config_path = path;
-	m_network_config = load_network_config(m_network_config_path);
-	reset_network();
+	const std::string from = path.empty() ? m_network_config_path : path;
+	take_network_config(load_network_config(from), from);
 }
-void Testbed::reload_network_from_json(const Json& json, const std::string& config_base_path) {
-	m_network_config_path = config_base_path;
-	m_network_config = json;
-	reset_network();
-}
+void Testbed::reload_network_from_json(const Json& json, const std::string& config_base_path) { take_network_config(json, config_base_path); }
 
 static ELossType string_to_loss_type(std::string s) {  // testbed.cu:2220-2240
 	std::transform(s.begin(), s.end(), s.begin(), ::tolower);

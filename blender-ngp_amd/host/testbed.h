@@ -289,6 +289,7 @@ public:
 	// ---- network (testbed.cu:120-194, 2249-2470)
 	void reload_network_from_file(const std::string& path = "");
 	void reload_network_from_json(const Json& json, const std::string& config_base_path = "");
+	void take_network_config(Json config, std::string path);
 	Json load_network_config(const std::string& path);
 	void reset_network(bool clear_density_grid = true);
 	void reset(bool reset_density_grid = true) { reset_network(reset_density_grid); }

@@ -499,3 +499,28 @@ def test_bright_images_give_the_loss_scale_back(cuda, tmp_path):
     first = tb.loss
     tb.train(1 << 18)
     assert tb.gridmlp_loss_scale == max(128.0, 2048.0 / 2.0 ** np.ceil(np.log2(max(1.0, first)) / 2))
+
+
+def test_a_refused_config_is_not_what_a_snapshot_names(cuda, tmp_path):
+    import msgpack
+    import scene
+    ds = scene.make_dataset(n_train=4, n_test=1, res=48, device=torch.device("cuda:0"))
+    mine = _config(tmp_path, "nerf/muon.json", encoding=dict(log2_hashmap_size=14))
+    tb = scene.build_testbed(ds, mine)
+    scene.train(tb, 2)
+    params = tb.debug_params("training").copy()
+    with pytest.raises(RuntimeError):
+        tb.reload_network_from_file(_config(tmp_path, "nerf/base.json", encoding=dict(log2_hashmap_size=19), network=dict(otype="GatedMLP")))
+    path = str(tmp_path / "kept.msgpack")
+    tb.save_snapshot(path, True)
+    saved = msgpack.unpackb(open(path, "rb").read(), raw=False)
+    assert saved["encoding"]["log2_hashmap_size"] == 14 and saved["network"]["otype"] == "FullyFusedMLP"
+    other = scene.build_testbed(ds, mine)
+    other.load_snapshot(path)
+    np.testing.assert_array_equal(other.debug_params("training"), params)
+    # without a path: the last config that was taken
+    again = scene.build_testbed(ds, mine)
+    with pytest.raises(RuntimeError):
+        again.reload_network_from_file(_config(tmp_path, "nerf/base.json", optimizer={"otype": "Shampoo"}))
+    again.reload_network_from_file("")
+    assert again.n_params() == tb.n_params()
